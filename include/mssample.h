@@ -48,7 +48,7 @@ enum {
                             ms_build_json_mask_noalloc (V > 262144) */
 };
 
-enum { MS_DTYPE_F32 = 0, MS_DTYPE_BF16 = 1 };
+enum { MS_DTYPE_F32 = 0, MS_DTYPE_BF16 = 1, MS_DTYPE_F16 = 2 /* decode-step operators only */ };
 
 /* row_status bits */
 enum {
@@ -63,9 +63,15 @@ enum {
                                  full vocabulary (top_k off or above kmax,
                                  a tie block past the candidate buffer, a
                                  non-finite logit); token -1 */
-  MS_ROW_PEER_TIMEOUT = 16    /* fused peer exchange only: a rank's record
+  MS_ROW_PEER_TIMEOUT = 16,   /* fused peer exchange only: a rank's record
                                  of the row had not arrived when
                                  ms_exchange_merge gave up waiting; token -1 */
+  /* decode-step operators */
+  MS_ROW_BAD_SLOT = 32,       /* ms_kv_append: slot past the cache; nothing is
+                                 written to the cache for the token */
+  MS_ROW_BAD_POSITION = 64    /* ms_kv_append: position outside the table;
+                                 nothing is written to the cache, the
+                                 token's q_out is zero */
 };
 
 /*
@@ -366,6 +372,56 @@ int ms_build_json_mask_noalloc(const uint32_t *states, int64_t B, const uint8_t 
  */
 int ms_mask_from_logits(const void *logits, int dtype, int64_t B, int64_t V, int64_t ld, uint32_t *mask,
                         int64_t mask_ld, ms_stream_t stream);
+
+/*
+ * Append new keys and values to a paged cache, the position rotation applied
+ * on the way, and rotate the same tokens' queries.
+ *
+ * The first `rotary` entries of every query and key head are rotated in
+ * pairs (a, b) -> (a c - b s, b c + a s), pair i being entries (i, i +
+ * rotary/2), or (2i, 2i + 1) when `interleaved`; c and s are the entries i
+ * and rotary/2 + i of row positions[t] of `table`.  The other entries and the
+ * values are copied.  The arithmetic is fp32, rounded once.
+ *
+ * Token t's key and value heads go to slot slots[t] = page * page_size +
+ * offset of the caches; a negative slot (padding) writes nothing there.  Slots
+ * of one call should differ: of two equal ones either token's entries may
+ * stay.  q_out may be q itself (the same strides).
+ *
+ * This struct is read on the host during the call; its pointers are device
+ * pointers and its strides count entries (the last dimension is contiguous).
+ * 16-byte accesses are used where head_dim and rotary are multiples of 16,
+ * strides of 8 and bases 16-byte aligned, single entries otherwise.
+ */
+typedef struct {
+  int32_t dtype;        /* MS_DTYPE_BF16 or MS_DTYPE_F16: q, k, v and the caches */
+  int32_t heads;        /* query heads; 0: no queries (q and q_out are not read) */
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t rotary;       /* even, <= head_dim; 0: nothing is rotated */
+  int32_t interleaved;
+  int64_t tokens;
+  const void *q;        /* [tokens, heads, head_dim] */
+  int64_t q_token, q_head;
+  const void *k;        /* [tokens, kv_heads, head_dim] */
+  int64_t k_token, k_head;
+  const void *v;        /* [tokens, kv_heads, head_dim] */
+  int64_t v_token, v_head;
+  void *q_out;          /* [tokens, heads, head_dim] */
+  int64_t q_out_token, q_out_head;
+  void *cache_k;        /* [pages, page_size, kv_heads, head_dim], any order of the first three */
+  int64_t ck_page, ck_token, ck_head;
+  void *cache_v;
+  int64_t cv_page, cv_token, cv_head;
+  int64_t pages, page_size;
+  const int64_t *slots; /* [tokens] */
+  const int64_t *positions; /* [tokens]; not read when rotary is 0 */
+  const float *table;   /* [table_rows, rotary]: rotary/2 cosines, then rotary/2 sines */
+  int64_t table_rows;
+  int32_t *status;      /* [tokens] MS_ROW_* bits out, or NULL */
+} ms_kv_append_args;
+
+int ms_kv_append(const ms_kv_append_args *args, ms_stream_t stream);
 
 /* Human-readable text for an MS_E_* code. */
 const char *ms_error_string(int code);

@@ -16,18 +16,35 @@ MS_OK = 0
 MS_E_TOO_LARGE = -5
 MS_DTYPE_F32 = 0
 MS_DTYPE_BF16 = 1
+MS_DTYPE_F16 = 2
 MS_ROW_OK = 0
 MS_ROW_ALL_MASKED = 1
 MS_ROW_BAD_TEMPERATURE = 2
 MS_ROW_NONFINITE = 4
 MS_ROW_UNSUPPORTED = 8
 MS_ROW_PEER_TIMEOUT = 16
+MS_ROW_BAD_SLOT = 32
+MS_ROW_BAD_POSITION = 64
 
 _lock = threading.Lock()
 _lib = None
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
+_I32 = ctypes.c_int32
+
+
+class KvAppendArgs(ctypes.Structure):
+    """ms_kv_append_args of include/mssample.h."""
+    _fields_ = [("dtype", _I32), ("heads", _I32), ("kv_heads", _I32), ("head_dim", _I32), ("rotary", _I32),
+                ("interleaved", _I32), ("tokens", _I64),
+                ("q", _P), ("q_token", _I64), ("q_head", _I64), ("k", _P), ("k_token", _I64), ("k_head", _I64),
+                ("v", _P), ("v_token", _I64), ("v_head", _I64), ("q_out", _P), ("q_out_token", _I64),
+                ("q_out_head", _I64), ("cache_k", _P), ("ck_page", _I64), ("ck_token", _I64), ("ck_head", _I64),
+                ("cache_v", _P), ("cv_page", _I64), ("cv_token", _I64), ("cv_head", _I64), ("pages", _I64),
+                ("page_size", _I64), ("slots", _P), ("positions", _P), ("table", _P), ("table_rows", _I64),
+                ("status", _P)]
+
 
 # name -> (restype, argtypes); every function include/mssample.h declares
 SIGNATURES = {
@@ -78,6 +95,7 @@ SIGNATURES = {
     "ms_build_json_mask_packed": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _I64, _P, _I64, _P, _P]),
     "ms_json_pack_vocab_ordered": (ctypes.c_int, [_P, _P, _I64, _P, _P, _P, _P]),
     "ms_build_json_mask_ordered": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _P, _I64, _P, _I64, _P, _P]),
+    "ms_kv_append": (ctypes.c_int, [ctypes.POINTER(KvAppendArgs), _P]),
     "ms_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ms_last_cuda_error": (ctypes.c_int, []),
     "ms_version": (ctypes.c_int, []),

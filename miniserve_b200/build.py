@@ -16,7 +16,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmssample.so")
-SOURCES = ["ms_sample.cu"]
+SOURCES = ["ms_sample.cu", "ms_kv.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -34,7 +34,7 @@ def build(verbose: bool = False, extra_flags=None) -> str:
         lib_m = os.path.getmtime(LIB)
         if all(os.path.getmtime(d) <= lib_m for d in deps):
             return LIB
-    cmd = [nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
+    cmd = [nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared", "-t", "0",
            "-Xptxas", "-v" if verbose else "-O3", "-o", LIB + ".tmp",
            *[os.path.join(CSRC, s) for s in SOURCES], *(extra_flags or [])]
     res = subprocess.run(cmd, capture_output=True, text=True)

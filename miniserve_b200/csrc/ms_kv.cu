@@ -1,0 +1,287 @@
+// ms_kv_append -- new keys and values into a paged cache, the position
+// rotation applied on the way (declared in include/mssample.h).
+//
+// Each rotated pair (a, b) of a head becomes (a c - b s, b c + a s) with the
+// cosine c and sine s of the token's position, from an fp32 table; the other
+// entries and the values are copied.  The arithmetic is fp32, rounded once to
+// the cache's type.
+//
+// Bound by bytes: every element is read once and written once, and one
+// table row of rotary fp32 pairs per token serves all its heads.  A thread
+// owns 16 entries of a head (two 16-byte loads and stores: eight pairs, or 16
+// copied entries), keeps its eight cosines and sines in registers and walks
+// over `per_thread` heads with them.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/mssample.h"
+#include "ms_host.h"
+
+namespace ms {
+
+template <typename T>
+__device__ __forceinline__ float2 kv_widen(uint32_t u);
+template <>
+__device__ __forceinline__ float2 kv_widen<__nv_bfloat16>(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+}
+template <>
+__device__ __forceinline__ float2 kv_widen<__half>(uint32_t u) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t kv_narrow(float x, float y);
+template <>
+__device__ __forceinline__ uint32_t kv_narrow<__nv_bfloat16>(float x, float y) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t kv_narrow<__half>(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float kv_to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float kv_to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ void kv_from_float(float x, __nv_bfloat16 &y) { y = __float2bfloat16_rn(x); }
+__device__ __forceinline__ void kv_from_float(float x, __half &y) { y = __float2half_rn(x); }
+
+struct KvArgs {
+  ms_kv_append_args a;
+  int per_token;   // threads of one token
+  int slots;       // head slots of one token: thread slot s walks over heads s, s + slots, ...
+  int tokens_cta;  // tokens of one CTA
+};
+
+// The token's cache row and status: bit set and no row for a bad slot or
+// position, no row and MS_ROW_OK for a negative slot.
+struct KvRow {
+  int64_t page;
+  int64_t offset;
+  int64_t position;
+  int32_t status;
+  bool write;
+};
+
+__device__ __forceinline__ KvRow kv_row(const ms_kv_append_args &a, int64_t t) {
+  KvRow r{0, 0, 0, MS_ROW_OK, false};
+  const int64_t slot = __ldg(a.slots + t);
+  if (slot >= a.pages * a.page_size) {
+    r.status |= MS_ROW_BAD_SLOT;
+  } else if (slot >= 0) {
+    if (slot < (1ll << 32)) {
+      r.page = (uint32_t)slot / (uint32_t)a.page_size;
+      r.offset = (uint32_t)slot - (uint32_t)r.page * (uint32_t)a.page_size;
+    } else {
+      r.page = slot / a.page_size;
+      r.offset = slot - r.page * a.page_size;
+    }
+    r.write = true;
+  }
+  if (a.rotary > 0) {
+    r.position = __ldg(a.positions + t);
+    if (r.position < 0 || r.position >= a.table_rows) {
+      r.status |= MS_ROW_BAD_POSITION;
+      r.position = 0;
+    }
+  }
+  if (r.status != MS_ROW_OK) r.write = false;
+  return r;
+}
+
+// Source and destination of head h of token t (null where nothing is written).
+template <typename T>
+__device__ __forceinline__ void kv_head(const ms_kv_append_args &a, const KvRow &r, int64_t t, int h, const T *&src,
+                                        T *&dst, bool &turn) {
+  turn = true;
+  if (h < a.heads) {
+    src = reinterpret_cast<const T *>(a.q) + t * a.q_token + h * a.q_head;
+    dst = reinterpret_cast<T *>(a.q_out) + t * a.q_out_token + h * a.q_out_head;
+    return;
+  }
+  h -= a.heads;
+  const bool key = h < a.kv_heads;
+  if (key) {
+    src = reinterpret_cast<const T *>(a.k) + t * a.k_token + h * a.k_head;
+    dst = reinterpret_cast<T *>(a.cache_k) + r.page * a.ck_page + r.offset * a.ck_token + h * a.ck_head;
+  } else {
+    h -= a.kv_heads;
+    src = reinterpret_cast<const T *>(a.v) + t * a.v_token + h * a.v_head;
+    dst = reinterpret_cast<T *>(a.cache_v) + r.page * a.cv_page + r.offset * a.cv_token + h * a.cv_head;
+    turn = false;
+  }
+  if (!r.write) dst = nullptr;
+}
+
+constexpr int kKvThreads = 256;
+
+// 16-byte path: head_dim and rotary multiples of 16, every stride a multiple
+// of 8 entries and every base 16-byte aligned (checked on the host).
+template <typename T, bool kInterleaved>
+__global__ void __launch_bounds__(kKvThreads) ms_kv_append_kernel(const __grid_constant__ KvArgs p) {
+  const ms_kv_append_args &a = p.a;
+  const int chunks = a.head_dim >> 4;
+  const int heads = a.heads + 2 * a.kv_heads;
+  const int64_t t0 = (int64_t)blockIdx.x * p.tokens_cta;
+  for (int u = threadIdx.x; u < p.tokens_cta * p.per_token; u += kKvThreads) {
+    const int tl = u / p.per_token, w = u - tl * p.per_token;
+    const int64_t t = t0 + tl;
+    if (t >= a.tokens) return;
+    const int slot = w / chunks, j = w - slot * chunks;
+    const KvRow r = kv_row(a, t);
+    if (w == 0 && a.status) a.status[t] = r.status;
+    const bool rotates = j * 16 < a.rotary;
+    // entries of the two 16-byte halves a rotating thread owns
+    const int lo = (!rotates || kInterleaved) ? j * 16 : j * 8;
+    const int hi = (!rotates || kInterleaved) ? lo + 8 : lo + (a.rotary >> 1);
+    float c[8], s[8];
+    if (rotates) {
+      const float *row = a.table + r.position * a.rotary + j * 8;
+      *reinterpret_cast<float4 *>(c) = __ldg(reinterpret_cast<const float4 *>(row));
+      *reinterpret_cast<float4 *>(c + 4) = __ldg(reinterpret_cast<const float4 *>(row) + 1);
+      row += a.rotary >> 1;
+      *reinterpret_cast<float4 *>(s) = __ldg(reinterpret_cast<const float4 *>(row));
+      *reinterpret_cast<float4 *>(s + 4) = __ldg(reinterpret_cast<const float4 *>(row) + 1);
+    }
+#pragma unroll 4
+    for (int h = slot; h < heads; h += p.slots) {
+      const T *src;
+      T *dst;
+      bool turn;
+      kv_head<T>(a, r, t, h, src, dst, turn);
+      if (!dst) continue;
+      if (r.status & MS_ROW_BAD_POSITION) {
+        *reinterpret_cast<uint4 *>(dst + lo) = *reinterpret_cast<uint4 *>(dst + hi) = make_uint4(0, 0, 0, 0);
+        continue;
+      }
+      uint4 x = *reinterpret_cast<const uint4 *>(src + lo), y = *reinterpret_cast<const uint4 *>(src + hi);
+      if (rotates && turn) {
+        uint32_t *xs = reinterpret_cast<uint32_t *>(&x), *ys = reinterpret_cast<uint32_t *>(&y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (kInterleaved) {  // word i of x is pair i, word i of y is pair 4 + i
+            const float2 f = kv_widen<T>(xs[i]), g = kv_widen<T>(ys[i]);
+            xs[i] = kv_narrow<T>(f.x * c[i] - f.y * s[i], f.y * c[i] + f.x * s[i]);
+            ys[i] = kv_narrow<T>(g.x * c[4 + i] - g.y * s[4 + i], g.y * c[4 + i] + g.x * s[4 + i]);
+          } else {  // word i holds the first (x) and second (y) entries of pairs 2i and 2i + 1
+            const float2 f = kv_widen<T>(xs[i]), g = kv_widen<T>(ys[i]);
+            const float c0 = c[2 * i], c1 = c[2 * i + 1], s0 = s[2 * i], s1 = s[2 * i + 1];
+            xs[i] = kv_narrow<T>(f.x * c0 - g.x * s0, f.y * c1 - g.y * s1);
+            ys[i] = kv_narrow<T>(g.x * c0 + f.x * s0, g.y * c1 + f.y * s1);
+          }
+        }
+      }
+      *reinterpret_cast<uint4 *>(dst + lo) = x;
+      *reinterpret_cast<uint4 *>(dst + hi) = y;
+    }
+  }
+}
+
+// Any head_dim, rotary and stride: a thread owns one pair, or two copied
+// entries, of a head.
+template <typename T, bool kInterleaved>
+__global__ void __launch_bounds__(kKvThreads) ms_kv_append_any_kernel(const __grid_constant__ KvArgs p) {
+  const ms_kv_append_args &a = p.a;
+  const int half = a.rotary >> 1;
+  const int units = half + (a.head_dim - a.rotary + 1) / 2;
+  const int heads = a.heads + 2 * a.kv_heads;
+  const int64_t t0 = (int64_t)blockIdx.x * p.tokens_cta;
+  for (int u = threadIdx.x; u < p.tokens_cta * p.per_token; u += kKvThreads) {
+    const int tl = u / p.per_token, w = u - tl * p.per_token;
+    const int64_t t = t0 + tl;
+    if (t >= a.tokens) return;
+    const int slot = w / units, j = w - slot * units;
+    const KvRow r = kv_row(a, t);
+    if (w == 0 && a.status) a.status[t] = r.status;
+    const bool rotates = j < half;
+    int lo, hi;
+    float c = 1.f, s = 0.f;
+    if (rotates) {
+      lo = kInterleaved ? 2 * j : j;
+      hi = kInterleaved ? 2 * j + 1 : j + half;
+      c = __ldg(a.table + r.position * a.rotary + j);
+      s = __ldg(a.table + r.position * a.rotary + half + j);
+    } else {
+      lo = a.rotary + 2 * (j - half);
+      hi = lo + 1;
+    }
+    for (int h = slot; h < heads; h += p.slots) {
+      const T *src;
+      T *dst;
+      bool turn;
+      kv_head<T>(a, r, t, h, src, dst, turn);
+      if (!dst) continue;
+      if (r.status & MS_ROW_BAD_POSITION) {
+        kv_from_float(0.f, dst[lo]);
+        if (hi < a.head_dim) kv_from_float(0.f, dst[hi]);
+      } else if (rotates && turn) {
+        const float x = kv_to_float(src[lo]), y = kv_to_float(src[hi]);
+        kv_from_float(x * c - y * s, dst[lo]);
+        kv_from_float(y * c + x * s, dst[hi]);
+      } else {
+        const T x = src[lo];
+        if (hi < a.head_dim) {
+          const T y = src[hi];
+          dst[hi] = y;
+        }
+        dst[lo] = x;
+      }
+    }
+  }
+}
+
+template <typename T>
+cudaError_t launch_kv_append(KvArgs &p, bool wide, cudaStream_t s) {
+  const ms_kv_append_args &a = p.a;
+  const int heads = a.heads + 2 * a.kv_heads;
+  const int units = wide ? a.head_dim / 16 : a.rotary / 2 + (a.head_dim - a.rotary + 1) / 2;
+  // one head a thread until the call fills the GPU's threads a few times
+  // over; then four, which share the thread's table row
+  const bool many = a.tokens * heads * units > 4ll * 148 * 2048;
+  p.slots = many ? (heads + 3) / 4 : heads;
+  p.per_token = units * p.slots;
+  p.tokens_cta = p.per_token < kKvThreads ? kKvThreads / p.per_token : 1;
+  const unsigned grid = (unsigned)((a.tokens + p.tokens_cta - 1) / p.tokens_cta);
+  if (wide && a.interleaved)
+    ms_kv_append_kernel<T, true><<<grid, kKvThreads, 0, s>>>(p);
+  else if (wide)
+    ms_kv_append_kernel<T, false><<<grid, kKvThreads, 0, s>>>(p);
+  else if (a.interleaved)
+    ms_kv_append_any_kernel<T, true><<<grid, kKvThreads, 0, s>>>(p);
+  else
+    ms_kv_append_any_kernel<T, false><<<grid, kKvThreads, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace ms
+
+extern "C" int ms_kv_append(const ms_kv_append_args *args, ms_stream_t stream) {
+  if (!args) return MS_E_INVALID;
+  ms::KvArgs p{};
+  p.a = *args;
+  const ms_kv_append_args &a = p.a;
+  if (a.dtype != MS_DTYPE_BF16 && a.dtype != MS_DTYPE_F16) return MS_E_DTYPE;
+  if (a.tokens < 0 || a.tokens > 0x7FFFFFFFll || a.heads < 0 || a.heads > 65536 || a.kv_heads < 1 ||
+      a.kv_heads > 65536 || a.head_dim < 1 || a.head_dim > 4096 || a.rotary < 0 || a.rotary > a.head_dim ||
+      (a.rotary & 1) || a.pages < 1 || a.page_size < 1 || a.page_size > 0x7FFFFFFFll ||
+      a.pages > (int64_t)(0x7FFFFFFFFFFFFFFFull / (uint64_t)a.page_size))
+    return MS_E_INVALID;
+  if (a.tokens == 0) return MS_OK;
+  if (!a.k || !a.v || !a.slots || !a.cache_k || !a.cache_v) return MS_E_INVALID;
+  if (a.heads > 0 && (!a.q || !a.q_out)) return MS_E_INVALID;
+  if (a.rotary > 0 && (!a.positions || !a.table || a.table_rows < 1)) return MS_E_INVALID;
+  bool wide = a.head_dim % 16 == 0 && a.rotary % 16 == 0 && ms::aligned16(a.k) && ms::aligned16(a.v) &&
+              ms::aligned16(a.cache_k) && ms::aligned16(a.cache_v) && (a.rotary == 0 || ms::aligned16(a.table)) &&
+              (a.heads == 0 || (ms::aligned16(a.q) && ms::aligned16(a.q_out)));
+  int64_t strides = a.k_token | a.k_head | a.v_token | a.v_head | a.ck_page | a.ck_token | a.ck_head | a.cv_page |
+                    a.cv_token | a.cv_head;
+  if (a.heads > 0) strides |= a.q_token | a.q_head | a.q_out_token | a.q_out_head;
+  wide = wide && (strides & 7) == 0;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e = a.dtype == MS_DTYPE_BF16 ? ms::launch_kv_append<__nv_bfloat16>(p, wide, s)
+                                           : ms::launch_kv_append<__half>(p, wide, s);
+  return e == cudaSuccess ? MS_OK : ms::cuda_fail(e);
+}

@@ -20,6 +20,7 @@
 #include "ms_common.cuh"
 #include "ms_generic.cuh"
 #include "ms_hook.cuh"
+#include "ms_host.h"
 #include "ms_json.cuh"
 #include "ms_exchange.cuh"
 #include "ms_shard.cuh"
@@ -28,13 +29,16 @@
 
 namespace {
 thread_local int g_last_cuda_error = 0;
+}
 
-int cuda_fail(cudaError_t e) {
+int ms::cuda_fail(cudaError_t e) {
   g_last_cuda_error = (int)e;
   return MS_E_CUDA;
 }
 
-constexpr int kMaxDevices = 64;
+namespace {
+using ms::cuda_fail;
+using ms::kMaxDevices;
 
 // The streaming kernel alone: one CTA per row, or in pair mode B clusters of
 // two CTAs.
@@ -125,7 +129,7 @@ const char *ms_error_string(int code) {
   switch (code) {
     case MS_OK: return "ok";
     case MS_E_INVALID: return "invalid argument (null pointer, B < 0, V < 1, V >= 2^31, ld < V or mask_ld too small)";
-    case MS_E_DTYPE: return "unsupported dtype (expected MS_DTYPE_F32 or MS_DTYPE_BF16)";
+    case MS_E_DTYPE: return "unsupported dtype (expected MS_DTYPE_F32 or MS_DTYPE_BF16; other entry points name theirs)";
     case MS_E_CUDA: return "CUDA error (see ms_last_cuda_error)";
     case MS_E_UNSUPPORTED: return "request outside what this build supports";
     case MS_E_TOO_LARGE: return "size beyond the fixed device array of the no-alloc entry point (V > 262144)";
