@@ -423,6 +423,41 @@ typedef struct {
 
 int ms_kv_append(const ms_kv_append_args *args, ms_stream_t stream);
 
+/*
+ * 8-bit integer product with a scale for each token and each output channel:
+ *
+ *   scale[t] = max_k |x[t, k]| / 127          (fp32 division)
+ *   q[t, k]  = rint(x[t, k] / scale[t])       (fp32 division, ties to even)
+ *   out[t, n] = (sum_k q[t, k] wq[n, k]) (scale[t] w_scale[n]) + bias[n]
+ *
+ * ms_quantize_rows makes q and scale from x [M, ldx] (fp32, bf16 or fp16): an
+ * all-zero row has scale 0, a row with a NaN or an infinity scale NaN, and
+ * both have zero integers, so that such a row's outputs are 0 (the bias) and
+ * NaN (the sampler then flags the row MS_ROW_NONFINITE).
+ *
+ * ms_int8_matmul takes xq [M, ldx] and wq [N, ldw] int8, K entries a row, the
+ * row strides multiples of 16 and the bases 16-byte aligned (entries past K
+ * are not used), and writes out [M, ldo] in out_dtype (fp32, bf16 or fp16;
+ * rounded once from fp32).  The sum is exact: K <= 131072.  bias may be NULL.
+ *
+ * ms_int8_linear is the two in one call: x [M, ldx] as it is, the integers and
+ * scales in `workspace` (ms_int8_workspace(M, K) bytes, 16-byte aligned, this
+ * call's until it has finished).  The logits of a quantised LM head, for
+ * ms_sample to read in place.
+ */
+int ms_quantize_rows(const void *x, int dtype, int64_t M, int64_t K, int64_t ldx, int8_t *q, int64_t ldq, float *scale,
+                     ms_stream_t stream);
+
+int ms_int8_matmul(const int8_t *xq, int64_t ldx, const float *x_scale, int64_t M, const int8_t *wq, int64_t ldw,
+                   const float *w_scale, int64_t N, int64_t K, const float *bias, void *out, int out_dtype,
+                   int64_t ldo, ms_stream_t stream);
+
+int64_t ms_int8_workspace(int64_t M, int64_t K);
+
+int ms_int8_linear(const void *x, int dtype, int64_t ldx, int64_t M, const int8_t *wq, int64_t ldw,
+                   const float *w_scale, int64_t N, int64_t K, const float *bias, void *out, int out_dtype,
+                   int64_t ldo, void *workspace, ms_stream_t stream);
+
 /* Human-readable text for an MS_E_* code. */
 const char *ms_error_string(int code);
 

@@ -96,6 +96,11 @@ SIGNATURES = {
     "ms_json_pack_vocab_ordered": (ctypes.c_int, [_P, _P, _I64, _P, _P, _P, _P]),
     "ms_build_json_mask_ordered": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _P, _I64, _P, _I64, _P, _P]),
     "ms_kv_append": (ctypes.c_int, [ctypes.POINTER(KvAppendArgs), _P]),
+    "ms_quantize_rows": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _I64, _P, _P]),
+    "ms_int8_matmul": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _P, ctypes.c_int, _I64, _P]),
+    "ms_int8_workspace": (_I64, [_I64, _I64]),
+    "ms_int8_linear": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, ctypes.c_int,
+                                      _I64, _P, _P]),
     "ms_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ms_last_cuda_error": (ctypes.c_int, []),
     "ms_version": (ctypes.c_int, []),

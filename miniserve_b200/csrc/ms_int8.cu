@@ -1,0 +1,448 @@
+// 8-bit integer product with a scale for each token and each output channel
+// (declared in include/mssample.h): ms_quantize_rows, ms_int8_matmul and the
+// two in one call, ms_int8_linear.
+//
+//   s_t = max_k |x[t, k]| / 127,  q[t, k] = rint(x[t, k] / s_t)
+//   out[t, n] = s_t w_n sum_k q[t, k] wq[n, k] + bias_n
+//
+// The sum is exact in int32 (K <= 131072, so |sum| <= 127^2 K < 2^31).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+
+#include "../../include/mssample.h"
+#include "ms_host.h"
+#include "ms_tc.cuh"
+
+namespace ms {
+
+// ------------------------------------------------------------ quantisation
+constexpr int kQuThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ void qu_load8(const T *p, float (&v)[8]);
+template <>
+__device__ __forceinline__ void qu_load8<float>(const float *p, float (&v)[8]) {
+  *reinterpret_cast<float4 *>(v) = __ldg(reinterpret_cast<const float4 *>(p));
+  *reinterpret_cast<float4 *>(v + 4) = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+}
+template <>
+__device__ __forceinline__ void qu_load8<__nv_bfloat16>(const __nv_bfloat16 *p, float (&v)[8]) {
+  const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+template <>
+__device__ __forceinline__ void qu_load8<__half>(const __half *p, float (&v)[8]) {
+  const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ float qu_float(float x) { return x; }
+__device__ __forceinline__ float qu_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float qu_float(__half x) { return __half2float(x); }
+
+__device__ __forceinline__ int qu_round(float x, float scale) {
+  return max(-127, min(127, __float2int_rn(__fdiv_rn(x, scale))));
+}
+
+// One CTA per token; the second reading of the row comes from the caches.
+// `wide`: rows of 16-byte aligned groups of eight.
+template <typename T>
+__global__ void __launch_bounds__(kQuThreads) ms_quantize_kernel(const T *x, int64_t ldx, int K, int8_t *q, int64_t ldq,
+                                                               float *scale, int wide) {
+  grid_release();
+  __shared__ uint32_t red[kQuThreads / 32];
+  const T *row = x + (int64_t)blockIdx.x * ldx;
+  int8_t *out = q + (int64_t)blockIdx.x * ldq;
+  const int tid = threadIdx.x;
+  const int K8 = wide ? K >> 3 : 0;
+  uint32_t top = 0;  // the largest magnitude's bits: NaN above infinity above finite
+  for (int i = tid; i < K8; i += kQuThreads) {
+    float v[8];
+    qu_load8<T>(row + i * 8, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+  }
+  for (int i = K8 * 8 + tid; i < K; i += kQuThreads) top = max(top, __float_as_uint(qu_float(row[i])) & 0x7FFFFFFFu);
+  top = __reduce_max_sync(0xFFFFFFFFu, top);
+  if ((tid & 31) == 0) red[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kQuThreads / 32; ++i) top = max(top, red[i]);
+  const bool finite = top < 0x7F800000u;
+  const float s = finite ? __fdiv_rn(__uint_as_float(top), 127.f) : __uint_as_float(0x7FC00000u);
+  const bool live = s > 0.f;  // false for an all-zero row and for a NaN scale: its integers are zero
+  if (tid == 0) scale[blockIdx.x] = s;
+  for (int i = tid; i < K8; i += kQuThreads) {
+    float v[8];
+    qu_load8<T>(row + i * 8, v);
+    uint32_t w[2] = {0, 0};
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)(uint8_t)qu_round(v[j], s) << (8 * (j & 3));
+    }
+    *reinterpret_cast<uint2 *>(out + i * 8) = make_uint2(w[0], w[1]);
+  }
+  for (int i = K8 * 8 + tid; i < K; i += kQuThreads) out[i] = live ? (int8_t)qu_round(qu_float(row[i]), s) : (int8_t)0;
+}
+
+static cudaError_t launch_quantize(const void *x, int dtype, int64_t M, int64_t K, int64_t ldx, int8_t *q, int64_t ldq,
+                                   float *scale, cudaStream_t s) {
+  const int esz = dtype == MS_DTYPE_F32 ? 4 : 2;
+  const int wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * esz) % 16 == 0 &&
+                   (reinterpret_cast<uintptr_t>(q) & 7) == 0 && ldq % 8 == 0;
+  if (dtype == MS_DTYPE_F32)
+    ms_quantize_kernel<<<(unsigned)M, kQuThreads, 0, s>>>(static_cast<const float *>(x), ldx, (int)K, q, ldq, scale,
+                                                          wide);
+  else if (dtype == MS_DTYPE_BF16)
+    ms_quantize_kernel<<<(unsigned)M, kQuThreads, 0, s>>>(static_cast<const __nv_bfloat16 *>(x), ldx, (int)K, q, ldq,
+                                                          scale, wide);
+  else
+    ms_quantize_kernel<<<(unsigned)M, kQuThreads, 0, s>>>(static_cast<const __half *>(x), ldx, (int)K, q, ldq, scale,
+                                                          wide);
+  return cudaGetLastError();
+}
+
+// ----------------------------------------------------------------- product
+// D[channel, token] = W[128 channels, K] X[tokens, K]^T on tcgen05 (kind::i8),
+// the channels on the 128 lanes of tensor memory and the tokens on its
+// columns: a small batch is a narrow N and the weights stream through once,
+// and in the epilogue a warp's 32 lanes are 32 consecutive channels of one
+// token, so its stores are whole lines.
+//
+// A persistent CTA per SM walks over (channel tile, token tile) pairs, token
+// tiles fastest, so that the weights of a channel tile come from HBM once.
+// Warp 0 loads K steps of 128 bytes with TMA (128-byte swizzle, zero beyond
+// K, channels or tokens), warp 1 issues the products into one of two
+// accumulators of 256 columns, warps 2-5 scale and store the other one.
+constexpr int kI8Threads = 192;
+constexpr int kI8Rows = 128;    // channels of a tile
+constexpr int kI8Step = 128;    // bytes of K of a stage
+constexpr int kI8MaxStages = 11;
+constexpr int kI8Cols = 256;    // columns of an accumulator
+constexpr int kI8Ring = 208 * 1024;
+
+struct I8Shared {
+  uint64_t full[kI8MaxStages], empty[kI8MaxStages];
+  uint64_t acc_full[2], acc_empty[2], drained;
+  uint32_t tmem;
+  volatile int dead;  // a wait ran out: the rest of the outputs are NaN
+  float xs[2][kI8Cols];
+};
+
+struct I8Args {
+  const float *x_scale, *w_scale, *bias;
+  void *out;
+  int64_t ldo;
+  int M, N, K;
+  int bn;      // tokens of a tile: a multiple of 16, at most 256
+  int stages;
+  int out_dtype;
+  int after_quantize;  // launched with the quantisation as its programmatic dependency
+};
+
+__device__ __forceinline__ void i8_store(void *out, int dtype, int64_t at, float y) {
+  if (dtype == MS_DTYPE_F32)
+    static_cast<float *>(out)[at] = y;
+  else if (dtype == MS_DTYPE_BF16)
+    static_cast<__nv_bfloat16 *>(out)[at] = __float2bfloat16_rn(y);
+  else
+    static_cast<__half *>(out)[at] = __float2half_rn(y);
+}
+
+__global__ void __launch_bounds__(kI8Threads, 1)
+    ms_int8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
+                   const __grid_constant__ I8Args a) {
+  extern __shared__ __align__(1024) unsigned char i8_raw[];
+  __shared__ I8Shared sh;
+  unsigned char *ring = i8_raw + ((1024u - (smem_addr(i8_raw) & 1023u)) & 1023u);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tok_tiles = (a.M + a.bn - 1) / a.bn;
+  const int64_t tiles = (int64_t)((a.N + kI8Rows - 1) / kI8Rows) * tok_tiles;
+  const int steps = (a.K + kI8Step - 1) / kI8Step;
+  const uint32_t wbytes = kI8Rows * kI8Step, xbytes = (uint32_t)a.bn * kI8Step;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.stages; ++i) {
+      bar_init(&sh.full[i], 1);
+      bar_init(&sh.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&sh.acc_full[i], 1);
+      bar_init(&sh.acc_empty[i], 4);
+    }
+    bar_init(&sh.drained, 1);
+    sh.dead = 0;
+    bar_init_fence();
+  }
+  if (warp == 1) tmem_alloc(&sh.tmem, 2 * kI8Cols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // the weights of the first stages need not wait for the quantisation
+      const int64_t mine = tiles > blockIdx.x ? (tiles - blockIdx.x - 1) / gridDim.x + 1 : 0;
+      const int64_t total = mine * steps;
+      const int ahead = (int)(total < a.stages ? total : a.stages);
+      for (int i = 0; i < ahead; ++i) {
+        const int64_t tile = blockIdx.x + (int64_t)(i / steps) * gridDim.x;
+        bar_expect(&sh.full[i], wbytes + xbytes);
+        tma_load_2d(ring + i * (wbytes + xbytes), &wmap, &sh.full[i], (i % steps) * kI8Step,
+                    (int)(tile / tok_tiles) * kI8Rows);
+      }
+      if (a.after_quantize) grid_wait();
+      int64_t it = 0;
+      int stage = 0, use = 0;
+      for (int64_t tile = blockIdx.x; tile < tiles && !sh.dead; tile += gridDim.x) {
+        const int n0 = (int)(tile / tok_tiles) * kI8Rows, t0 = (int)(tile % tok_tiles) * a.bn;
+        for (int k = 0; k < steps; ++k, ++it) {
+          unsigned char *st = ring + stage * (wbytes + xbytes);
+          if (it >= ahead) {
+            if (!bar_wait(&sh.empty[stage], (use & 1) ^ 1)) {
+              sh.dead = 1;
+              break;
+            }
+            bar_expect(&sh.full[stage], wbytes + xbytes);
+            tma_load_2d(st, &wmap, &sh.full[stage], k * kI8Step, n0);
+          }
+          tma_load_2d(st + wbytes, &xmap, &sh.full[stage], k * kI8Step, t0);
+          if (++stage == a.stages) stage = 0, ++use;
+        }
+      }
+      if (sh.dead) {  // copies in flight: their last phase of each stage, again bounded
+        for (int i = 0; i < a.stages; ++i) {
+          const int uses = use + (i < stage ? 1 : 0);
+          if (uses > 0 && it > i) bar_wait(&sh.full[i], (uses - 1) & 1);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = tc_idesc_i8(a.bn);
+      int stage = 0, phase = 0, n = 0;
+      for (int64_t tile = blockIdx.x; tile < tiles && !sh.dead; tile += gridDim.x, ++n) {
+        const int acc = n & 1;
+        if (!bar_wait(&sh.acc_empty[acc], ((n >> 1) & 1) ^ 1)) sh.dead = 1;
+        tc_fence_after();
+        for (int k = 0; k < steps && !sh.dead; ++k) {
+          if (!bar_wait(&sh.full[stage], phase)) {
+            sh.dead = 1;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t st = smem_addr(ring + stage * (wbytes + xbytes));
+          const uint64_t wd = tc_desc(st, 1024, 16), xd = tc_desc(st + wbytes, 1024, 16);
+#pragma unroll
+          for (int j = 0; j < kI8Step / 32; ++j)
+            tc_mma_i8(tmem + acc * kI8Cols, wd + 2 * j, xd + 2 * j, idesc, k > 0 || j > 0);
+          tc_commit(&sh.empty[stage]);
+          if (++stage == a.stages) stage = 0, phase ^= 1;
+        }
+        tc_commit(&sh.acc_full[acc]);
+      }
+      tc_commit(&sh.drained);
+      bar_wait(&sh.drained, 0);  // products in flight end before tensor memory is freed
+    }
+  } else {
+    const int quad = warp & 3;
+    const int et = threadIdx.x - 64;
+    if (a.after_quantize) grid_wait();
+    int n = 0;
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+      const int acc = n & 1;
+      const int n0 = (int)(tile / tok_tiles) * kI8Rows, t0 = (int)(tile % tok_tiles) * a.bn;
+      const int count = min(a.bn, a.M - t0);
+      for (int i = et; i < count; i += 128) sh.xs[acc][i] = __ldg(a.x_scale + t0 + i);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const int ch = n0 + quad * 32 + lane;
+      const float ws = ch < a.N ? __ldg(a.w_scale + ch) : 0.f;
+      const float bias = a.bias && ch < a.N ? __ldg(a.bias + ch) : 0.f;
+      if (!sh.dead && !bar_wait(&sh.acc_full[acc], (n >> 1) & 1)) sh.dead = 1;
+      __syncwarp();
+      tc_fence_after();
+      const bool dead = sh.dead != 0;
+      for (int c = 0; c < count; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + acc * kI8Cols + c, r);
+        tmem_wait_ld(r);
+        if (ch < a.N) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (c + i < count) {
+              float y = (float)(int)r[i] * (sh.xs[acc][c + i] * ws) + bias;
+              if (dead) y = __uint_as_float(0x7FC00000u);
+              i8_store(a.out, a.out_dtype, (int64_t)(t0 + c + i) * a.ldo + ch, y);
+            }
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&sh.acc_empty[acc]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_free(tmem, 2 * kI8Cols);
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// cuTensorMapEncodeTiled through the runtime, so that the library needs no
+// link to the driver.
+static cudaError_t encode_tiled(EncodeTiled *fn) {
+  static std::atomic<EncodeTiled> known{nullptr};
+  *fn = known.load(std::memory_order_acquire);
+  if (*fn) return cudaSuccess;
+  void *p = nullptr;
+  cudaDriverEntryPointQueryResult found;
+  cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found);
+  if (e != cudaSuccess) return e;
+  if (found != cudaDriverEntryPointSuccess || !p) return cudaErrorNotSupported;
+  *fn = reinterpret_cast<EncodeTiled>(p);
+  known.store(*fn, std::memory_order_release);
+  return cudaSuccess;
+}
+
+// A [rows, K] int8 matrix read in tiles of `box` rows and 128 bytes.
+static cudaError_t i8_map(CUtensorMap *map, const void *p, int64_t rows, int64_t K, int64_t ld, int box) {
+  EncodeTiled fn;
+  cudaError_t e = encode_tiled(&fn);
+  if (e != cudaSuccess) return e;
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t boxes[2] = {(cuuint32_t)kI8Step, (cuuint32_t)box};
+  const cuuint32_t unit[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(p), dims, strides, boxes, unit,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+static cudaError_t launch_int8(const int8_t *xq, int64_t ldx, const float *x_scale, int64_t M, const int8_t *wq,
+                               int64_t ldw, const float *w_scale, int64_t N, int64_t K, const float *bias, void *out,
+                               int out_dtype, int64_t ldo, bool after_quantize, cudaStream_t s) {
+  static std::atomic<int> ready[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(ms_int8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8Ring + 1024);
+    if (e != cudaSuccess) return e;
+    ready[dev].store(1, std::memory_order_release);
+  }
+  I8Args a{};
+  a.x_scale = x_scale, a.w_scale = w_scale, a.bias = bias, a.out = out, a.ldo = ldo;
+  a.M = (int)M, a.N = (int)N, a.K = (int)K, a.out_dtype = out_dtype, a.after_quantize = after_quantize;
+  // equal token tiles of at most 256, rounded up to the 16 that an N of the product allows
+  const int64_t parts = (M + kI8Cols - 1) / kI8Cols;
+  a.bn = (int)(((M + parts - 1) / parts + 15) / 16 * 16);
+  const int stage = (kI8Rows + a.bn) * kI8Step;
+  a.stages = kI8Ring / stage < kI8MaxStages ? kI8Ring / stage : kI8MaxStages;
+  CUtensorMap wmap, xmap;
+  e = i8_map(&wmap, wq, N, K, ldw, kI8Rows);
+  if (e == cudaSuccess) e = i8_map(&xmap, xq, M, K, ldx, a.bn);
+  if (e != cudaSuccess) return e;
+  int sms = 148;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int64_t tiles = ((N + kI8Rows - 1) / kI8Rows) * ((M + a.bn - 1) / a.bn);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles < sms ? tiles : sms));
+  cfg.blockDim = dim3(kI8Threads);
+  cfg.dynamicSmemBytes = a.stages * stage + 1024;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after_quantize ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, ms_int8_kernel, wmap, xmap, a);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+static bool i8_dtype(int d) { return d == MS_DTYPE_F32 || d == MS_DTYPE_BF16 || d == MS_DTYPE_F16; }
+static bool i8_rows(const void *p, int64_t ld, int64_t K) {  // what a tile load needs
+  return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld >= K && ld % 16 == 0 && ld < (1ll << 40);
+}
+constexpr int64_t kI8MaxK = 131072;
+constexpr int64_t kI8MaxRows = 0x7FFFFFFFll - 256;
+
+}  // namespace ms
+
+extern "C" {
+
+int ms_quantize_rows(const void *x, int dtype, int64_t M, int64_t K, int64_t ldx, int8_t *q, int64_t ldq, float *scale,
+                     ms_stream_t stream) {
+  if (!ms::i8_dtype(dtype)) return MS_E_DTYPE;
+  if (M < 0 || M > ms::kI8MaxRows || K < 1 || ldx < K || ldq < K) return MS_E_INVALID;
+  if (K > ms::kI8MaxK) return MS_E_UNSUPPORTED;
+  if (M == 0) return MS_OK;
+  if (!x || !q || !scale) return MS_E_INVALID;
+  cudaError_t e = ms::launch_quantize(x, dtype, M, K, ldx, q, ldq, scale, reinterpret_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? MS_OK : ms::cuda_fail(e);
+}
+
+static int int8_check(int64_t M, int64_t K, const int8_t *wq, int64_t ldw, const float *w_scale, int64_t N, void *out,
+                      int out_dtype, int64_t ldo) {
+  if (!ms::i8_dtype(out_dtype)) return MS_E_DTYPE;
+  if (M < 0 || M > ms::kI8MaxRows || N < 1 || N > ms::kI8MaxRows || K < 1 || ldo < N) return MS_E_INVALID;
+  if (K > ms::kI8MaxK) return MS_E_UNSUPPORTED;
+  if (M == 0) return MS_OK;
+  if (!ms::i8_rows(wq, ldw, K) || !w_scale || !out) return MS_E_INVALID;
+  return MS_OK;
+}
+
+int ms_int8_matmul(const int8_t *xq, int64_t ldx, const float *x_scale, int64_t M, const int8_t *wq, int64_t ldw,
+                   const float *w_scale, int64_t N, int64_t K, const float *bias, void *out, int out_dtype,
+                   int64_t ldo, ms_stream_t stream) {
+  const int rc = int8_check(M, K, wq, ldw, w_scale, N, out, out_dtype, ldo);
+  if (rc != MS_OK || M == 0) return rc;
+  if (!ms::i8_rows(xq, ldx, K) || !x_scale) return MS_E_INVALID;
+  cudaError_t e = ms::launch_int8(xq, ldx, x_scale, M, wq, ldw, w_scale, N, K, bias, out, out_dtype, ldo, false,
+                                  reinterpret_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? MS_OK : ms::cuda_fail(e);
+}
+
+int64_t ms_int8_workspace(int64_t M, int64_t K) {
+  if (M < 0 || K < 1 || M > ms::kI8MaxRows || K > ms::kI8MaxK) return 0;
+  return (M * 4 + 15) / 16 * 16 + M * ((K + 15) / 16 * 16);
+}
+
+int ms_int8_linear(const void *x, int dtype, int64_t ldx, int64_t M, const int8_t *wq, int64_t ldw,
+                   const float *w_scale, int64_t N, int64_t K, const float *bias, void *out, int out_dtype,
+                   int64_t ldo, void *workspace, ms_stream_t stream) {
+  if (!ms::i8_dtype(dtype)) return MS_E_DTYPE;
+  const int rc = int8_check(M, K, wq, ldw, w_scale, N, out, out_dtype, ldo);
+  if (rc != MS_OK || M == 0) return rc;
+  if (!x || ldx < K || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)) return MS_E_INVALID;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  float *scale = static_cast<float *>(workspace);
+  const int64_t ldq = (K + 15) / 16 * 16;
+  int8_t *q = static_cast<int8_t *>(workspace) + (M * 4 + 15) / 16 * 16;
+  cudaError_t e = ms::launch_quantize(x, dtype, M, K, ldx, q, ldq, scale, s);
+  if (e == cudaSuccess)
+    e = ms::launch_int8(q, ldq, scale, M, wq, ldw, w_scale, N, K, bias, out, out_dtype, ldo, true, s);
+  return e == cudaSuccess ? MS_OK : ms::cuda_fail(e);
+}
+
+}  // extern "C"
