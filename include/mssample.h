@@ -69,9 +69,14 @@ enum {
   /* decode-step operators */
   MS_ROW_BAD_SLOT = 32,       /* ms_kv_append: slot past the cache; nothing is
                                  written to the cache for the token */
-  MS_ROW_BAD_POSITION = 64    /* ms_kv_append: position outside the table;
+  MS_ROW_BAD_POSITION = 64,   /* ms_kv_append: position outside the table;
                                  nothing is written to the cache, the
                                  token's q_out is zero */
+  MS_ROW_BAD_LENGTH = 128,    /* ms_prefix_attention: length below 0 or past
+                                 the row's pages; the row's output is 0 and
+                                 its lse -inf */
+  MS_ROW_BAD_PAGE = 256       /* ms_prefix_attention: a page that the row or
+                                 the prefix uses is outside the cache; as above */
 };
 
 /*
@@ -422,6 +427,58 @@ typedef struct {
 } ms_kv_append_args;
 
 int ms_kv_append(const ms_kv_append_args *args, ms_stream_t stream);
+
+/*
+ * Attention of a batch of single tokens over a paged cache whose rows share a
+ * prefix.  Query head h of row b sees the prefix's keys 0..prefix_length-1
+ * (pages prefix_pages[j / page_size]) and its own keys 0..lengths[b]-1 (pages
+ * table[b, j / page_size]) of key head h / (heads / kv_heads):
+ *
+ *   out[b, h] = sum_j softmax_j(scale q[b, h] . k_j) v_j
+ *   lse[b, h] = log sum_j exp(scale q[b, h] . k_j)
+ *
+ * in fp32, the weights rounded to the cache's type for their product with v
+ * and out rounded once.  A row that sees no key has out 0 and lse -inf.  The
+ * cache past a row's keys is not used, whatever it holds (a part-full page,
+ * table entries past ceil(lengths[b] / page_size)).  prefix_length 0 is plain
+ * attention over the rows' own pages.
+ *
+ * head_dim is a multiple of 8, at most 128; the cache's strides are multiples
+ * of 8 entries and its bases 16-byte aligned (MS_E_UNSUPPORTED otherwise).
+ * scale is positive.  The struct is read on the host during the call, as for
+ * ms_kv_append.  workspace: ms_prefix_attention_workspace(...) bytes of the
+ * current device, 256-byte aligned, this call's until it has finished.
+ */
+typedef struct {
+  int32_t dtype;        /* MS_DTYPE_BF16 or MS_DTYPE_F16: q, the caches and out */
+  int32_t heads;
+  int32_t kv_heads;     /* divides heads */
+  int32_t head_dim;
+  int64_t rows;
+  const void *q;        /* [rows, heads, head_dim] */
+  int64_t q_row, q_head;
+  const void *cache_k;  /* [pages, page_size, kv_heads, head_dim], any order of the first three */
+  int64_t ck_page, ck_token, ck_head;
+  const void *cache_v;
+  int64_t cv_page, cv_token, cv_head;
+  int64_t pages, page_size;
+  const int32_t *table; /* [rows, table_width] own pages, rows table_row entries apart */
+  int64_t table_width, table_row;
+  const int32_t *lengths;      /* [rows] own keys */
+  const int32_t *prefix_pages; /* [ceil(prefix_length / page_size)] */
+  int64_t prefix_length;
+  float scale;
+  void *out;            /* [rows, heads, head_dim] */
+  int64_t out_row, out_head;
+  float *lse;           /* [rows, heads] */
+  int32_t *status;      /* [rows] MS_ROW_* bits */
+  void *workspace;
+  int64_t workspace_bytes;
+} ms_prefix_attention_args;
+
+int ms_prefix_attention(const ms_prefix_attention_args *args, ms_stream_t stream);
+
+int64_t ms_prefix_attention_workspace(int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim);
 
 /*
  * 8-bit integer product with a scale for each token and each output channel:

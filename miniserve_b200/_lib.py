@@ -25,6 +25,8 @@ MS_ROW_UNSUPPORTED = 8
 MS_ROW_PEER_TIMEOUT = 16
 MS_ROW_BAD_SLOT = 32
 MS_ROW_BAD_POSITION = 64
+MS_ROW_BAD_LENGTH = 128
+MS_ROW_BAD_PAGE = 256
 
 _lock = threading.Lock()
 _lib = None
@@ -44,6 +46,17 @@ class KvAppendArgs(ctypes.Structure):
                 ("cache_v", _P), ("cv_page", _I64), ("cv_token", _I64), ("cv_head", _I64), ("pages", _I64),
                 ("page_size", _I64), ("slots", _P), ("positions", _P), ("table", _P), ("table_rows", _I64),
                 ("status", _P)]
+
+
+class PrefixAttentionArgs(ctypes.Structure):
+    """ms_prefix_attention_args of include/mssample.h."""
+    _fields_ = [("dtype", _I32), ("heads", _I32), ("kv_heads", _I32), ("head_dim", _I32), ("rows", _I64),
+                ("q", _P), ("q_row", _I64), ("q_head", _I64), ("cache_k", _P), ("ck_page", _I64), ("ck_token", _I64),
+                ("ck_head", _I64), ("cache_v", _P), ("cv_page", _I64), ("cv_token", _I64), ("cv_head", _I64),
+                ("pages", _I64), ("page_size", _I64), ("table", _P), ("table_width", _I64), ("table_row", _I64),
+                ("lengths", _P), ("prefix_pages", _P), ("prefix_length", _I64), ("scale", ctypes.c_float),
+                ("out", _P), ("out_row", _I64), ("out_head", _I64), ("lse", _P), ("status", _P), ("workspace", _P),
+                ("workspace_bytes", _I64)]
 
 
 # name -> (restype, argtypes); every function include/mssample.h declares
@@ -101,6 +114,8 @@ SIGNATURES = {
     "ms_int8_workspace": (_I64, [_I64, _I64]),
     "ms_int8_linear": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, ctypes.c_int,
                                       _I64, _P, _P]),
+    "ms_prefix_attention": (ctypes.c_int, [ctypes.POINTER(PrefixAttentionArgs), _P]),
+    "ms_prefix_attention_workspace": (_I64, [_I64, _I32, _I32, _I32]),
     "ms_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ms_last_cuda_error": (ctypes.c_int, []),
     "ms_version": (ctypes.c_int, []),

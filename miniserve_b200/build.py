@@ -16,7 +16,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmssample.so")
-SOURCES = ["ms_sample.cu", "ms_kv.cu", "ms_int8.cu"]
+SOURCES = ["ms_sample.cu", "ms_kv.cu", "ms_attn.cu", "ms_int8.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -1,0 +1,150 @@
+// ms_prefix_attention -- single-token attention of a batch over a paged cache
+// (declared in include/mssample.h): every row sees the keys of a prefix that
+// the batch shares, then its own.
+//
+//   x_j = scale q . k_j,  o = sum_j exp(x_j - m) v_j / sum_j exp(x_j - m),
+//   lse = m + log sum_j exp(x_j - m),  m = max_j x_j
+//
+// Partial results over disjoint sets of keys combine exactly: each is kept as
+// (m, l = sum exp(x - m), O = sum exp(x - m) v) in fp32, and the merge weighs
+// them by exp(m - max m).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+
+#include "../../include/mssample.h"
+#include "ms_attn.cuh"
+#include "ms_host.h"
+
+namespace ms {
+
+// Workspace: a header, the rows' first tiles, and the pieces' records.
+struct AtLayout {
+  int64_t base, own_o, own_ml, bytes;
+};
+
+static int64_t at_round(int64_t n) { return (n + 255) / 256 * 256; }
+
+static AtLayout at_layout(const AtShape &s) {
+  AtLayout l;
+  int64_t at = 256;  // AtHeader
+  l.base = at, at = at_round(at + s.rows * 8);
+  const int64_t pieces = s.rows * s.kv_heads * s.chunks + s.split_warps;
+  l.own_o = at, at = at_round(at + pieces * s.chunk_rows * s.head_dim * 4);
+  l.own_ml = at, at = at_round(at + pieces * s.chunk_rows * 8);
+  l.bytes = at;
+  return l;
+}
+
+static int at_sms(int dev) {
+  int sms = 148;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+static AtShape at_shape(int64_t rows, int heads, int kv_heads, int head_dim, int sms) {
+  AtShape s;
+  s.rows = rows, s.heads = heads, s.kv_heads = kv_heads, s.head_dim = head_dim;
+  s.group = heads / kv_heads;
+  s.chunks = (s.group + kAtRows - 1) / kAtRows;
+  s.chunk_rows = s.group < kAtRows ? s.group : kAtRows;
+  s.split_warps = (int64_t)sms * kSpCtas * kSpWarps;
+  return s;
+}
+
+template <typename F>
+static cudaError_t at_allow_shared(F *kernel, int bytes, std::atomic<int> (&ready)[kMaxDevices], int dev) {
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  if (ready[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) ready[dev].store(1, std::memory_order_release);
+  return e;
+}
+
+template <typename K, typename... A>
+static cudaError_t at_launch(K *kernel, int64_t grid, int threads, int shared, cudaStream_t s, bool dependent,
+                             const A &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <typename T, int DP>
+static cudaError_t at_run(const AtArgs &a, int dev, cudaStream_t s) {
+  static std::atomic<int> split_ready[kMaxDevices];
+  cudaError_t e = at_allow_shared(ms_attn_split_kernel<T, DP>, kSpShared, split_ready, dev);
+  if (e != cudaSuccess) return e;
+  e = at_launch(ms_attn_split_kernel<T, DP>, a.shape.split_warps / kSpWarps, kSpWarps * 32, kSpShared, s, false, a);
+  if (e != cudaSuccess) return e;
+  return at_launch(ms_attn_merge_kernel<T>, a.shape.rows * a.shape.heads, kMgThreads, 0, s, true, a);
+}
+
+}  // namespace ms
+
+extern "C" {
+
+int64_t ms_prefix_attention_workspace(int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim) {
+  if (rows < 0 || rows > ms::kAtMaxRows || heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 65536 ||
+      head_dim < 1 || head_dim > 128)
+    return 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  return ms::at_layout(ms::at_shape(rows, heads, kv_heads, head_dim, ms::at_sms(dev))).bytes;
+}
+
+int ms_prefix_attention(const ms_prefix_attention_args *args, ms_stream_t stream) {
+  if (!args) return MS_E_INVALID;
+  const ms_prefix_attention_args &x = *args;
+  if (x.dtype != MS_DTYPE_BF16 && x.dtype != MS_DTYPE_F16) return MS_E_DTYPE;
+  if (x.rows < 0 || x.rows > ms::kAtMaxRows || x.heads < 1 || x.heads > 65536 || x.kv_heads < 1 ||
+      x.heads % x.kv_heads || x.head_dim < 1 || x.pages < 1 || x.pages > 0x7FFFFFFFll || x.page_size < 1 ||
+      x.page_size > 0x7FFFFFFFll || x.table_width < 0 || x.table_width > 0x7FFFFFFFll || x.table_row < 0 ||
+      x.prefix_length < 0 || x.prefix_length > ms::kAtMaxKeys || !(x.scale > 0.f) || x.scale > 3.0e38f)
+    return MS_E_INVALID;
+  if (x.rows * x.heads > 0x7FFFFFFFll) return MS_E_INVALID;
+  // 16-byte rows: what the copies of the cache read
+  const int64_t strides = x.ck_page | x.ck_token | x.ck_head | x.cv_page | x.cv_token | x.cv_head;
+  if (x.head_dim > 128 || x.head_dim % 8 || (strides & 7) || (reinterpret_cast<uintptr_t>(x.cache_k) & 15) ||
+      (reinterpret_cast<uintptr_t>(x.cache_v) & 15))
+    return MS_E_UNSUPPORTED;
+  if (x.rows == 0) return MS_OK;
+  if (!x.q || !x.cache_k || !x.cache_v || !x.lengths || !x.out || !x.lse || !x.status || !x.workspace ||
+      (reinterpret_cast<uintptr_t>(x.workspace) & 255) || (x.table_width > 0 && !x.table) ||
+      (x.prefix_length > 0 && !x.prefix_pages))
+    return MS_E_INVALID;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return ms::cuda_fail(e);
+  ms::AtArgs a{};
+  a.x = x;
+  a.shape = ms::at_shape(x.rows, x.heads, x.kv_heads, x.head_dim, ms::at_sms(dev));
+  const ms::AtLayout l = ms::at_layout(a.shape);
+  if (x.workspace_bytes < l.bytes) return MS_E_INVALID;
+  char *w = static_cast<char *>(x.workspace);
+  a.header = reinterpret_cast<ms::AtHeader *>(w);
+  a.base = reinterpret_cast<int64_t *>(w + l.base);
+  a.own_o = reinterpret_cast<float *>(w + l.own_o);
+  a.own_ml = reinterpret_cast<float2 *>(w + l.own_ml);
+  a.scale_log2 = x.scale * 1.4426950408889634f;
+  a.split_prefix = (int)x.prefix_length;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const bool narrow = x.head_dim <= 64;
+  if (x.dtype == MS_DTYPE_BF16)
+    e = narrow ? ms::at_run<__nv_bfloat16, 64>(a, dev, s) : ms::at_run<__nv_bfloat16, 128>(a, dev, s);
+  else
+    e = narrow ? ms::at_run<__half, 64>(a, dev, s) : ms::at_run<__half, 128>(a, dev, s);
+  return e == cudaSuccess ? MS_OK : ms::cuda_fail(e);
+}
+
+}  // extern "C"

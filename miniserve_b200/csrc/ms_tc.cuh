@@ -35,7 +35,7 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity) {
+static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity) {
   uint64_t t0, t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
   for (uint32_t it = 1;; ++it) {
