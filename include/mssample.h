@@ -478,7 +478,8 @@ typedef struct {
 
 int ms_prefix_attention(const ms_prefix_attention_args *args, ms_stream_t stream);
 
-int64_t ms_prefix_attention_workspace(int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim);
+int64_t ms_prefix_attention_workspace(int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                      int64_t prefix_length);
 
 /*
  * 8-bit integer product with a scale for each token and each output channel:

@@ -115,7 +115,7 @@ SIGNATURES = {
     "ms_int8_linear": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, ctypes.c_int,
                                       _I64, _P, _P]),
     "ms_prefix_attention": (ctypes.c_int, [ctypes.POINTER(PrefixAttentionArgs), _P]),
-    "ms_prefix_attention_workspace": (_I64, [_I64, _I32, _I32, _I32]),
+    "ms_prefix_attention_workspace": (_I64, [_I64, _I32, _I32, _I32, _I64]),
     "ms_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ms_last_cuda_error": (ctypes.c_int, []),
     "ms_version": (ctypes.c_int, []),

@@ -88,8 +88,8 @@ def prefix_attention(q, cache_k, cache_v, pages, lengths, *, prefix_pages=None, 
     a.out, a.out_row, a.out_head = out.data_ptr(), out.stride(0), out.stride(1)
     a.lse, a.status = lse.data_ptr(), status.data_ptr()
     with torch.cuda.device(dev):
-        workspace = torch.empty(L.ms_prefix_attention_workspace(B, heads, kv_heads, head_dim), dtype=torch.uint8,
-                                device=dev)
+        workspace = torch.empty(L.ms_prefix_attention_workspace(B, heads, kv_heads, head_dim, prefix_length),
+                                dtype=torch.uint8, device=dev)
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
         rc = L.ms_prefix_attention(ctypes.byref(a), torch.cuda.current_stream(dev).cuda_stream)
     _lib.check(rc, "ms_prefix_attention")

@@ -20,23 +20,7 @@
 
 namespace ms {
 
-// Workspace: a header, the rows' first tiles, and the pieces' records.
-struct AtLayout {
-  int64_t base, own_o, own_ml, bytes;
-};
-
 static int64_t at_round(int64_t n) { return (n + 255) / 256 * 256; }
-
-static AtLayout at_layout(const AtShape &s) {
-  AtLayout l;
-  int64_t at = 256;  // AtHeader
-  l.base = at, at = at_round(at + s.rows * 8);
-  const int64_t pieces = s.rows * s.kv_heads * s.chunks + s.split_warps;
-  l.own_o = at, at = at_round(at + pieces * s.chunk_rows * s.head_dim * 4);
-  l.own_ml = at, at = at_round(at + pieces * s.chunk_rows * 8);
-  l.bytes = at;
-  return l;
-}
 
 static int at_sms(int dev) {
   int sms = 148;
@@ -44,14 +28,56 @@ static int at_sms(int dev) {
   return sms;
 }
 
-static AtShape at_shape(int64_t rows, int heads, int kv_heads, int head_dim, int sms) {
-  AtShape s;
+// Parts of the prefix for the prefix kernel: the fewest waves of CTAs (two an
+// SM) times tiles of one CTA, each CTA costing about two tiles besides (its
+// queries, first copies and record).
+static int at_parts(int64_t ctas, int64_t tiles, int sms) {
+  int best = 1;
+  double least = 0;
+  for (int n = 1; n <= 2 * sms && n <= tiles; ++n) {
+    const double waves = (double)((ctas * n + 2 * sms - 1) / (2 * sms));
+    const double cost = waves * ((double)((tiles + n - 1) / n) + 2.0);
+    if (n == 1 || cost < least) best = n, least = cost;
+    if (ctas * n >= 4 * sms) break;
+  }
+  return best;
+}
+
+struct AtPlan {
+  AtShape shape;
+  int packed, split_prefix, pre_splits, pre_tiles;
+  // workspace: a header, the rows' first tiles, the split kernel's records, the prefix kernel's
+  int64_t base, own_o, own_ml, pre_o, pre_ml, bytes;
+};
+
+static AtPlan at_plan(int64_t rows, int heads, int kv_heads, int head_dim, int64_t prefix, int sms) {
+  AtPlan p{};
+  AtShape &s = p.shape;
   s.rows = rows, s.heads = heads, s.kv_heads = kv_heads, s.head_dim = head_dim;
   s.group = heads / kv_heads;
   s.chunks = (s.group + kAtRows - 1) / kAtRows;
   s.chunk_rows = s.group < kAtRows ? s.group : kAtRows;
   s.split_warps = (int64_t)sms * kSpCtas * kSpWarps;
-  return s;
+  p.packed = (int)(rows * s.group);
+  if (prefix > 0 && p.packed <= kAtRows) {
+    // one chunk of query rows: the split kernel reads the prefix once as well, with more warps at it
+    p.split_prefix = (int)prefix;
+    if (p.packed > s.chunk_rows) s.chunk_rows = p.packed;
+  } else if (prefix > 0) {
+    const int kt = head_dim <= 64 ? kPrKeys<64> : kPrKeys<128>;
+    p.pre_tiles = (p.packed + kPrRows - 1) / kPrRows;
+    p.pre_splits = at_parts((int64_t)p.pre_tiles * kv_heads, (prefix + kt - 1) / kt, sms);
+  }
+  const int64_t pieces = rows * kv_heads * s.chunks + (p.split_prefix ? kv_heads : 0) + s.split_warps;
+  const int64_t pre = (int64_t)p.pre_splits * kv_heads * p.packed;
+  int64_t at = 256;  // AtHeader
+  p.base = at, at = at_round(at + rows * 8);
+  p.own_o = at, at = at_round(at + pieces * s.chunk_rows * head_dim * 4);
+  p.own_ml = at, at = at_round(at + pieces * s.chunk_rows * 8);
+  p.pre_o = at, at = at_round(at + pre * head_dim * 4);
+  p.pre_ml = at, at = at_round(at + pre * 8);
+  p.bytes = at;
+  return p;
 }
 
 template <typename F>
@@ -82,10 +108,17 @@ static cudaError_t at_launch(K *kernel, int64_t grid, int threads, int shared, c
 
 template <typename T, int DP>
 static cudaError_t at_run(const AtArgs &a, int dev, cudaStream_t s) {
-  static std::atomic<int> split_ready[kMaxDevices];
+  static std::atomic<int> split_ready[kMaxDevices], prefix_ready[kMaxDevices];
   cudaError_t e = at_allow_shared(ms_attn_split_kernel<T, DP>, kSpShared, split_ready, dev);
+  if (e == cudaSuccess && a.pre_splits) {
+    e = at_allow_shared(ms_attn_prefix_kernel<T, DP>, kPrSharedBytes<DP>, prefix_ready, dev);
+    if (e == cudaSuccess)
+      e = at_launch(ms_attn_prefix_kernel<T, DP>, (int64_t)a.pre_tiles * a.shape.kv_heads * a.pre_splits, kPrThreads,
+                    kPrSharedBytes<DP>, s, false, a);
+  }
   if (e != cudaSuccess) return e;
-  e = at_launch(ms_attn_split_kernel<T, DP>, a.shape.split_warps / kSpWarps, kSpWarps * 32, kSpShared, s, false, a);
+  e = at_launch(ms_attn_split_kernel<T, DP>, a.shape.split_warps / kSpWarps, kSpWarps * 32, kSpShared, s,
+                a.pre_splits != 0, a);
   if (e != cudaSuccess) return e;
   return at_launch(ms_attn_merge_kernel<T>, a.shape.rows * a.shape.heads, kMgThreads, 0, s, true, a);
 }
@@ -94,13 +127,14 @@ static cudaError_t at_run(const AtArgs &a, int dev, cudaStream_t s) {
 
 extern "C" {
 
-int64_t ms_prefix_attention_workspace(int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim) {
-  if (rows < 0 || rows > ms::kAtMaxRows || heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 65536 ||
-      head_dim < 1 || head_dim > 128)
+int64_t ms_prefix_attention_workspace(int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                      int64_t prefix_length) {
+  if (prefix_length < 0 || prefix_length > ms::kAtMaxKeys || rows < 0 || rows > ms::kAtMaxRows || heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 65536 ||
+      head_dim < 1 || head_dim > 128 || rows * heads > 0x7FFFFFFFll)
     return 0;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  return ms::at_layout(ms::at_shape(rows, heads, kv_heads, head_dim, ms::at_sms(dev))).bytes;
+  return ms::at_plan(rows, heads, kv_heads, head_dim, prefix_length, ms::at_sms(dev)).bytes;
 }
 
 int ms_prefix_attention(const ms_prefix_attention_args *args, ms_stream_t stream) {
@@ -128,16 +162,19 @@ int ms_prefix_attention(const ms_prefix_attention_args *args, ms_stream_t stream
   if (e != cudaSuccess) return ms::cuda_fail(e);
   ms::AtArgs a{};
   a.x = x;
-  a.shape = ms::at_shape(x.rows, x.heads, x.kv_heads, x.head_dim, ms::at_sms(dev));
-  const ms::AtLayout l = ms::at_layout(a.shape);
-  if (x.workspace_bytes < l.bytes) return MS_E_INVALID;
+  const ms::AtPlan p = ms::at_plan(x.rows, x.heads, x.kv_heads, x.head_dim, x.prefix_length, ms::at_sms(dev));
+  if (x.workspace_bytes < p.bytes) return MS_E_INVALID;
+  a.shape = p.shape;
+  a.packed = p.packed, a.split_prefix = p.split_prefix, a.pre_splits = p.pre_splits, a.pre_tiles = p.pre_tiles;
   char *w = static_cast<char *>(x.workspace);
   a.header = reinterpret_cast<ms::AtHeader *>(w);
-  a.base = reinterpret_cast<int64_t *>(w + l.base);
-  a.own_o = reinterpret_cast<float *>(w + l.own_o);
-  a.own_ml = reinterpret_cast<float2 *>(w + l.own_ml);
+  a.base = reinterpret_cast<int64_t *>(w + p.base);
+  a.own_o = reinterpret_cast<float *>(w + p.own_o);
+  a.own_ml = reinterpret_cast<float2 *>(w + p.own_ml);
+  a.pre_o = reinterpret_cast<float *>(w + p.pre_o);
+  a.pre_ml = reinterpret_cast<float2 *>(w + p.pre_ml);
   a.scale_log2 = x.scale * 1.4426950408889634f;
-  a.split_prefix = (int)x.prefix_length;
+  a.q_wide = ((x.q_row | x.q_head) & 7) == 0 && (reinterpret_cast<uintptr_t>(x.q) & 15) == 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool narrow = x.head_dim <= 64;
   if (x.dtype == MS_DTYPE_BF16)

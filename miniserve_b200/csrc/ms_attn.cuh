@@ -31,7 +31,7 @@ struct AtShape {
   int heads, kv_heads, head_dim;
   int group;       // query heads of a key head
   int chunks;      // chunks of kAtRows query heads of a key head
-  int chunk_rows;  // query heads of a record
+  int chunk_rows;  // query rows of a record
   int64_t split_warps;
 };
 
@@ -39,11 +39,17 @@ struct AtArgs {
   ms_prefix_attention_args x;
   AtShape shape;
   AtHeader *header;
-  int64_t *base;    // [rows] tiles of the rows before
+  int64_t *base;    // [rows] the first tile of each row in the split kernel's sequence
   float *own_o;     // [pieces][chunk_rows][head_dim]
   float2 *own_ml;   // [pieces][chunk_rows] (m in units of log2, l)
+  float *pre_o;     // [splits][kv_heads][packed rows][head_dim], of the prefix kernel
+  float2 *pre_ml;   // [splits][kv_heads][packed rows]
   float scale_log2;
-  int split_prefix;  // keys of the prefix that every row's split tiles start with
+  int packed;        // rows * group: the prefix's query rows of one key head, row b's heads at b * group
+  int split_prefix;  // keys of the prefix that the split kernel takes: all or none
+  int pre_splits;    // parts of the prefix that the prefix kernel takes; 0 where it does not run
+  int pre_tiles;     // its query tiles of one key head
+  int q_wide;        // q's heads start 16-byte aligned
 };
 
 template <typename T>
@@ -106,7 +112,8 @@ __device__ __forceinline__ int at_length(const ms_prefix_attention_args &x, int6
   return n >= 0 && n <= kAtMaxKeys && (int64_t)n <= x.table_width * x.page_size ? n : 0;
 }
 
-// Walks over (row, key head and chunk, tile) in order.
+// Walks over (row, key head and chunk, tile) in order.  Row -1 is the prefix,
+// all rows' query heads of a key head being its one chunk.
 struct SpWalk {
   int64_t b;
   int hc, tile, tiles, keys;
@@ -114,14 +121,24 @@ struct SpWalk {
 };
 
 __device__ __forceinline__ void sp_row(const AtArgs &a, SpWalk &w) {
-  w.keys = a.split_prefix + at_length(a.x, w.b);
+  w.keys = w.b < 0 ? a.split_prefix : at_length(a.x, w.b);
   w.tiles = (w.keys + kSpTile - 1) / kSpTile;
+}
+__device__ __forceinline__ int sp_heads(const AtArgs &a, int64_t b) {  // (key head, chunk) pairs of a row
+  return b < 0 ? a.shape.kv_heads : a.shape.kv_heads * a.shape.chunks;
+}
+__device__ __forceinline__ int sp_head(const AtArgs &a, const SpWalk &w) {  // key head
+  return w.b < 0 ? w.hc : w.hc / a.shape.chunks;
+}
+// Index of a row's (key head, chunk) among the sequence's items.
+__device__ __forceinline__ int64_t sp_item(const AtArgs &a, int64_t b, int hc) {
+  return b < 0 ? hc : (a.split_prefix ? a.shape.kv_heads : 0) + b * a.shape.kv_heads * a.shape.chunks + hc;
 }
 __device__ __forceinline__ void sp_next(const AtArgs &a, SpWalk &w) {
   if (--w.left <= 0) return;
   if (++w.tile < w.tiles) return;
   w.tile = 0;
-  if (++w.hc < a.shape.kv_heads * a.shape.chunks) return;
+  if (++w.hc < sp_heads(a, w.b)) return;
   w.hc = 0;
   do {  // a later row has tiles: some are left
     ++w.b;
@@ -129,8 +146,8 @@ __device__ __forceinline__ void sp_next(const AtArgs &a, SpWalk &w) {
   } while (w.tiles == 0);
 }
 
-// Split kernel.  The tiles of 16 keys of all rows and key heads form one
-// sequence; every warp takes an equal, contiguous share of it, whatever the
+// Split kernel.  The tiles of 16 keys of all rows and key heads (and of the
+// prefix, where its query rows fit one chunk) form one sequence; every warp takes an equal, contiguous share of it, whatever the
 // rows' lengths, and works alone: a ring of tiles filled with 16-byte
 // asynchronous copies, a page lookup one tile ahead of its copies, and
 // products of m16n8k16 (the chunk's query heads are the M).  Where its share
@@ -160,7 +177,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
   const int64_t r0 = min(rows, tid * run), r1 = min(rows, r0 + run);
   {
     int64_t n = 0;
-    for (int64_t b = r0; b < r1; ++b) n += (a.split_prefix + at_length(x, b) + kSpTile - 1) / kSpTile;
+    for (int64_t b = r0; b < r1; ++b) n += (at_length(x, b) + kSpTile - 1) / kSpTile;
     sums[tid + 1] = n;
     if (tid == 0) sums[0] = 0, bad = 0;
     __syncthreads();
@@ -171,13 +188,14 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
       __syncthreads();
     }
   }
-  const int64_t total = sums[kSpWarps * 32] * hcs;
+  const int64_t before = (int64_t)((a.split_prefix + kSpTile - 1) / kSpTile) * a.shape.kv_heads;
+  const int64_t total = before + sums[kSpWarps * 32] * hcs;
   const int64_t share = max((int64_t)1, (total + a.shape.split_warps - 1) / a.shape.split_warps);
   if (blockIdx.x == 0) {  // for the merge: where each row's tiles start, and whether the prefix's pages are good
     int64_t n = sums[tid];
     for (int64_t b = r0; b < r1; ++b) {
-      a.base[b] = n;
-      n += (a.split_prefix + at_length(x, b) + kSpTile - 1) / kSpTile;
+      a.base[b] = before + n * hcs;
+      n += (at_length(x, b) + kSpTile - 1) / kSpTile;
     }
     const int64_t pages = (x.prefix_length + x.page_size - 1) / x.page_size;
     int seen = 0;
@@ -191,27 +209,34 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
   }
   const int64_t wid = (int64_t)blockIdx.x * kSpWarps + warp;
   const int64_t u0 = wid * share, u1 = min(total, u0 + share);
-  if (u0 >= u1) return;
+  if (u0 >= u1) {
+    grid_wait();
+    return;
+  }
   SpWalk load;
-  {  // the row that tile u0 of the sequence lies in: its thread's run, then the row
+  int64_t first = 0;
+  if (u0 < before) {
+    load.b = -1;
+    sp_row(a, load);
+  } else {  // the row that tile u0 of the sequence lies in: its thread's run, then the row
     int lo = 0, hi = kSpWarps * 32 - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (sums[mid + 1] * hcs > u0) hi = mid;
+      if (before + sums[mid + 1] * hcs > u0) hi = mid;
       else lo = mid + 1;
     }
     load.b = min(rows, lo * run);
-    int64_t first = sums[lo] * hcs;
+    first = before + sums[lo] * hcs;
     sp_row(a, load);
     while (first + (int64_t)load.tiles * hcs <= u0) {
       first += (int64_t)load.tiles * hcs;
       ++load.b;
       sp_row(a, load);
     }
-    load.hc = (int)((u0 - first) / load.tiles);
-    load.tile = (int)((u0 - first) - (int64_t)load.hc * load.tiles);
-    load.left = u1 - u0;
   }
+  load.hc = (int)((u0 - first) / load.tiles);
+  load.tile = (int)((u0 - first) - (int64_t)load.hc * load.tiles);
+  load.left = u1 - u0;
   SpWalk now = load;
   const uint32_t ring = smem_addr(sp_ring) + warp * kSpRing;
   const T *ck = static_cast<const T *>(x.cache_k), *cv = static_cast<const T *>(x.cache_v);
@@ -224,13 +249,11 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
     if (load.left > 0) {
       const int j = load.tile * kSpTile + (lane & 15);
       if (j < load.keys) {
-        const bool shared = j < a.split_prefix;
-        const int i = shared ? j : j - a.split_prefix;
-        const int p = i / page_size;
-        offset = i - p * page_size;
-        page = __ldg(shared ? x.prefix_pages + p : x.table + load.b * x.table_row + p);
+        const int p = j / page_size;
+        offset = j - p * page_size;
+        page = __ldg(load.b < 0 ? x.prefix_pages + p : x.table + load.b * x.table_row + p);
       }
-      head = load.hc / a.shape.chunks;
+      head = sp_head(a, load);
       sp_next(a, load);
     }
   };
@@ -270,10 +293,10 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
       look();
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    const int h = now.hc / a.shape.chunks, c = now.hc - h * a.shape.chunks;
+    // query rows of the item: a chunk of one row's heads, or all rows' heads for the prefix
+    const int h = sp_head(a, now), c = now.b < 0 ? 0 : now.hc - h * a.shape.chunks;
+    const int n = now.b < 0 ? a.packed : min(kAtRows, a.shape.group - c * kAtRows);
     if (fresh) {
-      const T *q = static_cast<const T *>(x.q) + now.b * x.q_row;
-      const int n = min(kAtRows, a.shape.group - c * kAtRows);
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k) {
 #pragma unroll
@@ -281,8 +304,10 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
           const int g = (lane >> 2) + (i & 1) * 8, d = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
           uint32_t u = 0;
           if (g < n && d < x.head_dim) {
-            const unsigned short *p = reinterpret_cast<const unsigned short *>(
-                q + (int64_t)(h * a.shape.group + c * kAtRows + g) * x.q_head + d);
+            const int64_t b = now.b < 0 ? g / a.shape.group : now.b;
+            const int head_q = h * a.shape.group + (now.b < 0 ? g % a.shape.group : c * kAtRows + g);
+            const unsigned short *p = reinterpret_cast<const unsigned short *>(static_cast<const T *>(x.q) +
+                                                                               b * x.q_row + head_q * x.q_head + d);
             u = (uint32_t)__ldg(p) | ((uint32_t)__ldg(p + 1) << 16);
           }
           qf[k][i] = u;
@@ -361,8 +386,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
     }
     __syncwarp();  // the stage is read: the next round's copies may overwrite it
     if (now.left == 1 || now.tile + 1 == now.tiles) {
-      const int64_t piece = now.b * hcs + now.hc + wid;
-      const int n = min(kAtRows, a.shape.group - c * kAtRows);
+      const int64_t piece = sp_item(a, now.b, now.hc) + wid;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
@@ -385,6 +409,351 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
     sp_next(a, now);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  grid_wait();  // the merge that follows this grid reads the prefix kernel's records too
+}
+
+// Prefix kernel, where the prefix has more query rows than one chunk.  The
+// rows' query heads of one key head are packed into tiles of 128 rows (M of
+// the tcgen05 products), and a CTA takes one such tile over one part of the
+// prefix, so that a key is read once for 128 query rows:
+//
+//   warps 0-3   softmax: a thread owns a row; scores from tensor memory, the
+//               weights (rounded to the cache's type) back to tensor memory
+//   warps 4-5   copies: 16-byte asynchronous copies of key and value tiles
+//               into a ring of swizzled 16 KB stages, pages looked up on the way
+//   warp 6      products: S = Q K^T of the next tile ahead of O += P V of this
+//
+// Two CTAs share an SM, so that one's products run under the other's softmax.
+// The maximum that the weights refer to moves only when a score passes it by
+// 2^8 (the weights then stay below 2^8, within fp16): O is rescaled rarely.
+//
+// Bound by the exponentials (16 a clock and SM): 128 x 128 scores are 1024
+// clocks, their products of 64-entry heads about 256.
+constexpr int kPrThreads = 224;
+constexpr int kPrRows = 128;
+constexpr int kPrStage = 16 * 1024;
+constexpr int kPrCols = 256;  // tensor memory: S, then P (two keys a column), then O
+template <int DP>
+constexpr int kPrKeys = kPrStage / (DP * 2);  // keys of a tile: 128, or 64 of 128-entry heads
+template <int DP>
+constexpr int kPrStages = DP == 64 ? 5 : 4;
+template <int DP>
+constexpr int kPrSharedBytes = 1024 + kPrRows * DP * 2 + kPrStages<DP> * kPrStage;
+
+struct PrShared {
+  uint64_t full[5], empty[5];
+  uint64_t q_full, s_full, p_ready, pv_done, drained;
+  uint32_t tmem;
+  volatile int dead;  // a wait ran out: the records are NaN
+};
+
+__device__ __forceinline__ void tmem_ld64(uint32_t addr, float (&r)[64]) {
+  uint32_t u[64];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) tmem_ld32(addr + 32 * i, u + 32 * i);
+  tmem_wait_ld64(u);
+#pragma unroll
+  for (int i = 0; i < 64; ++i) r[i] = __uint_as_float(u[i]);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kPrThreads, 2) ms_attn_prefix_kernel(const __grid_constant__ AtArgs a) {
+  constexpr int KT = kPrKeys<DP>, kStages = kPrStages<DP>;
+  constexpr uint32_t kP = KT, kO = KT + KT / 2;  // columns of P and O
+  extern __shared__ __align__(1024) unsigned char pr_raw[];
+  __shared__ PrShared sh;
+  grid_release();
+  unsigned char *qs = pr_raw + ((1024u - (smem_addr(pr_raw) & 1023u)) & 1023u);
+  unsigned char *ring = qs + kPrRows * DP * 2;
+  const ms_prefix_attention_args &x = a.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // query tiles fastest: CTAs that run together read the same keys
+  const int qt = blockIdx.x % a.pre_tiles;
+  const int hs = blockIdx.x / a.pre_tiles;
+  const int h = hs % a.shape.kv_heads, part = hs / a.shape.kv_heads;
+  const int keys = (int)x.prefix_length;
+  const int all = (keys + KT - 1) / KT;
+  const int t0 = (int)((int64_t)all * part / a.pre_splits), t1 = (int)((int64_t)all * (part + 1) / a.pre_splits);
+  const int tiles = t1 - t0;
+  const int r0 = qt * kPrRows;
+  const int live_rows = min(kPrRows, a.packed - r0);
+  const int live_warps = (live_rows + 31) / 32;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      bar_init(&sh.full[i], 2);
+      bar_init(&sh.empty[i], 1);
+    }
+    bar_init(&sh.q_full, 4);
+    bar_init(&sh.s_full, 1);
+    bar_init(&sh.p_ready, live_warps);
+    bar_init(&sh.pv_done, 1);
+    bar_init(&sh.drained, 1);
+    sh.dead = 0;
+    bar_init_fence();
+  }
+  if (warp == 6) tmem_alloc(&sh.tmem, kPrCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp < 4) {
+    // this thread's query row, in 128-byte swizzled panels of 64 entries
+    const int r = tid;
+    {
+      const int pr = r0 + r;
+      const bool live = pr < a.packed;
+      const int64_t b = live ? pr / a.shape.group : 0;
+      const int head = h * a.shape.group + (live ? pr - (int)b * a.shape.group : 0);
+      const T *src = static_cast<const T *>(x.q) + b * x.q_row + head * x.q_head;
+#pragma unroll
+      for (int c = 0; c < DP / 8; ++c) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (live && c * 8 < x.head_dim) {
+          if (a.q_wide) {
+            v = __ldg(reinterpret_cast<const uint4 *>(src + c * 8));
+          } else {
+            const unsigned short *p = reinterpret_cast<const unsigned short *>(src + c * 8);
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldg(p + 2 * i) | ((uint32_t)__ldg(p + 2 * i + 1) << 16);
+            v = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        *reinterpret_cast<uint4 *>(qs + (c >> 3) * kPrRows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+      }
+      fence_async_proxy();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&sh.q_full);
+    }
+    if (warp < live_warps) {
+      const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+      const float kNone = __uint_as_float(0xFF800000u);
+      float m = kNone, l = 0.f;
+      bool ok = true;
+      for (int i = 0; i < tiles && ok; ++i) {
+        ok = !sh.dead && bar_wait(&sh.s_full, i & 1);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const int key0 = (t0 + i) * KT;
+        const bool cut = key0 + KT > keys;
+        float s[64];
+        float top = kNone;
+#pragma unroll
+        for (int half = 0; half < KT / 64; ++half) {  // the last half stays in registers
+          tmem_ld64(lanes + half * 64, s);
+          if (cut) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (key0 + half * 64 + j >= keys) s[j] = kNone;
+          }
+#pragma unroll
+          for (int j = 0; j < 64; ++j) top = fmaxf(top, s[j]);
+        }
+        top *= a.scale_log2;
+        const bool moved = top > m + 8.f || (m == kNone && top != kNone);
+        bool waited = i == 0;
+        if (__any_sync(0xFFFFFFFFu, moved)) {
+          const float next = moved ? top : m;
+          const float f = m == next ? 1.f : at_exp2(m - next);
+          m = next;
+          l *= f;
+          if (i > 0) {
+            ok = __all_sync(0xFFFFFFFFu, bar_wait(&sh.pv_done, (i - 1) & 1));
+            if (!ok) break;
+            waited = true;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+              uint32_t u[32];
+              tmem_ld32(lanes + kO + c, u);
+              tmem_wait_ld32(u);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) u[j] = __float_as_uint(__uint_as_float(u[j]) * f);
+              tmem_st32(lanes + kO + c, u);
+            }
+          }
+        }
+        const float base = m == kNone ? 0.f : m;
+#pragma unroll
+        for (int half = KT / 64 - 1; half >= 0; --half) {
+          if (half != KT / 64 - 1) {
+            tmem_ld64(lanes + half * 64, s);
+                    if (cut) {
+#pragma unroll
+              for (int j = 0; j < 64; ++j)
+                if (key0 + half * 64 + j >= keys) s[j] = kNone;
+            }
+          }
+          uint32_t u[32];
+          float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float e0 = at_exp2(fmaf(s[2 * j], a.scale_log2, -base));
+            const float e1 = at_exp2(fmaf(s[2 * j + 1], a.scale_log2, -base));
+            sum0 += e0;
+            sum1 += e1;
+            u[j] = AtType<T>::pack(e0, e1);
+          }
+          l += sum0 + sum1;
+          if (!waited) {  // the previous tile's weights are still being read
+            ok = __all_sync(0xFFFFFFFFu, bar_wait(&sh.pv_done, (i - 1) & 1));
+            waited = true;
+            tc_fence_after();
+          }
+          tmem_st32(lanes + kP + half * 32, u);
+        }
+        if (!ok) break;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&sh.p_ready);
+      }
+      if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(&sh.pv_done, (tiles - 1) & 1));
+      if (!ok) sh.dead = 1;
+      tc_fence_after();
+      const int pr = r0 + r;
+      const int64_t rec = ((int64_t)part * a.shape.kv_heads + h) * a.packed + pr;
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t u[32];
+        tmem_ld32(lanes + kO + c, u);
+        tmem_wait_ld32(u);
+        if (pr < a.packed) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            if (c + j < x.head_dim)
+              *reinterpret_cast<uint4 *>(a.pre_o + rec * x.head_dim + c + j) =
+                  make_uint4(u[j], u[j + 1], u[j + 2], u[j + 3]);
+        }
+      }
+      if (pr < a.packed) a.pre_ml[rec] = ok ? make_float2(m, l) : make_float2(0.f, __uint_as_float(0x7FC00000u));
+    }
+  } else if (warp < 6) {
+    constexpr int kRowsWarp = KT / 2;          // rows of a tile that one warp copies
+    constexpr int kChunks = DP / 8;            // 16-byte chunks of a row
+    constexpr int kRowsStep = 32 / kChunks;    // rows of one copy instruction
+    constexpr int kLook = kRowsWarp / 32;      // rows that a lane looks up
+    const int w = warp - 4, page_size = (int)x.page_size;
+    const int count = 2 * tiles;  // loads: K0, then K(i + 1) and V(i) in turn, V of the last tile
+    auto tile_of = [&](int n, bool &value) {
+      // n = 0: K(0); 2i + 1: K(i + 1), 2i + 2: V(i); the last one is the last tile's V
+      value = n == count - 1 || (n > 0 && (n & 1) == 0);
+      return n == count - 1 ? tiles - 1 : value ? (n >> 1) - 1 : (n + 1) >> 1;
+    };
+    int page[kLook], offset[kLook];
+    auto look = [&](int n) {
+      bool value;
+      const int tile = n < count ? tile_of(n, value) : 0;
+#pragma unroll
+      for (int i = 0; i < kLook; ++i) {
+        const int j = (t0 + tile) * KT + w * kRowsWarp + i * 32 + lane;
+        page[i] = -1;
+        if (n < count && j < keys) {
+          const int p = j / page_size;
+          offset[i] = j - p * page_size;
+          page[i] = __ldg(x.prefix_pages + p);
+        }
+      }
+    };
+    look(0);
+    int stage = 0, phase = 1, sent = 0;
+    bool ok = true;
+    for (int n = 0; n < count; ++n) {
+      bool value;
+      tile_of(n, value);
+      int64_t at[kLook];
+#pragma unroll
+      for (int i = 0; i < kLook; ++i)
+        at[i] = page[i] < 0 || page[i] >= x.pages ? -1
+                : value ? page[i] * x.cv_page + offset[i] * x.cv_token + h * x.cv_head
+                        : page[i] * x.ck_page + offset[i] * x.ck_token + h * x.ck_head;
+      look(n + 1);
+      ok = !sh.dead && bar_wait(&sh.empty[stage], phase);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      const T *src = static_cast<const T *>(value ? x.cache_v : x.cache_k);
+      const uint32_t dst = smem_addr(ring) + stage * kPrStage;
+      const int chunk = lane % kChunks;
+#pragma unroll
+      for (int i = 0; i < kRowsWarp / kRowsStep; ++i) {
+        const int rr = i * kRowsStep + lane / kChunks;
+        const int64_t from = __shfl_sync(0xFFFFFFFFu, at[i * kRowsStep / 32], rr & 31);
+        const bool live = from >= 0 && chunk * 8 < x.head_dim;
+        const int row = w * kRowsWarp + rr;
+        copy16(dst + (chunk >> 3) * KT * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4),
+               src + (live ? from + chunk * 8 : 0), live);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (n >= 2) {  // two loads in flight: the one before them has landed
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&sh.full[sent]);
+        if (++sent == kStages) sent = 0;
+      }
+      if (++stage == kStages) stage = 0, phase ^= 1;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    fence_async_proxy();
+    __syncwarp();
+    if (ok) {
+      for (int n = count < 2 ? 0 : count - 2; n < count; ++n) {
+        if (lane == 0) bar_arrive(&sh.full[sent]);
+        if (++sent == kStages) sent = 0;
+      }
+    } else {
+      sh.dead = 1;
+    }
+  } else if (lane == 0) {
+    constexpr uint32_t kQk = tc_idesc_f16<T>(KT, false), kPv = tc_idesc_f16<T>(DP, true);
+    const uint32_t q0 = smem_addr(qs), k0 = smem_addr(ring);
+    int stage = 0, phase = 0;
+    bool ok = bar_wait(&sh.q_full, 0);
+    auto next = [&]() {
+      if (++stage == kStages) stage = 0, phase ^= 1;
+    };
+    auto scores = [&]() {  // S of the tile in the present stage
+      ok = ok && !sh.dead && bar_wait(&sh.full[stage], phase);
+      if (!ok) return;
+      tc_fence_after();
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t panel = k >> 2, step = (k & 3) * 32;
+        tc_mma_f16(tmem, tc_desc(q0 + panel * kPrRows * 128 + step, 1024, 16),
+                   tc_desc(k0 + stage * kPrStage + panel * KT * 128 + step, 1024, 16), kQk, k > 0);
+      }
+      tc_commit(&sh.empty[stage]);
+      tc_commit(&sh.s_full);
+      next();
+    };
+    scores();
+    for (int i = 0; i < tiles && ok; ++i) {
+      ok = !sh.dead && bar_wait(&sh.p_ready, i & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (i + 1 < tiles) scores();
+      ok = ok && bar_wait(&sh.full[stage], phase);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int k = 0; k < KT / 16; ++k)
+        tc_mma_f16_tmem(tmem + kO, tmem + kP + k * 8, tc_desc(k0 + stage * kPrStage + k * 2048, 1024, KT * 128), kPv,
+                        i > 0 || k > 0);
+      tc_commit(&sh.empty[stage]);
+      tc_commit(&sh.pv_done);
+      next();
+    }
+    if (!ok) sh.dead = 1;
+    tc_commit(&sh.drained);
+    bar_wait(&sh.drained, 0);  // products in flight end before tensor memory is freed
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 6) tmem_free(tmem, kPrCols);
 }
 
 // Merge: one CTA per (row, query head) weighs the records of its pieces; the
@@ -401,7 +770,7 @@ __global__ void __launch_bounds__(kMgThreads) ms_attn_merge_kernel(const __grid_
   const int64_t b = blockIdx.x / a.shape.heads;
   const int hq = (int)(blockIdx.x - b * a.shape.heads);
   const int h = hq / a.shape.group, g = hq - h * a.shape.group;
-  const int c = g / kAtRows, hcs = a.shape.kv_heads * a.shape.chunks, hc = h * a.shape.chunks + c;
+  const int c = g / kAtRows, hc = h * a.shape.chunks + c;
   const int raw = __ldg(x.lengths + b);
   const int len = at_length(x, b);
   if (tid == 0) flag = raw != len ? MS_ROW_BAD_LENGTH : MS_ROW_OK;
@@ -417,17 +786,36 @@ __global__ void __launch_bounds__(kMgThreads) ms_attn_merge_kernel(const __grid_
   }
   grid_wait();
   if (tid == 0 && a.header->prefix_bad) atomicOr(&flag, MS_ROW_BAD_PAGE);
-  const int64_t tiles = ((int64_t)a.split_prefix + len + kSpTile - 1) / kSpTile;
-  int64_t first = 0;
-  int pieces = 0;
-  if (tiles > 0) {
-    const int64_t share = a.header->share, u = a.base[b] * hcs + hc * tiles;
-    first = b * hcs + hc + u / share;
-    pieces = (int)((u + tiles - 1) / share - u / share) + 1;
+  // the records: the row's own pieces, then the prefix's (the split kernel's or the prefix kernel's)
+  const int64_t share = a.header->share;
+  int64_t own = 0, pre = 0;
+  int owns = 0, pres = 0;
+  {
+    const int64_t tiles = (len + kSpTile - 1) / kSpTile;
+    if (tiles > 0) {
+      const int64_t u = a.base[b] + hc * tiles;
+      own = (sp_item(a, b, hc) + u / share) * a.shape.chunk_rows + g - c * kAtRows;
+      owns = (int)((u + tiles - 1) / share - u / share) + 1;
+    }
   }
-  const int rr = g - c * kAtRows;
+  const int packed_row = (int)b * a.shape.group + g;
+  if (a.split_prefix) {
+    const int64_t tiles = (a.split_prefix + kSpTile - 1) / kSpTile, u = h * tiles;
+    pre = (sp_item(a, -1, h) + u / share) * a.shape.chunk_rows + packed_row;
+    pres = (int)((u + tiles - 1) / share - u / share) + 1;
+  } else if (a.pre_splits) {
+    pre = (int64_t)h * a.packed + packed_row;
+    pres = a.pre_splits;
+  }
+  const int64_t pre_step = a.split_prefix ? a.shape.chunk_rows : (int64_t)a.shape.kv_heads * a.packed;
+  const float2 *pre_ml = a.split_prefix ? a.own_ml : a.pre_ml;
+  const float *pre_o = a.split_prefix ? a.own_o : a.pre_o;
+  const int pieces = owns + pres;
+  auto ml_of = [&](int p) {
+    return p < owns ? a.own_ml[own + (int64_t)p * a.shape.chunk_rows] : pre_ml[pre + (p - owns) * pre_step];
+  };
   float top = __uint_as_float(0xFF800000u);
-  for (int p = tid; p < pieces; p += kMgThreads) top = fmaxf(top, a.own_ml[(first + p) * a.shape.chunk_rows + rr].x);
+  for (int p = tid; p < pieces; p += kMgThreads) top = fmaxf(top, ml_of(p).x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   if (lane == 0) red[warp] = top;
@@ -437,11 +825,11 @@ __global__ void __launch_bounds__(kMgThreads) ms_attn_merge_kernel(const __grid_
   const float base = top == __uint_as_float(0xFF800000u) ? 0.f : top;
   float sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
   for (int p = warp; p < pieces; p += kMgThreads / 32) {
-    const int64_t rec = (first + p) * a.shape.chunk_rows + rr;
-    const float2 ml = a.own_ml[rec];
+    const float2 ml = ml_of(p);
     const float w = at_exp2(ml.x - base);
     sum += w * ml.y;
-    const float *src = a.own_o + rec * x.head_dim;
+    const float *src = p < owns ? a.own_o + (own + (int64_t)p * a.shape.chunk_rows) * x.head_dim
+                                : pre_o + (pre + (p - owns) * pre_step) * x.head_dim;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int d = lane + 32 * i;

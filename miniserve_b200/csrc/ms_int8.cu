@@ -297,6 +297,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       if (lane == 0) bar_arrive(&sh.acc_empty[acc]);
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

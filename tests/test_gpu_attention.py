@@ -305,4 +305,4 @@ def test_c_entry_refuses_bad_arguments():
         setattr(a, field, bad)
         assert L.ms_prefix_attention(ctypes.byref(a), None) == code, field
         setattr(a, field, keep)
-    assert L.ms_prefix_attention_workspace(1, 3, 2, 64) == 0
+    assert L.ms_prefix_attention_workspace(1, 3, 2, 64, 0) == 0
