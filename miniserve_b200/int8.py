@@ -14,6 +14,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 from . import _lib
+from ._launch import launch
 from .sampler import _torch
 
 MAX_INNER = 131072  # the int32 sum of 127 * 127 * K stays exact
@@ -21,10 +22,13 @@ MAX_INNER = 131072  # the int32 sum of 127 * 127 * K stays exact
 
 def _dtype_code(dtype) -> int:
     torch = _torch()
-    codes = {torch.float32: _lib.MS_DTYPE_F32, torch.bfloat16: _lib.MS_DTYPE_BF16, torch.float16: _lib.MS_DTYPE_F16}
-    if dtype not in codes:
-        raise TypeError(f"dtype {dtype} is not float32, bfloat16 or float16")
-    return codes[dtype]
+    if dtype is torch.float32:
+        return _lib.MS_DTYPE_F32
+    if dtype is torch.bfloat16:
+        return _lib.MS_DTYPE_BF16
+    if dtype is torch.float16:
+        return _lib.MS_DTYPE_F16
+    raise TypeError(f"dtype {dtype} is not float32, bfloat16 or float16")
 
 
 def _matrix(name: str, t, dtype=None):
@@ -32,7 +36,7 @@ def _matrix(name: str, t, dtype=None):
     torch = _torch()
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
     if t.dim() != 2 or t.shape[1] < 1:
         raise ValueError(f"{name} must be a [rows, entries] matrix")
@@ -89,9 +93,8 @@ def quantize_rows(x) -> Tuple["object", "object"]:
     _check_inner(K)
     q = _empty_rows(M, K, x.device)
     scale = torch.empty(M, dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        rc = _lib.lib().ms_quantize_rows(x.data_ptr(), code, M, K, _pitch(x), q.data_ptr(), q.stride(0),
-                                         scale.data_ptr(), torch.cuda.current_stream(x.device).cuda_stream)
+    rc = launch(x.device, _lib.lib().ms_quantize_rows, x.data_ptr(), code, M, K, _pitch(x), q.data_ptr(), q.stride(0),
+                scale.data_ptr())
     _lib.check(rc, "ms_quantize_rows")
     return q, scale
 
@@ -123,11 +126,9 @@ def int8_matmul(xq, x_scale, wq, w_scale, *, bias=None, out_dtype=None, out=None
     if out_dtype is None:
         out_dtype = torch.float32 if out is None else out.dtype
     out = _output(out, out_dtype, M, N, xq.device)
-    with torch.cuda.device(xq.device):
-        rc = _lib.lib().ms_int8_matmul(xq.data_ptr(), ldx, x_scale.data_ptr(), M, wq.data_ptr(), ldw,
-                                       w_scale.data_ptr(), N, K, None if bias is None else bias.data_ptr(),
-                                       out.data_ptr(), _dtype_code(out_dtype), _pitch(out),
-                                       torch.cuda.current_stream(xq.device).cuda_stream)
+    rc = launch(xq.device, _lib.lib().ms_int8_matmul, xq.data_ptr(), ldx, x_scale.data_ptr(), M, wq.data_ptr(), ldw,
+                w_scale.data_ptr(), N, K, None if bias is None else bias.data_ptr(), out.data_ptr(),
+                _dtype_code(out_dtype), _pitch(out))
     _lib.check(rc, "ms_int8_matmul")
     return out
 
@@ -154,6 +155,8 @@ class Int8Linear:
             rows.copy_(weight)
             weight = rows
         self.weight = weight
+        self.shape = (N, K)
+        self._ldw = _check_rows("weight", weight)
 
     @classmethod
     def from_float(cls, weight, bias=None) -> "Int8Linear":
@@ -167,7 +170,7 @@ class Int8Linear:
         torch = _torch()
         _matrix("x", x)
         code = _dtype_code(x.dtype)
-        N, K = self.weight.shape
+        N, K = self.shape
         dev = self.weight.device
         M = x.shape[0]
         if x.shape[1] != K or x.device != dev:
@@ -177,10 +180,9 @@ class Int8Linear:
         out = _output(out, out_dtype, M, N, dev)
         L = _lib.lib()
         workspace = torch.empty(L.ms_int8_workspace(M, K), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            rc = L.ms_int8_linear(x.data_ptr(), code, _pitch(x), M, self.weight.data_ptr(), _pitch(self.weight),
-                                  self.scale.data_ptr(), N, K, None if self.bias is None else self.bias.data_ptr(),
-                                  out.data_ptr(), _dtype_code(out_dtype), _pitch(out), workspace.data_ptr(),
-                                  torch.cuda.current_stream(dev).cuda_stream)
-        _lib.check(rc, "ms_int8_linear")
+        rc = launch(dev, L.ms_int8_linear, x.data_ptr(), code, _pitch(x), M, self.weight.data_ptr(), self._ldw,
+                    self.scale.data_ptr(), N, K, None if self.bias is None else self.bias.data_ptr(), out.data_ptr(),
+                    _dtype_code(out_dtype), _pitch(out), workspace.data_ptr())
+        if rc:
+            _lib.check(rc, "ms_int8_linear")
         return out
