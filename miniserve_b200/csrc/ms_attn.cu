@@ -106,19 +106,31 @@ static cudaError_t at_launch(K *kernel, int64_t grid, int threads, int shared, c
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+template <typename T, int DP, int NQ, bool kWhole>
+static cudaError_t at_split(const AtArgs &a, int dev, cudaStream_t s) {
+  static std::atomic<int> ready[kMaxDevices];
+  cudaError_t e = at_allow_shared(ms_attn_split_kernel<T, DP, NQ, kWhole>, kSpShared, ready, dev);
+  if (e != cudaSuccess) return e;
+  return at_launch(ms_attn_split_kernel<T, DP, NQ, kWhole>, a.shape.split_warps / kSpWarps, kSpWarps * 32, kSpShared,
+                   s, a.pre_splits != 0, a);
+}
+
 template <typename T, int DP>
 static cudaError_t at_run(const AtArgs &a, int dev, cudaStream_t s) {
-  static std::atomic<int> split_ready[kMaxDevices], prefix_ready[kMaxDevices];
-  cudaError_t e = at_allow_shared(ms_attn_split_kernel<T, DP>, kSpShared, split_ready, dev);
-  if (e == cudaSuccess && a.pre_splits) {
-    e = at_allow_shared(ms_attn_prefix_kernel<T, DP>, kPrSharedBytes<DP>, prefix_ready, dev);
+  cudaError_t e = cudaSuccess;
+  if (a.pre_splits) {
+    static std::atomic<int> ready[kMaxDevices];
+    e = at_allow_shared(ms_attn_prefix_kernel<T, DP>, kPrSharedBytes<DP>, ready, dev);
     if (e == cudaSuccess)
       e = at_launch(ms_attn_prefix_kernel<T, DP>, (int64_t)a.pre_tiles * a.shape.kv_heads * a.pre_splits, kPrThreads,
                     kPrSharedBytes<DP>, s, false, a);
   }
-  if (e != cudaSuccess) return e;
-  e = at_launch(ms_attn_split_kernel<T, DP>, a.shape.split_warps / kSpWarps, kSpWarps * 32, kSpShared, s,
-                a.pre_splits != 0, a);
+  if (e == cudaSuccess) {
+    if (a.narrow)
+      e = a.whole ? at_split<T, DP, 1, true>(a, dev, s) : at_split<T, DP, 1, false>(a, dev, s);
+    else
+      e = a.whole ? at_split<T, DP, 2, true>(a, dev, s) : at_split<T, DP, 2, false>(a, dev, s);
+  }
   if (e != cudaSuccess) return e;
   return at_launch(ms_attn_merge_kernel<T>, a.shape.rows * a.shape.heads, kMgThreads, 0, s, true, a);
 }
@@ -175,6 +187,8 @@ int ms_prefix_attention(const ms_prefix_attention_args *args, ms_stream_t stream
   a.pre_ml = reinterpret_cast<float2 *>(w + p.pre_ml);
   a.scale_log2 = x.scale * 1.4426950408889634f;
   a.q_wide = ((x.q_row | x.q_head) & 7) == 0 && (reinterpret_cast<uintptr_t>(x.q) & 15) == 0;
+  a.narrow = p.shape.chunk_rows <= 8;
+  a.whole = x.page_size % ms::kSpTile == 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool narrow = x.head_dim <= 64;
   if (x.dtype == MS_DTYPE_BF16)

@@ -12,12 +12,13 @@
 
 namespace ms {
 
-constexpr int kAtRows = 16;              // query heads of one chunk: the M of the warp products
+constexpr int kAtRows = 16;              // query heads of one chunk: up to two Ns of the warp products
 constexpr int64_t kAtMaxRows = 1 << 20;  // rows of a call
 constexpr int kAtMaxKeys = 0x3FFFFFFF;   // of the prefix, and of a row: their sum is an int
 constexpr int kSpWarps = 4;              // warps of a split CTA
 constexpr int kSpCtas = 2;               // split CTAs of an SM
-constexpr int kSpTile = 16;              // keys of a split tile
+constexpr int kSpTile = 16;              // keys of a split tile: the M of the warp products
+constexpr int kSpItem = 2;               // cost of an item's queries and record, in tiles
 constexpr int kSpRing = 24 * 1024;       // bytes of one warp's ring of tiles
 constexpr int kSpShared = kSpRing * kSpWarps;
 
@@ -39,7 +40,7 @@ struct AtArgs {
   ms_prefix_attention_args x;
   AtShape shape;
   AtHeader *header;
-  int64_t *base;    // [rows] the first tile of each row in the split kernel's sequence
+  int64_t *base;    // [rows] where each row starts in the split kernel's sequence
   float *own_o;     // [pieces][chunk_rows][head_dim]
   float2 *own_ml;   // [pieces][chunk_rows] (m in units of log2, l)
   float *pre_o;     // [splits][kv_heads][packed rows][head_dim], of the prefix kernel
@@ -50,6 +51,8 @@ struct AtArgs {
   int pre_splits;    // parts of the prefix that the prefix kernel takes; 0 where it does not run
   int pre_tiles;     // its query tiles of one key head
   int q_wide;        // q's heads start 16-byte aligned
+  int narrow;        // at most 8 query rows an item
+  int whole;         // page_size is a multiple of kSpTile: a tile lies in one page
 };
 
 template <typename T>
@@ -112,51 +115,68 @@ __device__ __forceinline__ int at_length(const ms_prefix_attention_args &x, int6
   return n >= 0 && n <= kAtMaxKeys && (int64_t)n <= x.table_width * x.page_size ? n : 0;
 }
 
-// Walks over (row, key head and chunk, tile) in order.  Row -1 is the prefix,
-// all rows' query heads of a key head being its one chunk.
+// Transposed 8 x 8 matrix of 16-bit entries.
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// The split kernel's sequence: items (row, key head and chunk) in order, each
+// of kSpItem units and one unit a tile; items without keys are not in it.
+// Row -1 is the prefix, all rows' query heads of a key head being its one
+// chunk.
+__device__ __forceinline__ int64_t sp_tiles(int64_t keys) { return (keys + kSpTile - 1) / kSpTile; }
+__device__ __forceinline__ int64_t sp_units(int64_t keys) { return keys > 0 ? sp_tiles(keys) + kSpItem : 0; }
+// Index of an item among the items.
+__device__ __forceinline__ int64_t sp_item(const AtArgs &a, int64_t b, int hc) {
+  return b < 0 ? hc : (a.split_prefix ? a.shape.kv_heads : 0) + b * a.shape.kv_heads * a.shape.chunks + hc;
+}
+
+// Walks over a warp's tiles.
 struct SpWalk {
-  int64_t b;
-  int hc, tile, tiles, keys;
-  int64_t left;  // tiles of this warp still to visit, the present one among them
+  int64_t b, left;  // left: units of the share past this item
+  int hc, tile, end, tiles, keys;
 };
 
 __device__ __forceinline__ void sp_row(const AtArgs &a, SpWalk &w) {
   w.keys = w.b < 0 ? a.split_prefix : at_length(a.x, w.b);
-  w.tiles = (w.keys + kSpTile - 1) / kSpTile;
-}
-__device__ __forceinline__ int sp_heads(const AtArgs &a, int64_t b) {  // (key head, chunk) pairs of a row
-  return b < 0 ? a.shape.kv_heads : a.shape.kv_heads * a.shape.chunks;
+  w.tiles = (int)sp_tiles(w.keys);
 }
 __device__ __forceinline__ int sp_head(const AtArgs &a, const SpWalk &w) {  // key head
   return w.b < 0 ? w.hc : w.hc / a.shape.chunks;
 }
-// Index of a row's (key head, chunk) among the sequence's items.
-__device__ __forceinline__ int64_t sp_item(const AtArgs &a, int64_t b, int hc) {
-  return b < 0 ? hc : (a.split_prefix ? a.shape.kv_heads : 0) + b * a.shape.kv_heads * a.shape.chunks + hc;
+// The next item's tiles within the share; tile == end where none are left.
+__device__ __forceinline__ void sp_item_next(const AtArgs &a, SpWalk &w) {
+  w.tile = w.end = 0;
+  if (w.left <= kSpItem) return;
+  if (++w.hc >= (w.b < 0 ? a.shape.kv_heads : a.shape.kv_heads * a.shape.chunks)) {
+    w.hc = 0;
+    do {  // a later row has keys: units are left
+      ++w.b;
+      sp_row(a, w);
+    } while (w.tiles == 0);
+  }
+  const int64_t take = min(w.left, (int64_t)w.tiles + kSpItem);
+  w.left -= take;
+  w.end = (int)take - kSpItem;
 }
 __device__ __forceinline__ void sp_next(const AtArgs &a, SpWalk &w) {
-  if (--w.left <= 0) return;
-  if (++w.tile < w.tiles) return;
-  w.tile = 0;
-  if (++w.hc < sp_heads(a, w.b)) return;
-  w.hc = 0;
-  do {  // a later row has tiles: some are left
-    ++w.b;
-    sp_row(a, w);
-  } while (w.tiles == 0);
+  if (++w.tile >= w.end) sp_item_next(a, w);
 }
 
-// Split kernel.  The tiles of 16 keys of all rows and key heads (and of the
-// prefix, where its query rows fit one chunk) form one sequence; every warp takes an equal, contiguous share of it, whatever the
-// rows' lengths, and works alone: a ring of tiles filled with 16-byte
-// asynchronous copies, a page lookup one tile ahead of its copies, and
-// products of m16n8k16 (the chunk's query heads are the M).  Where its share
-// meets an item (row, key head, chunk), it leaves one record at index item +
-// warp, which is unique because both only grow along the sequence.
+// Split kernel.  All rows' items (and the prefix's, where its query rows fit
+// one chunk) form one sequence; every warp takes an equal, contiguous share of
+// it, whatever the rows' lengths, and works alone: a ring of tiles of 16 keys
+// filled with 16-byte asynchronous copies, a page lookup one tile ahead of its
+// copies, and products of m16n8k16 with the keys as M and the queries as N
+// (S^T = K Q^T, O^T += V^T P^T; P^T changes fragments with movmatrix), so that
+// 8 query heads leave no half of a product empty.  Where its share meets an
+// item's tiles, it leaves one record at index item + warp, which is unique
+// because both only grow along the sequence.
 //
-// Bound by the bytes of the cache: a tile of 64-entry heads is 4 KB and costs
-// the products of 16 rows whatever the group, far below their rate.
-template <typename T, int DP>
+// Bound by the bytes of the cache.
+template <typename T, int DP, int NQ, bool kWhole>
 __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
     ms_attn_split_kernel(const __grid_constant__ AtArgs a) {
   constexpr int kRow = DP * 2;                 // bytes of a key's row in the ring
@@ -164,42 +184,48 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
   constexpr int kStage = 2 * kSpTile * kRow;   // K, then V
   constexpr int kStages = kSpRing / kStage;
   constexpr int kRowsStep = 32 / kChunks;      // rows of one copy instruction
+  constexpr int kThreads = kSpWarps * 32;
+  const float kNone = __uint_as_float(0xFF800000u);
   extern __shared__ __align__(128) unsigned char sp_ring[];
-  __shared__ int64_t sums[kSpWarps * 32 + 1];
+  __shared__ int64_t sums[kThreads + 1];  // units of the rows before each thread's run of rows, of one key head and chunk
+  __shared__ int64_t warp_sums[kSpWarps];
   __shared__ int bad;
   grid_release();
   const ms_prefix_attention_args &x = a.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t rows = a.shape.rows;
   const int hcs = a.shape.kv_heads * a.shape.chunks;
-  // the rows' tiles before each thread's run of rows
-  const int64_t run = (rows + kSpWarps * 32 - 1) / (kSpWarps * 32);
+  const int64_t run = (rows + kThreads - 1) / kThreads;
   const int64_t r0 = min(rows, tid * run), r1 = min(rows, r0 + run);
   {
     int64_t n = 0;
-    for (int64_t b = r0; b < r1; ++b) n += (at_length(x, b) + kSpTile - 1) / kSpTile;
-    sums[tid + 1] = n;
+    for (int64_t b = r0; b < r1; ++b) n += sp_units(at_length(x, b));
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xFFFFFFFFu, n, o);
+      if (lane >= o) n += v;
+    }
+    if (lane == 31) warp_sums[warp] = n;
     if (tid == 0) sums[0] = 0, bad = 0;
     __syncthreads();
-    for (int o = 1; o < kSpWarps * 32; o <<= 1) {
-      const int64_t v = tid >= o ? sums[tid + 1 - o] : 0;
-      __syncthreads();
-      sums[tid + 1] += v;
-      __syncthreads();
-    }
+#pragma unroll
+    for (int i = 0; i < kSpWarps; ++i)
+      if (i < warp) n += warp_sums[i];
+    sums[tid + 1] = n;
+    __syncthreads();
   }
-  const int64_t before = (int64_t)((a.split_prefix + kSpTile - 1) / kSpTile) * a.shape.kv_heads;
-  const int64_t total = before + sums[kSpWarps * 32] * hcs;
-  const int64_t share = max((int64_t)1, (total + a.shape.split_warps - 1) / a.shape.split_warps);
-  if (blockIdx.x == 0) {  // for the merge: where each row's tiles start, and whether the prefix's pages are good
+  const int64_t before = sp_units(a.split_prefix) * a.shape.kv_heads;
+  const int64_t total = before + sums[kThreads] * hcs;
+  const int64_t share = max((int64_t)kSpItem + 1, (total + a.shape.split_warps - 1) / a.shape.split_warps);
+  if (blockIdx.x == 0) {  // for the merge: where each row starts, and whether the prefix's pages are good
     int64_t n = sums[tid];
     for (int64_t b = r0; b < r1; ++b) {
       a.base[b] = before + n * hcs;
-      n += (at_length(x, b) + kSpTile - 1) / kSpTile;
+      n += sp_units(at_length(x, b));
     }
     const int64_t pages = (x.prefix_length + x.page_size - 1) / x.page_size;
     int seen = 0;
-    for (int64_t p = tid; p < pages; p += kSpWarps * 32) {
+    for (int64_t p = tid; p < pages; p += kThreads) {
       const int32_t id = __ldg(x.prefix_pages + p);
       seen |= id < 0 || id >= x.pages;
     }
@@ -214,40 +240,49 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
     return;
   }
   SpWalk load;
-  int64_t first = 0;
-  if (u0 < before) {
-    load.b = -1;
-    sp_row(a, load);
-  } else {  // the row that tile u0 of the sequence lies in: its thread's run, then the row
-    int lo = 0, hi = kSpWarps * 32 - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (before + sums[mid + 1] * hcs > u0) hi = mid;
-      else lo = mid + 1;
-    }
-    load.b = min(rows, lo * run);
-    first = before + sums[lo] * hcs;
-    sp_row(a, load);
-    while (first + (int64_t)load.tiles * hcs <= u0) {
-      first += (int64_t)load.tiles * hcs;
-      ++load.b;
+  {
+    int64_t first = 0;  // the row that unit u0 lies in: its thread's run, then the row
+    if (u0 < before) {
+      load.b = -1;
       sp_row(a, load);
+    } else {
+      int lo = 0, hi = kThreads - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (before + sums[mid + 1] * hcs > u0) hi = mid;
+        else lo = mid + 1;
+      }
+      load.b = min(rows, lo * run);
+      first = before + sums[lo] * hcs;
+      sp_row(a, load);
+      while (first + sp_units(load.keys) * hcs <= u0) {
+        first += sp_units(load.keys) * hcs;
+        ++load.b;
+        sp_row(a, load);
+      }
     }
+    const int64_t units = load.tiles + kSpItem;
+    load.hc = (int)((u0 - first) / units);
+    const int64_t at = u0 - first - load.hc * units, take = min(u1 - u0, units - at);
+    load.left = u1 - u0 - take;
+    load.tile = (int)max((int64_t)0, at - kSpItem);
+    load.end = (int)(at + take) - kSpItem;
+    if (load.end <= load.tile) sp_item_next(a, load);
   }
-  load.hc = (int)((u0 - first) / load.tiles);
-  load.tile = (int)((u0 - first) - (int64_t)load.hc * load.tiles);
-  load.left = u1 - u0;
   SpWalk now = load;
   const uint32_t ring = smem_addr(sp_ring) + warp * kSpRing;
-  const T *ck = static_cast<const T *>(x.cache_k), *cv = static_cast<const T *>(x.cache_v);
   const int page_size = (int)x.page_size;
+  const int chunk = lane % kChunks;
+  const bool inside = chunk * 8 < x.head_dim;
 
-  // lanes 0-15 look up the tile's keys for K, lanes 16-31 for V
-  int page = -1, offset = 0, head = 0;
+  // One page for all lanes where tiles lie in one; else lanes 0-15 look up
+  // the tile's keys for K, lanes 16-31 for V.
+  int page = -1, offset = 0, head = 0, live_keys = 0;
   auto look = [&]() {
     page = -1;
-    if (load.left > 0) {
-      const int j = load.tile * kSpTile + (lane & 15);
+    if (load.tile < load.end) {
+      const int j = load.tile * kSpTile + (kWhole ? 0 : lane & 15);
+      live_keys = load.keys - load.tile * kSpTile;
       if (j < load.keys) {
         const int p = j / page_size;
         offset = j - p * page_size;
@@ -257,20 +292,44 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
       sp_next(a, load);
     }
   };
+  const int64_t kstep = (int64_t)(lane / kChunks) * x.ck_token + chunk * 8;
+  const int64_t vstep = (int64_t)(lane / kChunks) * x.cv_token + chunk * 8;
   auto issue = [&](int stage) {
-    int64_t at = -1;
-    if (page >= 0 && page < x.pages)
-      at = lane < 16 ? page * x.ck_page + offset * x.ck_token + head * x.ck_head
-                     : page * x.cv_page + offset * x.cv_token + head * x.cv_head;
-    const uint32_t dst = ring + stage * kStage;
-    const int chunk = lane % kChunks;
+    const uint32_t dst = ring + stage * kStage + (lane / kChunks) * kRow;
+    const bool good = page >= 0 && page < x.pages;
+    if (kWhole) {
+      const T *ks = static_cast<const T *>(x.cache_k), *vs = static_cast<const T *>(x.cache_v);
+      if (good) {
+        ks += page * x.ck_page + offset * x.ck_token + head * x.ck_head + kstep;
+        vs += page * x.cv_page + offset * x.cv_token + head * x.cv_head + vstep;
+      }
 #pragma unroll
-    for (int i = 0; i < 2 * kSpTile / kRowsStep; ++i) {
-      const int r = i * kRowsStep + lane / kChunks;  // 0-15: K, 16-31: V
-      const int64_t from = __shfl_sync(0xFFFFFFFFu, at, r);
-      const bool live = from >= 0 && chunk * 8 < x.head_dim;
-      const T *src = (r < kSpTile ? ck : cv) + (live ? from + chunk * 8 : 0);
-      copy16(dst + r * kRow + ((chunk ^ (r & 7)) << 4), src, live);
+      for (int i = 0; i < kSpTile / kRowsStep; ++i) {
+        const int r = i * kRowsStep + lane / kChunks;
+        const bool live = good && inside && r < live_keys;
+        copy16(dst + i * kRowsStep * kRow + ((chunk ^ (r & 7)) << 4), live ? ks : x.cache_k, live);
+        ks += kRowsStep * x.ck_token;
+      }
+#pragma unroll
+      for (int i = 0; i < kSpTile / kRowsStep; ++i) {
+        const int r = i * kRowsStep + lane / kChunks;
+        const bool live = good && inside && r < live_keys;
+        copy16(dst + (kSpTile + i * kRowsStep) * kRow + ((chunk ^ (r & 7)) << 4), live ? vs : x.cache_v, live);
+        vs += kRowsStep * x.cv_token;
+      }
+    } else {
+      int64_t at = -1;
+      if (good)
+        at = lane < 16 ? page * x.ck_page + offset * x.ck_token + head * x.ck_head
+                       : page * x.cv_page + offset * x.cv_token + head * x.cv_head;
+#pragma unroll
+      for (int i = 0; i < 2 * kSpTile / kRowsStep; ++i) {
+        const int r = i * kRowsStep + lane / kChunks;  // 0-15: K, 16-31: V
+        const int64_t from = __shfl_sync(0xFFFFFFFFu, at, r);
+        const bool live = from >= 0 && inside;
+        const T *src = static_cast<const T *>(r < kSpTile ? x.cache_k : x.cache_v) + (live ? from + chunk * 8 : 0);
+        copy16(dst + i * kRowsStep * kRow + ((chunk ^ (r & 7)) << 4), src, live);
+      }
     }
   };
 
@@ -281,125 +340,123 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
     look();
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  uint32_t qf[DP / 16][4];
-  float o[DP / 8][4];
-  float m[2], l[2];
+  uint32_t qf[NQ][DP / 16][2];
+  float o[NQ][DP / 16][4];
+  float m[NQ][2], l[NQ][2];
   bool fresh = true;
   int stage = 0;
-  while (now.left > 0) {
-    {
-      const int ahead = stage == 0 ? kStages - 1 : stage - 1;
-      issue(ahead);
-      look();
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
+  while (now.tile < now.end) {
+    issue(stage == 0 ? kStages - 1 : stage - 1);
+    look();
+    asm volatile("cp.async.commit_group;" ::: "memory");
     // query rows of the item: a chunk of one row's heads, or all rows' heads for the prefix
     const int h = sp_head(a, now), c = now.b < 0 ? 0 : now.hc - h * a.shape.chunks;
     const int n = now.b < 0 ? a.packed : min(kAtRows, a.shape.group - c * kAtRows);
     if (fresh) {
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
+      for (int t = 0; t < NQ; ++t) {
+        const int g = t * 8 + (lane >> 2);
+        const int64_t b = now.b < 0 ? g / a.shape.group : now.b;
+        const int head_q = h * a.shape.group + (now.b < 0 ? g % a.shape.group : c * kAtRows + g);
+        const T *q = static_cast<const T *>(x.q) + (g < n ? b * x.q_row + head_q * x.q_head : 0) + (lane & 3) * 2;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int g = (lane >> 2) + (i & 1) * 8, d = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
+        for (int k = 0; k < DP / 8; ++k) {
           uint32_t u = 0;
-          if (g < n && d < x.head_dim) {
-            const int64_t b = now.b < 0 ? g / a.shape.group : now.b;
-            const int head_q = h * a.shape.group + (now.b < 0 ? g % a.shape.group : c * kAtRows + g);
-            const unsigned short *p = reinterpret_cast<const unsigned short *>(static_cast<const T *>(x.q) +
-                                                                               b * x.q_row + head_q * x.q_head + d);
-            u = (uint32_t)__ldg(p) | ((uint32_t)__ldg(p + 1) << 16);
+          if (g < n && k * 8 < x.head_dim) {
+            if (a.q_wide) {
+              u = __ldg(reinterpret_cast<const unsigned int *>(q + k * 8));
+            } else {
+              const unsigned short *p = reinterpret_cast<const unsigned short *>(q + k * 8);
+              u = (uint32_t)__ldg(p) | ((uint32_t)__ldg(p + 1) << 16);
+            }
           }
-          qf[k][i] = u;
+          qf[t][k >> 1][k & 1] = u;
         }
-      }
 #pragma unroll
-      for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-      m[0] = m[1] = __uint_as_float(0xFF800000u);
-      l[0] = l[1] = 0.f;
+        for (int i = 0; i < DP / 16; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+        m[t][0] = m[t][1] = kNone;
+        l[t][0] = l[t][1] = 0.f;
+      }
       fresh = false;
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     __syncwarp();
     const uint32_t kst = ring + stage * kStage, vst = kst + kSpTile * kRow;
-    float sc[2][4] = {};
+    float sc[NQ][2][4] = {};
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
-      const int r = (lane & 7) + ((lane >> 4) << 3), chunk = 2 * k + ((lane >> 3) & 1);
-      uint32_t b[4];
-      ldmatrix4(b, kst + r * kRow + ((chunk ^ (r & 7)) << 4));
-      AtType<T>::mma(sc[0], qf[k], b[0], b[1]);
-      AtType<T>::mma(sc[1], qf[k], b[2], b[3]);
+      const int r = lane & 15, ch = 2 * k + (lane >> 4);
+      uint32_t f[4];
+      ldmatrix4(f, kst + r * kRow + ((ch ^ (r & 7)) << 4));
+#pragma unroll
+      for (int t = 0; t < NQ; ++t) AtType<T>::mma(sc[t][k & 1], f, qf[t][k][0], qf[t][k][1]);
     }
-    // scores in units of log2; keys past the end leave nothing
-    const int j0 = now.tile * kSpTile + (lane & 3) * 2;
-    float top[2] = {m[0], m[1]};
+    // scores in units of log2: entries 0, 1 of key lane / 4, queries 2 (lane % 4) and the next; 2, 3 of key + 8
+    const int left = now.keys - now.tile * kSpTile;
+    uint32_t p[NQ][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < NQ; ++t) {
+      float w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool seen = j0 + t * 8 + (i & 1) < now.keys;
-        sc[t][i] = seen ? sc[t][i] * a.scale_log2 : __uint_as_float(0xFF800000u);
-        top[i >> 1] = fmaxf(top[i >> 1], sc[t][i]);
+      for (int i = 0; i < 4; ++i) w[i] = (sc[t][0][i] + sc[t][1][i]) * a.scale_log2;
+      if (left < kSpTile) {  // keys past the end leave nothing
+        if ((lane >> 2) >= left) w[0] = w[1] = kNone;
+        if ((lane >> 2) + 8 >= left) w[2] = w[3] = kNone;
       }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 1));
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 2));
-    }
-    if (__any_sync(0xFFFFFFFFu, top[0] != m[0] || top[1] != m[1])) {
+      float top[2] = {fmaxf(w[0], w[2]), fmaxf(w[1], w[3])};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        // both -inf (no score yet above it): nothing to rescale
-        const float f = m[i] == top[i] ? 1.f : at_exp2(m[i] - top[i]);
-        m[i] = top[i];
-        l[i] *= f;
 #pragma unroll
-        for (int n = 0; n < DP / 8; ++n) o[n][2 * i] *= f, o[n][2 * i + 1] *= f;
+        for (int s = 4; s < 32; s <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], s));
+        top[i] = fmaxf(top[i], m[t][i]);
       }
-    }
-    uint32_t p[4];
-    {
-      float w[2][4];
+      if (__any_sync(0xFFFFFFFFu, top[0] != m[t][0] || top[1] != m[t][1])) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int i = 0; i < 2; ++i) {
+          // both -inf (no score yet above it): nothing to rescale
+          const float f = m[t][i] == top[i] ? 1.f : at_exp2(m[t][i] - top[i]);
+          m[t][i] = top[i];
+          l[t][i] *= f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float base = m[i >> 1];
-          w[t][i] = sc[t][i] == __uint_as_float(0xFF800000u) ? 0.f : at_exp2(sc[t][i] - base);
+          for (int k = 0; k < DP / 16; ++k) o[t][k][i] *= f, o[t][k][2 + i] *= f;
         }
-      l[0] += (w[0][0] + w[0][1]) + (w[1][0] + w[1][1]);
-      l[1] += (w[0][2] + w[0][3]) + (w[1][2] + w[1][3]);
-      p[0] = AtType<T>::pack(w[0][0], w[0][1]);
-      p[1] = AtType<T>::pack(w[0][2], w[0][3]);
-      p[2] = AtType<T>::pack(w[1][0], w[1][1]);
-      p[3] = AtType<T>::pack(w[1][2], w[1][3]);
+      }
+      // a score of -inf has weight 0 whatever the maximum
+      const float base[2] = {m[t][0] == kNone ? 0.f : m[t][0], m[t][1] == kNone ? 0.f : m[t][1]};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = at_exp2(w[i] - base[i & 1]);
+      l[t][0] += w[0] + w[2];
+      l[t][1] += w[1] + w[3];
+      p[t][0] = movmatrix(AtType<T>::pack(w[0], w[1]));
+      p[t][1] = movmatrix(AtType<T>::pack(w[2], w[3]));
     }
 #pragma unroll
-    for (int n = 0; n < DP / 16; ++n) {
-      const int r = (lane & 7) + (((lane >> 3) & 1) << 3), chunk = 2 * n + (lane >> 4);
-      uint32_t b[4];
-      ldmatrix4t(b, vst + r * kRow + ((chunk ^ (r & 7)) << 4));
-      AtType<T>::mma(o[2 * n], p, b[0], b[1]);
-      AtType<T>::mma(o[2 * n + 1], p, b[2], b[3]);
+    for (int k = 0; k < DP / 16; ++k) {
+      const int r = (lane & 7) + ((lane >> 4) << 3), ch = 2 * k + ((lane >> 3) & 1);
+      uint32_t f[4];
+      ldmatrix4t(f, vst + r * kRow + ((ch ^ (r & 7)) << 4));
+#pragma unroll
+      for (int t = 0; t < NQ; ++t) AtType<T>::mma(o[t][k], f, p[t][0], p[t][1]);
     }
     __syncwarp();  // the stage is read: the next round's copies may overwrite it
-    if (now.left == 1 || now.tile + 1 == now.tiles) {
+    if (now.tile + 1 == now.end) {
       const int64_t piece = sp_item(a, now.b, now.hc) + wid;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
-        const int g = (lane >> 2) + i * 8;
-        if (g < n) {
-          const int64_t rec = piece * a.shape.chunk_rows + g;
-          if ((lane & 3) == 0) a.own_ml[rec] = make_float2(m[i], l[i]);
-          float *dst = a.own_o + rec * x.head_dim;
+      for (int t = 0; t < NQ; ++t) {
 #pragma unroll
-          for (int t = 0; t < DP / 8; ++t) {
-            const int d = t * 8 + (lane & 3) * 2;
-            if (d < x.head_dim) *reinterpret_cast<float2 *>(dst + d) = make_float2(o[t][2 * i], o[t][2 * i + 1]);
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int s = 4; s < 32; s <<= 1) l[t][i] += __shfl_xor_sync(0xFFFFFFFFu, l[t][i], s);
+          const int g = t * 8 + (lane & 3) * 2 + i;
+          if (g < n) {
+            const int64_t rec = piece * a.shape.chunk_rows + g;
+            if (lane < 4) a.own_ml[rec] = make_float2(m[t][i], l[t][i]);
+            float *dst = a.own_o + rec * x.head_dim + (lane >> 2);
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+              if (k * 16 < x.head_dim) dst[k * 16] = o[t][k][i];
+              if (k * 16 + 8 < x.head_dim) dst[k * 16 + 8] = o[t][k][2 + i];
+            }
           }
         }
       }
@@ -791,18 +848,18 @@ __global__ void __launch_bounds__(kMgThreads) ms_attn_merge_kernel(const __grid_
   int64_t own = 0, pre = 0;
   int owns = 0, pres = 0;
   {
-    const int64_t tiles = (len + kSpTile - 1) / kSpTile;
-    if (tiles > 0) {
-      const int64_t u = a.base[b] + hc * tiles;
-      own = (sp_item(a, b, hc) + u / share) * a.shape.chunk_rows + g - c * kAtRows;
-      owns = (int)((u + tiles - 1) / share - u / share) + 1;
+    const int64_t units = sp_units(len);
+    if (units > 0) {  // the warps whose shares meet the item's tiles
+      const int64_t u = a.base[b] + hc * units, w = (u + kSpItem) / share;
+      own = (sp_item(a, b, hc) + w) * a.shape.chunk_rows + g - c * kAtRows;
+      owns = (int)((u + units - 1) / share - w) + 1;
     }
   }
   const int packed_row = (int)b * a.shape.group + g;
   if (a.split_prefix) {
-    const int64_t tiles = (a.split_prefix + kSpTile - 1) / kSpTile, u = h * tiles;
-    pre = (sp_item(a, -1, h) + u / share) * a.shape.chunk_rows + packed_row;
-    pres = (int)((u + tiles - 1) / share - u / share) + 1;
+    const int64_t units = sp_units(a.split_prefix), u = h * units, w = (u + kSpItem) / share;
+    pre = (sp_item(a, -1, h) + w) * a.shape.chunk_rows + packed_row;
+    pres = (int)((u + units - 1) / share - w) + 1;
   } else if (a.pre_splits) {
     pre = (int64_t)h * a.packed + packed_row;
     pres = a.pre_splits;
