@@ -29,14 +29,14 @@ static int at_sms(int dev) {
 }
 
 // Parts of the prefix for the prefix kernel: the fewest waves of CTAs (two an
-// SM) times tiles of one CTA, each CTA costing about two tiles besides (its
+// SM) times tiles of one CTA, each CTA costing about four tiles besides (its
 // queries, first copies and record).
 static int at_parts(int64_t ctas, int64_t tiles, int sms) {
   int best = 1;
   double least = 0;
   for (int n = 1; n <= 2 * sms && n <= tiles; ++n) {
     const double waves = (double)((ctas * n + 2 * sms - 1) / (2 * sms));
-    const double cost = waves * ((double)((tiles + n - 1) / n) + 2.0);
+    const double cost = waves * ((double)((tiles + n - 1) / n) + 4.0);
     if (n == 1 || cost < least) best = n, least = cost;
     if (ctas * n >= 4 * sms) break;
   }
@@ -64,9 +64,8 @@ static AtPlan at_plan(int64_t rows, int heads, int kv_heads, int head_dim, int64
     p.split_prefix = (int)prefix;
     if (p.packed > s.chunk_rows) s.chunk_rows = p.packed;
   } else if (prefix > 0) {
-    const int kt = head_dim <= 64 ? kPrKeys<64> : kPrKeys<128>;
     p.pre_tiles = (p.packed + kPrRows - 1) / kPrRows;
-    p.pre_splits = at_parts((int64_t)p.pre_tiles * kv_heads, (prefix + kt - 1) / kt, sms);
+    p.pre_splits = at_parts((int64_t)p.pre_tiles * kv_heads, (prefix + kPrKeys - 1) / kPrKeys, sms);
   }
   const int64_t pieces = rows * kv_heads * s.chunks + (p.split_prefix ? kv_heads : 0) + s.split_warps;
   const int64_t pre = (int64_t)p.pre_splits * kv_heads * p.packed;
@@ -115,15 +114,41 @@ static cudaError_t at_split(const AtArgs &a, int dev, cudaStream_t s) {
                    s, a.pre_splits != 0, a);
 }
 
+// One of the caches as [pages, kv_heads, page_size, head_dim], read in boxes of
+// one page's or half a tile's tokens and 64 entries (128 bytes, swizzled).
+// False where the layout cannot be described so.
+static bool at_map(CUtensorMap *map, const ms_prefix_attention_args &x, const void *base, int64_t page, int64_t token,
+                   int64_t head) {
+  const bool inner = x.page_size % 8 == 0 && (x.page_size % kPrHalf == 0 || kPrHalf % x.page_size == 0);
+  EncodeTiled fn;
+  if (!inner || encode_tiled(&fn) != cudaSuccess) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)x.head_dim, (cuuint64_t)x.page_size, (cuuint64_t)x.kv_heads,
+                              (cuuint64_t)x.pages};
+  // a dimension of one entry may have any stride: one that a map accepts
+  const int64_t row = (int64_t)x.head_dim;
+  const cuuint64_t strides[3] = {(cuuint64_t)(x.page_size > 1 ? token : row) * 2,
+                                 (cuuint64_t)(x.kv_heads > 1 ? head : row) * 2,
+                                 (cuuint64_t)(x.pages > 1 ? page : row) * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)(x.page_size < kPrHalf ? x.page_size : kPrHalf), 1, 1};
+  const cuuint32_t unit[4] = {1, 1, 1, 1};
+  return fn(map, x.dtype == MS_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+            const_cast<void *>(base), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int DP>
-static cudaError_t at_run(const AtArgs &a, int dev, cudaStream_t s) {
+static cudaError_t at_run(AtArgs &a, int dev, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
   if (a.pre_splits) {
     static std::atomic<int> ready[kMaxDevices];
     e = at_allow_shared(ms_attn_prefix_kernel<T, DP>, kPrSharedBytes<DP>, ready, dev);
+    CUtensorMap kmap{}, vmap{};
+    a.tma = at_map(&kmap, a.x, a.x.cache_k, a.x.ck_page, a.x.ck_token, a.x.ck_head) &&
+            at_map(&vmap, a.x, a.x.cache_v, a.x.cv_page, a.x.cv_token, a.x.cv_head);
     if (e == cudaSuccess)
       e = at_launch(ms_attn_prefix_kernel<T, DP>, (int64_t)a.pre_tiles * a.shape.kv_heads * a.pre_splits, kPrThreads,
-                    kPrSharedBytes<DP>, s, false, a);
+                    kPrSharedBytes<DP>, s, false, a, kmap, vmap);
   }
   if (e == cudaSuccess) {
     if (a.narrow)
@@ -132,7 +157,9 @@ static cudaError_t at_run(const AtArgs &a, int dev, cudaStream_t s) {
       e = a.whole ? at_split<T, DP, 2, true>(a, dev, s) : at_split<T, DP, 2, false>(a, dev, s);
   }
   if (e != cudaSuccess) return e;
-  return at_launch(ms_attn_merge_kernel<T>, a.shape.rows * a.shape.heads, kMgThreads, 0, s, true, a);
+  const int64_t outputs = a.shape.rows * a.shape.heads;
+  if (a.merge_wide) return at_launch(ms_attn_merge_kernel<T, DP, 8>, outputs, kMgThreads, 0, s, true, a);
+  return at_launch(ms_attn_merge_kernel<T, DP, 1>, (outputs + 7) / 8, kMgThreads, 0, s, true, a);
 }
 
 }  // namespace ms
@@ -187,6 +214,7 @@ int ms_prefix_attention(const ms_prefix_attention_args *args, ms_stream_t stream
   a.pre_ml = reinterpret_cast<float2 *>(w + p.pre_ml);
   a.scale_log2 = x.scale * 1.4426950408889634f;
   a.q_wide = ((x.q_row | x.q_head) & 7) == 0 && (reinterpret_cast<uintptr_t>(x.q) & 15) == 0;
+  a.merge_wide = x.rows * x.heads <= 8 * ms::at_sms(dev);
   a.narrow = p.shape.chunk_rows <= 8;
   a.whole = x.page_size % ms::kSpTile == 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -2,6 +2,7 @@
 // and the prefix's where few rows share it) and the merge.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -23,9 +24,12 @@ constexpr int kSpRing = 24 * 1024;       // bytes of one warp's ring of tiles
 constexpr int kSpShared = kSpRing * kSpWarps;
 
 struct AtHeader {
-  int64_t share;       // tiles of one split warp
-  int32_t prefix_bad;  // a page of the prefix is outside the cache
+  int64_t share;  // units of one split warp
 };
+
+// l of a record that met a page outside the cache (its keys count as zeros
+// there; the merge flags the rows that read the record).
+constexpr float kAtBadPage = -1.f;
 
 struct AtShape {
   int64_t rows;
@@ -51,6 +55,8 @@ struct AtArgs {
   int pre_splits;    // parts of the prefix that the prefix kernel takes; 0 where it does not run
   int pre_tiles;     // its query tiles of one key head
   int q_wide;        // q's heads start 16-byte aligned
+  int tma;           // the cache can be read in boxes of half a tile, or of pages that divide it
+  int merge_wide;    // the merge gives each output a CTA
   int narrow;        // at most 8 query rows an item
   int whole;         // page_size is a multiple of kSpTile: a tile lies in one page
 };
@@ -189,7 +195,6 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
   extern __shared__ __align__(128) unsigned char sp_ring[];
   __shared__ int64_t sums[kThreads + 1];  // units of the rows before each thread's run of rows, of one key head and chunk
   __shared__ int64_t warp_sums[kSpWarps];
-  __shared__ int bad;
   grid_release();
   const ms_prefix_attention_args &x = a.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -206,7 +211,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
       if (lane >= o) n += v;
     }
     if (lane == 31) warp_sums[warp] = n;
-    if (tid == 0) sums[0] = 0, bad = 0;
+    if (tid == 0) sums[0] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kSpWarps; ++i)
@@ -217,21 +222,13 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
   const int64_t before = sp_units(a.split_prefix) * a.shape.kv_heads;
   const int64_t total = before + sums[kThreads] * hcs;
   const int64_t share = max((int64_t)kSpItem + 1, (total + a.shape.split_warps - 1) / a.shape.split_warps);
-  if (blockIdx.x == 0) {  // for the merge: where each row starts, and whether the prefix's pages are good
+  if (blockIdx.x == 0) {  // for the merge: where each row starts
     int64_t n = sums[tid];
     for (int64_t b = r0; b < r1; ++b) {
       a.base[b] = before + n * hcs;
       n += sp_units(at_length(x, b));
     }
-    const int64_t pages = (x.prefix_length + x.page_size - 1) / x.page_size;
-    int seen = 0;
-    for (int64_t p = tid; p < pages; p += kThreads) {
-      const int32_t id = __ldg(x.prefix_pages + p);
-      seen |= id < 0 || id >= x.pages;
-    }
-    if (seen) bad = 1;
-    __syncthreads();
-    if (tid == 0) a.header->share = share, a.header->prefix_bad = bad;
+    if (tid == 0) a.header->share = share;
   }
   const int64_t wid = (int64_t)blockIdx.x * kSpWarps + warp;
   const int64_t u0 = wid * share, u1 = min(total, u0 + share);
@@ -278,8 +275,10 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
   // One page for all lanes where tiles lie in one; else lanes 0-15 look up
   // the tile's keys for K, lanes 16-31 for V.
   int page = -1, offset = 0, head = 0, live_keys = 0;
+  uint32_t met = 0;  // bit i: the tile issued i tiles ago met a bad page
   auto look = [&]() {
     page = -1;
+    live_keys = 0;
     if (load.tile < load.end) {
       const int j = load.tile * kSpTile + (kWhole ? 0 : lane & 15);
       live_keys = load.keys - load.tile * kSpTile;
@@ -297,6 +296,8 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
   auto issue = [&](int stage) {
     const uint32_t dst = ring + stage * kStage + (lane / kChunks) * kRow;
     const bool good = page >= 0 && page < x.pages;
+    const bool wrong = !good && (kWhole ? 0 : lane & 15) < live_keys;
+    met = (met << 1) | (kWhole ? wrong : __any_sync(0xFFFFFFFFu, wrong));
     if (kWhole) {
       const T *ks = static_cast<const T *>(x.cache_k), *vs = static_cast<const T *>(x.cache_v);
       if (good) {
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
   uint32_t qf[NQ][DP / 16][2];
   float o[NQ][DP / 16][4];
   float m[NQ][2], l[NQ][2];
-  bool fresh = true;
+  bool fresh = true, broken = false;
   int stage = 0;
   while (now.tile < now.end) {
     issue(stage == 0 ? kStages - 1 : stage - 1);
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
         m[t][0] = m[t][1] = kNone;
         l[t][0] = l[t][1] = 0.f;
       }
-      fresh = false;
+      fresh = broken = false;
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     __syncwarp();
@@ -392,6 +393,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
       for (int t = 0; t < NQ; ++t) AtType<T>::mma(sc[t][k & 1], f, qf[t][k][0], qf[t][k][1]);
     }
     // scores in units of log2: entries 0, 1 of key lane / 4, queries 2 (lane % 4) and the next; 2, 3 of key + 8
+    broken |= (met >> (kStages - 1)) & 1;
     const int left = now.keys - now.tile * kSpTile;
     uint32_t p[NQ][2];
 #pragma unroll
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
           const int g = t * 8 + (lane & 3) * 2 + i;
           if (g < n) {
             const int64_t rec = piece * a.shape.chunk_rows + g;
-            if (lane < 4) a.own_ml[rec] = make_float2(m[t][i], l[t][i]);
+            if (lane < 4) a.own_ml[rec] = make_float2(m[t][i], broken ? kAtBadPage : l[t][i]);
             float *dst = a.own_o + rec * x.head_dim + (lane >> 2);
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) {
@@ -474,49 +476,81 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
 // the tcgen05 products), and a CTA takes one such tile over one part of the
 // prefix, so that a key is read once for 128 query rows:
 //
-//   warps 0-3   softmax: a thread owns a row; scores from tensor memory, the
-//               weights (rounded to the cache's type) back to tensor memory
-//   warps 4-5   copies: 16-byte asynchronous copies of key and value tiles
-//               into a ring of swizzled 16 KB stages, pages looked up on the way
-//   warp 6      products: S = Q K^T of the next tile ahead of O += P V of this
+//   warps 0-3   softmax: a thread owns a row; 64 scores from tensor memory,
+//               the weights (rounded to the cache's type) back over them
+//   warps 4-5   copies of tiles of 64 keys or values, half a tile each, into a
+//               ring of swizzled stages: TMA boxes where a half tile is whole
+//               pages or within one, 16-byte asynchronous copies for other page
+//               sizes and for the part-full last tile (what lies past the prefix
+//               has to be zero)
+//   warp 6      products: S = Q K^T into two buffers in turn, so that a tile's
+//               scores are there when the last tile's weights are done; O += P V
 //
-// Two CTAs share an SM, so that one's products run under the other's softmax.
-// The maximum that the weights refer to moves only when a score passes it by
-// 2^8 (the weights then stay below 2^8, within fp16): O is rescaled rarely.
+// Two CTAs share an SM, so that one's latencies pass under the other's
+// exponentials.  The maximum that the weights refer to moves only when a score
+// passes it by 2^8 (the weights then stay below 2^8, within fp16): O is
+// rescaled rarely.
 //
-// Bound by the exponentials (16 a clock and SM): 128 x 128 scores are 1024
-// clocks, their products of 64-entry heads about 256.
+// Bound by the exponentials (16 a clock and SM): 128 x 64 scores are 512
+// clocks, their products of 64-entry heads 64 each way.
 constexpr int kPrThreads = 224;
 constexpr int kPrRows = 128;
-constexpr int kPrStage = 16 * 1024;
-constexpr int kPrCols = 256;  // tensor memory: S, then P (two keys a column), then O
+constexpr int kPrKeys = 64;    // keys of a tile
+constexpr int kPrHalf = 32;    // keys that one warp copies
+constexpr int kPrCols = 256;   // tensor memory: two buffers of S (P over it, two keys a column), then O
+constexpr uint32_t kPrO = 2 * kPrKeys;
 template <int DP>
-constexpr int kPrKeys = kPrStage / (DP * 2);  // keys of a tile: 128, or 64 of 128-entry heads
+constexpr int kPrStage = kPrKeys * DP * 2;
 template <int DP>
-constexpr int kPrStages = DP == 64 ? 5 : 4;
+constexpr int kPrStages = DP == 64 ? 8 : 4;
 template <int DP>
-constexpr int kPrSharedBytes = 1024 + kPrRows * DP * 2 + kPrStages<DP> * kPrStage;
+constexpr int kPrSharedBytes = 1024 + kPrRows * DP * 2 + kPrStages<DP> * kPrStage<DP>;
 
 struct PrShared {
-  uint64_t full[5], empty[5];
-  uint64_t q_full, s_full, p_ready, pv_done, drained;
+  uint64_t full[8], empty[8];
+  uint64_t q_full, s_full[2], p_ready[2], pv_done, drained;
   uint32_t tmem;
   volatile int dead;  // a wait ran out: the records are NaN
+  volatile int bad;   // a page of this part is outside the cache
 };
 
-__device__ __forceinline__ void tmem_ld64(uint32_t addr, float (&r)[64]) {
-  uint32_t u[64];
+// The largest of 64 values.
+__device__ __forceinline__ float at_max64(const float (&s)[64]) {
+  float t[8];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) tmem_ld32(addr + 32 * i, u + 32 * i);
-  tmem_wait_ld64(u);
+  for (int i = 0; i < 8; ++i) {
+    t[i] = fmaxf(s[i], s[i + 8]);
 #pragma unroll
-  for (int i = 0; i < 64; ++i) r[i] = __uint_as_float(u[i]);
+    for (int j = 16; j < 64; j += 8) t[i] = fmaxf(t[i], s[i + j]);
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < o; ++i) t[i] = fmaxf(t[i], t[i + o]);
+  return t[0];
+}
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 at_fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)),
+        "l"(*reinterpret_cast<uint64_t *>(&c)));
+  return *reinterpret_cast<float2 *>(&d);
+}
+__device__ __forceinline__ float2 at_add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+  return *reinterpret_cast<float2 *>(&d);
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kPrThreads, 2) ms_attn_prefix_kernel(const __grid_constant__ AtArgs a) {
-  constexpr int KT = kPrKeys<DP>, kStages = kPrStages<DP>;
-  constexpr uint32_t kP = KT, kO = KT + KT / 2;  // columns of P and O
+__global__ void __launch_bounds__(kPrThreads, 2)
+    ms_attn_prefix_kernel(const __grid_constant__ AtArgs a, const __grid_constant__ CUtensorMap kmap,
+                          const __grid_constant__ CUtensorMap vmap) {
+  constexpr int KT = kPrKeys, kStages = kPrStages<DP>, kStage = kPrStage<DP>;
   extern __shared__ __align__(1024) unsigned char pr_raw[];
   __shared__ PrShared sh;
   grid_release();
@@ -541,11 +575,15 @@ __global__ void __launch_bounds__(kPrThreads, 2) ms_attn_prefix_kernel(const __g
       bar_init(&sh.empty[i], 1);
     }
     bar_init(&sh.q_full, 4);
-    bar_init(&sh.s_full, 1);
-    bar_init(&sh.p_ready, live_warps);
+    bar_init(&sh.s_full[0], 1);
+    bar_init(&sh.s_full[1], 1);
+    // one for each buffer: softmax may be two tiles ahead of the products' wait
+    bar_init(&sh.p_ready[0], live_warps);
+    bar_init(&sh.p_ready[1], live_warps);
     bar_init(&sh.pv_done, 1);
     bar_init(&sh.drained, 1);
     sh.dead = 0;
+    sh.bad = 0;
     bar_init_fence();
   }
   if (warp == 6) tmem_alloc(&sh.tmem, kPrCols);
@@ -586,88 +624,65 @@ __global__ void __launch_bounds__(kPrThreads, 2) ms_attn_prefix_kernel(const __g
     if (warp < live_warps) {
       const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
       const float kNone = __uint_as_float(0xFF800000u);
-      float m = kNone, l = 0.f;
+      const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
+      float m = kNone;
+      float2 l[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       bool ok = true;
-      for (int i = 0; i < tiles && ok; ++i) {
-        ok = !sh.dead && bar_wait(&sh.s_full, i & 1);
+      for (int i = 0; i < tiles; ++i) {
+        const uint32_t buffer = lanes + (i & 1) * KT;
+        ok = !sh.dead && bar_wait(&sh.s_full[i & 1], (i >> 1) & 1);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         tc_fence_after();
-        const int key0 = (t0 + i) * KT;
-        const bool cut = key0 + KT > keys;
         float s[64];
-        float top = kNone;
+        tmem_ld64(buffer, s);
+        const int left = keys - (t0 + i) * KT;
+        if (left < KT) {  // keys past the end leave nothing
 #pragma unroll
-        for (int half = 0; half < KT / 64; ++half) {  // the last half stays in registers
-          tmem_ld64(lanes + half * 64, s);
-          if (cut) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j)
-              if (key0 + half * 64 + j >= keys) s[j] = kNone;
-          }
-#pragma unroll
-          for (int j = 0; j < 64; ++j) top = fmaxf(top, s[j]);
+          for (int j = 0; j < 64; ++j)
+            if (j >= left) s[j] = kNone;
         }
-        top *= a.scale_log2;
+        const float top = at_max64(s) * a.scale_log2;
         const bool moved = top > m + 8.f || (m == kNone && top != kNone);
-        bool waited = i == 0;
         if (__any_sync(0xFFFFFFFFu, moved)) {
           const float next = moved ? top : m;
           const float f = m == next ? 1.f : at_exp2(m - next);
           m = next;
-          l *= f;
-          if (i > 0) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) l[j].x *= f, l[j].y *= f;
+          if (i > 0) {  // O is at rest once the last tile's product is done (the one before is: S was waited for)
             ok = __all_sync(0xFFFFFFFFu, bar_wait(&sh.pv_done, (i - 1) & 1));
             if (!ok) break;
-            waited = true;
             tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < DP; c += 32) {
-              uint32_t u[32];
-              tmem_ld32(lanes + kO + c, u);
-              tmem_wait_ld32(u);
+            for (int c = 0; c < DP; c += 16) {
+              uint32_t u[16];
+              tmem_ld16(lanes + kPrO + c, u);
+              tmem_wait_ld(u);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) u[j] = __float_as_uint(__uint_as_float(u[j]) * f);
-              tmem_st32(lanes + kO + c, u);
+              for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(__uint_as_float(u[j]) * f);
+              tmem_st16(lanes + kPrO + c, u);
             }
           }
         }
         const float base = m == kNone ? 0.f : m;
+        const float2 base2 = make_float2(-base, -base);
+        uint32_t u[32];
 #pragma unroll
-        for (int half = KT / 64 - 1; half >= 0; --half) {
-          if (half != KT / 64 - 1) {
-            tmem_ld64(lanes + half * 64, s);
-                    if (cut) {
-#pragma unroll
-              for (int j = 0; j < 64; ++j)
-                if (key0 + half * 64 + j >= keys) s[j] = kNone;
-            }
-          }
-          uint32_t u[32];
-          float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float e0 = at_exp2(fmaf(s[2 * j], a.scale_log2, -base));
-            const float e1 = at_exp2(fmaf(s[2 * j + 1], a.scale_log2, -base));
-            sum0 += e0;
-            sum1 += e1;
-            u[j] = AtType<T>::pack(e0, e1);
-          }
-          l += sum0 + sum1;
-          if (!waited) {  // the previous tile's weights are still being read
-            ok = __all_sync(0xFFFFFFFFu, bar_wait(&sh.pv_done, (i - 1) & 1));
-            waited = true;
-            tc_fence_after();
-          }
-          tmem_st32(lanes + kP + half * 32, u);
+        for (int j = 0; j < 32; ++j) {
+          const float2 e = at_fma2(make_float2(s[2 * j], s[2 * j + 1]), scale2, base2);
+          const float2 w = make_float2(at_exp2(e.x), at_exp2(e.y));
+          l[j & 1] = at_add2(l[j & 1], w);
+          u[j] = AtType<T>::pack(w.x, w.y);
         }
-        if (!ok) break;
+        tmem_st32(buffer, u);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) bar_arrive(&sh.p_ready);
+        if (lane == 0) bar_arrive(&sh.p_ready[i & 1]);
       }
-      if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(&sh.pv_done, (tiles - 1) & 1));
+      // not pv_done: its phase may be two behind here, which its parity cannot tell from done
+      if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(&sh.drained, 0)) && !sh.dead;
       if (!ok) sh.dead = 1;
       tc_fence_after();
       const int pr = r0 + r;
@@ -675,7 +690,7 @@ __global__ void __launch_bounds__(kPrThreads, 2) ms_attn_prefix_kernel(const __g
 #pragma unroll
       for (int c = 0; c < DP; c += 32) {
         uint32_t u[32];
-        tmem_ld32(lanes + kO + c, u);
+        tmem_ld32(lanes + kPrO + c, u);
         tmem_wait_ld32(u);
         if (pr < a.packed) {
 #pragma unroll
@@ -685,122 +700,162 @@ __global__ void __launch_bounds__(kPrThreads, 2) ms_attn_prefix_kernel(const __g
                   make_uint4(u[j], u[j + 1], u[j + 2], u[j + 3]);
         }
       }
-      if (pr < a.packed) a.pre_ml[rec] = ok ? make_float2(m, l) : make_float2(0.f, __uint_as_float(0x7FC00000u));
+      if (pr < a.packed) {
+        // the copies' warps set `bad` before the last products could start
+        const float sum = sh.bad ? kAtBadPage : (l[0].x + l[0].y) + (l[1].x + l[1].y);
+        a.pre_ml[rec] = ok ? make_float2(m, sum) : make_float2(0.f, __uint_as_float(0x7FC00000u));
+      }
     }
   } else if (warp < 6) {
-    constexpr int kRowsWarp = KT / 2;          // rows of a tile that one warp copies
+    constexpr int kHalf = kPrHalf;             // rows of a tile that one warp copies: a lane looks one up
     constexpr int kChunks = DP / 8;            // 16-byte chunks of a row
     constexpr int kRowsStep = 32 / kChunks;    // rows of one copy instruction
-    constexpr int kLook = kRowsWarp / 32;      // rows that a lane looks up
+    constexpr int kPanels = DP / 64;
     const int w = warp - 4, page_size = (int)x.page_size;
-    const int count = 2 * tiles;  // loads: K0, then K(i + 1) and V(i) in turn, V of the last tile
+    const int count = 2 * tiles;  // loads: K(0), then K(i + 1) and V(i) in turn, V of the last tile
     auto tile_of = [&](int n, bool &value) {
-      // n = 0: K(0); 2i + 1: K(i + 1), 2i + 2: V(i); the last one is the last tile's V
       value = n == count - 1 || (n > 0 && (n & 1) == 0);
       return n == count - 1 ? tiles - 1 : value ? (n >> 1) - 1 : (n + 1) >> 1;
     };
-    int page[kLook], offset[kLook];
+    const int box = min(kHalf, page_size);  // rows of a TMA box
+    int page = -1, offset = 0;
+    bool live_key = false;
     auto look = [&](int n) {
       bool value;
       const int tile = n < count ? tile_of(n, value) : 0;
-#pragma unroll
-      for (int i = 0; i < kLook; ++i) {
-        const int j = (t0 + tile) * KT + w * kRowsWarp + i * 32 + lane;
-        page[i] = -1;
-        if (n < count && j < keys) {
-          const int p = j / page_size;
-          offset[i] = j - p * page_size;
-          page[i] = __ldg(x.prefix_pages + p);
-        }
+      // a lane's key, or with TMA the first key of a lane's box
+      const int in = a.tma ? lane / kPanels * box : lane;
+      const int j = (t0 + tile) * KT + w * kHalf + in;
+      page = -1;
+      live_key = n < count && in < kHalf && j < keys;
+      if (live_key) {
+        const int p = j / page_size;
+        offset = j - p * page_size;
+        page = __ldg(x.prefix_pages + p);
       }
     };
     look(0);
     int stage = 0, phase = 1, sent = 0;
     bool ok = true;
-    for (int n = 0; n < count; ++n) {
+    const int chunk = lane % kChunks;
+    const bool inside = chunk * 8 < x.head_dim;
+    int n = 0;
+    for (; n < count; ++n) {
       bool value;
-      tile_of(n, value);
-      int64_t at[kLook];
-#pragma unroll
-      for (int i = 0; i < kLook; ++i)
-        at[i] = page[i] < 0 || page[i] >= x.pages ? -1
-                : value ? page[i] * x.cv_page + offset[i] * x.cv_token + h * x.cv_head
-                        : page[i] * x.ck_page + offset[i] * x.ck_token + h * x.ck_head;
+      const int tile = tile_of(n, value);
+      const bool whole = a.tma && (t0 + tile + 1) * KT <= keys;
+      if (a.tma && !whole) {  // a lane's key instead of a box's
+        const int j = (t0 + tile) * KT + w * kHalf + lane;
+        page = -1;
+        live_key = j < keys;
+        if (live_key) {
+          const int p = j / page_size;
+          offset = j - p * page_size;
+          page = __ldg(x.prefix_pages + p);
+        }
+      }
+      const bool good = page >= 0 && page < x.pages;
+      if (live_key && !good) sh.bad = 1;
+      const int page_now = page, offset_now = offset;
+      const bool live_now = live_key;
       look(n + 1);
       ok = !sh.dead && bar_wait(&sh.empty[stage], phase);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
-      const T *src = static_cast<const T *>(value ? x.cache_v : x.cache_k);
-      const uint32_t dst = smem_addr(ring) + stage * kPrStage;
-      const int chunk = lane % kChunks;
-#pragma unroll
-      for (int i = 0; i < kRowsWarp / kRowsStep; ++i) {
-        const int rr = i * kRowsStep + lane / kChunks;
-        const int64_t from = __shfl_sync(0xFFFFFFFFu, at[i * kRowsStep / 32], rr & 31);
-        const bool live = from >= 0 && chunk * 8 < x.head_dim;
-        const int row = w * kRowsWarp + rr;
-        copy16(dst + (chunk >> 3) * KT * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4),
-               src + (live ? from + chunk * 8 : 0), live);
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (n >= 2) {  // two loads in flight: the one before them has landed
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
-        fence_async_proxy();
+      unsigned char *to = ring + stage * kStage;
+      if (whole) {
+        if (lane == 0) bar_expect(&sh.full[stage], kStage / 2);
         __syncwarp();
-        if (lane == 0) bar_arrive(&sh.full[sent]);
-        if (++sent == kStages) sent = 0;
+        // a page outside the cache is outside the map: zeros
+        if (live_now) {
+          const int panel = lane % kPanels;
+          tma_load_4d(to + panel * KT * 128 + (w * kHalf + lane / kPanels * box) * 128, value ? &vmap : &kmap,
+                      &sh.full[stage], panel * 64, offset_now, h, good ? page_now : -1);
+        }
+      } else {
+        const int64_t at = !good ? -1
+                           : value ? page_now * x.cv_page + offset_now * x.cv_token + h * x.cv_head
+                                   : page_now * x.ck_page + offset_now * x.ck_token + h * x.ck_head;
+        const T *src = static_cast<const T *>(value ? x.cache_v : x.cache_k);
+        const uint32_t dst = smem_addr(to) + (chunk >> 3) * KT * 128;
+#pragma unroll
+        for (int i = 0; i < kHalf / kRowsStep; ++i) {
+          const int rr = i * kRowsStep + lane / kChunks;
+          const int64_t from = __shfl_sync(0xFFFFFFFFu, at, rr);
+          const bool live = from >= 0 && inside;
+          const int row = w * kHalf + rr;
+          copy16(dst + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), src + (live ? from + chunk * 8 : 0), live);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (a.tma) {
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+          fence_async_proxy();
+          __syncwarp();
+          if (lane == 0) bar_arrive(&sh.full[stage]);
+        } else if (n >= 2) {  // two loads in flight: the one before them has landed
+          asm volatile("cp.async.wait_group 2;" ::: "memory");
+          fence_async_proxy();
+          __syncwarp();
+          if (lane == 0) bar_arrive(&sh.full[sent]);
+          if (++sent == kStages) sent = 0;
+        }
       }
       if (++stage == kStages) stage = 0, phase ^= 1;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    fence_async_proxy();
-    __syncwarp();
-    if (ok) {
-      for (int n = count < 2 ? 0 : count - 2; n < count; ++n) {
+    if (!ok) sh.dead = 1;
+    if (!a.tma) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_async_proxy();
+      __syncwarp();
+      for (int i = 0; i < 2 && ok; ++i) {  // at least two loads: K and V of a tile
         if (lane == 0) bar_arrive(&sh.full[sent]);
         if (++sent == kStages) sent = 0;
       }
-    } else {
-      sh.dead = 1;
+    } else if (!ok) {  // copies in flight: every stage's last phase, again bounded
+      for (int i = 0; i < kStages; ++i)
+        if (i < stage || n >= kStages) bar_wait(&sh.full[i], i < stage ? phase ^ 1 : phase);
     }
   } else if (lane == 0) {
     constexpr uint32_t kQk = tc_idesc_f16<T>(KT, false), kPv = tc_idesc_f16<T>(DP, true);
-    const uint32_t q0 = smem_addr(qs), k0 = smem_addr(ring);
+    // descriptors of the first stage: later ones, and steps of a product, are added in units of 16 bytes
+    const uint64_t qd = tc_desc(smem_addr(qs), 1024, 16), kd = tc_desc(smem_addr(ring), 1024, 16),
+                   vd = tc_desc(smem_addr(ring), 1024, KT * 128);
     int stage = 0, phase = 0;
     bool ok = bar_wait(&sh.q_full, 0);
-    auto next = [&]() {
+    auto take = [&]() {  // the present stage, loaded
+      ok = ok && !sh.dead && bar_wait(&sh.full[stage], phase);
+      tc_fence_after();
+      return stage * (kStage >> 4);
+    };
+    auto give = [&]() {
+      tc_commit(&sh.empty[stage]);
       if (++stage == kStages) stage = 0, phase ^= 1;
     };
-    auto scores = [&]() {  // S of the tile in the present stage
-      ok = ok && !sh.dead && bar_wait(&sh.full[stage], phase);
+    auto scores = [&](int i) {
+      const uint64_t k = kd + take();
       if (!ok) return;
-      tc_fence_after();
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        const uint32_t panel = k >> 2, step = (k & 3) * 32;
-        tc_mma_f16(tmem, tc_desc(q0 + panel * kPrRows * 128 + step, 1024, 16),
-                   tc_desc(k0 + stage * kPrStage + panel * KT * 128 + step, 1024, 16), kQk, k > 0);
-      }
-      tc_commit(&sh.empty[stage]);
-      tc_commit(&sh.s_full);
-      next();
+      for (int d = 0; d < DP / 16; ++d)
+        tc_mma_f16(tmem + (i & 1) * KT, qd + (d >> 2) * (kPrRows * 8) + (d & 3) * 2, k + (d >> 2) * (KT * 8) + (d & 3) * 2,
+                   kQk, d > 0);
+      give();
+      tc_commit(&sh.s_full[i & 1]);
     };
-    scores();
+    scores(0);
+    if (tiles > 1) scores(1);
     for (int i = 0; i < tiles && ok; ++i) {
-      ok = !sh.dead && bar_wait(&sh.p_ready, i & 1);
+      ok = !sh.dead && bar_wait(&sh.p_ready[i & 1], (i >> 1) & 1);
+      const uint64_t v = vd + take();
       if (!ok) break;
-      tc_fence_after();
-      if (i + 1 < tiles) scores();
-      ok = ok && bar_wait(&sh.full[stage], phase);
-      if (!ok) break;
-      tc_fence_after();
 #pragma unroll
-      for (int k = 0; k < KT / 16; ++k)
-        tc_mma_f16_tmem(tmem + kO, tmem + kP + k * 8, tc_desc(k0 + stage * kPrStage + k * 2048, 1024, KT * 128), kPv,
-                        i > 0 || k > 0);
-      tc_commit(&sh.empty[stage]);
+      for (int d = 0; d < KT / 16; ++d)
+        tc_mma_f16_tmem(tmem + kPrO, tmem + (i & 1) * KT + d * 8, v + d * 128, kPv, i > 0 || d > 0);
+      give();
       tc_commit(&sh.pv_done);
-      next();
+      if (i + 2 < tiles) {  // into the buffer whose weights have just been used
+        ok = bar_wait(&sh.pv_done, i & 1);
+        if (ok) scores(i + 2);
+      }
     }
     if (!ok) sh.dead = 1;
     tc_commit(&sh.drained);
@@ -813,47 +868,39 @@ __global__ void __launch_bounds__(kPrThreads, 2) ms_attn_prefix_kernel(const __g
   if (warp == 6) tmem_free(tmem, kPrCols);
 }
 
-// Merge: one CTA per (row, query head) weighs the records of its pieces; the
+// Merge: the records of a (row, query head) weighed by one warp, or by the
+// eight of a CTA where there are too few rows to fill the GPU with such CTAs
+// (kWarps); a record's entries are loaded before its weight is known.  The
 // rows' statuses are found here.
-constexpr int kMgThreads = 128;
+constexpr int kMgThreads = 256;
 
-template <typename T>
+template <typename T, int DP, int kWarps>
 __global__ void __launch_bounds__(kMgThreads) ms_attn_merge_kernel(const __grid_constant__ AtArgs a) {
-  __shared__ float red[2 * kMgThreads / 32];
-  __shared__ int flag;
-  __shared__ float acc[kMgThreads / 32][128];
+  constexpr int kLanes = DP / 4;        // lanes of a record: four entries each
+  constexpr int kSide = 32 / kLanes;    // records side by side
+  constexpr int kBatch = 4;             // records in flight of a lane
+  constexpr int kStep = kWarps * kSide;
+  const float kNone = __uint_as_float(0xFF800000u);
+  __shared__ float4 part[kWarps > 1 ? kMgThreads / 32 : 1][kLanes];
+  __shared__ float2 part_ml[kMgThreads / 32];
   const ms_prefix_attention_args &x = a.x;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t b = blockIdx.x / a.shape.heads;
-  const int hq = (int)(blockIdx.x - b * a.shape.heads);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t out_row = kWarps > 1 ? blockIdx.x : (int64_t)blockIdx.x * (kMgThreads / 32) + warp;
+  if (out_row >= a.shape.rows * a.shape.heads) return;  // warps alone
+  const int64_t b = out_row / a.shape.heads;
+  const int hq = (int)(out_row - b * a.shape.heads);
   const int h = hq / a.shape.group, g = hq - h * a.shape.group;
   const int c = g / kAtRows, hc = h * a.shape.chunks + c;
-  const int raw = __ldg(x.lengths + b);
-  const int len = at_length(x, b);
-  if (tid == 0) flag = raw != len ? MS_ROW_BAD_LENGTH : MS_ROW_OK;
-  __syncthreads();
-  {
-    const int64_t pages = ((int64_t)len + x.page_size - 1) / x.page_size;
-    bool bad = false;
-    for (int64_t p = tid; p < pages; p += kMgThreads) {
-      const int32_t id = __ldg(x.table + b * x.table_row + p);
-      bad |= id < 0 || id >= x.pages;
-    }
-    if (bad) atomicOr(&flag, MS_ROW_BAD_PAGE);
-  }
+  const int raw = __ldg(x.lengths + b), len = at_length(x, b);
   grid_wait();
-  if (tid == 0 && a.header->prefix_bad) atomicOr(&flag, MS_ROW_BAD_PAGE);
   // the records: the row's own pieces, then the prefix's (the split kernel's or the prefix kernel's)
-  const int64_t share = a.header->share;
+  const int64_t share = a.header->share, start = a.base[b];
   int64_t own = 0, pre = 0;
   int owns = 0, pres = 0;
-  {
-    const int64_t units = sp_units(len);
-    if (units > 0) {  // the warps whose shares meet the item's tiles
-      const int64_t u = a.base[b] + hc * units, w = (u + kSpItem) / share;
-      own = (sp_item(a, b, hc) + w) * a.shape.chunk_rows + g - c * kAtRows;
-      owns = (int)((u + units - 1) / share - w) + 1;
-    }
+  if (len > 0) {  // the warps whose shares meet the item's tiles
+    const int64_t units = sp_units(len), u = start + hc * units, w = (u + kSpItem) / share;
+    own = (sp_item(a, b, hc) + w) * a.shape.chunk_rows + g - c * kAtRows;
+    owns = (int)((u + units - 1) / share - w) + 1;
   }
   const int packed_row = (int)b * a.shape.group + g;
   if (a.split_prefix) {
@@ -868,51 +915,75 @@ __global__ void __launch_bounds__(kMgThreads) ms_attn_merge_kernel(const __grid_
   const float2 *pre_ml = a.split_prefix ? a.own_ml : a.pre_ml;
   const float *pre_o = a.split_prefix ? a.own_o : a.pre_o;
   const int pieces = owns + pres;
-  auto ml_of = [&](int p) {
-    return p < owns ? a.own_ml[own + (int64_t)p * a.shape.chunk_rows] : pre_ml[pre + (p - owns) * pre_step];
-  };
-  float top = __uint_as_float(0xFF800000u);
-  for (int p = tid; p < pieces; p += kMgThreads) top = fmaxf(top, ml_of(p).x);
+  const int side = lane / kLanes, d = (lane % kLanes) * 4;
+  float top = kNone, sum = 0.f;
+  bool broken = false;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = (kWarps > 1 ? warp * kSide : 0) + side; __any_sync(0xFFFFFFFFu, p0 < pieces); p0 += kStep * kBatch) {
+    float2 ml[kBatch];
+    float4 v[kBatch];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  if (lane == 0) red[warp] = top;
-  __syncthreads();
+    for (int i = 0; i < kBatch; ++i) {
+      const int p = p0 + i * kStep;
+      ml[i] = make_float2(kNone, 0.f);
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (p < pieces) {
+        const int64_t rec = p < owns ? own + (int64_t)p * a.shape.chunk_rows : pre + (p - owns) * pre_step;
+        ml[i] = (p < owns ? a.own_ml : pre_ml)[rec];
+        if (d < x.head_dim)
+          v[i] = *reinterpret_cast<const float4 *>((p < owns ? a.own_o : pre_o) + rec * x.head_dim + d);
+      }
+    }
+    float next = top;
 #pragma unroll
-  for (int i = 0; i < kMgThreads / 32; ++i) top = fmaxf(top, red[i]);
-  const float base = top == __uint_as_float(0xFF800000u) ? 0.f : top;
-  float sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int p = warp; p < pieces; p += kMgThreads / 32) {
-    const float2 ml = ml_of(p);
-    const float w = at_exp2(ml.x - base);
-    sum += w * ml.y;
-    const float *src = p < owns ? a.own_o + (own + (int64_t)p * a.shape.chunk_rows) * x.head_dim
-                                : pre_o + (pre + (p - owns) * pre_step) * x.head_dim;
+    for (int i = 0; i < kBatch; ++i) next = fmaxf(next, ml[i].x);
+    const float f = top == next ? 1.f : at_exp2(top - next);
+    top = next;
+    sum *= f, y.x *= f, y.y *= f, y.z *= f, y.w *= f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 32 * i;
-      if (d < x.head_dim) y[i] += w * src[d];
+    for (int i = 0; i < kBatch; ++i) {
+      const float w = at_exp2(ml[i].x - (top == kNone ? 0.f : top));
+      broken |= ml[i].y == kAtBadPage;
+      sum += w * ml[i].y;
+      y.x += w * v[i].x, y.y += w * v[i].y, y.z += w * v[i].z, y.w += w * v[i].w;
     }
   }
-  if (lane == 0) red[kMgThreads / 32 + warp] = sum;
+  auto join = [&](float other, float other_sum, float4 other_y) {
+    const float next = fmaxf(top, other), base = next == kNone ? 0.f : next;
+    const float f = at_exp2(top - base), e = at_exp2(other - base);
+    top = next;
+    sum = sum * f + other_sum * e;
+    y.x = y.x * f + other_y.x * e, y.y = y.y * f + other_y.y * e;
+    y.z = y.z * f + other_y.z * e, y.w = y.w * f + other_y.w * e;
+  };
 #pragma unroll
-  for (int i = 0; i < 4; ++i) acc[warp][lane + 32 * i] = y[i];
-  __syncthreads();
-  sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < kMgThreads / 32; ++i) sum += red[kMgThreads / 32 + i];
-  const int st = flag;
-  const bool empty = st != MS_ROW_OK || sum == 0.f;
-  if (tid < x.head_dim) {
-    float v = 0.f;
-#pragma unroll
-    for (int i = 0; i < kMgThreads / 32; ++i) v += acc[i][tid];
-    T *dst = static_cast<T *>(x.out) + b * x.out_row + hq * x.out_head;
-    dst[tid] = AtType<T>::narrow(empty ? 0.f : v / sum);
+  for (int o = kLanes; o < 32; o <<= 1) {
+    const float other = __shfl_xor_sync(0xFFFFFFFFu, top, o), other_sum = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    float4 v;
+    v.x = __shfl_xor_sync(0xFFFFFFFFu, y.x, o), v.y = __shfl_xor_sync(0xFFFFFFFFu, y.y, o);
+    v.z = __shfl_xor_sync(0xFFFFFFFFu, y.z, o), v.w = __shfl_xor_sync(0xFFFFFFFFu, y.w, o);
+    join(other, other_sum, v);
   }
-  if (tid == 0) {
-    x.lse[b * a.shape.heads + hq] =
-        empty ? __uint_as_float(0xFF800000u) : (base + log2f(sum)) * 0.6931471805599453f;
-    if (hq == 0) x.status[b] = st;
+  broken = __any_sync(0xFFFFFFFFu, broken);
+  if (kWarps > 1) {
+    if (lane < kLanes) part[warp][lane] = y;
+    if (lane == 0) part_ml[warp] = make_float2(top, sum);
+    broken = __syncthreads_or(broken);
+    if (warp != 0) return;
+    for (int i = 1; i < kWarps; ++i) join(part_ml[i].x, part_ml[i].y, part[i][lane % kLanes]);
+  }
+  const int status = (raw != len ? MS_ROW_BAD_LENGTH : MS_ROW_OK) | (broken ? MS_ROW_BAD_PAGE : MS_ROW_OK);
+  const bool empty = status != MS_ROW_OK || sum == 0.f;
+  if (lane < kLanes && d < x.head_dim) {
+    T *dst = static_cast<T *>(x.out) + b * x.out_row + hq * x.out_head + d;
+    const float inv = 1.f / sum;
+    const float e[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[i] = AtType<T>::narrow(empty ? 0.f : e[i]);
+  }
+  if (lane == 0) {
+    x.lse[out_row] = empty ? kNone : (top + log2f(sum)) * 0.6931471805599453f;
+    if (hq == 0) x.status[b] = status;
   }
 }
 

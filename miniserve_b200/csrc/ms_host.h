@@ -1,7 +1,10 @@
 // Host helpers shared by the library's source files.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
+
+#include <atomic>
 
 namespace ms {
 
@@ -9,5 +12,25 @@ constexpr int kMaxDevices = 64;
 
 // Records a failed CUDA call for ms_last_cuda_error and returns MS_E_CUDA.
 __attribute__((visibility("hidden"))) int cuda_fail(cudaError_t e);
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// cuTensorMapEncodeTiled through the runtime, so that the library needs no
+// link to the driver.
+inline cudaError_t encode_tiled(EncodeTiled *fn) {
+  static std::atomic<EncodeTiled> known{nullptr};
+  *fn = known.load(std::memory_order_acquire);
+  if (*fn) return cudaSuccess;
+  void *p = nullptr;
+  cudaDriverEntryPointQueryResult found;
+  cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found);
+  if (e != cudaSuccess) return e;
+  if (found != cudaDriverEntryPointSuccess || !p) return cudaErrorNotSupported;
+  *fn = reinterpret_cast<EncodeTiled>(p);
+  known.store(*fn, std::memory_order_release);
+  return cudaSuccess;
+}
 
 }  // namespace ms

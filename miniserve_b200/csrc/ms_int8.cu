@@ -304,26 +304,6 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   if (warp == 1) tmem_free(tmem, 2 * kI8Cols);
 }
 
-typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// cuTensorMapEncodeTiled through the runtime, so that the library needs no
-// link to the driver.
-static cudaError_t encode_tiled(EncodeTiled *fn) {
-  static std::atomic<EncodeTiled> known{nullptr};
-  *fn = known.load(std::memory_order_acquire);
-  if (*fn) return cudaSuccess;
-  void *p = nullptr;
-  cudaDriverEntryPointQueryResult found;
-  cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found);
-  if (e != cudaSuccess) return e;
-  if (found != cudaDriverEntryPointSuccess || !p) return cudaErrorNotSupported;
-  *fn = reinterpret_cast<EncodeTiled>(p);
-  known.store(*fn, std::memory_order_release);
-  return cudaSuccess;
-}
-
 // A [rows, K] int8 matrix read in tiles of `box` rows and 128 bytes.
 static cudaError_t i8_map(CUtensorMap *map, const void *p, int64_t rows, int64_t K, int64_t ld, int box) {
   EncodeTiled fn;

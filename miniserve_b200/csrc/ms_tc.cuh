@@ -69,6 +69,13 @@ __device__ __forceinline__ void tma_load_2d(void *dst, const void *map, uint64_t
       "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_4d(void *dst, const void *map, uint64_t *bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(smem_addr(dst)),
+      "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
 
 // ---------------------------------------------------------------- tcgen05
 // Called by one whole warp; `cols` is a power of two, at least 32.
@@ -162,6 +169,22 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld64(uint32_t addr, float (&r)[64]) {
+  uint32_t u[64];
+  tmem_ld32(addr, u);
+  tmem_ld32(addr + 32, u + 32);
+  tmem_wait_ld64(u);
+#pragma unroll
+  for (int i = 0; i < 64; ++i) r[i] = __uint_as_float(u[i]);
 }
 
 // 16-bit floats x 16-bit floats -> fp32, M = 128: A [128, 16] K-major (shared

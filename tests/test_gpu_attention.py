@@ -146,6 +146,17 @@ def test_sharp_and_growing_scores(dtype, prefix):
 
 
 @gpu
+@pytest.mark.parametrize("B,H,Hkv,D,prefix", [(512, 14, 2, 64, 4097), (512, 14, 2, 64, 700), (300, 32, 4, 128, 1500),
+                                              (1000, 8, 1, 64, 257), (64, 64, 8, 128, 3000)])
+def test_grids_of_every_sm(B, H, Hkv, D, prefix):
+    """Two CTAs on every SM, and more than one wave of them."""
+    p = Problem(B, H, Hkv, D, prefix, [(7 * i) % 40 for i in range(B)], 16, "nhd", torch.bfloat16, seed=B)
+    p.check(*p.run(), rows=[0, 1, B // 3, B // 2, B - 2, B - 1])
+    first, second = p.run(), p.run()
+    assert torch.equal(first[0], second[0]) and bool(first[0].isfinite().all())
+
+
+@gpu
 @pytest.mark.parametrize("scale", [1e-3, 0.5, 1.0])
 def test_scale_and_strided_tensors(scale):
     p = Problem(33, 6, 2, 64, 200, [(5 * i) % 77 for i in range(33)], 16, "nhd", torch.bfloat16, seed=4)
