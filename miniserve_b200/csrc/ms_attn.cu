@@ -115,11 +115,11 @@ static cudaError_t at_split(const AtArgs &a, int dev, cudaStream_t s) {
 }
 
 // One of the caches as [pages, kv_heads, page_size, head_dim], read in boxes of
-// one page's or half a tile's tokens and 64 entries (128 bytes, swizzled).
+// one page's or a tile's tokens and 64 entries (128 bytes, swizzled).
 // False where the layout cannot be described so.
 static bool at_map(CUtensorMap *map, const ms_prefix_attention_args &x, const void *base, int64_t page, int64_t token,
                    int64_t head) {
-  const bool inner = x.page_size % 8 == 0 && (x.page_size % kPrHalf == 0 || kPrHalf % x.page_size == 0);
+  const bool inner = x.page_size % 8 == 0 && (x.page_size % kPrKeys == 0 || kPrKeys % x.page_size == 0);
   EncodeTiled fn;
   if (!inner || encode_tiled(&fn) != cudaSuccess) return false;
   const cuuint64_t dims[4] = {(cuuint64_t)x.head_dim, (cuuint64_t)x.page_size, (cuuint64_t)x.kv_heads,
@@ -129,7 +129,7 @@ static bool at_map(CUtensorMap *map, const ms_prefix_attention_args &x, const vo
   const cuuint64_t strides[3] = {(cuuint64_t)(x.page_size > 1 ? token : row) * 2,
                                  (cuuint64_t)(x.kv_heads > 1 ? head : row) * 2,
                                  (cuuint64_t)(x.pages > 1 ? page : row) * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)(x.page_size < kPrHalf ? x.page_size : kPrHalf), 1, 1};
+  const cuuint32_t box[4] = {64, (cuuint32_t)(x.page_size < kPrKeys ? x.page_size : kPrKeys), 1, 1};
   const cuuint32_t unit[4] = {1, 1, 1, 1};
   return fn(map, x.dtype == MS_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
             const_cast<void *>(base), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -214,6 +214,9 @@ int ms_prefix_attention(const ms_prefix_attention_args *args, ms_stream_t stream
   a.pre_ml = reinterpret_cast<float2 *>(w + p.pre_ml);
   a.scale_log2 = x.scale * 1.4426950408889634f;
   a.q_wide = ((x.q_row | x.q_head) & 7) == 0 && (reinterpret_cast<uintptr_t>(x.q) & 15) == 0;
+  a.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (x.page_size == 1ll << i) a.page_shift = i;
   a.merge_wide = x.rows * x.heads <= 8 * ms::at_sms(dev);
   a.narrow = p.shape.chunk_rows <= 8;
   a.whole = x.page_size % ms::kSpTile == 0;

@@ -55,7 +55,8 @@ struct AtArgs {
   int pre_splits;    // parts of the prefix that the prefix kernel takes; 0 where it does not run
   int pre_tiles;     // its query tiles of one key head
   int q_wide;        // q's heads start 16-byte aligned
-  int tma;           // the cache can be read in boxes of half a tile, or of pages that divide it
+  int tma;           // the cache can be read in boxes of a tile, or of pages that divide it
+  int page_shift;    // log2 of the page size, or -1
   int merge_wide;    // the merge gives each output a CTA
   int narrow;        // at most 8 query rows an item
   int whole;         // page_size is a multiple of kSpTile: a tile lies in one page
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
       const int j = load.tile * kSpTile + (kWhole ? 0 : lane & 15);
       live_keys = load.keys - load.tile * kSpTile;
       if (j < load.keys) {
-        const int p = j / page_size;
+        const int p = a.page_shift >= 0 ? j >> a.page_shift : j / page_size;
         offset = j - p * page_size;
         page = __ldg(load.b < 0 ? x.prefix_pages + p : x.table + load.b * x.table_row + p);
       }
@@ -478,11 +479,11 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
 //
 //   warps 0-3   softmax: a thread owns a row; 64 scores from tensor memory,
 //               the weights (rounded to the cache's type) back over them
-//   warps 4-5   copies of tiles of 64 keys or values, half a tile each, into a
-//               ring of swizzled stages: TMA boxes where a half tile is whole
-//               pages or within one, 16-byte asynchronous copies for other page
-//               sizes and for the part-full last tile (what lies past the prefix
-//               has to be zero)
+//   warps 4-5   copies of tiles of 64 keys (warp 4) and of their values (warp
+//               5) into a ring of swizzled stages each: TMA boxes where a tile is
+//               whole pages or within one, 16-byte asynchronous copies for other
+//               page sizes and for the part-full last tile (what lies past the
+//               prefix has to be zero)
 //   warp 6      products: S = Q K^T into two buffers in turn, so that a tile's
 //               scores are there when the last tile's weights are done; O += P V
 //
@@ -496,18 +497,17 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
 constexpr int kPrThreads = 224;
 constexpr int kPrRows = 128;
 constexpr int kPrKeys = 64;    // keys of a tile
-constexpr int kPrHalf = 32;    // keys that one warp copies
 constexpr int kPrCols = 256;   // tensor memory: two buffers of S (P over it, two keys a column), then O
 constexpr uint32_t kPrO = 2 * kPrKeys;
 template <int DP>
 constexpr int kPrStage = kPrKeys * DP * 2;
 template <int DP>
-constexpr int kPrStages = DP == 64 ? 8 : 4;
+constexpr int kPrStages = DP == 64 ? 4 : 2;  // of keys, and of values
 template <int DP>
-constexpr int kPrSharedBytes = 1024 + kPrRows * DP * 2 + kPrStages<DP> * kPrStage<DP>;
+constexpr int kPrSharedBytes = 1024 + kPrRows * DP * 2 + 2 * kPrStages<DP> * kPrStage<DP>;
 
 struct PrShared {
-  uint64_t full[8], empty[8];
+  uint64_t full[2][4], empty[2][4];  // of keys, of values
   uint64_t q_full, s_full[2], p_ready[2], pv_done, drained;
   uint32_t tmem;
   volatile int dead;  // a wait ran out: the records are NaN
@@ -570,9 +570,9 @@ __global__ void __launch_bounds__(kPrThreads, 2)
   const int live_rows = min(kPrRows, a.packed - r0);
   const int live_warps = (live_rows + 31) / 32;
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      bar_init(&sh.full[i], 2);
-      bar_init(&sh.empty[i], 1);
+    for (int i = 0; i < 2 * kStages; ++i) {
+      bar_init(&sh.full[i / kStages][i % kStages], 1);
+      bar_init(&sh.empty[i / kStages][i % kStages], 1);
     }
     bar_init(&sh.q_full, 4);
     bar_init(&sh.s_full[0], 1);
@@ -707,151 +707,129 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       }
     }
   } else if (warp < 6) {
-    constexpr int kHalf = kPrHalf;             // rows of a tile that one warp copies: a lane looks one up
     constexpr int kChunks = DP / 8;            // 16-byte chunks of a row
     constexpr int kRowsStep = 32 / kChunks;    // rows of one copy instruction
     constexpr int kPanels = DP / 64;
-    const int w = warp - 4, page_size = (int)x.page_size;
-    const int count = 2 * tiles;  // loads: K(0), then K(i + 1) and V(i) in turn, V of the last tile
-    auto tile_of = [&](int n, bool &value) {
-      value = n == count - 1 || (n > 0 && (n & 1) == 0);
-      return n == count - 1 ? tiles - 1 : value ? (n >> 1) - 1 : (n + 1) >> 1;
+    const bool value = warp == 5;
+    const int page_size = (int)x.page_size;
+    uint64_t *full = sh.full[value], *empty = sh.empty[value];
+    unsigned char *mine = ring + value * kStages * kStage;
+    auto find = [&](int j, int &page, int &offset) {
+      const int p = a.page_shift >= 0 ? j >> a.page_shift : j / page_size;
+      offset = j - p * page_size;
+      page = __ldg(x.prefix_pages + p);
     };
-    const int box = min(kHalf, page_size);  // rows of a TMA box
-    int page = -1, offset = 0;
-    bool live_key = false;
-    auto look = [&](int n) {
-      bool value;
-      const int tile = n < count ? tile_of(n, value) : 0;
-      // a lane's key, or with TMA the first key of a lane's box
-      const int in = a.tma ? lane / kPanels * box : lane;
-      const int j = (t0 + tile) * KT + w * kHalf + in;
-      page = -1;
-      live_key = n < count && in < kHalf && j < keys;
-      if (live_key) {
-        const int p = j / page_size;
-        offset = j - p * page_size;
-        page = __ldg(x.prefix_pages + p);
-      }
-    };
-    look(0);
-    int stage = 0, phase = 1, sent = 0;
+    int stage = 0, phase = 1, i = 0;
     bool ok = true;
+    if (a.tma) {  // tiles that lie in the prefix as a whole
+      const int box = min(KT, page_size);  // rows of a TMA box: a lane's panel of one
+      const int row = lane / kPanels * box, panel = lane % kPanels;
+      const CUtensorMap *map = value ? &vmap : &kmap;
+      const int last = min(tiles, keys / KT - t0);
+      int page = 0, offset = 0;
+      if (row < KT && last > 0) find(t0 * KT + row, page, offset);
+      for (; i < last; ++i) {
+        const int page_now = page, offset_now = offset;
+        if (row < KT && i + 1 < last) find((t0 + i + 1) * KT + row, page, offset);
+        ok = !sh.dead && bar_wait(&empty[stage], phase);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        if (lane == 0) bar_expect(&full[stage], kStage);
+        __syncwarp();
+        if (row < KT) {  // a page outside the cache is outside the map: zeros
+          const bool good = page_now >= 0 && page_now < x.pages;
+          if (!good) sh.bad = 1;
+          tma_load_4d(mine + stage * kStage + panel * KT * 128 + row * 128, map, &full[stage], panel * 64, offset_now, h,
+                      good ? page_now : -1);
+        }
+        if (++stage == kStages) stage = 0, phase ^= 1;
+      }
+    }
+    // the rest: a copy's tile is announced once the next one's has been issued
+    const T *cache = static_cast<const T *>(value ? x.cache_v : x.cache_k);
+    const int64_t step_page = value ? x.cv_page : x.ck_page, step_token = value ? x.cv_token : x.ck_token,
+                  step_head = value ? x.cv_head : x.ck_head;
     const int chunk = lane % kChunks;
     const bool inside = chunk * 8 < x.head_dim;
-    int n = 0;
-    for (; n < count; ++n) {
-      bool value;
-      const int tile = tile_of(n, value);
-      const bool whole = a.tma && (t0 + tile + 1) * KT <= keys;
-      if (a.tma && !whole) {  // a lane's key instead of a box's
-        const int j = (t0 + tile) * KT + w * kHalf + lane;
-        page = -1;
-        live_key = j < keys;
-        if (live_key) {
-          const int p = j / page_size;
-          offset = j - p * page_size;
-          page = __ldg(x.prefix_pages + p);
+    int waiting = -1;  // stage of the tile issued last
+    for (; i < tiles && ok; ++i) {
+      int64_t at[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {  // a lane looks up two keys
+        const int j = (t0 + i) * KT + k * 32 + lane;
+        at[k] = -1;
+        if (j < keys) {
+          int page, offset;
+          find(j, page, offset);
+          if (page >= 0 && page < x.pages) at[k] = page * step_page + offset * step_token + h * step_head;
+          else sh.bad = 1;
         }
       }
-      const bool good = page >= 0 && page < x.pages;
-      if (live_key && !good) sh.bad = 1;
-      const int page_now = page, offset_now = offset;
-      const bool live_now = live_key;
-      look(n + 1);
-      ok = !sh.dead && bar_wait(&sh.empty[stage], phase);
+      ok = !sh.dead && bar_wait(&empty[stage], phase);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
-      unsigned char *to = ring + stage * kStage;
-      if (whole) {
-        if (lane == 0) bar_expect(&sh.full[stage], kStage / 2);
-        __syncwarp();
-        // a page outside the cache is outside the map: zeros
-        if (live_now) {
-          const int panel = lane % kPanels;
-          tma_load_4d(to + panel * KT * 128 + (w * kHalf + lane / kPanels * box) * 128, value ? &vmap : &kmap,
-                      &sh.full[stage], panel * 64, offset_now, h, good ? page_now : -1);
-        }
-      } else {
-        const int64_t at = !good ? -1
-                           : value ? page_now * x.cv_page + offset_now * x.cv_token + h * x.cv_head
-                                   : page_now * x.ck_page + offset_now * x.ck_token + h * x.ck_head;
-        const T *src = static_cast<const T *>(value ? x.cache_v : x.cache_k);
-        const uint32_t dst = smem_addr(to) + (chunk >> 3) * KT * 128;
+      const uint32_t dst = smem_addr(mine) + stage * kStage + (chunk >> 3) * KT * 128;
 #pragma unroll
-        for (int i = 0; i < kHalf / kRowsStep; ++i) {
-          const int rr = i * kRowsStep + lane / kChunks;
-          const int64_t from = __shfl_sync(0xFFFFFFFFu, at, rr);
-          const bool live = from >= 0 && inside;
-          const int row = w * kHalf + rr;
-          copy16(dst + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), src + (live ? from + chunk * 8 : 0), live);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (a.tma) {
-          asm volatile("cp.async.wait_group 0;" ::: "memory");
-          fence_async_proxy();
-          __syncwarp();
-          if (lane == 0) bar_arrive(&sh.full[stage]);
-        } else if (n >= 2) {  // two loads in flight: the one before them has landed
-          asm volatile("cp.async.wait_group 2;" ::: "memory");
-          fence_async_proxy();
-          __syncwarp();
-          if (lane == 0) bar_arrive(&sh.full[sent]);
-          if (++sent == kStages) sent = 0;
-        }
+      for (int k = 0; k < KT / kRowsStep; ++k) {
+        const int row = k * kRowsStep + lane / kChunks;
+        const int64_t from = __shfl_sync(0xFFFFFFFFu, at[k * kRowsStep / 32], row & 31);
+        const bool live = from >= 0 && inside;
+        copy16(dst + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), cache + (live ? from + chunk * 8 : 0), live);
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (waiting >= 0) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&full[waiting]);
+      }
+      waiting = stage;
       if (++stage == kStages) stage = 0, phase ^= 1;
     }
-    if (!ok) sh.dead = 1;
-    if (!a.tma) {
-      asm volatile("cp.async.wait_all;" ::: "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (waiting >= 0) {
       fence_async_proxy();
       __syncwarp();
-      for (int i = 0; i < 2 && ok; ++i) {  // at least two loads: K and V of a tile
-        if (lane == 0) bar_arrive(&sh.full[sent]);
-        if (++sent == kStages) sent = 0;
-      }
-    } else if (!ok) {  // copies in flight: every stage's last phase, again bounded
-      for (int i = 0; i < kStages; ++i)
-        if (i < stage || n >= kStages) bar_wait(&sh.full[i], i < stage ? phase ^ 1 : phase);
+      if (lane == 0) bar_arrive(&full[waiting]);
+    }
+    if (!ok) {  // boxes in flight: every stage's last phase, again bounded
+      sh.dead = 1;
+      for (int k = 0; k < kStages; ++k)
+        if (k < stage || i >= kStages) bar_wait(&full[k], k < stage ? phase ^ 1 : phase);
     }
   } else if (lane == 0) {
     constexpr uint32_t kQk = tc_idesc_f16<T>(KT, false), kPv = tc_idesc_f16<T>(DP, true);
     // descriptors of the first stage: later ones, and steps of a product, are added in units of 16 bytes
     const uint64_t qd = tc_desc(smem_addr(qs), 1024, 16), kd = tc_desc(smem_addr(ring), 1024, 16),
-                   vd = tc_desc(smem_addr(ring), 1024, KT * 128);
-    int stage = 0, phase = 0;
+                   vd = tc_desc(smem_addr(ring + kStages * kStage), 1024, KT * 128);
     bool ok = bar_wait(&sh.q_full, 0);
-    auto take = [&]() {  // the present stage, loaded
-      ok = ok && !sh.dead && bar_wait(&sh.full[stage], phase);
-      tc_fence_after();
-      return stage * (kStage >> 4);
-    };
-    auto give = [&]() {
-      tc_commit(&sh.empty[stage]);
-      if (++stage == kStages) stage = 0, phase ^= 1;
-    };
     auto scores = [&](int i) {
-      const uint64_t k = kd + take();
+      const int stage = i % kStages;
+      ok = ok && !sh.dead && bar_wait(&sh.full[0][stage], (i / kStages) & 1);
       if (!ok) return;
+      tc_fence_after();
+      const uint64_t k = kd + stage * (kStage >> 4);
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d)
         tc_mma_f16(tmem + (i & 1) * KT, qd + (d >> 2) * (kPrRows * 8) + (d & 3) * 2, k + (d >> 2) * (KT * 8) + (d & 3) * 2,
                    kQk, d > 0);
-      give();
       tc_commit(&sh.s_full[i & 1]);
+      tc_commit(&sh.empty[0][stage]);
     };
     scores(0);
     if (tiles > 1) scores(1);
     for (int i = 0; i < tiles && ok; ++i) {
-      ok = !sh.dead && bar_wait(&sh.p_ready[i & 1], (i >> 1) & 1);
-      const uint64_t v = vd + take();
+      const int stage = i % kStages;
+      ok = !sh.dead && bar_wait(&sh.full[1][stage], (i / kStages) & 1) &&
+           bar_wait(&sh.p_ready[i & 1], (i >> 1) & 1);
       if (!ok) break;
+      tc_fence_after();
+      const uint64_t v = vd + stage * (kStage >> 4);
 #pragma unroll
       for (int d = 0; d < KT / 16; ++d)
         tc_mma_f16_tmem(tmem + kPrO, tmem + (i & 1) * KT + d * 8, v + d * 128, kPv, i > 0 || d > 0);
-      give();
       tc_commit(&sh.pv_done);
+      tc_commit(&sh.empty[1][stage]);
       if (i + 2 < tiles) {  // into the buffer whose weights have just been used
         ok = bar_wait(&sh.pv_done, i & 1);
         if (ok) scores(i + 2);
