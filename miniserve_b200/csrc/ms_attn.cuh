@@ -630,8 +630,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       bool ok = true;
       for (int i = 0; i < tiles; ++i) {
         const uint32_t buffer = lanes + (i & 1) * KT;
-        ok = !sh.dead && bar_wait(&sh.s_full[i & 1], (i >> 1) & 1);
-        ok = __all_sync(0xFFFFFFFFu, ok);
+        ok = bar_wait_warp(&sh.s_full[i & 1], (i >> 1) & 1, sh.dead);
         if (!ok) break;
         tc_fence_after();
         float s[64];
@@ -651,7 +650,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
 #pragma unroll
           for (int j = 0; j < 2; ++j) l[j].x *= f, l[j].y *= f;
           if (i > 0) {  // O is at rest once the last tile's product is done (the one before is: S was waited for)
-            ok = __all_sync(0xFFFFFFFFu, bar_wait(&sh.pv_done, (i - 1) & 1));
+            ok = bar_wait_warp(&sh.pv_done, (i - 1) & 1, sh.dead);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -682,7 +681,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
         if (lane == 0) bar_arrive(&sh.p_ready[i & 1]);
       }
       // not pv_done: its phase may be two behind here, which its parity cannot tell from done
-      if (ok) ok = __all_sync(0xFFFFFFFFu, bar_wait(&sh.drained, 0)) && !sh.dead;
+      if (ok) ok = bar_wait_warp(&sh.drained, 0, sh.dead) && !sh.dead;
       if (!ok) sh.dead = 1;
       tc_fence_after();
       const int pr = r0 + r;
@@ -731,8 +730,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       for (; i < last; ++i) {
         const int page_now = page, offset_now = offset;
         if (row < KT && i + 1 < last) find((t0 + i + 1) * KT + row, page, offset);
-        ok = !sh.dead && bar_wait(&empty[stage], phase);
-        ok = __all_sync(0xFFFFFFFFu, ok);
+        ok = bar_wait_warp(&empty[stage], phase, sh.dead);
         if (!ok) break;
         if (lane == 0) bar_expect(&full[stage], kStage);
         __syncwarp();
@@ -765,8 +763,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
           else sh.bad = 1;
         }
       }
-      ok = !sh.dead && bar_wait(&empty[stage], phase);
-      ok = __all_sync(0xFFFFFFFFu, ok);
+      ok = bar_wait_warp(&empty[stage], phase, sh.dead);
       if (!ok) break;
       const uint32_t dst = smem_addr(mine) + stage * kStage + (chunk >> 3) * KT * 128;
 #pragma unroll
@@ -797,46 +794,47 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       for (int k = 0; k < kStages; ++k)
         if (k < stage || i >= kStages) bar_wait(&full[k], k < stage ? phase ^ 1 : phase);
     }
-  } else if (lane == 0) {
+  } else {
+    const uint32_t leader = tc_leader();
     constexpr uint32_t kQk = tc_idesc_f16<T>(KT, false), kPv = tc_idesc_f16<T>(DP, true);
     // descriptors of the first stage: later ones, and steps of a product, are added in units of 16 bytes
     const uint64_t qd = tc_desc(smem_addr(qs), 1024, 16), kd = tc_desc(smem_addr(ring), 1024, 16),
                    vd = tc_desc(smem_addr(ring + kStages * kStage), 1024, KT * 128);
-    bool ok = bar_wait(&sh.q_full, 0);
+    bool ok = bar_wait_warp(&sh.q_full, 0, sh.dead);
     auto scores = [&](int i) {
       const int stage = i % kStages;
-      ok = ok && !sh.dead && bar_wait(&sh.full[0][stage], (i / kStages) & 1);
+      ok = ok && bar_wait_warp(&sh.full[0][stage], (i / kStages) & 1, sh.dead);
       if (!ok) return;
       tc_fence_after();
       const uint64_t k = kd + stage * (kStage >> 4);
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d)
-        tc_mma_f16(tmem + (i & 1) * KT, qd + (d >> 2) * (kPrRows * 8) + (d & 3) * 2, k + (d >> 2) * (KT * 8) + (d & 3) * 2,
+        tc_mma_f16(leader, tmem + (i & 1) * KT, qd + (d >> 2) * (kPrRows * 8) + (d & 3) * 2, k + (d >> 2) * (KT * 8) + (d & 3) * 2,
                    kQk, d > 0);
-      tc_commit(&sh.s_full[i & 1]);
-      tc_commit(&sh.empty[0][stage]);
+      tc_commit(leader, &sh.s_full[i & 1]);
+      tc_commit(leader, &sh.empty[0][stage]);
     };
     scores(0);
     if (tiles > 1) scores(1);
     for (int i = 0; i < tiles && ok; ++i) {
       const int stage = i % kStages;
-      ok = !sh.dead && bar_wait(&sh.full[1][stage], (i / kStages) & 1) &&
-           bar_wait(&sh.p_ready[i & 1], (i >> 1) & 1);
+      ok = bar_wait_warp(&sh.full[1][stage], (i / kStages) & 1, sh.dead) &&
+           bar_wait_warp(&sh.p_ready[i & 1], (i >> 1) & 1, sh.dead);
       if (!ok) break;
       tc_fence_after();
       const uint64_t v = vd + stage * (kStage >> 4);
 #pragma unroll
       for (int d = 0; d < KT / 16; ++d)
-        tc_mma_f16_tmem(tmem + kPrO, tmem + (i & 1) * KT + d * 8, v + d * 128, kPv, i > 0 || d > 0);
-      tc_commit(&sh.pv_done);
-      tc_commit(&sh.empty[1][stage]);
+        tc_mma_f16_tmem(leader, tmem + kPrO, tmem + (i & 1) * KT + d * 8, v + d * 128, kPv, i > 0 || d > 0);
+      tc_commit(leader, &sh.pv_done);
+      tc_commit(leader, &sh.empty[1][stage]);
       if (i + 2 < tiles) {  // into the buffer whose weights have just been used
-        ok = bar_wait(&sh.pv_done, i & 1);
+        ok = bar_wait_warp(&sh.pv_done, i & 1, sh.dead);
         if (ok) scores(i + 2);
       }
     }
     if (!ok) sh.dead = 1;
-    tc_commit(&sh.drained);
+    tc_commit(leader, &sh.drained);
     bar_wait(&sh.drained, 0);  // products in flight end before tensor memory is freed
   }
   __syncwarp();

@@ -232,32 +232,31 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = tc_idesc_i8(a.bn);
-      int stage = 0, phase = 0, n = 0;
-      for (int64_t tile = blockIdx.x; tile < tiles && !sh.dead; tile += gridDim.x, ++n) {
-        const int acc = n & 1;
-        if (!bar_wait(&sh.acc_empty[acc], ((n >> 1) & 1) ^ 1)) sh.dead = 1;
+    const uint32_t leader = tc_leader();
+    const uint32_t idesc = tc_idesc_i8(a.bn);
+    int stage = 0, phase = 0, n = 0;
+    bool ok = true;
+    for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++n) {
+      const int acc = n & 1;
+      ok = bar_wait_warp(&sh.acc_empty[acc], ((n >> 1) & 1) ^ 1, sh.dead);
+      tc_fence_after();
+      for (int k = 0; k < steps && ok; ++k) {
+        ok = bar_wait_warp(&sh.full[stage], phase, sh.dead);
+        if (!ok) break;
         tc_fence_after();
-        for (int k = 0; k < steps && !sh.dead; ++k) {
-          if (!bar_wait(&sh.full[stage], phase)) {
-            sh.dead = 1;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t st = smem_addr(ring + stage * (wbytes + xbytes));
-          const uint64_t wd = tc_desc(st, 1024, 16), xd = tc_desc(st + wbytes, 1024, 16);
+        const uint32_t st = smem_addr(ring + stage * (wbytes + xbytes));
+        const uint64_t wd = tc_desc(st, 1024, 16), xd = tc_desc(st + wbytes, 1024, 16);
 #pragma unroll
-          for (int j = 0; j < kI8Step / 32; ++j)
-            tc_mma_i8(tmem + acc * kI8Cols, wd + 2 * j, xd + 2 * j, idesc, k > 0 || j > 0);
-          tc_commit(&sh.empty[stage]);
-          if (++stage == a.stages) stage = 0, phase ^= 1;
-        }
-        tc_commit(&sh.acc_full[acc]);
+        for (int j = 0; j < kI8Step / 32; ++j)
+          tc_mma_i8(leader, tmem + acc * kI8Cols, wd + 2 * j, xd + 2 * j, idesc, k > 0 || j > 0);
+        tc_commit(leader, &sh.empty[stage]);
+        if (++stage == a.stages) stage = 0, phase ^= 1;
       }
-      tc_commit(&sh.drained);
-      bar_wait(&sh.drained, 0);  // products in flight end before tensor memory is freed
+      if (ok) tc_commit(leader, &sh.acc_full[acc]);
     }
+    if (!ok) sh.dead = 1;
+    tc_commit(leader, &sh.drained);
+    bar_wait(&sh.drained, 0);  // products in flight end before tensor memory is freed
   } else {
     const int quad = warp & 3;
     const int et = threadIdx.x - 64;

@@ -53,6 +53,11 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity) {
   const uint32_t b = smem_addr(bar);
   return bar_try(b, parity) || bar_wait_slow(b, parity);
 }
+// For a whole warp: false, for all its lanes, where the wait ran out or another
+// warp's had.
+__device__ __forceinline__ bool bar_wait_warp(uint64_t *bar, uint32_t parity, const volatile int &dead) {
+  return __all_sync(0xFFFFFFFFu, !dead && bar_wait(bar, parity));
+}
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -89,10 +94,21 @@ __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// The barrier is arrived at when every product this thread issued has finished.
-__device__ __forceinline__ void tc_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-               : "memory");
+// The lane that issues a warp's products.  The whole warp walks through the
+// code around them, so that descriptors and addresses stay in uniform
+// registers; inside one lane's branch every product costs moves of them.
+__device__ __forceinline__ uint32_t tc_leader() {
+  uint32_t one;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xFFFFFFFF; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+  return one;
+}
+// The barrier is arrived at when every product the leader issued has finished.
+__device__ __forceinline__ void tc_commit(uint32_t leader, uint64_t *bar) {
+  asm volatile(
+      "{ .reg .pred q; setp.ne.u32 q, %1, 0; @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 "
+      "[%0]; }" ::"r"(smem_addr(bar)),
+      "r"(leader)
+      : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -108,10 +124,10 @@ __device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t stride, uint
 __device__ __forceinline__ uint32_t tc_idesc_i8(int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void tc_mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void tc_mma_i8(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p; }" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{ .reg .pred p, q; setp.ne.u32 p, %4, 0; setp.ne.u32 q, %5, 0; @q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p; }" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(leader)
       : "memory");
 }
 
@@ -200,16 +216,16 @@ template <>
 __device__ __forceinline__ constexpr uint32_t tc_idesc_f16<__half>(int n, bool transposed) {
   return (1u << 4) | ((transposed ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void tc_mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void tc_mma_f16(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{ .reg .pred p, q; setp.ne.u32 p, %4, 0; setp.ne.u32 q, %5, 0; @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void tc_mma_f16_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void tc_mma_f16_tmem(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{ .reg .pred p, q; setp.ne.u32 p, %4, 0; setp.ne.u32 q, %5, 0; @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(leader)
       : "memory");
 }
 
