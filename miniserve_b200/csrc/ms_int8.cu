@@ -140,7 +140,7 @@ struct I8Shared {
   uint64_t acc_full[2], acc_empty[2], drained;
   uint32_t tmem;
   volatile int dead;  // a wait ran out: the rest of the outputs are NaN
-  float xs[2][kI8Cols];
+  alignas(16) float xs[2][kI8Cols];
 };
 
 struct I8Args {
@@ -150,19 +150,30 @@ struct I8Args {
   int M, N, K;
   int bn;      // tokens of a tile: a multiple of 16, at most 256
   int stages;
-  int out_dtype;
   int after_quantize;  // launched with the quantisation as its programmatic dependency
 };
 
-__device__ __forceinline__ void i8_store(void *out, int dtype, int64_t at, float y) {
-  if (dtype == MS_DTYPE_F32)
-    static_cast<float *>(out)[at] = y;
-  else if (dtype == MS_DTYPE_BF16)
-    static_cast<__nv_bfloat16 *>(out)[at] = __float2bfloat16_rn(y);
-  else
-    static_cast<__half *>(out)[at] = __float2half_rn(y);
+__device__ __forceinline__ void i8_store(float *p, float y) { *p = y; }
+__device__ __forceinline__ void i8_store(__nv_bfloat16 *p, float y) { *p = __float2bfloat16_rn(y); }
+__device__ __forceinline__ void i8_store(__half *p, float y) { *p = __float2half_rn(y); }
+
+// 16 columns (tokens) of a lane's channel, scaled and stored ldo apart.
+template <typename T, bool kAll>
+__device__ __forceinline__ void i8_columns(const uint32_t (&r)[16], const float *xs, float ws, float bias, T *out,
+                                           int64_t ldo, int count) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const float4 s = *reinterpret_cast<const float4 *>(xs + i);
+    const float e[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (kAll || i + j < count) i8_store(out, fmaf((float)(int)r[i + j], e[j] * ws, bias));
+      out += ldo;
+    }
+  }
 }
 
+template <typename T>
 __global__ void __launch_bounds__(kI8Threads, 1)
     ms_int8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                    const __grid_constant__ I8Args a) {
@@ -275,21 +286,28 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       __syncwarp();
       tc_fence_after();
       const bool dead = sh.dead != 0;
-      for (int c = 0; c < count; c += 16) {
-        uint32_t r[16];
-        tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + acc * kI8Cols + c, r);
-        tmem_wait_ld(r);
-        if (ch < a.N) {
+      T *out = static_cast<T *>(a.out) + (int64_t)t0 * a.ldo + ch;
+      const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + acc * kI8Cols;
+      const float scale = dead ? __uint_as_float(0x7FC00000u) : ws;
+      uint32_t r[2][16];  // the next 16 columns are read under the stores of these
+      tmem_ld16(from, r[0]);
+#pragma unroll 1
+      for (int c = 0; c < count; c += 32) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (c + i < count) {
-              float y = (float)(int)r[i] * (sh.xs[acc][c + i] * ws) + bias;
-              if (dead) y = __uint_as_float(0x7FC00000u);
-              i8_store(a.out, a.out_dtype, (int64_t)(t0 + c + i) * a.ldo + ch, y);
-            }
+        for (int k = 0; k < 2; ++k) {
+          const int at = c + 16 * k;
+          if (at >= count) break;
+          tmem_wait_ld(r[k]);
+          if (at + 16 < count) tmem_ld16(from + at + 16, r[k ^ 1]);
+          if (ch < a.N) {
+            if (at + 16 <= count)
+              i8_columns<T, true>(r[k], sh.xs[acc] + at, scale, bias, out, a.ldo, 16);
+            else
+              i8_columns<T, false>(r[k], sh.xs[acc] + at, scale, bias, out, a.ldo, count - at);
           }
+          __syncwarp();
+          out += 16 * a.ldo;
         }
-        __syncwarp();
       }
       tc_fence_before();
       __syncwarp();
@@ -318,22 +336,23 @@ static cudaError_t i8_map(CUtensorMap *map, const void *p, int64_t rows, int64_t
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-static cudaError_t launch_int8(const int8_t *xq, int64_t ldx, const float *x_scale, int64_t M, const int8_t *wq,
-                               int64_t ldw, const float *w_scale, int64_t N, int64_t K, const float *bias, void *out,
-                               int out_dtype, int64_t ldo, bool after_quantize, cudaStream_t s) {
+template <typename T>
+static cudaError_t launch_int8_as(const int8_t *xq, int64_t ldx, const float *x_scale, int64_t M, const int8_t *wq,
+                                  int64_t ldw, const float *w_scale, int64_t N, int64_t K, const float *bias,
+                                  void *out, int64_t ldo, bool after_quantize, cudaStream_t s) {
   static std::atomic<int> ready[kMaxDevices];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(ms_int8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8Ring + 1024);
+    e = cudaFuncSetAttribute(ms_int8_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8Ring + 1024);
     if (e != cudaSuccess) return e;
     ready[dev].store(1, std::memory_order_release);
   }
   I8Args a{};
   a.x_scale = x_scale, a.w_scale = w_scale, a.bias = bias, a.out = out, a.ldo = ldo;
-  a.M = (int)M, a.N = (int)N, a.K = (int)K, a.out_dtype = out_dtype, a.after_quantize = after_quantize;
+  a.M = (int)M, a.N = (int)N, a.K = (int)K, a.after_quantize = after_quantize;
   // equal token tiles of at most 256, rounded up to the 16 that an N of the product allows
   const int64_t parts = (M + kI8Cols - 1) / kI8Cols;
   a.bn = (int)(((M + parts - 1) / parts + 15) / 16 * 16);
@@ -356,8 +375,17 @@ static cudaError_t launch_int8(const int8_t *xq, int64_t ldx, const float *x_sca
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = after_quantize ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, ms_int8_kernel, wmap, xmap, a);
+  e = cudaLaunchKernelEx(&cfg, ms_int8_kernel<T>, wmap, xmap, a);
   return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+static cudaError_t launch_int8(const int8_t *xq, int64_t ldx, const float *x_scale, int64_t M, const int8_t *wq,
+                               int64_t ldw, const float *w_scale, int64_t N, int64_t K, const float *bias, void *out,
+                               int out_dtype, int64_t ldo, bool after_quantize, cudaStream_t s) {
+  const auto run = out_dtype == MS_DTYPE_F32    ? launch_int8_as<float>
+                   : out_dtype == MS_DTYPE_BF16 ? launch_int8_as<__nv_bfloat16>
+                                                : launch_int8_as<__half>;
+  return run(xq, ldx, x_scale, M, wq, ldw, w_scale, N, K, bias, out, ldo, after_quantize, s);
 }
 
 static bool i8_dtype(int d) { return d == MS_DTYPE_F32 || d == MS_DTYPE_BF16 || d == MS_DTYPE_F16; }
