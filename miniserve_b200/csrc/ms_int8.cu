@@ -127,8 +127,9 @@ static cudaError_t launch_quantize(const void *x, int dtype, int64_t M, int64_t 
 // tiles fastest, so that the weights of a channel tile come from HBM once.
 // Warp 0 loads K steps of 128 bytes with TMA (128-byte swizzle, zero beyond
 // K, channels or tokens), warp 1 issues the products into one of two
-// accumulators of 256 columns, warps 2-5 scale and store the other one.
-constexpr int kI8Threads = 192;
+// accumulators of 256 columns, warps 2-9 scale and store the other one.
+constexpr int kI8Epilogue = 8;  // warps: two for each 32 lanes of tensor memory, on alternate 16 columns
+constexpr int kI8Threads = 64 + 32 * kI8Epilogue;
 constexpr int kI8Rows = 128;    // channels of a tile
 constexpr int kI8Step = 128;    // bytes of K of a stage
 constexpr int kI8MaxStages = 11;
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(&sh.acc_full[i], 1);
-      bar_init(&sh.acc_empty[i], 4);
+      bar_init(&sh.acc_empty[i], kI8Epilogue);
     }
     bar_init(&sh.drained, 1);
     sh.dead = 0;
@@ -277,8 +278,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       const int acc = n & 1;
       const int n0 = (int)(tile / tok_tiles) * kI8Rows, t0 = (int)(tile % tok_tiles) * a.bn;
       const int count = min(a.bn, a.M - t0);
-      for (int i = et; i < count; i += 128) sh.xs[acc][i] = __ldg(a.x_scale + t0 + i);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int i = et; i < count; i += 32 * kI8Epilogue) sh.xs[acc][i] = __ldg(a.x_scale + t0 + i);
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kI8Epilogue) : "memory");
       const int ch = n0 + quad * 32 + lane;
       const float ws = ch < a.N ? __ldg(a.w_scale + ch) : 0.f;
       const float bias = a.bias && ch < a.N ? __ldg(a.bias + ch) : 0.f;
@@ -286,19 +287,21 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       __syncwarp();
       tc_fence_after();
       const bool dead = sh.dead != 0;
-      T *out = static_cast<T *>(a.out) + (int64_t)t0 * a.ldo + ch;
+      const int first = (warp - 2) / 4 * 16;
+      T *out = static_cast<T *>(a.out) + (int64_t)(t0 + first) * a.ldo + ch;
       const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + acc * kI8Cols;
       const float scale = dead ? __uint_as_float(0x7FC00000u) : ws;
+      constexpr int kNext = kI8Epilogue * 4;  // columns to this warp's next 16
       uint32_t r[2][16];  // the next 16 columns are read under the stores of these
-      tmem_ld16(from, r[0]);
+      if (first < count) tmem_ld16(from + first, r[0]);
 #pragma unroll 1
-      for (int c = 0; c < count; c += 32) {
+      for (int c = first; c < count; c += 2 * kNext) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int at = c + 16 * k;
+          const int at = c + kNext * k;
           if (at >= count) break;
           tmem_wait_ld(r[k]);
-          if (at + 16 < count) tmem_ld16(from + at + 16, r[k ^ 1]);
+          if (at + kNext < count) tmem_ld16(from + at + kNext, r[k ^ 1]);
           if (ch < a.N) {
             if (at + 16 <= count)
               i8_columns<T, true>(r[k], sh.xs[acc] + at, scale, bias, out, a.ldo, 16);
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
               i8_columns<T, false>(r[k], sh.xs[acc] + at, scale, bias, out, a.ldo, count - at);
           }
           __syncwarp();
-          out += 16 * a.ldo;
+          out += kNext * a.ldo;
         }
       }
       tc_fence_before();
