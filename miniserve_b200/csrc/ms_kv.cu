@@ -9,8 +9,8 @@
 // Bound by bytes: every element is read once and written once, and one
 // table row of rotary fp32 pairs per token serves all its heads.  A thread
 // owns 16 entries of a head (two 16-byte loads and stores: eight pairs, or 16
-// copied entries), keeps its eight cosines and sines in registers and walks
-// over `per_thread` heads with them.
+// copied entries), keeps its eight cosines and sines in registers and turns
+// one to kKvHeads heads with them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -90,51 +90,59 @@ __device__ __forceinline__ KvRow kv_row(const ms_kv_append_args &a, int64_t t) {
   return r;
 }
 
-// Source and destination of head h of token t (null where nothing is written).
+// Source of head h of token t.
 template <typename T>
-__device__ __forceinline__ void kv_head(const ms_kv_append_args &a, const KvRow &r, int64_t t, int h, const T *&src,
-                                        T *&dst, bool &turn) {
-  turn = true;
-  if (h < a.heads) {
-    src = reinterpret_cast<const T *>(a.q) + t * a.q_token + h * a.q_head;
-    dst = reinterpret_cast<T *>(a.q_out) + t * a.q_out_token + h * a.q_out_head;
-    return;
-  }
+__device__ __forceinline__ const T *kv_source(const ms_kv_append_args &a, int64_t t, int h) {
+  if (h < a.heads) return static_cast<const T *>(a.q) + t * a.q_token + h * a.q_head;
   h -= a.heads;
-  const bool key = h < a.kv_heads;
-  if (key) {
-    src = reinterpret_cast<const T *>(a.k) + t * a.k_token + h * a.k_head;
-    dst = reinterpret_cast<T *>(a.cache_k) + r.page * a.ck_page + r.offset * a.ck_token + h * a.ck_head;
-  } else {
-    h -= a.kv_heads;
-    src = reinterpret_cast<const T *>(a.v) + t * a.v_token + h * a.v_head;
-    dst = reinterpret_cast<T *>(a.cache_v) + r.page * a.cv_page + r.offset * a.cv_token + h * a.cv_head;
-    turn = false;
-  }
-  if (!r.write) dst = nullptr;
+  if (h < a.kv_heads) return static_cast<const T *>(a.k) + t * a.k_token + h * a.k_head;
+  return static_cast<const T *>(a.v) + t * a.v_token + (h - a.kv_heads) * a.v_head;
+}
+// Its destination (null where nothing is written).
+template <typename T>
+__device__ __forceinline__ T *kv_target(const ms_kv_append_args &a, const KvRow &r, int64_t t, int h) {
+  if (h < a.heads) return static_cast<T *>(a.q_out) + t * a.q_out_token + h * a.q_out_head;
+  if (!r.write) return nullptr;
+  h -= a.heads;
+  if (h < a.kv_heads) return static_cast<T *>(a.cache_k) + r.page * a.ck_page + r.offset * a.ck_token + h * a.ck_head;
+  return static_cast<T *>(a.cache_v) + r.page * a.cv_page + r.offset * a.cv_token + (h - a.kv_heads) * a.cv_head;
 }
 
 constexpr int kKvThreads = 256;
+constexpr int kKvHeads = 4;
 
 // 16-byte path: head_dim and rotary multiples of 16, every stride a multiple
-// of 8 entries and every base 16-byte aligned (checked on the host).
-template <typename T, bool kInterleaved>
+// of 8 entries and every base 16-byte aligned (checked on the host).  The
+// loads of a thread's kHeads heads are issued before anything that depends on
+// the token's slot, position and table row.
+template <typename T, bool kInterleaved, int kHeads>
 __global__ void __launch_bounds__(kKvThreads) ms_kv_append_kernel(const __grid_constant__ KvArgs p) {
   const ms_kv_append_args &a = p.a;
   const int chunks = a.head_dim >> 4;
   const int heads = a.heads + 2 * a.kv_heads;
+  const int turned = a.heads + a.kv_heads;
   const int64_t t0 = (int64_t)blockIdx.x * p.tokens_cta;
   for (int u = threadIdx.x; u < p.tokens_cta * p.per_token; u += kKvThreads) {
     const int tl = u / p.per_token, w = u - tl * p.per_token;
     const int64_t t = t0 + tl;
     if (t >= a.tokens) return;
     const int slot = w / chunks, j = w - slot * chunks;
-    const KvRow r = kv_row(a, t);
-    if (w == 0 && a.status) a.status[t] = r.status;
     const bool rotates = j * 16 < a.rotary;
     // entries of the two 16-byte halves a rotating thread owns
     const int lo = (!rotates || kInterleaved) ? j * 16 : j * 8;
     const int hi = (!rotates || kInterleaved) ? lo + 8 : lo + (a.rotary >> 1);
+    uint4 x[kHeads], y[kHeads];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      const int h = slot + i * p.slots;
+      if (h < heads) {
+        const T *src = kv_source<T>(a, t, h);
+        x[i] = *reinterpret_cast<const uint4 *>(src + lo);
+        y[i] = *reinterpret_cast<const uint4 *>(src + hi);
+      }
+    }
+    const KvRow r = kv_row(a, t);
+    if (w == 0 && a.status) a.status[t] = r.status;
     float c[8], s[8];
     if (rotates) {
       const float *row = a.table + r.position * a.rotary + j * 8;
@@ -144,36 +152,31 @@ __global__ void __launch_bounds__(kKvThreads) ms_kv_append_kernel(const __grid_c
       *reinterpret_cast<float4 *>(s) = __ldg(reinterpret_cast<const float4 *>(row));
       *reinterpret_cast<float4 *>(s + 4) = __ldg(reinterpret_cast<const float4 *>(row) + 1);
     }
-#pragma unroll 4
-    for (int h = slot; h < heads; h += p.slots) {
-      const T *src;
-      T *dst;
-      bool turn;
-      kv_head<T>(a, r, t, h, src, dst, turn);
-      if (!dst) continue;
-      if (r.status & MS_ROW_BAD_POSITION) {
-        *reinterpret_cast<uint4 *>(dst + lo) = *reinterpret_cast<uint4 *>(dst + hi) = make_uint4(0, 0, 0, 0);
-        continue;
-      }
-      uint4 x = *reinterpret_cast<const uint4 *>(src + lo), y = *reinterpret_cast<const uint4 *>(src + hi);
-      if (rotates && turn) {
-        uint32_t *xs = reinterpret_cast<uint32_t *>(&x), *ys = reinterpret_cast<uint32_t *>(&y);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (kInterleaved) {  // word i of x is pair i, word i of y is pair 4 + i
-            const float2 f = kv_widen<T>(xs[i]), g = kv_widen<T>(ys[i]);
-            xs[i] = kv_narrow<T>(f.x * c[i] - f.y * s[i], f.y * c[i] + f.x * s[i]);
-            ys[i] = kv_narrow<T>(g.x * c[4 + i] - g.y * s[4 + i], g.y * c[4 + i] + g.x * s[4 + i]);
-          } else {  // word i holds the first (x) and second (y) entries of pairs 2i and 2i + 1
-            const float2 f = kv_widen<T>(xs[i]), g = kv_widen<T>(ys[i]);
-            const float c0 = c[2 * i], c1 = c[2 * i + 1], s0 = s[2 * i], s1 = s[2 * i + 1];
-            xs[i] = kv_narrow<T>(f.x * c0 - g.x * s0, f.y * c1 - g.y * s1);
-            ys[i] = kv_narrow<T>(g.x * c0 + f.x * s0, g.y * c1 + f.y * s1);
+    for (int i = 0; i < kHeads; ++i) {
+      const int h = slot + i * p.slots;
+      if (h >= heads) break;
+      T *dst = kv_target<T>(a, r, t, h);
+      if (!dst) continue;
+      uint32_t *xs = reinterpret_cast<uint32_t *>(&x[i]), *ys = reinterpret_cast<uint32_t *>(&y[i]);
+      if (r.status & MS_ROW_BAD_POSITION) {
+        x[i] = y[i] = make_uint4(0, 0, 0, 0);
+      } else if (rotates && h < turned) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = kv_widen<T>(xs[k]), g = kv_widen<T>(ys[k]);
+          if (kInterleaved) {  // word k of x is pair k, word k of y is pair 4 + k
+            xs[k] = kv_narrow<T>(f.x * c[k] - f.y * s[k], f.y * c[k] + f.x * s[k]);
+            ys[k] = kv_narrow<T>(g.x * c[4 + k] - g.y * s[4 + k], g.y * c[4 + k] + g.x * s[4 + k]);
+          } else {  // word k holds the first (x) and second (y) entries of pairs 2k and 2k + 1
+            const float c0 = c[2 * k], c1 = c[2 * k + 1], s0 = s[2 * k], s1 = s[2 * k + 1];
+            xs[k] = kv_narrow<T>(f.x * c0 - g.x * s0, f.y * c1 - g.y * s1);
+            ys[k] = kv_narrow<T>(g.x * c0 + f.x * s0, g.y * c1 + f.y * s1);
           }
         }
       }
-      *reinterpret_cast<uint4 *>(dst + lo) = x;
-      *reinterpret_cast<uint4 *>(dst + hi) = y;
+      *reinterpret_cast<uint4 *>(dst + lo) = x[i];
+      *reinterpret_cast<uint4 *>(dst + hi) = y[i];
     }
   }
 }
@@ -207,15 +210,13 @@ __global__ void __launch_bounds__(kKvThreads) ms_kv_append_any_kernel(const __gr
       hi = lo + 1;
     }
     for (int h = slot; h < heads; h += p.slots) {
-      const T *src;
-      T *dst;
-      bool turn;
-      kv_head<T>(a, r, t, h, src, dst, turn);
+      const T *src = kv_source<T>(a, t, h);
+      T *dst = kv_target<T>(a, r, t, h);
       if (!dst) continue;
       if (r.status & MS_ROW_BAD_POSITION) {
         kv_from_float(0.f, dst[lo]);
         if (hi < a.head_dim) kv_from_float(0.f, dst[hi]);
-      } else if (rotates && turn) {
+      } else if (rotates && h < a.heads + a.kv_heads) {
         const float x = kv_to_float(src[lo]), y = kv_to_float(src[hi]);
         kv_from_float(x * c - y * s, dst[lo]);
         kv_from_float(y * c + x * s, dst[hi]);
@@ -237,20 +238,18 @@ cudaError_t launch_kv_append(KvArgs &p, bool wide, cudaStream_t s) {
   const int heads = a.heads + 2 * a.kv_heads;
   const int units = wide ? a.head_dim / 16 : a.rotary / 2 + (a.head_dim - a.rotary + 1) / 2;
   // one head a thread until the call fills the GPU's threads a few times
-  // over; then four, which share the thread's table row
+  // over; then kKvHeads, which share the thread's table row
   const bool many = a.tokens * heads * units > 4ll * 148 * 2048;
-  p.slots = many ? (heads + 3) / 4 : heads;
+  p.slots = many ? (heads + kKvHeads - 1) / kKvHeads : heads;
   p.per_token = units * p.slots;
   p.tokens_cta = p.per_token < kKvThreads ? kKvThreads / p.per_token : 1;
   const unsigned grid = (unsigned)((a.tokens + p.tokens_cta - 1) / p.tokens_cta);
-  if (wide && a.interleaved)
-    ms_kv_append_kernel<T, true><<<grid, kKvThreads, 0, s>>>(p);
+  auto *kernel = a.interleaved ? ms_kv_append_any_kernel<T, true> : ms_kv_append_any_kernel<T, false>;
+  if (wide && many)
+    kernel = a.interleaved ? ms_kv_append_kernel<T, true, kKvHeads> : ms_kv_append_kernel<T, false, kKvHeads>;
   else if (wide)
-    ms_kv_append_kernel<T, false><<<grid, kKvThreads, 0, s>>>(p);
-  else if (a.interleaved)
-    ms_kv_append_any_kernel<T, true><<<grid, kKvThreads, 0, s>>>(p);
-  else
-    ms_kv_append_any_kernel<T, false><<<grid, kKvThreads, 0, s>>>(p);
+    kernel = a.interleaved ? ms_kv_append_kernel<T, true, 1> : ms_kv_append_kernel<T, false, 1>;
+  kernel<<<grid, kKvThreads, 0, s>>>(p);
   return cudaGetLastError();
 }
 
