@@ -49,9 +49,11 @@ __device__ __forceinline__ void kv_from_float(float x, __half &y) { y = __float2
 
 struct KvArgs {
   ms_kv_append_args a;
-  int per_token;   // threads of one token
-  int slots;       // head slots of one token: thread slot s walks over heads s, s + slots, ...
-  int tokens_cta;  // tokens of one CTA
+  int page_shift;         // log2 of the page size, or -1
+  int slots;              // head slots of one token
+  int q_slots, kv_slots;  // of them, of the queries, and of the keys and the values each
+  int per_token;          // threads of one token, where a token's threads are not a block's dimensions
+  int tokens_cta;         // tokens of one CTA
 };
 
 // The token's cache row and status: bit set and no row for a bad slot or
@@ -64,13 +66,17 @@ struct KvRow {
   bool write;
 };
 
-__device__ __forceinline__ KvRow kv_row(const ms_kv_append_args &a, int64_t t) {
+__device__ __forceinline__ KvRow kv_row(const KvArgs &p, int64_t t) {
+  const ms_kv_append_args &a = p.a;
   KvRow r{0, 0, 0, MS_ROW_OK, false};
   const int64_t slot = __ldg(a.slots + t);
   if (slot >= a.pages * a.page_size) {
     r.status |= MS_ROW_BAD_SLOT;
   } else if (slot >= 0) {
-    if (slot < (1ll << 32)) {
+    if (p.page_shift >= 0) {
+      r.page = slot >> p.page_shift;
+      r.offset = slot & (a.page_size - 1);
+    } else if (slot < (1ll << 32)) {
       r.page = (uint32_t)slot / (uint32_t)a.page_size;
       r.offset = (uint32_t)slot - (uint32_t)r.page * (uint32_t)a.page_size;
     } else {
@@ -109,42 +115,50 @@ __device__ __forceinline__ T *kv_target(const ms_kv_append_args &a, const KvRow 
 }
 
 constexpr int kKvThreads = 256;
-constexpr int kKvHeads = 4;
+constexpr int kKvHeads = 2;
 
 // 16-byte path: head_dim and rotary multiples of 16, every stride a multiple
-// of 8 entries and every base 16-byte aligned (checked on the host).  The
-// loads of a thread's kHeads heads are issued before anything that depends on
-// the token's slot, position and table row.
+// of 8 entries and every base 16-byte aligned (checked on the host).  Threads
+// are (chunk of 16 entries, head slot, token); a slot is up to kHeads heads of
+// one of q, k and v, so that a thread finds its addresses once and steps along
+// them.  Its loads are issued before anything that depends on the token's
+// slot, position and table row.
 template <typename T, bool kInterleaved, int kHeads>
-__global__ void __launch_bounds__(kKvThreads) ms_kv_append_kernel(const __grid_constant__ KvArgs p) {
+__global__ void __launch_bounds__(kKvThreads, 4) ms_kv_append_kernel(const __grid_constant__ KvArgs p) {
   const ms_kv_append_args &a = p.a;
-  const int chunks = a.head_dim >> 4;
-  const int heads = a.heads + 2 * a.kv_heads;
-  const int turned = a.heads + a.kv_heads;
-  const int64_t t0 = (int64_t)blockIdx.x * p.tokens_cta;
-  for (int u = threadIdx.x; u < p.tokens_cta * p.per_token; u += kKvThreads) {
-    const int tl = u / p.per_token, w = u - tl * p.per_token;
-    const int64_t t = t0 + tl;
-    if (t >= a.tokens) return;
-    const int slot = w / chunks, j = w - slot * chunks;
-    const bool rotates = j * 16 < a.rotary;
-    // entries of the two 16-byte halves a rotating thread owns
-    const int lo = (!rotates || kInterleaved) ? j * 16 : j * 8;
-    const int hi = (!rotates || kInterleaved) ? lo + 8 : lo + (a.rotary >> 1);
+  const int j = threadIdx.x;
+  const int64_t t = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
+  if (t >= a.tokens) return;
+  const bool rotates = j * 16 < a.rotary;
+  // entries of the two 16-byte halves a rotating thread owns
+  const int lo = (!rotates || kInterleaved) ? j * 16 : j * 8;
+  const int hi = (!rotates || kInterleaved) ? lo + 8 : lo + (a.rotary >> 1);
+  for (int slot = threadIdx.y; slot < p.slots; slot += blockDim.y) {
+    // the slot's heads: h, h + step, ... of q, k or v
+    const bool query = slot < p.q_slots, key = !query && slot < p.q_slots + p.kv_slots;
+    const int h = slot - (query ? 0 : key ? p.q_slots : p.q_slots + p.kv_slots);
+    const int step = query ? p.q_slots : p.kv_slots, heads = query ? a.heads : a.kv_heads;
+    const int64_t src_head = query ? a.q_head : key ? a.k_head : a.v_head;
+    const T *src = static_cast<const T *>(query ? a.q : key ? a.k : a.v) +
+                   t * (query ? a.q_token : key ? a.k_token : a.v_token) + h * src_head;
     uint4 x[kHeads], y[kHeads];
+    {
+      const T *from = src;
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      const int h = slot + i * p.slots;
-      if (h < heads) {
-        const T *src = kv_source<T>(a, t, h);
-        x[i] = *reinterpret_cast<const uint4 *>(src + lo);
-        y[i] = *reinterpret_cast<const uint4 *>(src + hi);
+      for (int i = 0; i < kHeads; ++i) {
+        if (h + i * step < heads) {
+          x[i] = *reinterpret_cast<const uint4 *>(from + lo);
+          y[i] = *reinterpret_cast<const uint4 *>(from + hi);
+        }
+        from += step * src_head;
       }
     }
-    const KvRow r = kv_row(a, t);
-    if (w == 0 && a.status) a.status[t] = r.status;
+    const KvRow r = kv_row(p, t);
+    if (slot == 0 && j == 0 && a.status) a.status[t] = r.status;
+    if (!query && !r.write) continue;
     float c[8], s[8];
-    if (rotates) {
+    const bool turns = rotates && (query || key);
+    if (turns) {
       const float *row = a.table + r.position * a.rotary + j * 8;
       *reinterpret_cast<float4 *>(c) = __ldg(reinterpret_cast<const float4 *>(row));
       *reinterpret_cast<float4 *>(c + 4) = __ldg(reinterpret_cast<const float4 *>(row) + 1);
@@ -152,16 +166,18 @@ __global__ void __launch_bounds__(kKvThreads) ms_kv_append_kernel(const __grid_c
       *reinterpret_cast<float4 *>(s) = __ldg(reinterpret_cast<const float4 *>(row));
       *reinterpret_cast<float4 *>(s + 4) = __ldg(reinterpret_cast<const float4 *>(row) + 1);
     }
+    const int64_t dst_head = query ? a.q_out_head : key ? a.ck_head : a.cv_head;
+    T *dst = static_cast<T *>(query ? a.q_out : key ? a.cache_k : a.cache_v) + h * dst_head;
+    if (query) dst += t * a.q_out_token;
+    else if (key) dst += r.page * a.ck_page + r.offset * a.ck_token;
+    else dst += r.page * a.cv_page + r.offset * a.cv_token;
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
-      const int h = slot + i * p.slots;
-      if (h >= heads) break;
-      T *dst = kv_target<T>(a, r, t, h);
-      if (!dst) continue;
+      if (h + i * step >= heads) break;
       uint32_t *xs = reinterpret_cast<uint32_t *>(&x[i]), *ys = reinterpret_cast<uint32_t *>(&y[i]);
       if (r.status & MS_ROW_BAD_POSITION) {
         x[i] = y[i] = make_uint4(0, 0, 0, 0);
-      } else if (rotates && h < turned) {
+      } else if (turns) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float2 f = kv_widen<T>(xs[k]), g = kv_widen<T>(ys[k]);
@@ -177,6 +193,7 @@ __global__ void __launch_bounds__(kKvThreads) ms_kv_append_kernel(const __grid_c
       }
       *reinterpret_cast<uint4 *>(dst + lo) = x[i];
       *reinterpret_cast<uint4 *>(dst + hi) = y[i];
+      dst += step * dst_head;
     }
   }
 }
@@ -195,7 +212,7 @@ __global__ void __launch_bounds__(kKvThreads) ms_kv_append_any_kernel(const __gr
     const int64_t t = t0 + tl;
     if (t >= a.tokens) return;
     const int slot = w / units, j = w - slot * units;
-    const KvRow r = kv_row(a, t);
+    const KvRow r = kv_row(p, t);
     if (w == 0 && a.status) a.status[t] = r.status;
     const bool rotates = j < half;
     int lo, hi;
@@ -238,17 +255,25 @@ cudaError_t launch_kv_append(KvArgs &p, bool wide, cudaStream_t s) {
   const int heads = a.heads + 2 * a.kv_heads;
   const int units = wide ? a.head_dim / 16 : a.rotary / 2 + (a.head_dim - a.rotary + 1) / 2;
   // one head a thread until the call fills the GPU's threads a few times
-  // over; then kKvHeads, which share the thread's table row
-  const bool many = a.tokens * heads * units > 4ll * 148 * 2048;
-  p.slots = many ? (heads + kKvHeads - 1) / kKvHeads : heads;
+  // over; then up to kKvHeads, which share the thread's table row
+  const int each = a.tokens * heads * units > 4ll * 148 * 2048 ? kKvHeads : 1;
+  if (wide) {
+    p.q_slots = (a.heads + each - 1) / each;
+    p.kv_slots = (a.kv_heads + each - 1) / each;
+    p.slots = p.q_slots + 2 * p.kv_slots;
+    const int y = p.slots < kKvThreads / units ? p.slots : kKvThreads / units;
+    const int z = kKvThreads / (units * y) < 64 ? kKvThreads / (units * y) : 64;
+    auto *kernel = a.interleaved ? ms_kv_append_kernel<T, true, 1> : ms_kv_append_kernel<T, false, 1>;
+    if (each > 1)
+      kernel = a.interleaved ? ms_kv_append_kernel<T, true, kKvHeads> : ms_kv_append_kernel<T, false, kKvHeads>;
+    kernel<<<(unsigned)((a.tokens + z - 1) / z), dim3(units, y, z), 0, s>>>(p);
+    return cudaGetLastError();
+  }
+  p.slots = (heads + each - 1) / each;
   p.per_token = units * p.slots;
   p.tokens_cta = p.per_token < kKvThreads ? kKvThreads / p.per_token : 1;
   const unsigned grid = (unsigned)((a.tokens + p.tokens_cta - 1) / p.tokens_cta);
   auto *kernel = a.interleaved ? ms_kv_append_any_kernel<T, true> : ms_kv_append_any_kernel<T, false>;
-  if (wide && many)
-    kernel = a.interleaved ? ms_kv_append_kernel<T, true, kKvHeads> : ms_kv_append_kernel<T, false, kKvHeads>;
-  else if (wide)
-    kernel = a.interleaved ? ms_kv_append_kernel<T, true, 1> : ms_kv_append_kernel<T, false, 1>;
   kernel<<<grid, kKvThreads, 0, s>>>(p);
   return cudaGetLastError();
 }
@@ -275,6 +300,9 @@ extern "C" int ms_kv_append(const ms_kv_append_args *args, ms_stream_t stream) {
   bool wide = a.head_dim % 16 == 0 && a.rotary % 16 == 0 && ms::aligned16(a.k) && ms::aligned16(a.v) &&
               ms::aligned16(a.cache_k) && ms::aligned16(a.cache_v) && (a.rotary == 0 || ms::aligned16(a.table)) &&
               (a.heads == 0 || (ms::aligned16(a.q) && ms::aligned16(a.q_out)));
+  p.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (a.page_size == 1ll << i) p.page_shift = i;
   int64_t strides = a.k_token | a.k_head | a.v_token | a.v_head | a.ck_page | a.ck_token | a.ck_head | a.cv_page |
                     a.cv_token | a.cv_head;
   if (a.heads > 0) strides |= a.q_token | a.q_head | a.q_out_token | a.q_out_head;
