@@ -593,29 +593,40 @@ __global__ void __launch_bounds__(kPrThreads, 2)
   const uint32_t tmem = sh.tmem;
 
   if (warp < 4) {
-    // this thread's query row, in 128-byte swizzled panels of 64 entries
+    // the warp's 32 query rows, in 128-byte swizzled panels of 64 entries: a row is read by neighbouring lanes
     const int r = tid;
     {
+      constexpr int kChunks = DP / 8, kRowsStep = 32 / kChunks;
       const int pr = r0 + r;
-      const bool live = pr < a.packed;
-      const int64_t b = live ? pr / a.shape.group : 0;
-      const int head = h * a.shape.group + (live ? pr - (int)b * a.shape.group : 0);
-      const T *src = static_cast<const T *>(x.q) + b * x.q_row + head * x.q_head;
+      int64_t at = -1;
+      if (pr < a.packed) {
+        const int64_t b = pr / a.shape.group;
+        at = b * x.q_row + (int64_t)(h * a.shape.group + (pr - (int)b * a.shape.group)) * x.q_head;
+      }
+      const int chunk = lane % kChunks;
+      uint4 v[32 / kRowsStep];
 #pragma unroll
-      for (int c = 0; c < DP / 8; ++c) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (live && c * 8 < x.head_dim) {
+      for (int i = 0; i < 32 / kRowsStep; ++i) {
+        const int64_t from = __shfl_sync(0xFFFFFFFFu, at, i * kRowsStep + lane / kChunks);
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (from >= 0 && chunk * 8 < x.head_dim) {
+          const T *src = static_cast<const T *>(x.q) + from + chunk * 8;
           if (a.q_wide) {
-            v = __ldg(reinterpret_cast<const uint4 *>(src + c * 8));
+            v[i] = __ldg(reinterpret_cast<const uint4 *>(src));
           } else {
-            const unsigned short *p = reinterpret_cast<const unsigned short *>(src + c * 8);
+            const unsigned short *p = reinterpret_cast<const unsigned short *>(src);
             uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldg(p + 2 * i) | ((uint32_t)__ldg(p + 2 * i + 1) << 16);
-            v = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int k = 0; k < 4; ++k) w[k] = (uint32_t)__ldg(p + 2 * k) | ((uint32_t)__ldg(p + 2 * k + 1) << 16);
+            v[i] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
-        *reinterpret_cast<uint4 *>(qs + (c >> 3) * kPrRows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+      }
+#pragma unroll
+      for (int i = 0; i < 32 / kRowsStep; ++i) {
+        const int row = warp * 32 + i * kRowsStep + lane / kChunks;
+        *reinterpret_cast<uint4 *>(qs + (chunk >> 3) * kPrRows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
+            v[i];
       }
       fence_async_proxy();
       __syncwarp();
@@ -686,18 +697,28 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       tc_fence_after();
       const int pr = r0 + r;
       const int64_t rec = ((int64_t)part * a.shape.kv_heads + h) * a.packed + pr;
-#pragma unroll
+      // 32 columns at a time through the queries' memory (they have been used), so that a record's row is
+      // written by neighbouring lanes
+      unsigned char *turn = qs + warp * 4096;
+#pragma unroll 1
       for (int c = 0; c < DP; c += 32) {
         uint32_t u[32];
         tmem_ld32(lanes + kPrO + c, u);
         tmem_wait_ld32(u);
-        if (pr < a.packed) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            if (c + j < x.head_dim)
-              *reinterpret_cast<uint4 *>(a.pre_o + rec * x.head_dim + c + j) =
-                  make_uint4(u[j], u[j + 1], u[j + 2], u[j + 3]);
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<uint4 *>(turn + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+              make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+        __syncwarp();
+        const int j = lane & 7;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = i * 4 + (lane >> 3);
+          const uint4 v = *reinterpret_cast<const uint4 *>(turn + row * 128 + ((j ^ (row & 7)) << 4));
+          if (r0 + warp * 32 + row < a.packed && c + j * 4 < x.head_dim)
+            *reinterpret_cast<uint4 *>(a.pre_o + (rec - lane + row) * x.head_dim + c + j * 4) = v;
         }
+        __syncwarp();
       }
       if (pr < a.packed) {
         // the copies' warps set `bad` before the last products could start
