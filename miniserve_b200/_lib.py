@@ -28,8 +28,11 @@ MS_ROW_BAD_POSITION = 64
 MS_ROW_BAD_LENGTH = 128
 MS_ROW_BAD_PAGE = 256
 
+BINDING_PATH = os.path.join(HERE, "_binding.so")
+
 _lock = threading.Lock()
 _lib = None
+_binding = None
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -144,6 +147,36 @@ def lib():
                 fn.argtypes = args
             _lib = handle
     return _lib
+
+
+def binding():
+    """Load _binding.so once, with the library's entry points; raise if it has
+    not been built for this torch."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    import importlib.machinery
+    import importlib.util
+
+    import torch
+    handle = lib()
+    with _lock:
+        if _binding is None:
+            if not os.path.exists(BINDING_PATH):
+                raise SamplerLibraryError(
+                    f"{BINDING_PATH} is missing: build it with `python -m miniserve_b200.build`")
+            loader = importlib.machinery.ExtensionFileLoader("miniserve_b200._binding", BINDING_PATH)
+            module = importlib.util.module_from_spec(
+                importlib.util.spec_from_file_location("miniserve_b200._binding", BINDING_PATH, loader=loader))
+            loader.exec_module(module)
+            if module.torch_version != torch.__version__.split("+")[0]:
+                raise SamplerLibraryError(f"{BINDING_PATH} was built for torch {module.torch_version}, this is "
+                                          f"{torch.__version__}: build it again")
+            module.bind(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in (
+                "ms_kv_append", "ms_prefix_attention", "ms_prefix_attention_workspace", "ms_int8_linear",
+                "ms_int8_workspace")))
+            _binding = module
+    return _binding
 
 
 def check(rc: int, what: str) -> None:

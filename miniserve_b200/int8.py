@@ -155,8 +155,6 @@ class Int8Linear:
             rows.copy_(weight)
             weight = rows
         self.weight = weight
-        self.shape = (N, K)
-        self._ldw = _check_rows("weight", weight)
 
     @classmethod
     def from_float(cls, weight, bias=None) -> "Int8Linear":
@@ -167,22 +165,9 @@ class Int8Linear:
     def __call__(self, x, *, out_dtype=None, out=None):
         """[M, N] of ``x`` [M, K] (fp32, bf16 or fp16) in ``out_dtype``
         (default: out's type, or fp32 as the sampler's logits)."""
-        torch = _torch()
-        _matrix("x", x)
-        code = _dtype_code(x.dtype)
-        N, K = self.shape
-        dev = self.weight.device
-        M = x.shape[0]
-        if x.shape[1] != K or x.device != dev:
-            raise ValueError(f"x must be a [M, {K}] tensor on {dev}")
-        if out_dtype is None:
-            out_dtype = torch.float32 if out is None else out.dtype
-        out = _output(out, out_dtype, M, N, dev)
-        L = _lib.lib()
-        workspace = torch.empty(L.ms_int8_workspace(M, K), dtype=torch.uint8, device=dev)
-        rc = launch(dev, L.ms_int8_linear, x.data_ptr(), code, _pitch(x), M, self.weight.data_ptr(), self._ldw,
-                    self.scale.data_ptr(), N, K, None if self.bias is None else self.bias.data_ptr(), out.data_ptr(),
-                    _dtype_code(out_dtype), _pitch(out), workspace.data_ptr())
-        if rc:
-            _lib.check(rc, "ms_int8_linear")
-        return out
+        entry = _lib.binding()
+        try:
+            return entry.int8_linear(x, self.weight, self.scale, self.bias, out_dtype, out)
+        except entry.CallError as e:
+            _lib.check(e.args[0], "ms_int8_linear")
+            raise
