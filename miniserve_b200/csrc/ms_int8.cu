@@ -128,6 +128,13 @@ static cudaError_t launch_quantize(const void *x, int dtype, int64_t M, int64_t 
 // Warp 0 loads K steps of 128 bytes with TMA (128-byte swizzle, zero beyond
 // K, channels or tokens), warp 1 issues the products into one of two
 // accumulators of 256 columns, warps 2-9 scale and store the other one.
+//
+// Large batches are bound by what an SM can read (64 bytes a clock): a tile of
+// 128 channels x 256 tokens reads 96 bytes a clock at the products' full rate.
+// There two SMs take a tile of 256 channels together (kPair: a cluster of two,
+// products of cta_group::2): each loads its 128 channels and half of the
+// tokens, 64 bytes a clock, the first CTA issues the products for both, and
+// each stores its own channels.
 constexpr int kI8Epilogue = 8;  // warps: two for each 32 lanes of tensor memory, on alternate 16 columns
 constexpr int kI8Threads = 64 + 32 * kI8Epilogue;
 constexpr int kI8Rows = 128;    // channels of a tile
@@ -135,6 +142,7 @@ constexpr int kI8Step = 128;    // bytes of K of a stage
 constexpr int kI8MaxStages = 11;
 constexpr int kI8Cols = 256;    // columns of an accumulator
 constexpr int kI8Ring = 208 * 1024;
+constexpr int kI8PairRows = 128;  // tokens above which two SMs share a tile
 
 struct I8Shared {
   uint64_t full[kI8MaxStages], empty[kI8MaxStages];
@@ -150,6 +158,7 @@ struct I8Args {
   int64_t ldo;
   int M, N, K;
   int bn;      // tokens of a tile: a multiple of 16, at most 256
+  int rows;    // channels of a tile, at most kI8Rows
   int stages;
   int after_quantize;  // launched with the quantisation as its programmatic dependency
 };
@@ -174,7 +183,7 @@ __device__ __forceinline__ void i8_columns(const uint32_t (&r)[16], const float 
   }
 }
 
-template <typename T>
+template <typename T, bool kPair>
 __global__ void __launch_bounds__(kI8Threads, 1)
     ms_int8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                    const __grid_constant__ I8Args a) {
@@ -182,10 +191,16 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   __shared__ I8Shared sh;
   unsigned char *ring = i8_raw + ((1024u - (smem_addr(i8_raw) & 1023u)) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // this CTA's or pair's tiles, and this CTA's channels and tokens of one
+  constexpr int kCtas = kPair ? 2 : 1;
+  const uint32_t rank = kPair ? cluster_rank() : 0;
+  const int64_t worker = blockIdx.x / kCtas, workers = gridDim.x / kCtas;
   const int tok_tiles = (a.M + a.bn - 1) / a.bn;
-  const int64_t tiles = (int64_t)((a.N + kI8Rows - 1) / kI8Rows) * tok_tiles;
+  const int span = a.rows * kCtas;
+  const int64_t tiles = (int64_t)((a.N + span - 1) / span) * tok_tiles;
   const int steps = (a.K + kI8Step - 1) / kI8Step;
-  const uint32_t wbytes = kI8Rows * kI8Step, xbytes = (uint32_t)a.bn * kI8Step;
+  constexpr uint32_t wbytes = kI8Rows * kI8Step;
+  const uint32_t xbytes = (uint32_t)(a.bn / kCtas) * kI8Step, both = (uint32_t)a.rows * kI8Step + xbytes;
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
       bar_init(&sh.full[i], 1);
@@ -193,35 +208,47 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(&sh.acc_full[i], 1);
-      bar_init(&sh.acc_empty[i], kI8Epilogue);
+      bar_init(&sh.acc_empty[i], kI8Epilogue * kCtas);
     }
     bar_init(&sh.drained, 1);
     sh.dead = 0;
     bar_init_fence();
   }
-  if (warp == 1) tmem_alloc(&sh.tmem, 2 * kI8Cols);
+  if (warp == 1) {
+    if (kPair) tmem_alloc_pair(&sh.tmem, 2 * kI8Cols);
+    else tmem_alloc(&sh.tmem, 2 * kI8Cols);
+  }
   tc_fence_before();
   __syncthreads();
+  if (kPair) cluster_sync();  // the other CTA's barriers are ready
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
   if (warp == 0) {
     if (lane == 0) {
+      auto load = [&](int stage, unsigned char *dst, const CUtensorMap *map, int x, int y) {
+        if (kPair) tma_load_2d_pair(dst, map, leader_addr(&sh.full[stage]), x, y);
+        else tma_load_2d(dst, map, &sh.full[stage], x, y);
+      };
+      auto expect = [&](int stage) {  // the first CTA's barrier counts both CTAs' bytes
+        if (rank == 0) bar_expect(&sh.full[stage], both * kCtas);
+      };
       // the weights of the first stages need not wait for the quantisation
-      const int64_t mine = tiles > blockIdx.x ? (tiles - blockIdx.x - 1) / gridDim.x + 1 : 0;
+      const int64_t mine = tiles > worker ? (tiles - worker - 1) / workers + 1 : 0;
       const int64_t total = mine * steps;
       const int ahead = (int)(total < a.stages ? total : a.stages);
       for (int i = 0; i < ahead; ++i) {
-        const int64_t tile = blockIdx.x + (int64_t)(i / steps) * gridDim.x;
-        bar_expect(&sh.full[i], wbytes + xbytes);
-        tma_load_2d(ring + i * (wbytes + xbytes), &wmap, &sh.full[i], (i % steps) * kI8Step,
-                    (int)(tile / tok_tiles) * kI8Rows);
+        const int64_t tile = worker + (int64_t)(i / steps) * workers;
+        expect(i);
+        load(i, ring + i * (wbytes + xbytes), &wmap, (i % steps) * kI8Step,
+             (int)(tile / tok_tiles) * span + (int)rank * a.rows);
       }
       if (a.after_quantize) grid_wait();
       int64_t it = 0;
       int stage = 0, use = 0;
-      for (int64_t tile = blockIdx.x; tile < tiles && !sh.dead; tile += gridDim.x) {
-        const int n0 = (int)(tile / tok_tiles) * kI8Rows, t0 = (int)(tile % tok_tiles) * a.bn;
+      for (int64_t tile = worker; tile < tiles && !sh.dead; tile += workers) {
+        const int n0 = (int)(tile / tok_tiles) * span + (int)rank * a.rows;
+        const int t0 = (int)(tile % tok_tiles) * a.bn + (int)rank * (a.bn / kCtas);
         for (int k = 0; k < steps; ++k, ++it) {
           unsigned char *st = ring + stage * (wbytes + xbytes);
           if (it >= ahead) {
@@ -229,15 +256,15 @@ __global__ void __launch_bounds__(kI8Threads, 1)
               sh.dead = 1;
               break;
             }
-            bar_expect(&sh.full[stage], wbytes + xbytes);
-            tma_load_2d(st, &wmap, &sh.full[stage], k * kI8Step, n0);
+            expect(stage);
+            load(stage, st, &wmap, k * kI8Step, n0);
           }
-          tma_load_2d(st + wbytes, &xmap, &sh.full[stage], k * kI8Step, t0);
+          load(stage, st + wbytes, &xmap, k * kI8Step, t0);
           if (++stage == a.stages) stage = 0, ++use;
         }
       }
       if (sh.dead) {  // copies in flight: their last phase of each stage, again bounded
-        for (int i = 0; i < a.stages; ++i) {
+        for (int i = 0; i < a.stages && rank == 0; ++i) {
           const int uses = use + (i < stage ? 1 : 0);
           if (uses > 0 && it > i) bar_wait(&sh.full[i], (uses - 1) & 1);
         }
@@ -245,10 +272,14 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
   } else if (warp == 1) {
     const uint32_t leader = tc_leader();
-    const uint32_t idesc = tc_idesc_i8(a.bn);
+    const uint32_t idesc = tc_idesc_i8(kI8Rows * kCtas, a.bn);
     int stage = 0, phase = 0, n = 0;
     bool ok = true;
-    for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++n) {
+    auto commit = [&](uint64_t *bar) {
+      if (kPair) tc_commit_pair(leader, bar);
+      else tc_commit(leader, bar);
+    };
+    for (int64_t tile = worker; tile < tiles && ok && rank == 0; tile += workers, ++n) {
       const int acc = n & 1;
       ok = bar_wait_warp(&sh.acc_empty[acc], ((n >> 1) & 1) ^ 1, sh.dead);
       tc_fence_after();
@@ -259,28 +290,30 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         const uint32_t st = smem_addr(ring + stage * (wbytes + xbytes));
         const uint64_t wd = tc_desc(st, 1024, 16), xd = tc_desc(st + wbytes, 1024, 16);
 #pragma unroll
-        for (int j = 0; j < kI8Step / 32; ++j)
-          tc_mma_i8(leader, tmem + acc * kI8Cols, wd + 2 * j, xd + 2 * j, idesc, k > 0 || j > 0);
-        tc_commit(leader, &sh.empty[stage]);
+        for (int j = 0; j < kI8Step / 32; ++j) {
+          if (kPair) tc_mma_i8_pair(leader, tmem + acc * kI8Cols, wd + 2 * j, xd + 2 * j, idesc, k > 0 || j > 0);
+          else tc_mma_i8(leader, tmem + acc * kI8Cols, wd + 2 * j, xd + 2 * j, idesc, k > 0 || j > 0);
+        }
+        commit(&sh.empty[stage]);
         if (++stage == a.stages) stage = 0, phase ^= 1;
       }
-      if (ok) tc_commit(leader, &sh.acc_full[acc]);
+      if (ok) commit(&sh.acc_full[acc]);
     }
     if (!ok) sh.dead = 1;
-    tc_commit(leader, &sh.drained);
+    if (rank == 0) commit(&sh.drained);
     bar_wait(&sh.drained, 0);  // products in flight end before tensor memory is freed
   } else {
     const int quad = warp & 3;
     const int et = threadIdx.x - 64;
     if (a.after_quantize) grid_wait();
     int n = 0;
-    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+    for (int64_t tile = worker; tile < tiles; tile += workers, ++n) {
       const int acc = n & 1;
-      const int n0 = (int)(tile / tok_tiles) * kI8Rows, t0 = (int)(tile % tok_tiles) * a.bn;
+      const int n0 = (int)(tile / tok_tiles) * span + (int)rank * a.rows, t0 = (int)(tile % tok_tiles) * a.bn;
       const int count = min(a.bn, a.M - t0);
       for (int i = et; i < count; i += 32 * kI8Epilogue) sh.xs[acc][i] = __ldg(a.x_scale + t0 + i);
       asm volatile("bar.sync 1, %0;" ::"n"(32 * kI8Epilogue) : "memory");
-      const int ch = n0 + quad * 32 + lane;
+      const int ch = quad * 32 + lane < a.rows ? n0 + quad * 32 + lane : a.N;  // a.N: not a channel of this tile
       const float ws = ch < a.N ? __ldg(a.w_scale + ch) : 0.f;
       const float bias = a.bias && ch < a.N ? __ldg(a.bias + ch) : 0.f;
       if (!sh.dead && !bar_wait(&sh.acc_full[acc], (n >> 1) & 1)) sh.dead = 1;
@@ -314,14 +347,21 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) bar_arrive(&sh.acc_empty[acc]);
+      if (lane == 0) {
+        if (kPair) bar_arrive_leader(&sh.acc_empty[acc]);
+        else bar_arrive(&sh.acc_empty[acc]);
+      }
     }
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (kPair) cluster_sync();  // neither CTA's memory or barriers are used by the other any more
   tc_fence_after();
-  if (warp == 1) tmem_free(tmem, 2 * kI8Cols);
+  if (warp == 1) {
+    if (kPair) tmem_free_pair(tmem, 2 * kI8Cols);
+    else tmem_free(tmem, 2 * kI8Cols);
+  }
 }
 
 // A [rows, K] int8 matrix read in tiles of `box` rows and 128 bytes.
@@ -339,56 +379,84 @@ static cudaError_t i8_map(CUtensorMap *map, const void *p, int64_t rows, int64_t
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-template <typename T>
-static cudaError_t launch_int8_as(const int8_t *xq, int64_t ldx, const float *x_scale, int64_t M, const int8_t *wq,
-                                  int64_t ldw, const float *w_scale, int64_t N, int64_t K, const float *bias,
-                                  void *out, int64_t ldo, bool after_quantize, cudaStream_t s) {
+template <typename T, bool kPair>
+static cudaError_t launch_int8_as(I8Args &a, const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, int dev,
+                                  cudaStream_t s) {
   static std::atomic<int> ready[kMaxDevices];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  constexpr int kCtas = kPair ? 2 : 1;
+  cudaError_t e = cudaSuccess;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(ms_int8_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8Ring + 1024);
+    e = cudaFuncSetAttribute(ms_int8_kernel<T, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8Ring + 1024);
     if (e != cudaSuccess) return e;
     ready[dev].store(1, std::memory_order_release);
   }
-  I8Args a{};
-  a.x_scale = x_scale, a.w_scale = w_scale, a.bias = bias, a.out = out, a.ldo = ldo;
-  a.M = (int)M, a.N = (int)N, a.K = (int)K, a.after_quantize = after_quantize;
-  // equal token tiles of at most 256, rounded up to the 16 that an N of the product allows
-  const int64_t parts = (M + kI8Cols - 1) / kI8Cols;
-  a.bn = (int)(((M + parts - 1) / parts + 15) / 16 * 16);
-  const int stage = (kI8Rows + a.bn) * kI8Step;
-  a.stages = kI8Ring / stage < kI8MaxStages ? kI8Ring / stage : kI8MaxStages;
-  CUtensorMap wmap, xmap;
-  e = i8_map(&wmap, wq, N, K, ldw, kI8Rows);
-  if (e == cudaSuccess) e = i8_map(&xmap, xq, M, K, ldx, a.bn);
-  if (e != cudaSuccess) return e;
   int sms = 148;
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int64_t tiles = ((N + kI8Rows - 1) / kI8Rows) * ((M + a.bn - 1) / a.bn);
+  // equal token tiles of at most 256, rounded up to what an N of the product and half of it for a pair allow
+  const int64_t parts = (a.M + (int64_t)kI8Cols - 1) / kI8Cols;
+  a.bn = (int)(((a.M + parts - 1) / parts + 16 * kCtas - 1) / (16 * kCtas) * (16 * kCtas));
+  const int64_t tok_tiles = (a.M + (int64_t)a.bn - 1) / a.bn;
+  a.rows = kI8Rows;
+  // Where the weights are most of the bytes (few tokens), as many rounds of tiles as 128 channels a tile need,
+  // with the channels spread evenly over them: 1 x 896 x 151936 takes 26.8 us, 28.0 us in tiles of 128.  Else
+  // tiles of 128, whose stores are whole lines: 512 tokens take 102 us, 117 us with odd tiles.
+  if (!kPair && a.M * (int64_t)sizeof(T) * 8 <= a.K) {
+    const int64_t rounds = ((a.N + (int64_t)kI8Rows - 1) / kI8Rows * tok_tiles + sms - 1) / sms;
+    const int64_t most = rounds * sms / tok_tiles;  // at least ceil(N / kI8Rows)
+    a.rows = (int)((a.N + most - 1) / most);
+  }
+  const int stage = (kI8Rows + a.bn / kCtas) * kI8Step;
+  a.stages = kI8Ring / stage < kI8MaxStages ? kI8Ring / stage : kI8MaxStages;
+  const int64_t span = (int64_t)a.rows * kCtas;
+  const int64_t tiles = (a.N + span - 1) / span * tok_tiles;
+  CUtensorMap wmap, xmap;
+  e = i8_map(&wmap, wq, a.N, a.K, ldw, a.rows);
+  if (e == cudaSuccess) e = i8_map(&xmap, xq, a.M, a.K, ldx, a.bn / kCtas);
+  if (e != cudaSuccess) return e;
+  const int64_t workers = tiles < sms / kCtas ? tiles : sms / kCtas;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles < sms ? tiles : sms));
+  cfg.gridDim = dim3((unsigned)(workers * kCtas));
   cfg.blockDim = dim3(kI8Threads);
   cfg.dynamicSmemBytes = a.stages * stage + 1024;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  cfg.numAttrs = after_quantize ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, ms_int8_kernel<T>, wmap, xmap, a);
+  if (kPair) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = 2;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (a.after_quantize) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  e = cudaLaunchKernelEx(&cfg, ms_int8_kernel<T, kPair>, wmap, xmap, a);
   return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t launch_int8_out(I8Args &a, const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, int dev,
+                                   cudaStream_t s) {
+  return a.M > kI8PairRows ? launch_int8_as<T, true>(a, xq, ldx, wq, ldw, dev, s)
+                           : launch_int8_as<T, false>(a, xq, ldx, wq, ldw, dev, s);
 }
 
 static cudaError_t launch_int8(const int8_t *xq, int64_t ldx, const float *x_scale, int64_t M, const int8_t *wq,
                                int64_t ldw, const float *w_scale, int64_t N, int64_t K, const float *bias, void *out,
                                int out_dtype, int64_t ldo, bool after_quantize, cudaStream_t s) {
-  const auto run = out_dtype == MS_DTYPE_F32    ? launch_int8_as<float>
-                   : out_dtype == MS_DTYPE_BF16 ? launch_int8_as<__nv_bfloat16>
-                                                : launch_int8_as<__half>;
-  return run(xq, ldx, x_scale, M, wq, ldw, w_scale, N, K, bias, out, ldo, after_quantize, s);
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  I8Args a{};
+  a.x_scale = x_scale, a.w_scale = w_scale, a.bias = bias, a.out = out, a.ldo = ldo;
+  a.M = (int)M, a.N = (int)N, a.K = (int)K, a.after_quantize = after_quantize;
+  if (out_dtype == MS_DTYPE_F32) return launch_int8_out<float>(a, xq, ldx, wq, ldw, dev, s);
+  if (out_dtype == MS_DTYPE_BF16) return launch_int8_out<__nv_bfloat16>(a, xq, ldx, wq, ldw, dev, s);
+  return launch_int8_out<__half>(a, xq, ldx, wq, ldw, dev, s);
 }
 
 static bool i8_dtype(int d) { return d == MS_DTYPE_F32 || d == MS_DTYPE_BF16 || d == MS_DTYPE_F16; }

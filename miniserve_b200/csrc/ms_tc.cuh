@@ -112,6 +112,52 @@ __device__ __forceinline__ void tc_commit(uint32_t leader, uint64_t *bar) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// ---- pairs of CTAs (clusters of two) that issue one product over both
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of the pair's first CTA's copy of a shared variable.
+__device__ __forceinline__ uint32_t leader_addr(const void *p) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_addr(p)));
+  return r;
+}
+__device__ __forceinline__ void bar_arrive_leader(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+}
+// A tile into this CTA's memory, announced to the first CTA's barrier.
+__device__ __forceinline__ void tma_load_2d_pair(void *dst, const void *map, uint32_t leader_bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4}], [%2];" ::"r"(smem_addr(dst)),
+      "l"(map), "r"(leader_bar), "r"(x), "r"(y)
+      : "memory");
+}
+// By one warp of each CTA of the pair.
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t *slot, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free_pair(uint32_t base, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+}
+// Arrives at the barrier of both CTAs.
+__device__ __forceinline__ void tc_commit_pair(uint32_t leader, uint64_t *bar) {
+  asm volatile(
+      "{ .reg .pred q; setp.ne.u32 q, %1, 0; @q "
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2; }" ::"r"(
+          smem_addr(bar)),
+      "r"(leader), "h"((uint16_t)3)
+      : "memory");
+}
+
 // Shared-memory operand in 128-byte swizzled rows: groups of eight rows are
 // `stride` bytes apart; `lead` is the distance of 64-element panels of a
 // transposed operand (unused otherwise).
@@ -120,9 +166,18 @@ __device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t stride, uint
          ((uint64_t)((stride >> 4) & 0x3FFF) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// int8 x int8 -> int32, M = 128: A [128, 32], B [n, 32], both K-major.
-__device__ __forceinline__ uint32_t tc_idesc_i8(int n) {
-  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+// int8 x int8 -> int32: A [m, 32], B [n, 32], both K-major; m is 128, or 256
+// over a pair (each CTA has half of A's rows, B's rows and D's rows).
+__device__ __forceinline__ uint32_t tc_idesc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma_i8_pair(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                               bool accumulate) {
+  asm volatile(
+      "{ .reg .pred p, q; setp.ne.u32 p, %4, 0; setp.ne.u32 q, %5, 0; @q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, "
+      "%2, %3, p; }" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(leader)
+      : "memory");
 }
 __device__ __forceinline__ void tc_mma_i8(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
