@@ -128,8 +128,10 @@ __device__ __forceinline__ uint32_t leader_addr(const void *p) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_addr(p)));
   return r;
 }
+// Relaxed: it orders nothing but tensor memory reads that have been waited for
+// (tc_fence_before); a release at cluster scope would wait for the stores.
 __device__ __forceinline__ void bar_arrive_leader(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
 }
 // A tile into this CTA's memory, announced to the first CTA's barrier.
 __device__ __forceinline__ void tma_load_2d_pair(void *dst, const void *map, uint32_t leader_bar, int x, int y) {
