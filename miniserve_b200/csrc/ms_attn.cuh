@@ -515,19 +515,20 @@ struct PrShared {
 };
 
 // The largest of 64 values.
+__device__ __forceinline__ float at_max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 __device__ __forceinline__ float at_max64(const float (&s)[64]) {
-  float t[8];
+  float t[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    t[i] = fmaxf(s[i], s[i + 8]);
+  for (int i = 0; i < 4; ++i) {
+    t[i] = s[i];
 #pragma unroll
-    for (int j = 16; j < 64; j += 8) t[i] = fmaxf(t[i], s[i + j]);
+    for (int j = 4; j + 4 < 60; j += 8) t[i] = at_max3(t[i], s[i + j], s[i + j + 4]);
   }
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < o; ++i) t[i] = fmaxf(t[i], t[i + o]);
-  return t[0];
+  return at_max3(at_max3(t[0], t[1], at_max3(s[60], s[61], s[62])), t[2], fmaxf(t[3], s[63]));
 }
 // Two fp32 operations an instruction.
 __device__ __forceinline__ float2 at_fma2(float2 a, float2 b, float2 c) {

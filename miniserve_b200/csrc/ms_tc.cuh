@@ -37,12 +37,13 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity) {
+static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, const volatile int *dead) {
   uint64_t t0, t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
   for (uint32_t it = 1;; ++it) {
     if (bar_try(bar, parity)) return true;
-    if ((it & 1023u) == 0u) {
+    if ((it & 63u) == 0u) {
+      if (dead && *dead) return false;
       asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
       if (t - t0 > 1000000000ull) return false;
     }
@@ -51,12 +52,14 @@ static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity)
 // Waits for the phase of the given parity; false after about 1 s.
 __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity) {
   const uint32_t b = smem_addr(bar);
-  return bar_try(b, parity) || bar_wait_slow(b, parity);
+  return bar_try(b, parity) || bar_wait_slow(b, parity, nullptr);
 }
 // For a whole warp: false, for all its lanes, where the wait ran out or another
 // warp's had.
 __device__ __forceinline__ bool bar_wait_warp(uint64_t *bar, uint32_t parity, const volatile int &dead) {
-  return __all_sync(0xFFFFFFFFu, !dead && bar_wait(bar, parity));
+  const uint32_t b = smem_addr(bar);
+  if (__all_sync(0xFFFFFFFFu, bar_try(b, parity))) return true;
+  return __all_sync(0xFFFFFFFFu, bar_wait_slow(b, parity, &dead));
 }
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
