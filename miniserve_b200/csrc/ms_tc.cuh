@@ -28,6 +28,14 @@ __device__ __forceinline__ void bar_arrive(uint64_t *bar) {
 __device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
 }
+// By the one lane of a converged warp that has `leader` set.
+__device__ __forceinline__ void bar_expect(uint32_t leader, uint64_t *bar, uint32_t bytes) {
+  asm volatile(
+      "{ .reg .pred q; setp.ne.u32 q, %2, 0; @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1; }" ::"r"(
+          smem_addr(bar)),
+      "r"(bytes), "r"(leader)
+      : "memory");
+}
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
@@ -70,11 +78,13 @@ __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // -------------------------------------------------------------------- TMA
-__device__ __forceinline__ void tma_load_2d(void *dst, const void *map, uint64_t *bar, int x, int y) {
+// By the one lane of a converged warp that has `leader` set.
+__device__ __forceinline__ void tma_load_2d(uint32_t leader, uint32_t dst, const void *map, uint32_t bar, int x, int y) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          smem_addr(dst)),
-      "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y)
+      "{ .reg .pred q; setp.ne.u32 q, %5, 0; @q "
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2]; "
+      "}" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(y), "r"(leader)
       : "memory");
 }
 __device__ __forceinline__ void tma_load_4d(void *dst, const void *map, uint64_t *bar, int x, int y, int z, int w) {
@@ -137,11 +147,13 @@ __device__ __forceinline__ void bar_arrive_leader(uint64_t *bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
 }
 // A tile into this CTA's memory, announced to the first CTA's barrier.
-__device__ __forceinline__ void tma_load_2d_pair(void *dst, const void *map, uint32_t leader_bar, int x, int y) {
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t leader, uint32_t dst, const void *map, uint32_t leader_bar,
+                                                 int x, int y) {
   asm volatile(
+      "{ .reg .pred q; setp.ne.u32 q, %5, 0; @q "
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
-      "%4}], [%2];" ::"r"(smem_addr(dst)),
-      "l"(map), "r"(leader_bar), "r"(x), "r"(y)
+      "%4}], [%2]; }" ::"r"(dst),
+      "l"(map), "r"(leader_bar), "r"(x), "r"(y), "r"(leader)
       : "memory");
 }
 // By one warp of each CTA of the pair.
