@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "../../include/mssample.h"
@@ -30,13 +31,14 @@ static int at_sms(int dev) {
 
 // Parts of the prefix for the prefix kernel: the fewest waves of CTAs (two an
 // SM) times tiles of one CTA, each CTA costing about four tiles besides (its
-// queries, first copies and record).
-static int at_parts(int64_t ctas, int64_t tiles, int sms) {
+// queries, first copies and record), and the records' way through L2, written
+// and read (about 3 MB a tile's time).
+static int at_parts(int64_t ctas, int64_t tiles, int64_t record_bytes, int sms) {
   int best = 1;
   double least = 0;
   for (int n = 1; n <= 2 * sms && n <= tiles; ++n) {
     const double waves = (double)((ctas * n + 2 * sms - 1) / (2 * sms));
-    const double cost = waves * ((double)((tiles + n - 1) / n) + 4.0);
+    const double cost = waves * ((double)((tiles + n - 1) / n) + 4.0) + (double)n * record_bytes * 2 / 3e6;
     if (n == 1 || cost < least) best = n, least = cost;
     if (ctas * n >= 4 * sms) break;
   }
@@ -57,7 +59,7 @@ static AtPlan at_plan(int64_t rows, int heads, int kv_heads, int head_dim, int64
   s.group = heads / kv_heads;
   s.chunks = (s.group + kAtRows - 1) / kAtRows;
   s.chunk_rows = s.group < kAtRows ? s.group : kAtRows;
-  s.split_warps = (int64_t)sms * kSpCtas * kSpWarps;
+  s.split_warps = (int64_t)sms * (head_dim <= 64 ? kSpCtas<64> : kSpCtas<128>) * kSpWarps;
   p.packed = (int)(rows * s.group);
   if (prefix > 0 && p.packed <= kAtRows) {
     // one chunk of query rows: the split kernel reads the prefix once as well, with more warps at it
@@ -65,7 +67,8 @@ static AtPlan at_plan(int64_t rows, int heads, int kv_heads, int head_dim, int64
     if (p.packed > s.chunk_rows) s.chunk_rows = p.packed;
   } else if (prefix > 0) {
     p.pre_tiles = (p.packed + kPrRows - 1) / kPrRows;
-    p.pre_splits = at_parts((int64_t)p.pre_tiles * kv_heads, (prefix + kPrKeys - 1) / kPrKeys, sms);
+    p.pre_splits = at_parts((int64_t)p.pre_tiles * kv_heads, (prefix + kPrKeys - 1) / kPrKeys,
+                            (int64_t)p.packed * kv_heads * head_dim * 4, sms);
   }
   const int64_t pieces = rows * kv_heads * s.chunks + (p.split_prefix ? kv_heads : 0) + s.split_warps;
   const int64_t pre = (int64_t)p.pre_splits * kv_heads * p.packed;
@@ -78,6 +81,21 @@ static AtPlan at_plan(int64_t rows, int heads, int kv_heads, int head_dim, int64
   p.bytes = at;
   return p;
 }
+
+// About how many records an output may have: the split kernel's warps spread
+// over its items, but no more than the longest item has room for.
+static int64_t at_records(const AtArgs &a) {
+  const AtShape &s = a.shape;
+  auto pieces = [&](int64_t keys, int64_t items) {
+    return std::min(s.split_warps / items + 1, (sp_tiles(keys) + kSpItem) / (kSpItem + 1) + 1);
+  };
+  int64_t n = a.pre_splits;
+  if (a.split_prefix) n += pieces(a.split_prefix, s.kv_heads);
+  const int64_t room = a.x.table_width * a.x.page_size;
+  if (room > 0) n += pieces(room, s.rows * s.kv_heads * s.chunks);
+  return n;
+}
+constexpr int64_t kMgMany = 24;
 
 template <typename F>
 static cudaError_t at_allow_shared(F *kernel, int bytes, std::atomic<int> (&ready)[kMaxDevices], int dev) {
@@ -108,9 +126,9 @@ static cudaError_t at_launch(K *kernel, int64_t grid, int threads, int shared, c
 template <typename T, int DP, int NQ, bool kWhole>
 static cudaError_t at_split(const AtArgs &a, int dev, cudaStream_t s) {
   static std::atomic<int> ready[kMaxDevices];
-  cudaError_t e = at_allow_shared(ms_attn_split_kernel<T, DP, NQ, kWhole>, kSpShared, ready, dev);
+  cudaError_t e = at_allow_shared(ms_attn_split_kernel<T, DP, NQ, kWhole>, kSpShared<DP>, ready, dev);
   if (e != cudaSuccess) return e;
-  return at_launch(ms_attn_split_kernel<T, DP, NQ, kWhole>, a.shape.split_warps / kSpWarps, kSpWarps * 32, kSpShared,
+  return at_launch(ms_attn_split_kernel<T, DP, NQ, kWhole>, a.shape.split_warps / kSpWarps, kSpWarps * 32, kSpShared<DP>,
                    s, a.pre_splits != 0, a);
 }
 
@@ -158,8 +176,9 @@ static cudaError_t at_run(AtArgs &a, int dev, cudaStream_t s) {
   }
   if (e != cudaSuccess) return e;
   const int64_t outputs = a.shape.rows * a.shape.heads;
-  if (a.merge_wide) return at_launch(ms_attn_merge_kernel<T, DP, 8>, outputs, kMgThreads, 0, s, true, a);
-  return at_launch(ms_attn_merge_kernel<T, DP, 1>, (outputs + 7) / 8, kMgThreads, 0, s, true, a);
+  if (a.merge_wide) return at_launch(ms_attn_merge_kernel<T, DP, kMgWide>, outputs, kMgWide * 32, 0, s, true, a);
+  return at_launch(ms_attn_merge_kernel<T, DP, 1>, (outputs + kMgNarrow - 1) / kMgNarrow, kMgNarrow * 32, 0, s, true,
+                   a);
 }
 
 }  // namespace ms
@@ -217,7 +236,7 @@ int ms_prefix_attention(const ms_prefix_attention_args *args, ms_stream_t stream
   a.page_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (x.page_size == 1ll << i) a.page_shift = i;
-  a.merge_wide = x.rows * x.heads <= 8 * ms::at_sms(dev);
+  a.merge_wide = ms::at_records(a) > ms::kMgMany;
   a.narrow = p.shape.chunk_rows <= 8;
   a.whole = x.page_size % ms::kSpTile == 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -17,11 +17,15 @@ constexpr int kAtRows = 16;              // query heads of one chunk: up to two 
 constexpr int64_t kAtMaxRows = 1 << 20;  // rows of a call
 constexpr int kAtMaxKeys = 0x3FFFFFFF;   // of the prefix, and of a row: their sum is an int
 constexpr int kSpWarps = 4;              // warps of a split CTA
-constexpr int kSpCtas = 2;               // split CTAs of an SM
+template <int DP>
+constexpr int kSpCtas = DP == 64 ? 4 : 2;  // split CTAs of an SM
 constexpr int kSpTile = 16;              // keys of a split tile: the M of the warp products
 constexpr int kSpItem = 2;               // cost of an item's queries and record, in tiles
-constexpr int kSpRing = 24 * 1024;       // bytes of one warp's ring of tiles
-constexpr int kSpShared = kSpRing * kSpWarps;
+constexpr int kSpStages = 2;             // tiles of a warp's ring: one is copied while the other is used
+template <int DP>
+constexpr int kSpStage = 2 * kSpTile * DP * 2;  // K, then V
+template <int DP>
+constexpr int kSpShared = kSpStages * kSpStage<DP> * kSpWarps;
 
 struct AtHeader {
   int64_t share;  // units of one split warp
@@ -133,7 +137,7 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 // of kSpItem units and one unit a tile; items without keys are not in it.
 // Row -1 is the prefix, all rows' query heads of a key head being its one
 // chunk.
-__device__ __forceinline__ int64_t sp_tiles(int64_t keys) { return (keys + kSpTile - 1) / kSpTile; }
+__host__ __device__ __forceinline__ int64_t sp_tiles(int64_t keys) { return (keys + kSpTile - 1) / kSpTile; }
 __device__ __forceinline__ int64_t sp_units(int64_t keys) { return keys > 0 ? sp_tiles(keys) + kSpItem : 0; }
 // Index of an item among the items.
 __device__ __forceinline__ int64_t sp_item(const AtArgs &a, int64_t b, int hc) {
@@ -184,12 +188,11 @@ __device__ __forceinline__ void sp_next(const AtArgs &a, SpWalk &w) {
 //
 // Bound by the bytes of the cache.
 template <typename T, int DP, int NQ, bool kWhole>
-__global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
+__global__ void __launch_bounds__(kSpWarps * 32, kSpCtas<DP>)
     ms_attn_split_kernel(const __grid_constant__ AtArgs a) {
   constexpr int kRow = DP * 2;                 // bytes of a key's row in the ring
   constexpr int kChunks = DP / 8;              // 16-byte chunks of a row
-  constexpr int kStage = 2 * kSpTile * kRow;   // K, then V
-  constexpr int kStages = kSpRing / kStage;
+  constexpr int kStage = kSpStage<DP>, kStages = kSpStages;
   constexpr int kRowsStep = 32 / kChunks;      // rows of one copy instruction
   constexpr int kThreads = kSpWarps * 32;
   const float kNone = __uint_as_float(0xFF800000u);
@@ -268,7 +271,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas)
     if (load.end <= load.tile) sp_item_next(a, load);
   }
   SpWalk now = load;
-  const uint32_t ring = smem_addr(sp_ring) + warp * kSpRing;
+  const uint32_t ring = smem_addr(sp_ring) + warp * kStages * kStage;
   const int page_size = (int)x.page_size;
   const int chunk = lane % kChunks;
   const bool inside = chunk * 8 < x.head_dim;
@@ -866,24 +869,26 @@ __global__ void __launch_bounds__(kPrThreads, 2)
   if (warp == 6) tmem_free(tmem, kPrCols);
 }
 
-// Merge: the records of a (row, query head) weighed by one warp, or by the
-// eight of a CTA where there are too few rows to fill the GPU with such CTAs
-// (kWarps); a record's entries are loaded before its weight is known.  The
-// rows' statuses are found here.
-constexpr int kMgThreads = 256;
+// Merge: the records of a (row, query head) weighed by one warp of eight in a
+// CTA, or by all sixteen of a CTA where there may be many records (kWarps); a
+// record's entries are loaded before its weight is known.  The rows' statuses
+// are found here.
+constexpr int kMgNarrow = 8;  // warps of a CTA that each have an output of their own
+constexpr int kMgWide = 16;   // warps of a CTA that share one
 
 template <typename T, int DP, int kWarps>
-__global__ void __launch_bounds__(kMgThreads) ms_attn_merge_kernel(const __grid_constant__ AtArgs a) {
+__global__ void __launch_bounds__((kWarps > 1 ? kWarps : kMgNarrow) * 32)
+    ms_attn_merge_kernel(const __grid_constant__ AtArgs a) {
   constexpr int kLanes = DP / 4;        // lanes of a record: four entries each
   constexpr int kSide = 32 / kLanes;    // records side by side
   constexpr int kBatch = 4;             // records in flight of a lane
   constexpr int kStep = kWarps * kSide;
   const float kNone = __uint_as_float(0xFF800000u);
-  __shared__ float4 part[kWarps > 1 ? kMgThreads / 32 : 1][kLanes];
-  __shared__ float2 part_ml[kMgThreads / 32];
+  __shared__ float4 part[kWarps][kLanes];
+  __shared__ float2 part_ml[kWarps];
   const ms_prefix_attention_args &x = a.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t out_row = kWarps > 1 ? blockIdx.x : (int64_t)blockIdx.x * (kMgThreads / 32) + warp;
+  const int64_t out_row = kWarps > 1 ? blockIdx.x : (int64_t)blockIdx.x * kMgNarrow + warp;
   if (out_row >= a.shape.rows * a.shape.heads) return;  // warps alone
   const int64_t b = out_row / a.shape.heads;
   const int hq = (int)(out_row - b * a.shape.heads);
@@ -968,6 +973,7 @@ __global__ void __launch_bounds__(kMgThreads) ms_attn_merge_kernel(const __grid_
     if (lane == 0) part_ml[warp] = make_float2(top, sum);
     broken = __syncthreads_or(broken);
     if (warp != 0) return;
+#pragma unroll 5
     for (int i = 1; i < kWarps; ++i) join(part_ml[i].x, part_ml[i].y, part[i][lane % kLanes]);
   }
   const int status = (raw != len ? MS_ROW_BAD_LENGTH : MS_ROW_OK) | (broken ? MS_ROW_BAD_PAGE : MS_ROW_OK);
