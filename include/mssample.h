@@ -445,7 +445,7 @@ int ms_kv_append(const ms_kv_append_args *args, ms_stream_t stream);
  *
  * head_dim is a multiple of 8, at most 128; the cache's strides are multiples
  * of 8 entries and its bases 16-byte aligned (MS_E_UNSUPPORTED otherwise).
- * scale is positive.  The struct is read on the host during the call, as for
+ * scale is positive, at most 2e38.  The struct is read on the host during the call, as for
  * ms_kv_append.  workspace: ms_prefix_attention_workspace(...) bytes of the
  * current device, 256-byte aligned, this call's until it has finished.
  */
@@ -496,7 +496,9 @@ int64_t ms_prefix_attention_workspace(int64_t rows, int32_t heads, int32_t kv_he
  * ms_int8_matmul takes xq [M, ldx] and wq [N, ldw] int8, K entries a row, the
  * row strides multiples of 16 and the bases 16-byte aligned (entries past K
  * are not used), and writes out [M, ldo] in out_dtype (fp32, bf16 or fp16;
- * rounded once from fp32).  The sum is exact: K <= 131072.  bias may be NULL.
+ * rounded once from fp32).  The sum is exact for K <= 131072 and xq within
+ * [-127, 127], as ms_quantize_rows makes it (wq may hold -128).  bias may be
+ * NULL.
  *
  * ms_int8_linear is the two in one call: x [M, ldx] as it is, the integers and
  * scales in `workspace` (ms_int8_workspace(M, K) bytes, 16-byte aligned, this

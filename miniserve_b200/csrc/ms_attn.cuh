@@ -208,6 +208,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas<DP>)
   const int64_t r0 = min(rows, tid * run), r1 = min(rows, r0 + run);
   {
     int64_t n = 0;
+#pragma unroll 8
     for (int64_t b = r0; b < r1; ++b) n += sp_units(at_length(x, b));
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas<DP>)
   const int64_t before = sp_units(a.split_prefix) * a.shape.kv_heads;
   const int64_t total = before + sums[kThreads] * hcs;
   const int64_t share = max((int64_t)kSpItem + 1, (total + a.shape.split_warps - 1) / a.shape.split_warps);
-  if (blockIdx.x == 0) {  // for the merge: where each row starts
+  if (blockIdx.x == gridDim.x - 1) {  // for the merge: where each row starts (this CTA's own share is the last, often short)
     int64_t n = sums[tid];
     for (int64_t b = r0; b < r1; ++b) {
       a.base[b] = before + n * hcs;
@@ -495,8 +496,12 @@ __global__ void __launch_bounds__(kSpWarps * 32, kSpCtas<DP>)
 // passes it by 2^8 (the weights then stay below 2^8, within fp16): O is
 // rescaled rarely.
 //
-// Bound by the exponentials (16 a clock and SM): 128 x 64 scores are 512
-// clocks, their products of 64-entry heads 64 each way.
+// Bound by the exponentials (16 a clock and SM) and, with two CTAs, by the
+// latencies between them: 128 x 64 scores are 512 clocks of exponentials and
+// take about 700 (two CTAs on an SM: 1400 each), their products of 64-entry
+// heads 64 each way.  512 rows of 14 / 2 heads of 64 behind 8192 keys: 29 us
+// (15.3 GFLOP; the exponentials alone 14 us, the products 9).  A quarter of the
+// exponentials as polynomials on the FMA pipe gained 1 % and is not done.
 constexpr int kPrThreads = 224;
 constexpr int kPrRows = 128;
 constexpr int kPrKeys = 64;    // keys of a tile

@@ -5,7 +5,8 @@
 //   s_t = max_k |x[t, k]| / 127,  q[t, k] = rint(x[t, k] / s_t)
 //   out[t, n] = s_t w_n sum_k q[t, k] wq[n, k] + bias_n
 //
-// The sum is exact in int32 (K <= 131072, so |sum| <= 127^2 K < 2^31).
+// The sum is exact in int32: with |q| <= 127 and K <= 131072 its magnitude is
+// at most 127 * 128 K < 2^31.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -169,6 +170,12 @@ static cudaError_t launch_quantize(const void *x, int dtype, int64_t M, int64_t 
 // products of cta_group::2): each loads its 128 channels and half of the
 // tokens, 64 bytes a clock, the first CTA issues the products for both, and
 // each stores its own channels.
+//
+// With their quantisation: 1 x 896 x 151936 to fp32 26.7 us (137 MB of weights,
+// 5.1 TB/s); 512 x 896 x 151936 90 us (449 MB, 77 % of the measured copy rate;
+// the stores are what is left: 71 us without them); 2048 x 4096 x 8192 to bf16
+// 56 us (2.4 POP/s, tensor pipe 79 % busy; 256 tiles over 74 pairs leave 13 %
+// of the last round idle).
 constexpr int kI8Epilogue = 8;  // warps: two for each 32 lanes of tensor memory, on alternate 16 columns
 constexpr int kI8Threads = 64 + 32 * kI8Epilogue;
 constexpr int kI8Rows = 128;    // channels of a tile

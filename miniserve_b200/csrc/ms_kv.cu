@@ -10,7 +10,10 @@
 // table row of rotary fp32 pairs per token serves all its heads.  A thread
 // owns 16 entries of a head (two 16-byte loads and stores: eight pairs, or 16
 // copied entries), keeps its eight cosines and sines in registers and turns
-// one to kKvHeads heads with them.
+// one to kKvHeads heads with them.  30011 tokens of 14 + 2 + 2 heads of 64
+// (139 MB): 29 us, 4.8 TB/s, 74 % of the measured copy rate; issue slots are
+// 60 % busy (address arithmetic and conversions) with four CTAs an SM.  512
+// tokens of 32 + 8 + 8 heads of 128 (12.7 MB): 4.1 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -115,6 +118,7 @@ __device__ __forceinline__ T *kv_target(const ms_kv_append_args &a, const KvRow 
 }
 
 constexpr int kKvThreads = 256;
+// heads of a thread: 30011 tokens take 34.8 us with one, 29.0 with two, 31.5 with three (registers)
 constexpr int kKvHeads = 2;
 
 // 16-byte path: head_dim and rotary multiples of 16, every stride a multiple

@@ -108,7 +108,8 @@ def _check_rows(name: str, t) -> int:
 
 def int8_matmul(xq, x_scale, wq, w_scale, *, bias=None, out_dtype=None, out=None):
     """``(xq @ wq.T) * x_scale[:, None] * w_scale + bias`` of integer matrices
-    ``xq`` [M, K] and ``wq`` [N, K] with fp32 scales, rows 16-byte aligned.
+    ``xq`` [M, K] and ``wq`` [N, K] with fp32 scales, rows 16-byte aligned;
+    ``xq`` within [-127, 127], as ``quantize_rows`` makes it.
     Returns [M, N] in ``out_dtype`` (default: out's type, or fp32)."""
     torch = _torch()
     _matrix("xq", xq, torch.int8)

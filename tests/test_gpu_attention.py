@@ -147,7 +147,8 @@ def test_sharp_and_growing_scores(dtype, prefix):
 
 @gpu
 @pytest.mark.parametrize("B,H,Hkv,D,prefix", [(512, 14, 2, 64, 4097), (512, 14, 2, 64, 700), (300, 32, 4, 128, 1500),
-                                              (1000, 8, 1, 64, 257), (64, 64, 8, 128, 3000)])
+                                              (1000, 8, 1, 64, 257), (64, 64, 8, 128, 3000), (5000, 4, 2, 64, 100),
+                                              (5000, 4, 2, 64, 0)])
 def test_grids_of_every_sm(B, H, Hkv, D, prefix):
     """Two CTAs on every SM, and more than one wave of them."""
     p = Problem(B, H, Hkv, D, prefix, [(7 * i) % 40 for i in range(B)], 16, "nhd", torch.bfloat16, seed=B)
