@@ -160,9 +160,10 @@ static cudaError_t launch_quantize(const void *x, int dtype, int64_t M, int64_t 
 //
 // A persistent CTA per SM walks over (channel tile, token tile) pairs, token
 // tiles fastest, so that the weights of a channel tile come from HBM once.
-// Warp 0 loads K steps of 128 bytes with TMA (128-byte swizzle, zero beyond
-// K, channels or tokens), warp 1 issues the products into one of two
-// accumulators of 256 columns, warps 2-9 scale and store the other one.
+// Warps 0 and 10 load K steps of 128 bytes of the channels and of the tokens
+// with TMA (128-byte swizzle, zero beyond K, channels or tokens), warp 1
+// issues the products into one of two accumulators of 256 columns, warps 2-9
+// scale and store the other one.
 //
 // Large batches are bound by what an SM can read (64 bytes a clock): a tile of
 // 128 channels x 256 tokens reads 96 bytes a clock at the products' full rate.
@@ -177,7 +178,7 @@ static cudaError_t launch_quantize(const void *x, int dtype, int64_t M, int64_t 
 // 56 us (2.4 POP/s, tensor pipe 79 % busy; 256 tiles over 74 pairs leave 13 %
 // of the last round idle).
 constexpr int kI8Epilogue = 8;  // warps: two for each 32 lanes of tensor memory, on alternate 16 columns
-constexpr int kI8Threads = 64 + 32 * kI8Epilogue;
+constexpr int kI8Threads = 64 + 32 * kI8Epilogue + 32;
 constexpr int kI8Rows = 128;    // channels of a tile
 constexpr int kI8Step = 128;    // bytes of K of a stage
 constexpr int kI8MaxStages = 11;
@@ -264,51 +265,34 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
-  if (warp == 0) {
+  if (warp == 0 || warp == kI8Threads / 32 - 1) {
+    // weights (announced with the tokens' bytes; they need not wait for the quantisation), and tokens
+    const bool tokens = warp != 0;
     const uint32_t leader = tc_leader();
-    const uint32_t ring0 = smem_addr(ring), full0 = kPair ? leader_addr(&sh.full[0]) : smem_addr(&sh.full[0]);
-    auto load = [&](int stage, uint32_t dst, const CUtensorMap *map, int x, int y) {
-      if (kPair) tma_load_2d_pair(leader, dst, map, full0 + stage * 8, x, y);
-      else tma_load_2d(leader, dst, map, full0 + stage * 8, x, y);
-    };
-    auto expect = [&](int stage) {  // the first CTA's barrier counts both CTAs' bytes
-      if (rank == 0) bar_expect(leader, &sh.full[stage], both * kCtas);
-    };
-    // the weights of the first stages need not wait for the quantisation
-    const int64_t mine = tiles > worker ? (tiles - worker - 1) / workers + 1 : 0;
-    const int64_t total = mine * steps;
-    const int ahead = (int)(total < a.stages ? total : a.stages);
-    for (int i = 0; i < ahead; ++i) {
-      const int64_t tile = worker + (int64_t)(i / steps) * workers;
-      expect(i);
-      load(i, ring0 + i * (wbytes + xbytes), &wmap, (i % steps) * kI8Step,
-           (int)(tile / tok_tiles) * span + (int)rank * a.rows);
-    }
-    if (a.after_quantize) grid_wait();
-    int64_t it = 0;
-    int stage = 0, use = 0;
+    const uint32_t dst0 = smem_addr(ring) + (tokens ? wbytes : 0), bytes = wbytes + xbytes;
+    const uint32_t full0 = kPair ? leader_addr(&sh.full[0]) : smem_addr(&sh.full[0]);
+    const CUtensorMap *map = tokens ? &xmap : &wmap;
+    if (tokens && a.after_quantize) grid_wait();
+    int stage = 0, phase = 1, issued = 0;
     bool ok = true;
     for (int64_t tile = worker; tile < tiles && ok; tile += workers) {
-      const int n0 = (int)(tile / tok_tiles) * span + (int)rank * a.rows;
-      const int t0 = (int)(tile % tok_tiles) * a.bn + (int)rank * (a.bn / kCtas);
-      for (int k = 0; k < steps; ++k, ++it) {
-        const uint32_t st = ring0 + stage * (wbytes + xbytes);
-        if (it >= ahead) {
-          ok = bar_wait_warp(&sh.empty[stage], (use & 1) ^ 1, sh.dead);
-          if (!ok) break;
-          expect(stage);
-          load(stage, st, &wmap, k * kI8Step, n0);
-        }
-        load(stage, st + wbytes, &xmap, k * kI8Step, t0);
-        if (++stage == a.stages) stage = 0, ++use;
+      const int row = tokens ? (int)(tile % tok_tiles) * a.bn + (int)rank * (a.bn / kCtas)
+                             : (int)(tile / tok_tiles) * span + (int)rank * a.rows;
+      for (int k = 0; k < steps; ++k) {
+        ok = bar_wait_warp(&sh.empty[stage], phase, sh.dead);
+        if (!ok) break;
+        // the first CTA's barrier counts both CTAs' bytes
+        if (!tokens && rank == 0) bar_expect(leader, &sh.full[stage], both * kCtas);
+        if (kPair) tma_load_2d_pair(leader, dst0 + stage * bytes, map, full0 + stage * 8, k * kI8Step, row);
+        else tma_load_2d(leader, dst0 + stage * bytes, map, full0 + stage * 8, k * kI8Step, row);
+        issued = min(issued + 1, a.stages);
+        if (++stage == a.stages) stage = 0, phase ^= 1;
       }
     }
     if (!ok) {  // copies in flight: their last phase of each stage, again bounded
       sh.dead = 1;
-      for (int i = 0; i < a.stages && rank == 0; ++i) {
-        const int uses = use + (i < stage ? 1 : 0);
-        if (uses > 0 && it > i) bar_wait(&sh.full[i], (uses - 1) & 1);
-      }
+      for (int i = 0; i < a.stages && rank == 0; ++i)
+        if (i < stage || issued == a.stages) bar_wait(&sh.full[i], i < stage ? phase ^ 1 : phase);
     }
   } else if (warp == 1) {
     const uint32_t leader = tc_leader();
