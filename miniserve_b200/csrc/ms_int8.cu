@@ -330,24 +330,36 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     const int quad = warp & 3;
     const int et = threadIdx.x - 64;
     if (a.after_quantize) grid_wait();
+    // a tile's scales are loaded under the tile before: a token's by each thread, this lane's channel's
+    static_assert(32 * kI8Epilogue == kI8Cols, "a thread for each token of a tile");
+    float xs = 0.f, ws = 0.f, bias = 0.f;
+    auto scales = [&](int64_t tile) {
+      if (tile >= tiles) return;
+      const int ch = (int)(tile / tok_tiles) * span + (int)rank * a.rows + quad * 32 + lane;
+      const int t = (int)(tile % tok_tiles) * a.bn + et;
+      if (et < a.bn && t < a.M) xs = __ldg(a.x_scale + t);
+      const bool live = quad * 32 + lane < a.rows && ch < a.N;
+      ws = live ? __ldg(a.w_scale + ch) : 0.f;
+      bias = live && a.bias ? __ldg(a.bias + ch) : 0.f;
+    };
+    scales(worker);
     int n = 0;
     for (int64_t tile = worker; tile < tiles; tile += workers, ++n) {
       const int acc = n & 1;
       const int n0 = (int)(tile / tok_tiles) * span + (int)rank * a.rows, t0 = (int)(tile % tok_tiles) * a.bn;
       const int count = min(a.bn, a.M - t0);
-      for (int i = et; i < count; i += 32 * kI8Epilogue) sh.xs[acc][i] = __ldg(a.x_scale + t0 + i);
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * kI8Epilogue) : "memory");
       const int ch = quad * 32 + lane < a.rows ? n0 + quad * 32 + lane : a.N;  // a.N: not a channel of this tile
-      const float ws = ch < a.N ? __ldg(a.w_scale + ch) : 0.f;
-      const float bias = a.bias && ch < a.N ? __ldg(a.bias + ch) : 0.f;
+      const float scale = ws, add = bias;
+      sh.xs[acc][et] = xs;
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kI8Epilogue) : "memory");
+      scales(tile + workers);
       if (!sh.dead && !bar_wait(&sh.acc_full[acc], (n >> 1) & 1)) sh.dead = 1;
       __syncwarp();
       tc_fence_after();
-      const bool dead = sh.dead != 0;
+      const float factor = sh.dead ? __uint_as_float(0x7FC00000u) : scale;
       const int first = (warp - 2) / 4 * 16;
       T *out = static_cast<T *>(a.out) + (int64_t)(t0 + first) * a.ldo + ch;
       const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + acc * kI8Cols;
-      const float scale = dead ? __uint_as_float(0x7FC00000u) : ws;
       constexpr int kNext = kI8Epilogue * 4;  // columns to this warp's next 16
       uint32_t r[2][16];  // the next 16 columns are read under the stores of these
       if (first < count) tmem_ld16(from + first, r[0]);
@@ -361,9 +373,9 @@ __global__ void __launch_bounds__(kI8Threads, 1)
           if (at + kNext < count) tmem_ld16(from + at + kNext, r[k ^ 1]);
           if (ch < a.N) {
             if (at + 16 <= count)
-              i8_columns<T, true>(r[k], sh.xs[acc] + at, scale, bias, out, a.ldo, 16);
+              i8_columns<T, true>(r[k], sh.xs[acc] + at, factor, add, out, a.ldo, 16);
             else
-              i8_columns<T, false>(r[k], sh.xs[acc] + at, scale, bias, out, a.ldo, count - at);
+              i8_columns<T, false>(r[k], sh.xs[acc] + at, factor, add, out, a.ldo, count - at);
           }
           __syncwarp();
           out += kNext * a.ldo;
