@@ -396,7 +396,8 @@ int ms_mask_from_logits(const void *logits, int dtype, int64_t B, int64_t V, int
  * This struct is read on the host during the call; its pointers are device
  * pointers and its strides count entries (the last dimension is contiguous).
  * 16-byte accesses are used where head_dim and rotary are multiples of 16,
- * strides of 8 and bases 16-byte aligned, single entries otherwise.
+ * strides of 8 and bases 16-byte aligned, 8-byte ones for half of that, single
+ * entries otherwise.
  */
 typedef struct {
   int32_t dtype;        /* MS_DTYPE_BF16 or MS_DTYPE_F16: q, k, v and the caches */

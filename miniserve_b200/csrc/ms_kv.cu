@@ -121,22 +121,34 @@ constexpr int kKvThreads = 256;
 // heads of a thread: 30011 tokens take 34.8 us with one, 29.0 with two, 31.5 with three (registers)
 constexpr int kKvHeads = 2;
 
-// 16-byte path: head_dim and rotary multiples of 16, every stride a multiple
-// of 8 entries and every base 16-byte aligned (checked on the host).  Threads
-// are (chunk of 16 entries, head slot, token); a slot is up to kHeads heads of
-// one of q, k and v, so that a thread finds its addresses once and steps along
-// them.  Its loads are issued before anything that depends on the token's
-// slot, position and table row.
-template <typename T, bool kInterleaved, int kHeads>
+// kV entries (8: 16 bytes, 4: 8 bytes) at once: the halves that a thread owns.
+template <int kV>
+struct KvVec;
+template <>
+struct KvVec<8> {
+  uint4 v;
+};
+template <>
+struct KvVec<4> {
+  uint2 v;
+};
+
+// Wide path: head_dim and rotary multiples of 2 kV, every stride a multiple of
+// kV entries and every base aligned to them (checked on the host).  Threads
+// are (chunk of 2 kV entries, head slot, token); a slot is up to kHeads heads
+// of one of q, k and v, so that a thread finds its addresses once and steps
+// along them.  Its loads are issued before anything that depends on the
+// token's slot, position and table row.
+template <typename T, bool kInterleaved, int kHeads, int kV>
 __global__ void __launch_bounds__(kKvThreads, 4) ms_kv_append_kernel(const __grid_constant__ KvArgs p) {
   const ms_kv_append_args &a = p.a;
   const int j = threadIdx.x;
   const int64_t t = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
   if (t >= a.tokens) return;
-  const bool rotates = j * 16 < a.rotary;
-  // entries of the two 16-byte halves a rotating thread owns
-  const int lo = (!rotates || kInterleaved) ? j * 16 : j * 8;
-  const int hi = (!rotates || kInterleaved) ? lo + 8 : lo + (a.rotary >> 1);
+  const bool rotates = j * 2 * kV < a.rotary;
+  // entries of the two halves a rotating thread owns
+  const int lo = (!rotates || kInterleaved) ? j * 2 * kV : j * kV;
+  const int hi = (!rotates || kInterleaved) ? lo + kV : lo + (a.rotary >> 1);
   for (int slot = threadIdx.y; slot < p.slots; slot += blockDim.y) {
     // the slot's heads: h, h + step, ... of q, k or v
     const bool query = slot < p.q_slots, key = !query && slot < p.q_slots + p.kv_slots;
@@ -145,14 +157,14 @@ __global__ void __launch_bounds__(kKvThreads, 4) ms_kv_append_kernel(const __gri
     const int64_t src_head = query ? a.q_head : key ? a.k_head : a.v_head;
     const T *src = static_cast<const T *>(query ? a.q : key ? a.k : a.v) +
                    t * (query ? a.q_token : key ? a.k_token : a.v_token) + h * src_head;
-    uint4 x[kHeads], y[kHeads];
+    KvVec<kV> x[kHeads], y[kHeads];
     {
       const T *from = src;
 #pragma unroll
       for (int i = 0; i < kHeads; ++i) {
         if (h + i * step < heads) {
-          x[i] = *reinterpret_cast<const uint4 *>(from + lo);
-          y[i] = *reinterpret_cast<const uint4 *>(from + hi);
+          x[i] = *reinterpret_cast<const KvVec<kV> *>(from + lo);
+          y[i] = *reinterpret_cast<const KvVec<kV> *>(from + hi);
         }
         from += step * src_head;
       }
@@ -160,15 +172,15 @@ __global__ void __launch_bounds__(kKvThreads, 4) ms_kv_append_kernel(const __gri
     const KvRow r = kv_row(p, t);
     if (slot == 0 && j == 0 && a.status) a.status[t] = r.status;
     if (!query && !r.write) continue;
-    float c[8], s[8];
+    float c[kV], s[kV];
     const bool turns = rotates && (query || key);
     if (turns) {
-      const float *row = a.table + r.position * a.rotary + j * 8;
-      *reinterpret_cast<float4 *>(c) = __ldg(reinterpret_cast<const float4 *>(row));
-      *reinterpret_cast<float4 *>(c + 4) = __ldg(reinterpret_cast<const float4 *>(row) + 1);
-      row += a.rotary >> 1;
-      *reinterpret_cast<float4 *>(s) = __ldg(reinterpret_cast<const float4 *>(row));
-      *reinterpret_cast<float4 *>(s + 4) = __ldg(reinterpret_cast<const float4 *>(row) + 1);
+      const float *row = a.table + r.position * a.rotary + j * kV;
+#pragma unroll
+      for (int i = 0; i < kV; i += 4) {
+        *reinterpret_cast<float4 *>(c + i) = __ldg(reinterpret_cast<const float4 *>(row + i));
+        *reinterpret_cast<float4 *>(s + i) = __ldg(reinterpret_cast<const float4 *>(row + (a.rotary >> 1) + i));
+      }
     }
     const int64_t dst_head = query ? a.q_out_head : key ? a.ck_head : a.cv_head;
     T *dst = static_cast<T *>(query ? a.q_out : key ? a.cache_k : a.cache_v) + h * dst_head;
@@ -180,14 +192,14 @@ __global__ void __launch_bounds__(kKvThreads, 4) ms_kv_append_kernel(const __gri
       if (h + i * step >= heads) break;
       uint32_t *xs = reinterpret_cast<uint32_t *>(&x[i]), *ys = reinterpret_cast<uint32_t *>(&y[i]);
       if (r.status & MS_ROW_BAD_POSITION) {
-        x[i] = y[i] = make_uint4(0, 0, 0, 0);
+        x[i] = y[i] = KvVec<kV>{};
       } else if (turns) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < kV / 2; ++k) {
           const float2 f = kv_widen<T>(xs[k]), g = kv_widen<T>(ys[k]);
-          if (kInterleaved) {  // word k of x is pair k, word k of y is pair 4 + k
+          if (kInterleaved) {  // word k of x is pair k, word k of y is pair kV / 2 + k
             xs[k] = kv_narrow<T>(f.x * c[k] - f.y * s[k], f.y * c[k] + f.x * s[k]);
-            ys[k] = kv_narrow<T>(g.x * c[4 + k] - g.y * s[4 + k], g.y * c[4 + k] + g.x * s[4 + k]);
+            ys[k] = kv_narrow<T>(g.x * c[kV / 2 + k] - g.y * s[kV / 2 + k], g.y * c[kV / 2 + k] + g.x * s[kV / 2 + k]);
           } else {  // word k holds the first (x) and second (y) entries of pairs 2k and 2k + 1
             const float c0 = c[2 * k], c1 = c[2 * k + 1], s0 = s[2 * k], s1 = s[2 * k + 1];
             xs[k] = kv_narrow<T>(f.x * c0 - g.x * s0, f.y * c1 - g.y * s1);
@@ -195,8 +207,8 @@ __global__ void __launch_bounds__(kKvThreads, 4) ms_kv_append_kernel(const __gri
           }
         }
       }
-      *reinterpret_cast<uint4 *>(dst + lo) = x[i];
-      *reinterpret_cast<uint4 *>(dst + hi) = y[i];
+      *reinterpret_cast<KvVec<kV> *>(dst + lo) = x[i];
+      *reinterpret_cast<KvVec<kV> *>(dst + hi) = y[i];
       dst += step * dst_head;
     }
   }
@@ -253,36 +265,44 @@ __global__ void __launch_bounds__(kKvThreads) ms_kv_append_any_kernel(const __gr
   }
 }
 
-template <typename T>
-cudaError_t launch_kv_append(KvArgs &p, bool wide, cudaStream_t s) {
+template <typename T, int kV>
+void launch_kv_wide(KvArgs &p, int each, cudaStream_t s) {
   const ms_kv_append_args &a = p.a;
-  const int heads = a.heads + 2 * a.kv_heads;
-  const int units = wide ? a.head_dim / 16 : a.rotary / 2 + (a.head_dim - a.rotary + 1) / 2;
-  // one head a thread until the call fills the GPU's threads a few times
-  // over; then up to kKvHeads, which share the thread's table row
-  const int each = a.tokens * heads * units > 4ll * 148 * 2048 ? kKvHeads : 1;
-  if (wide) {
-    p.q_slots = (a.heads + each - 1) / each;
-    p.kv_slots = (a.kv_heads + each - 1) / each;
-    p.slots = p.q_slots + 2 * p.kv_slots;
-    const int y = p.slots < kKvThreads / units ? p.slots : kKvThreads / units;
-    const int z = kKvThreads / (units * y) < 64 ? kKvThreads / (units * y) : 64;
-    auto *kernel = a.interleaved ? ms_kv_append_kernel<T, true, 1> : ms_kv_append_kernel<T, false, 1>;
-    if (each > 1)
-      kernel = a.interleaved ? ms_kv_append_kernel<T, true, kKvHeads> : ms_kv_append_kernel<T, false, kKvHeads>;
-    kernel<<<(unsigned)((a.tokens + z - 1) / z), dim3(units, y, z), 0, s>>>(p);
-    return cudaGetLastError();
-  }
-  p.slots = (heads + each - 1) / each;
-  p.per_token = units * p.slots;
-  p.tokens_cta = p.per_token < kKvThreads ? kKvThreads / p.per_token : 1;
-  const unsigned grid = (unsigned)((a.tokens + p.tokens_cta - 1) / p.tokens_cta);
-  auto *kernel = a.interleaved ? ms_kv_append_any_kernel<T, true> : ms_kv_append_any_kernel<T, false>;
-  kernel<<<grid, kKvThreads, 0, s>>>(p);
-  return cudaGetLastError();
+  const int units = a.head_dim / (2 * kV);
+  p.q_slots = (a.heads + each - 1) / each;
+  p.kv_slots = (a.kv_heads + each - 1) / each;
+  p.slots = p.q_slots + 2 * p.kv_slots;
+  const int y = p.slots < kKvThreads / units ? p.slots : kKvThreads / units;
+  const int z = kKvThreads / (units * y) < 64 ? kKvThreads / (units * y) : 64;
+  auto *kernel = a.interleaved ? ms_kv_append_kernel<T, true, 1, kV> : ms_kv_append_kernel<T, false, 1, kV>;
+  if (each > 1)
+    kernel = a.interleaved ? ms_kv_append_kernel<T, true, kKvHeads, kV> : ms_kv_append_kernel<T, false, kKvHeads, kV>;
+  kernel<<<(unsigned)((a.tokens + z - 1) / z), dim3(units, y, z), 0, s>>>(p);
 }
 
-static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// `wide`: entries that can be moved at once (8, 4 or 1).
+template <typename T>
+cudaError_t launch_kv_append(KvArgs &p, int wide, cudaStream_t s) {
+  const ms_kv_append_args &a = p.a;
+  const int heads = a.heads + 2 * a.kv_heads;
+  // one head a thread until the call fills the GPU's threads a few times
+  // over; then up to kKvHeads, which share the thread's table row
+  const int each = a.tokens * heads * a.head_dim > 16 * 4ll * 148 * 2048 ? kKvHeads : 1;
+  if (wide == 8) {
+    launch_kv_wide<T, 8>(p, each, s);
+  } else if (wide == 4) {
+    launch_kv_wide<T, 4>(p, each, s);
+  } else {
+    const int units = a.rotary / 2 + (a.head_dim - a.rotary + 1) / 2;
+    p.slots = (heads + each - 1) / each;
+    p.per_token = units * p.slots;
+    p.tokens_cta = p.per_token < kKvThreads ? kKvThreads / p.per_token : 1;
+    const unsigned grid = (unsigned)((a.tokens + p.tokens_cta - 1) / p.tokens_cta);
+    auto *kernel = a.interleaved ? ms_kv_append_any_kernel<T, true> : ms_kv_append_any_kernel<T, false>;
+    kernel<<<grid, kKvThreads, 0, s>>>(p);
+  }
+  return cudaGetLastError();
+}
 
 }  // namespace ms
 
@@ -301,16 +321,22 @@ extern "C" int ms_kv_append(const ms_kv_append_args *args, ms_stream_t stream) {
   if (!a.k || !a.v || !a.slots || !a.cache_k || !a.cache_v) return MS_E_INVALID;
   if (a.heads > 0 && (!a.q || !a.q_out)) return MS_E_INVALID;
   if (a.rotary > 0 && (!a.positions || !a.table || a.table_rows < 1)) return MS_E_INVALID;
-  bool wide = a.head_dim % 16 == 0 && a.rotary % 16 == 0 && ms::aligned16(a.k) && ms::aligned16(a.v) &&
-              ms::aligned16(a.cache_k) && ms::aligned16(a.cache_v) && (a.rotary == 0 || ms::aligned16(a.table)) &&
-              (a.heads == 0 || (ms::aligned16(a.q) && ms::aligned16(a.q_out)));
+  // the widest pieces that sizes, strides and bases allow (the table is read in 16 bytes either way)
+  uint64_t bases = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                   reinterpret_cast<uintptr_t>(a.cache_k) | reinterpret_cast<uintptr_t>(a.cache_v);
+  if (a.heads > 0) bases |= reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out);
   p.page_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (a.page_size == 1ll << i) p.page_shift = i;
   int64_t strides = a.k_token | a.k_head | a.v_token | a.v_head | a.ck_page | a.ck_token | a.ck_head | a.cv_page |
                     a.cv_token | a.cv_head;
   if (a.heads > 0) strides |= a.q_token | a.q_head | a.q_out_token | a.q_out_head;
-  wide = wide && (strides & 7) == 0;
+  const bool table = a.rotary == 0 || (reinterpret_cast<uintptr_t>(a.table) & 15) == 0;
+  auto fits = [&](int v) {
+    return a.head_dim % (2 * v) == 0 && a.head_dim / (2 * v) <= ms::kKvThreads && a.rotary % (2 * v) == 0 && table &&
+           (strides & (v - 1)) == 0 && (bases & (2 * v - 1)) == 0;
+  };
+  const int wide = fits(8) ? 8 : fits(4) ? 4 : 1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = a.dtype == MS_DTYPE_BF16 ? ms::launch_kv_append<__nv_bfloat16>(p, wide, s)
                                            : ms::launch_kv_append<__half>(p, wide, s);

@@ -117,9 +117,9 @@ def test_table_is_the_definition():
 
 
 @gpu
-@pytest.mark.parametrize("dim,offset", [(64, 0), (64, 1), (40, 0)])
+@pytest.mark.parametrize("dim,offset", [(64, 0), (64, 4), (64, 1), (40, 0)])
 def test_in_place_and_unaligned(dim, offset):
-    """q rotated in place; bases off the 16-byte grid take the single-entry path."""
+    """q rotated in place; bases off the 16-byte grid take the 8-byte or the single-entry path."""
     from miniserve_b200.kvcache import append_kv, rope_table
     dtype, T, H = torch.bfloat16, 19, 4
     gen = torch.Generator(device="cuda").manual_seed(3)
