@@ -59,7 +59,7 @@ static AtPlan at_plan(int64_t rows, int heads, int kv_heads, int head_dim, int64
   s.group = heads / kv_heads;
   s.chunks = (s.group + kAtRows - 1) / kAtRows;
   s.chunk_rows = s.group < kAtRows ? s.group : kAtRows;
-  s.split_warps = (int64_t)sms * (head_dim <= 64 ? kSpCtas<64> : kSpCtas<128>) * kSpWarps;
+  s.split_warps = (int64_t)sms * sp_ctas(head_dim) * kSpWarps;
   p.packed = (int)(rows * s.group);
   if (prefix > 0 && p.packed <= kAtRows) {
     // one chunk of query rows: the split kernel reads the prefix once as well, with more warps at it
@@ -125,13 +125,19 @@ static cudaError_t at_launch(K *kernel, int64_t grid, int threads, int shared, c
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-template <typename T, int DP, int NQ, bool kWhole>
+template <typename T, int DP, int NQ, bool kWhole, int kCtas>
 static cudaError_t at_split(const AtArgs &a, int dev, cudaStream_t s) {
   static std::atomic<int> ready[kMaxDevices];
-  cudaError_t e = at_allow_shared(ms_attn_split_kernel<T, DP, NQ, kWhole>, kSpShared<DP>, ready, dev);
+  auto *kernel = ms_attn_split_kernel<T, DP, NQ, kWhole, kCtas>;
+  cudaError_t e = at_allow_shared(kernel, kSpShared<DP>, ready, dev);
   if (e != cudaSuccess) return e;
-  return at_launch(ms_attn_split_kernel<T, DP, NQ, kWhole>, a.shape.split_warps / kSpWarps, kSpWarps * 32, kSpShared<DP>,
-                   s, a.pre_splits != 0, a);
+  return at_launch(kernel, a.shape.split_warps / kSpWarps, kSpWarps * 32, kSpShared<DP>, s, a.pre_splits != 0, a);
+}
+
+template <typename T, int DP, int kCtas>
+static cudaError_t at_split_as(const AtArgs &a, int dev, cudaStream_t s) {
+  if (a.narrow) return a.whole ? at_split<T, DP, 1, true, kCtas>(a, dev, s) : at_split<T, DP, 1, false, kCtas>(a, dev, s);
+  return a.whole ? at_split<T, DP, 2, true, kCtas>(a, dev, s) : at_split<T, DP, 2, false, kCtas>(a, dev, s);
 }
 
 // One of the caches as [pages, kv_heads, page_size, head_dim], read in boxes of
@@ -170,12 +176,11 @@ static cudaError_t at_run(AtArgs &a, int dev, cudaStream_t s) {
       e = at_launch(ms_attn_prefix_kernel<T, DP>, (int64_t)a.pre_tiles * a.shape.kv_heads * a.pre_splits, kPrThreads,
                     kPrSharedBytes<DP>, s, false, a, kmap, vmap);
   }
-  if (e == cudaSuccess) {
-    if (a.narrow)
-      e = a.whole ? at_split<T, DP, 1, true>(a, dev, s) : at_split<T, DP, 1, false>(a, dev, s);
-    else
-      e = a.whole ? at_split<T, DP, 2, true>(a, dev, s) : at_split<T, DP, 2, false>(a, dev, s);
-  }
+  if (e != cudaSuccess) return e;
+  if constexpr (DP == 64)
+    e = at_split_as<T, DP, sp_ctas(64)>(a, dev, s);
+  else
+    e = a.x.head_dim <= 96 ? at_split_as<T, DP, sp_ctas(96)>(a, dev, s) : at_split_as<T, DP, sp_ctas(128)>(a, dev, s);
   if (e != cudaSuccess) return e;
   const int64_t outputs = a.shape.rows * a.shape.heads;
   if (a.merge_wide) return at_launch(ms_attn_merge_kernel<T, DP, kMgWide>, outputs, kMgWide * 32, 0, s, true, a);

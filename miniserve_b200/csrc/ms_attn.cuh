@@ -17,8 +17,10 @@ constexpr int kAtRows = 16;              // query heads of one chunk: up to two 
 constexpr int64_t kAtMaxRows = 1 << 20;  // rows of a call
 constexpr int kAtMaxKeys = 0x3FFFFFFF;   // of the prefix, and of a row: their sum is an int
 constexpr int kSpWarps = 4;              // warps of a split CTA
-template <int DP>
-constexpr int kSpCtas = DP == 64 ? 4 : 2;  // split CTAs of an SM
+// Split CTAs of an SM: what heads of fewer entries leave of the latencies is
+// hidden by more warps (64 rows of 4 key heads of 80: 76 us with two, 66 with
+// three; of 128: 90 with two, 96 with three).
+__host__ __device__ constexpr int sp_ctas(int head_dim) { return head_dim <= 64 ? 4 : head_dim <= 96 ? 3 : 2; }
 constexpr int kSpTile = 16;              // keys of a split tile: the M of the warp products
 constexpr int kSpItem = 2;               // cost of an item's queries and record, in tiles
 constexpr int kSpStages = 2;             // tiles of a warp's ring: one is copied while the other is used
@@ -187,8 +189,8 @@ __device__ __forceinline__ void sp_next(const AtArgs &a, SpWalk &w) {
 // because both only grow along the sequence.
 //
 // Bound by the bytes of the cache.
-template <typename T, int DP, int NQ, bool kWhole>
-__global__ void __launch_bounds__(kSpWarps * 32, kSpCtas<DP>)
+template <typename T, int DP, int NQ, bool kWhole, int kCtas>
+__global__ void __launch_bounds__(kSpWarps * 32, kCtas)
     ms_attn_split_kernel(const __grid_constant__ AtArgs a) {
   constexpr int kRow = DP * 2;                 // bytes of a key's row in the ring
   constexpr int kChunks = DP / 8;              // 16-byte chunks of a row

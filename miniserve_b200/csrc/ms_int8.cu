@@ -172,11 +172,10 @@ static cudaError_t launch_quantize(const void *x, int dtype, int64_t M, int64_t 
 // tokens, 64 bytes a clock, the first CTA issues the products for both, and
 // each stores its own channels.
 //
-// With their quantisation: 1 x 896 x 151936 to fp32 26.7 us (137 MB of weights,
-// 5.1 TB/s); 512 x 896 x 151936 90 us (449 MB, 77 % of the measured copy rate;
-// the stores are what is left: 71 us without them); 2048 x 4096 x 8192 to bf16
-// 56 us (2.4 POP/s, tensor pipe 79 % busy; 256 tiles over 74 pairs leave 13 %
-// of the last round idle).
+// With their quantisation: 1 x 896 x 151936 to fp32 26.1 us (137 MB of weights,
+// 5.3 TB/s); 512 x 896 x 151936 85 us (449 MB, 5.3 TB/s, 81 % of the measured
+// copy rate); 2048 x 4096 x 8192 to bf16 56 us (2.4 POP/s, tensor pipe 79 %
+// busy; 256 tiles over 74 pairs leave 13 % of the rounds idle).
 constexpr int kI8Epilogue = 8;  // warps: two for each 32 lanes of tensor memory, on alternate 16 columns
 constexpr int kI8Threads = 64 + 32 * kI8Epilogue + 32;
 constexpr int kI8Rows = 128;    // channels of a tile
