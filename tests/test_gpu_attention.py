@@ -120,6 +120,10 @@ CASES = [
     (3, 4, 2, 64, 0, [0, 0, 0], 16, "nhd"),
     (3, 6, 2, 56, 0, [0, 5000, 1], 16, "nhd"),
     (8, 8, 2, 64, 20000, [3] * 8, 16, "nhd"),
+    (40, 4, 2, 48, 300, [i % 19 for i in range(40)], 16, "nhd"),   # boxes wider than a head
+    (40, 4, 1, 24, 200, [i % 7 for i in range(40)], 32, "hnd"),
+    (40, 4, 1, 72, 333, [i % 33 for i in range(40)], 128, "nhd"),
+    (21, 5, 5, 88, 640, [40] * 21, 8, "hnd"),
     (2, 2, 1, 128, 9000, [6000, 7], 48, "nhd"),
 ]
 
