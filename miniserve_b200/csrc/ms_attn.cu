@@ -108,30 +108,13 @@ static cudaError_t at_allow_shared(F *kernel, int bytes, std::atomic<int> (&read
   return e;
 }
 
-template <typename K, typename... A>
-static cudaError_t at_launch(K *kernel, int64_t grid, int threads, int shared, cudaStream_t s, bool dependent,
-                             const A &...args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = shared;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 1 : 0;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-  return e != cudaSuccess ? e : cudaGetLastError();
-}
-
 template <typename T, int DP, int NQ, bool kWhole, int kCtas>
 static cudaError_t at_split(const AtArgs &a, int dev, cudaStream_t s) {
   static std::atomic<int> ready[kMaxDevices];
   auto *kernel = ms_attn_split_kernel<T, DP, NQ, kWhole, kCtas>;
   cudaError_t e = at_allow_shared(kernel, kSpShared<DP>, ready, dev);
   if (e != cudaSuccess) return e;
-  return at_launch(kernel, a.shape.split_warps / kSpWarps, kSpWarps * 32, kSpShared<DP>, s, a.pre_splits != 0, a);
+  return launch_dependent(kernel, (unsigned)(a.shape.split_warps / kSpWarps), kSpWarps * 32, kSpShared<DP>, s, a);
 }
 
 template <typename T, int DP, int kCtas>
@@ -173,8 +156,8 @@ static cudaError_t at_run(AtArgs &a, int dev, cudaStream_t s) {
     a.tma = at_map(&kmap, a.x, a.x.cache_k, a.x.ck_page, a.x.ck_token, a.x.ck_head) &&
             at_map(&vmap, a.x, a.x.cache_v, a.x.cv_page, a.x.cv_token, a.x.cv_head);
     if (e == cudaSuccess)
-      e = at_launch(ms_attn_prefix_kernel<T, DP>, (int64_t)a.pre_tiles * a.shape.kv_heads * a.pre_splits, kPrThreads,
-                    kPrSharedBytes<DP>, s, false, a, kmap, vmap);
+      e = launch_dependent(ms_attn_prefix_kernel<T, DP>, (unsigned)((int64_t)a.pre_tiles * a.shape.kv_heads * a.pre_splits),
+                           kPrThreads, kPrSharedBytes<DP>, s, a, kmap, vmap);
   }
   if (e != cudaSuccess) return e;
   if constexpr (DP == 64)
@@ -183,9 +166,10 @@ static cudaError_t at_run(AtArgs &a, int dev, cudaStream_t s) {
     e = a.x.head_dim <= 96 ? at_split_as<T, DP, sp_ctas(96)>(a, dev, s) : at_split_as<T, DP, sp_ctas(128)>(a, dev, s);
   if (e != cudaSuccess) return e;
   const int64_t outputs = a.shape.rows * a.shape.heads;
-  if (a.merge_wide) return at_launch(ms_attn_merge_kernel<T, DP, kMgWide>, outputs, kMgWide * 32, 0, s, true, a);
-  return at_launch(ms_attn_merge_kernel<T, DP, 1>, (outputs + kMgNarrow - 1) / kMgNarrow, kMgNarrow * 32, 0, s, true,
-                   a);
+  if (a.merge_wide)
+    return launch_dependent(ms_attn_merge_kernel<T, DP, kMgWide>, (unsigned)outputs, kMgWide * 32, 0, s, a);
+  return launch_dependent(ms_attn_merge_kernel<T, DP, 1>, (unsigned)((outputs + kMgNarrow - 1) / kMgNarrow),
+                          kMgNarrow * 32, 0, s, a);
 }
 
 }  // namespace ms

@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kCtas)
   extern __shared__ __align__(128) unsigned char sp_ring[];
   __shared__ int64_t sums[kThreads + 1];  // units of the rows before each thread's run of rows, of one key head and chunk
   __shared__ int64_t warp_sums[kSpWarps];
+  if (!a.pre_splits) grid_wait();  // the call's first kernel
   grid_release();
   const ms_prefix_attention_args &x = a.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -564,7 +565,6 @@ __global__ void __launch_bounds__(kPrThreads, 2)
   constexpr int KT = kPrKeys, kStages = kPrStages<DP>, kStage = kPrStage<DP>;
   extern __shared__ __align__(1024) unsigned char pr_raw[];
   __shared__ PrShared sh;
-  grid_release();
   unsigned char *qs = pr_raw + ((1024u - (smem_addr(pr_raw) & 1023u)) & 1023u);
   unsigned char *ring = qs + kPrRows * DP * 2;
   const ms_prefix_attention_args &x = a.x;
@@ -602,6 +602,8 @@ __global__ void __launch_bounds__(kPrThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
+  grid_wait();  // the call's first kernel
+  grid_release();
 
   if (warp < 4) {
     // the warp's 32 query rows, in 128-byte swizzled panels of 64 entries: a row is read by neighbouring lanes

@@ -68,7 +68,8 @@ constexpr int kQuKeep = 4;
 template <typename T, bool kWide>
 __global__ void __launch_bounds__(kQuThreads) ms_quantize_kernel(const T *x, int64_t ldx, int K, int8_t *q, int64_t ldq,
                                                                float *scale) {
-  grid_release();
+  grid_wait();     // the call's first kernel: what it reads, and the weights, are in memory
+  grid_release();  // before the product may load weights
   __shared__ uint32_t red[kQuThreads / 32];
   constexpr int kEach = kWide ? 8 : 1;  // entries of a unit
   constexpr int kKeep = kWide ? kQuKeep : 4 * kQuKeep;
@@ -134,10 +135,10 @@ __global__ void __launch_bounds__(kQuThreads) ms_quantize_kernel(const T *x, int
 }
 
 template <typename T>
-static void run_quantize(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q, int64_t ldq, float *scale,
+static cudaError_t run_quantize(const void *x, int64_t M, int64_t K, int64_t ldx, int8_t *q, int64_t ldq, float *scale,
                          bool wide, cudaStream_t s) {
   auto *kernel = wide ? ms_quantize_kernel<T, true> : ms_quantize_kernel<T, false>;
-  kernel<<<(unsigned)M, kQuThreads, 0, s>>>(static_cast<const T *>(x), ldx, (int)K, q, ldq, scale);
+  return launch_dependent(kernel, (unsigned)M, kQuThreads, 0, s, static_cast<const T *>(x), ldx, (int)K, q, ldq, scale);
 }
 
 static cudaError_t launch_quantize(const void *x, int dtype, int64_t M, int64_t K, int64_t ldx, int8_t *q, int64_t ldq,
@@ -145,10 +146,9 @@ static cudaError_t launch_quantize(const void *x, int dtype, int64_t M, int64_t 
   const int esz = dtype == MS_DTYPE_F32 ? 4 : 2;
   const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * esz) % 16 == 0 &&
                     (reinterpret_cast<uintptr_t>(q) & 7) == 0 && ldq % 8 == 0;
-  if (dtype == MS_DTYPE_F32) run_quantize<float>(x, M, K, ldx, q, ldq, scale, wide, s);
-  else if (dtype == MS_DTYPE_BF16) run_quantize<__nv_bfloat16>(x, M, K, ldx, q, ldq, scale, wide, s);
-  else run_quantize<__half>(x, M, K, ldx, q, ldq, scale, wide, s);
-  return cudaGetLastError();
+  if (dtype == MS_DTYPE_F32) return run_quantize<float>(x, M, K, ldx, q, ldq, scale, wide, s);
+  if (dtype == MS_DTYPE_BF16) return run_quantize<__nv_bfloat16>(x, M, K, ldx, q, ldq, scale, wide, s);
+  return run_quantize<__half>(x, M, K, ldx, q, ldq, scale, wide, s);
 }
 
 // ----------------------------------------------------------------- product

@@ -20,6 +20,7 @@
 
 #include "../../include/mssample.h"
 #include "ms_host.h"
+#include "ms_tc.cuh"
 
 namespace ms {
 
@@ -141,6 +142,7 @@ struct KvVec<4> {
 // token's slot, position and table row.
 template <typename T, bool kInterleaved, int kHeads, int kV>
 __global__ void __launch_bounds__(kKvThreads, 4) ms_kv_append_kernel(const __grid_constant__ KvArgs p) {
+  grid_wait();
   const ms_kv_append_args &a = p.a;
   const int j = threadIdx.x;
   const int64_t t = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
@@ -218,6 +220,7 @@ __global__ void __launch_bounds__(kKvThreads, 4) ms_kv_append_kernel(const __gri
 // entries, of a head.
 template <typename T, bool kInterleaved>
 __global__ void __launch_bounds__(kKvThreads) ms_kv_append_any_kernel(const __grid_constant__ KvArgs p) {
+  grid_wait();
   const ms_kv_append_args &a = p.a;
   const int half = a.rotary >> 1;
   const int units = half + (a.head_dim - a.rotary + 1) / 2;
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(kKvThreads) ms_kv_append_any_kernel(const __gr
 }
 
 template <typename T, int kV>
-void launch_kv_wide(KvArgs &p, int each, cudaStream_t s) {
+cudaError_t launch_kv_wide(KvArgs &p, int each, cudaStream_t s) {
   const ms_kv_append_args &a = p.a;
   const int units = a.head_dim / (2 * kV);
   p.q_slots = (a.heads + each - 1) / each;
@@ -277,7 +280,7 @@ void launch_kv_wide(KvArgs &p, int each, cudaStream_t s) {
   auto *kernel = a.interleaved ? ms_kv_append_kernel<T, true, 1, kV> : ms_kv_append_kernel<T, false, 1, kV>;
   if (each > 1)
     kernel = a.interleaved ? ms_kv_append_kernel<T, true, kKvHeads, kV> : ms_kv_append_kernel<T, false, kKvHeads, kV>;
-  kernel<<<(unsigned)((a.tokens + z - 1) / z), dim3(units, y, z), 0, s>>>(p);
+  return launch_dependent(kernel, (unsigned)((a.tokens + z - 1) / z), dim3(units, y, z), 0, s, p);
 }
 
 // `wide`: entries that can be moved at once (8, 4 or 1).
@@ -288,20 +291,15 @@ cudaError_t launch_kv_append(KvArgs &p, int wide, cudaStream_t s) {
   // one head a thread until the call fills the GPU's threads a few times
   // over; then up to kKvHeads, which share the thread's table row
   const int each = a.tokens * heads * a.head_dim > 16 * 4ll * 148 * 2048 ? kKvHeads : 1;
-  if (wide == 8) {
-    launch_kv_wide<T, 8>(p, each, s);
-  } else if (wide == 4) {
-    launch_kv_wide<T, 4>(p, each, s);
-  } else {
-    const int units = a.rotary / 2 + (a.head_dim - a.rotary + 1) / 2;
-    p.slots = (heads + each - 1) / each;
-    p.per_token = units * p.slots;
-    p.tokens_cta = p.per_token < kKvThreads ? kKvThreads / p.per_token : 1;
-    const unsigned grid = (unsigned)((a.tokens + p.tokens_cta - 1) / p.tokens_cta);
-    auto *kernel = a.interleaved ? ms_kv_append_any_kernel<T, true> : ms_kv_append_any_kernel<T, false>;
-    kernel<<<grid, kKvThreads, 0, s>>>(p);
-  }
-  return cudaGetLastError();
+  if (wide == 8) return launch_kv_wide<T, 8>(p, each, s);
+  if (wide == 4) return launch_kv_wide<T, 4>(p, each, s);
+  const int units = a.rotary / 2 + (a.head_dim - a.rotary + 1) / 2;
+  p.slots = (heads + each - 1) / each;
+  p.per_token = units * p.slots;
+  p.tokens_cta = p.per_token < kKvThreads ? kKvThreads / p.per_token : 1;
+  const unsigned grid = (unsigned)((a.tokens + p.tokens_cta - 1) / p.tokens_cta);
+  auto *kernel = a.interleaved ? ms_kv_append_any_kernel<T, true> : ms_kv_append_any_kernel<T, false>;
+  return launch_dependent(kernel, grid, kKvThreads, 0, s, p);
 }
 
 }  // namespace ms
