@@ -517,6 +517,8 @@ constexpr int kPrStages = DP == 64 ? 4 : 2;  // of keys, and of values
 template <int DP>
 constexpr int kPrSharedBytes = 1024 + kPrRows * DP * 2 + 2 * kPrStages<DP> * kPrStage<DP>;
 
+constexpr float kAtFar = 1048576.f;  // references (units of log2) above this are not used in a fused exponent
+
 struct PrShared {
   uint64_t full[2][4], empty[2][4];  // of keys, of values
   uint64_t q_full, s_full[2], p_ready[2], pv_done, drained;
@@ -649,7 +651,8 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
       const float kNone = __uint_as_float(0xFF800000u);
       const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
-      float m = kNone;
+      float m = kNone;    // a score, raw
+      float ref = kNone;  // it in units of log2: what the weights refer to
       float2 l[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       bool ok = true;
       for (int i = 0; i < tiles; ++i) {
@@ -665,12 +668,13 @@ __global__ void __launch_bounds__(kPrThreads, 2)
           for (int j = 0; j < 64; ++j)
             if (j >= left) s[j] = kNone;
         }
-        const float top = at_max64(s) * a.scale_log2;
-        const bool moved = top > m + 8.f || (m == kNone && top != kNone);
+        const float top = at_max64(s);
+        const bool moved = (top - m) * a.scale_log2 > 8.f;  // not where both are -inf (a NaN)
         if (__any_sync(0xFFFFFFFFu, moved)) {
-          const float next = moved ? top : m;
-          const float f = m == next ? 1.f : at_exp2(m - next);
-          m = next;
+          const float next = moved ? top * a.scale_log2 : ref;
+          const float f = ref == next ? 1.f : at_exp2(ref - next);
+          ref = next;
+          m = moved ? top : m;
 #pragma unroll
           for (int j = 0; j < 2; ++j) l[j].x *= f, l[j].y *= f;
           if (i > 0) {  // O is at rest once the last tile's product is done (the one before is: S was waited for)
@@ -688,7 +692,16 @@ __global__ void __launch_bounds__(kPrThreads, 2)
             }
           }
         }
-        const float base = m == kNone ? 0.f : m;
+        // Past 2^20 the fused exponent s scale - ref would keep what rounding took from ref (whole units and more:
+        // weights of 0 or infinity); there the difference of the raw scores, which is exact at the top, is scaled.
+        float base = ref == kNone ? 0.f : ref;
+        const bool far = fabsf(base) > kAtFar;
+        if (__any_sync(0xFFFFFFFFu, far)) {
+          const float from = far ? m : 0.f;
+#pragma unroll
+          for (int j = 0; j < 64; ++j) s[j] -= from;
+          base = far ? 0.f : base;
+        }
         const float2 base2 = make_float2(-base, -base);
         uint32_t u[32];
 #pragma unroll
@@ -736,7 +749,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       if (pr < a.packed) {
         // the copies' warps set `bad` before the last products could start
         const float sum = sh.bad ? kAtBadPage : (l[0].x + l[0].y) + (l[1].x + l[1].y);
-        a.pre_ml[rec] = ok ? make_float2(m, sum) : make_float2(0.f, __uint_as_float(0x7FC00000u));
+        a.pre_ml[rec] = ok ? make_float2(ref, sum) : make_float2(0.f, __uint_as_float(0x7FC00000u));
       }
     }
   } else if (warp < 6) {

@@ -255,6 +255,34 @@ def test_cache_offsets_past_32_bits():
 
 
 @gpu
+@pytest.mark.parametrize("dtype,top", [(torch.bfloat16, 1e6), (torch.float16, 6e4)])
+@pytest.mark.parametrize("prefix,own", [(200, 20), (0, 200)])
+def test_scores_past_the_integers_of_fp32(dtype, top, prefix, own):
+    """Finite scores of 1e9 and more, where neighbouring fp32 numbers are
+    hundreds apart: a key ahead of the others by half of that has weight 1 and
+    they have none, so that out is its value (two fp32 roundings and the
+    type's) and lse its score (the product's, the scale's and lse's own
+    roundings: 2^-22 of it)."""
+    p = Problem(40, 8, 2, 64, prefix, [own] * 40, 16, "nhd", dtype, seed=31)
+    gen = torch.Generator(device="cuda").manual_seed(32)
+    factor = (0.5 + torch.rand((40, 8), generator=gen, device="cuda")) * 0.6 * top
+    p.q.zero_()
+    p.q[..., 0] = factor.to(dtype)
+    near = torch.rand(p.ck.shape[:3], generator=gen, device="cuda") * 0.5 * top
+    p.ck[..., 0] = torch.where(p.ck[..., 0].isnan(), math.nan, near).to(dtype)
+    pages = p.prefix_pages[None].expand(40, -1) if prefix else p.pages
+    at = (pages[:, 77 // 16].long(), 77 % 16)  # key 77 of the prefix, or of every row
+    p.ck[(*at, slice(None), 0)] = top
+    out, lse, status = p.run(scale=1.0)
+    assert not status.any()
+    want = p.cv[at].double().repeat_interleave(4, 1)
+    bound = want.abs() * (UNIT[dtype] + 2.0 ** -22)
+    assert bool(((out.double() - want).abs() <= bound).all())
+    score = p.q[..., 0].double() * torch.tensor(top, device="cuda").to(dtype).double()
+    assert bool(((lse.double() - score).abs() <= score * 2.0 ** -22).all())
+
+
+@gpu
 def test_reads_what_append_wrote():
     from miniserve_b200.kvcache import append_kv, rope_table
     p = Problem(6, 8, 2, 64, 40, [3, 16, 0, 20, 31, 8], 16, "nhd", torch.bfloat16, seed=21, hole=0.0)
