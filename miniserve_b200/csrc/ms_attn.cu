@@ -6,8 +6,8 @@
 //   lse = m + log sum_j exp(x_j - m),  m = max_j x_j
 //
 // Partial results over disjoint sets of keys combine exactly: each is kept as
-// (m, l = sum exp(x - m), O = sum exp(x - m) v) in fp32, and the merge weighs
-// them by exp(m - max m).
+// (m, l = sum exp(x - m), O = sum exp(x - m) v) in fp32 for a reference m near
+// its maximum, and the merge weighs them by exp(m - max m).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -52,7 +52,7 @@ struct AtArgs {
   AtHeader *header;
   int64_t *base;    // [rows] where each row starts in the split kernel's sequence
   float *own_o;     // [pieces][chunk_rows][head_dim]
-  float2 *own_ml;   // [pieces][chunk_rows] (m in units of log2, l)
+  float2 *own_ml;   // [pieces][chunk_rows] (reference in units of log2, l)
   float *pre_o;     // [splits][kv_heads][packed rows][head_dim], of the prefix kernel
   float2 *pre_ml;   // [splits][kv_heads][packed rows]
   float scale_log2;
@@ -98,6 +98,28 @@ struct AtType<__half> {
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
+
+constexpr float kAtFar = 1048576.f;  // references (units of log2) above this are not used in a fused exponent
+
+// What weights refer to for a running maximum m, both in units of log2.  The
+// weights are rounded to the cache's type for their product with V, which
+// then runs on the tensor cores with both operands of one type; the sum and
+// O stay in fp32.  fp16 loses bits below 2^-14, so its weights are scaled up
+// by 2^kUp, which records carry along exactly; bf16 has fp32's range.
+template <typename T, int kUp>
+__device__ __forceinline__ float at_reference(float m) {
+  return m;
+}
+template <>
+__device__ __forceinline__ float at_reference<__half, 15>(float m) {
+  return fabsf(m) <= kAtFar / 2 ? m - 15.f : m;  // further off, m - 15 would be rounded past fp16's largest weight
+}
+template <>
+__device__ __forceinline__ float at_reference<__half, 7>(float m) {
+  return fabsf(m) <= kAtFar / 2 ? m - 7.f : m;
+}
+constexpr int kSpUp = 15;  // the split kernel's weights are at most 2^0 of the running maximum,
+constexpr int kPrUp = 7;   // the prefix kernel's 2^8
 
 __device__ __forceinline__ float at_exp2(float x) {
   float y;
@@ -424,7 +446,8 @@ __global__ void __launch_bounds__(kSpWarps * 32, kCtas)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           // both -inf (no score yet above it): nothing to rescale
-          const float f = m[t][i] == top[i] ? 1.f : at_exp2(m[t][i] - top[i]);
+          const float f =
+              m[t][i] == top[i] ? 1.f : at_exp2(at_reference<T, kSpUp>(m[t][i]) - at_reference<T, kSpUp>(top[i]));
           m[t][i] = top[i];
           l[t][i] *= f;
 #pragma unroll
@@ -432,7 +455,8 @@ __global__ void __launch_bounds__(kSpWarps * 32, kCtas)
         }
       }
       // a score of -inf has weight 0 whatever the maximum
-      const float base[2] = {m[t][0] == kNone ? 0.f : m[t][0], m[t][1] == kNone ? 0.f : m[t][1]};
+      const float base[2] = {m[t][0] == kNone ? 0.f : at_reference<T, kSpUp>(m[t][0]),
+                             m[t][1] == kNone ? 0.f : at_reference<T, kSpUp>(m[t][1])};
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = at_exp2(w[i] - base[i & 1]);
       l[t][0] += w[0] + w[2];
@@ -460,7 +484,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kCtas)
           const int g = t * 8 + (lane & 3) * 2 + i;
           if (g < n) {
             const int64_t rec = piece * a.shape.chunk_rows + g;
-            if (lane < 4) a.own_ml[rec] = make_float2(m[t][i], broken ? kAtBadPage : l[t][i]);
+            if (lane < 4) a.own_ml[rec] = make_float2(at_reference<T, kSpUp>(m[t][i]), broken ? kAtBadPage : l[t][i]);
             float *dst = a.own_o + rec * x.head_dim + (lane >> 2);
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) {
@@ -496,8 +520,8 @@ __global__ void __launch_bounds__(kSpWarps * 32, kCtas)
 //
 // Two CTAs share an SM, so that one's latencies pass under the other's
 // exponentials.  The maximum that the weights refer to moves only when a score
-// passes it by 2^8 (the weights then stay below 2^8, within fp16): O is
-// rescaled rarely.
+// passes it by 2^8 (the weights then stay below 2^8, or 2^15 in fp16, see
+// at_reference): O is rescaled rarely.
 //
 // Bound by the exponentials (16 a clock and SM) and, with two CTAs, by the
 // latencies between them: 128 x 64 scores are 512 clocks of exponentials and
@@ -516,8 +540,6 @@ template <int DP>
 constexpr int kPrStages = DP == 64 ? 4 : 2;  // of keys, and of values
 template <int DP>
 constexpr int kPrSharedBytes = 1024 + kPrRows * DP * 2 + 2 * kPrStages<DP> * kPrStage<DP>;
-
-constexpr float kAtFar = 1048576.f;  // references (units of log2) above this are not used in a fused exponent
 
 struct PrShared {
   uint64_t full[2][4], empty[2][4];  // of keys, of values
@@ -652,7 +674,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       const float kNone = __uint_as_float(0xFF800000u);
       const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
       float m = kNone;    // a score, raw
-      float ref = kNone;  // it in units of log2: what the weights refer to
+      float ref = kNone;  // what the weights refer to, in units of log2
       float2 l[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       bool ok = true;
       for (int i = 0; i < tiles; ++i) {
@@ -671,7 +693,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
         const float top = at_max64(s);
         const bool moved = (top - m) * a.scale_log2 > 8.f;  // not where both are -inf (a NaN)
         if (__any_sync(0xFFFFFFFFu, moved)) {
-          const float next = moved ? top * a.scale_log2 : ref;
+          const float next = moved ? at_reference<T, kPrUp>(top * a.scale_log2) : ref;
           const float f = ref == next ? 1.f : at_exp2(ref - next);
           ref = next;
           m = moved ? top : m;

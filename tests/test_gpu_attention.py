@@ -283,6 +283,38 @@ def test_scores_past_the_integers_of_fp32(dtype, top, prefix, own):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("prefix,own", [(500, 3), (3, 500), (0, 700)])
+@pytest.mark.parametrize("drop", [9.7, 13.9, 16.264])
+def test_keys_far_below_the_largest_keep_their_share(dtype, prefix, own, drop):
+    """A first key takes nearly all the weight and has a value of zero, as
+    trained heads' first tokens do; what is left comes from keys exp(-drop)
+    below it.  Their weights are rounded to the type relative to themselves
+    down to 2^-21 of the largest (fp16's normal range, the weights scaled up
+    by at least 2^7), by 2^-32 of the largest below that."""
+    p = Problem(40, 8, 2, 64, prefix, [own] * 40, 16, "nhd", dtype, seed=33)
+    gen = torch.Generator(device="cuda").manual_seed(34)
+    p.q.zero_()
+    p.q[..., 0] = 8.0  # a score is k[0], as the scale is 1 / 8
+    p.ck[..., 0] = torch.where(p.ck[..., 0].isnan(), math.nan, -drop).to(dtype)
+    p.cv[:] = torch.where(p.cv.isnan(), math.nan, 500 + 1000 * torch.rand(p.cv.shape, generator=gen, device="cuda"))
+    first = p.prefix_pages[:1] if prefix else p.pages[:, 0]
+    p.ck[first.long(), 0, :, 0] = 0
+    p.cv[first.long(), 0] = 0
+    out, lse, status = p.run()
+    assert not status.any()
+    u = UNIT[dtype]
+    for b in (0, 17, 39):
+        k, v = (p.keys(b, c).repeat_interleave(4, 1).transpose(0, 1) for c in (p.ck, p.cv))
+        s = (p.q[b].double()[:, None] * k).sum(-1) / 8
+        want = (torch.softmax(s, -1)[..., None] * v).sum(1)
+        e, sums = 72 * 2.0 ** -23 * drop, (k.shape[1] + 64) * 2.0 ** -23
+        bound = (2 * u + 4 * e + 2.0 ** -19 + 2 * sums) * want + 2.0 ** -32 * v.sum(1) + 2.0 ** -25
+        err = (out[b].double() - want).abs()
+        assert bool((err <= bound).all()), (b, float((err / want).max()))
+
+
+@gpu
 def test_reads_what_append_wrote():
     from miniserve_b200.kvcache import append_kv, rope_table
     p = Problem(6, 8, 2, 64, 40, [3, 16, 0, 20, 31, 8], 16, "nhd", torch.bfloat16, seed=21, hole=0.0)
