@@ -75,8 +75,12 @@ enum {
   MS_ROW_BAD_LENGTH = 128,    /* ms_prefix_attention: length below 0 or past
                                  the row's pages; the row's output is 0 and
                                  its lse -inf */
-  MS_ROW_BAD_PAGE = 256       /* ms_prefix_attention: a page that the row or
+  MS_ROW_BAD_PAGE = 256,      /* ms_prefix_attention: a page that the row or
                                  the prefix uses is outside the cache; as above */
+  MS_ROW_WAIT_TIMEOUT = 512   /* ms_prefix_attention: a wait inside the kernel
+                                 of the shared prefix was given up after 1 s;
+                                 the heads concerned have output 0 and lse
+                                 -inf */
 };
 
 /*

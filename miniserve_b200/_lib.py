@@ -27,6 +27,7 @@ MS_ROW_BAD_SLOT = 32
 MS_ROW_BAD_POSITION = 64
 MS_ROW_BAD_LENGTH = 128
 MS_ROW_BAD_PAGE = 256
+MS_ROW_WAIT_TIMEOUT = 512
 
 BINDING_PATH = os.path.join(HERE, "_binding.so")
 

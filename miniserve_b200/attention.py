@@ -28,7 +28,9 @@ def prefix_attention(q, cache_k, cache_v, pages, lengths, *, prefix_pages=None, 
     logarithm of the softmax's sum [B, heads] fp32, and [B] int32 MS_ROW_* bits.
     Heads are up to 128 entries, a multiple of 8, and start 16-byte aligned.
     A row that sees no key has out 0 and lse -inf; so has a row flagged
-    MS_ROW_BAD_LENGTH or MS_ROW_BAD_PAGE.
+    MS_ROW_BAD_LENGTH or MS_ROW_BAD_PAGE, and the heads of a row flagged
+    MS_ROW_WAIT_TIMEOUT that lost a part of the prefix (a wait inside its kernel
+    was given up after 1 s).
     """
     entry = _lib.binding()
     try:

@@ -34,8 +34,10 @@ struct AtHeader {
 };
 
 // l of a record that met a page outside the cache (its keys count as zeros
-// there; the merge flags the rows that read the record).
+// there), and of one whose CTA gave up a wait: the merge flags the rows that
+// read the record.
 constexpr float kAtBadPage = -1.f;
+constexpr float kAtLate = -2.f;
 
 struct AtShape {
   int64_t rows;
@@ -256,6 +258,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kCtas)
     int64_t n = sums[tid];
     for (int64_t b = r0; b < r1; ++b) {
       a.base[b] = before + n * hcs;
+      x.status[b] = at_length(x, b) != __ldg(x.lengths + b) ? MS_ROW_BAD_LENGTH : MS_ROW_OK;
       n += sp_units(at_length(x, b));
     }
     if (tid == 0) a.header->share = share;
@@ -545,7 +548,7 @@ struct PrShared {
   uint64_t full[2][4], empty[2][4];  // of keys, of values
   uint64_t q_full, s_full[2], p_ready[2], pv_done, drained;
   uint32_t tmem;
-  volatile int dead;  // a wait ran out: the records are NaN
+  volatile int dead;  // a wait ran out: the records are kAtLate
   volatile int bad;   // a page of this part is outside the cache
 };
 
@@ -771,7 +774,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
       if (pr < a.packed) {
         // the copies' warps set `bad` before the last products could start
         const float sum = sh.bad ? kAtBadPage : (l[0].x + l[0].y) + (l[1].x + l[1].y);
-        a.pre_ml[rec] = ok ? make_float2(ref, sum) : make_float2(0.f, __uint_as_float(0x7FC00000u));
+        a.pre_ml[rec] = ok ? make_float2(ref, sum) : make_float2(0.f, kAtLate);
       }
     }
   } else if (warp < 6) {
@@ -915,8 +918,8 @@ __global__ void __launch_bounds__(kPrThreads, 2)
 
 // Merge: the records of a (row, query head) weighed by one warp of eight in a
 // CTA, or by all sixteen of a CTA where there may be many records (kWarps); a
-// record's entries are loaded before its weight is known.  The rows' statuses
-// are found here.
+// record's entries are loaded before its weight is known.  What records stand
+// for no result is added to the rows' statuses here.
 constexpr int kMgNarrow = 8;  // warps of a CTA that each have an output of their own
 constexpr int kMgWide = 16;   // warps of a CTA that share one
 
@@ -930,6 +933,7 @@ __global__ void __launch_bounds__((kWarps > 1 ? kWarps : kMgNarrow) * 32)
   const float kNone = __uint_as_float(0xFF800000u);
   __shared__ float4 part[kWarps][kLanes];
   __shared__ float2 part_ml[kWarps];
+  __shared__ int part_flags[kWarps];
   const ms_prefix_attention_args &x = a.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t out_row = kWarps > 1 ? blockIdx.x : (int64_t)blockIdx.x * kMgNarrow + warp;
@@ -964,7 +968,7 @@ __global__ void __launch_bounds__((kWarps > 1 ? kWarps : kMgNarrow) * 32)
   const int pieces = owns + pres;
   const int side = lane / kLanes, d = (lane % kLanes) * 4;
   float top = kNone, sum = 0.f;
-  bool broken = false;
+  int flags = 0;  // MS_ROW_* bits that the records stand for
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int p0 = (kWarps > 1 ? warp * kSide : 0) + side; __any_sync(0xFFFFFFFFu, p0 < pieces); p0 += kStep * kBatch) {
     float2 ml[kBatch];
@@ -990,7 +994,7 @@ __global__ void __launch_bounds__((kWarps > 1 ? kWarps : kMgNarrow) * 32)
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const float w = at_exp2(ml[i].x - (top == kNone ? 0.f : top));
-      broken |= ml[i].y == kAtBadPage;
+      if (ml[i].y < 0.f) flags |= ml[i].y == kAtBadPage ? MS_ROW_BAD_PAGE : MS_ROW_WAIT_TIMEOUT;
       sum += w * ml[i].y;
       y.x += w * v[i].x, y.y += w * v[i].y, y.z += w * v[i].z, y.w += w * v[i].w;
     }
@@ -1011,17 +1015,17 @@ __global__ void __launch_bounds__((kWarps > 1 ? kWarps : kMgNarrow) * 32)
     v.z = __shfl_xor_sync(0xFFFFFFFFu, y.z, o), v.w = __shfl_xor_sync(0xFFFFFFFFu, y.w, o);
     join(other, other_sum, v);
   }
-  broken = __any_sync(0xFFFFFFFFu, broken);
+  flags = __reduce_or_sync(0xFFFFFFFFu, flags);
   if (kWarps > 1) {
     if (lane < kLanes) part[warp][lane] = y;
-    if (lane == 0) part_ml[warp] = make_float2(top, sum);
-    broken = __syncthreads_or(broken);
+    if (lane == 0) part_ml[warp] = make_float2(top, sum), part_flags[warp] = flags;
+    __syncthreads();
     if (warp != 0) return;
 #pragma unroll 5
     for (int i = 1; i < kWarps; ++i) join(part_ml[i].x, part_ml[i].y, part[i][lane % kLanes]);
+    flags = __reduce_or_sync(0xFFFFFFFFu, part_flags[lane % kWarps]);
   }
-  const int status = (raw != len ? MS_ROW_BAD_LENGTH : MS_ROW_OK) | (broken ? MS_ROW_BAD_PAGE : MS_ROW_OK);
-  const bool empty = status != MS_ROW_OK || sum == 0.f;
+  const bool empty = raw != len || flags != 0 || sum == 0.f;
   if (lane < kLanes && d < x.head_dim) {
     T *dst = static_cast<T *>(x.out) + b * x.out_row + hq * x.out_head + d;
     const float inv = 1.f / sum;
@@ -1031,7 +1035,7 @@ __global__ void __launch_bounds__((kWarps > 1 ? kWarps : kMgNarrow) * 32)
   }
   if (lane == 0) {
     x.lse[out_row] = empty ? kNone : (top + log2f(sum)) * 0.6931471805599453f;
-    if (hq == 0) x.status[b] = status;
+    if (flags) atomicOr(x.status + b, flags);  // one head's record may be late and another's not
   }
 }
 
