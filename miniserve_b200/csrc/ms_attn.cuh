@@ -148,7 +148,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool live)
 // A row's own keys: its length, or 0 where the length does not fit its pages
 // or is past kAtMaxKeys (the merge flags the row).
 __device__ __forceinline__ int at_length(const ms_prefix_attention_args &x, int64_t b) {
-  const int n = __ldg(x.lengths + b);
+  const int n = load_in(x.lengths + b);
   return n >= 0 && n <= kAtMaxKeys && (int64_t)n <= x.table_width * x.page_size ? n : 0;
 }
 
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kCtas)
     int64_t n = sums[tid];
     for (int64_t b = r0; b < r1; ++b) {
       a.base[b] = before + n * hcs;
-      x.status[b] = at_length(x, b) != __ldg(x.lengths + b) ? MS_ROW_BAD_LENGTH : MS_ROW_OK;
+      x.status[b] = at_length(x, b) != load_in(x.lengths + b) ? MS_ROW_BAD_LENGTH : MS_ROW_OK;
       n += sp_units(at_length(x, b));
     }
     if (tid == 0) a.header->share = share;
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kSpWarps * 32, kCtas)
       if (j < load.keys) {
         const int p = a.page_shift >= 0 ? j >> a.page_shift : j / page_size;
         offset = j - p * page_size;
-        page = __ldg(load.b < 0 ? x.prefix_pages + p : x.table + load.b * x.table_row + p);
+        page = load_in(load.b < 0 ? x.prefix_pages + p : x.table + load.b * x.table_row + p);
       }
       head = sp_head(a, load);
       sp_next(a, load);
@@ -398,10 +398,10 @@ __global__ void __launch_bounds__(kSpWarps * 32, kCtas)
           uint32_t u = 0;
           if (g < n && k * 8 < x.head_dim) {
             if (a.q_wide) {
-              u = __ldg(reinterpret_cast<const unsigned int *>(q + k * 8));
+              u = load_in(reinterpret_cast<const unsigned int *>(q + k * 8));
             } else {
               const unsigned short *p = reinterpret_cast<const unsigned short *>(q + k * 8);
-              u = (uint32_t)__ldg(p) | ((uint32_t)__ldg(p + 1) << 16);
+              u = (uint32_t)load_in(p) | ((uint32_t)load_in(p + 1) << 16);
             }
           }
           qf[t][k >> 1][k & 1] = u;
@@ -652,12 +652,12 @@ __global__ void __launch_bounds__(kPrThreads, 2)
         if (from >= 0 && chunk * 8 < x.head_dim) {
           const T *src = static_cast<const T *>(x.q) + from + chunk * 8;
           if (a.q_wide) {
-            v[i] = __ldg(reinterpret_cast<const uint4 *>(src));
+            v[i] = load_in(reinterpret_cast<const uint4 *>(src));
           } else {
             const unsigned short *p = reinterpret_cast<const unsigned short *>(src);
             uint32_t w[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = (uint32_t)__ldg(p + 2 * k) | ((uint32_t)__ldg(p + 2 * k + 1) << 16);
+            for (int k = 0; k < 4; ++k) w[k] = (uint32_t)load_in(p + 2 * k) | ((uint32_t)load_in(p + 2 * k + 1) << 16);
             v[i] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(kPrThreads, 2)
     auto find = [&](int j, int &page, int &offset) {
       const int p = a.page_shift >= 0 ? j >> a.page_shift : j / page_size;
       offset = j - p * page_size;
-      page = __ldg(x.prefix_pages + p);
+      page = load_in(x.prefix_pages + p);
     };
     int stage = 0, phase = 1, i = 0;
     bool ok = true;
@@ -942,7 +942,7 @@ __global__ void __launch_bounds__((kWarps > 1 ? kWarps : kMgNarrow) * 32)
   const int hq = (int)(out_row - b * a.shape.heads);
   const int h = hq / a.shape.group, g = hq - h * a.shape.group;
   const int c = g / kAtRows, hc = h * a.shape.chunks + c;
-  const int raw = __ldg(x.lengths + b), len = at_length(x, b);
+  const int raw = load_in(x.lengths + b), len = at_length(x, b);
   grid_wait();
   // the records: the row's own pieces, then the prefix's (the split kernel's or the prefix kernel's)
   const int64_t share = a.header->share, start = a.base[b];

@@ -28,12 +28,12 @@ template <typename T>
 __device__ __forceinline__ void qu_load8(const T *p, float (&v)[8]);
 template <>
 __device__ __forceinline__ void qu_load8<float>(const float *p, float (&v)[8]) {
-  *reinterpret_cast<float4 *>(v) = __ldg(reinterpret_cast<const float4 *>(p));
-  *reinterpret_cast<float4 *>(v + 4) = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+  *reinterpret_cast<float4 *>(v) = load_in(reinterpret_cast<const float4 *>(p));
+  *reinterpret_cast<float4 *>(v + 4) = load_in(reinterpret_cast<const float4 *>(p) + 1);
 }
 template <>
 __device__ __forceinline__ void qu_load8<__nv_bfloat16>(const __nv_bfloat16 *p, float (&v)[8]) {
-  const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
+  const uint4 u = load_in(reinterpret_cast<const uint4 *>(p));
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -43,7 +43,7 @@ __device__ __forceinline__ void qu_load8<__nv_bfloat16>(const __nv_bfloat16 *p, 
 }
 template <>
 __device__ __forceinline__ void qu_load8<__half>(const __half *p, float (&v)[8]) {
-  const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
+  const uint4 u = load_in(reinterpret_cast<const uint4 *>(p));
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -336,10 +336,10 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       if (tile >= tiles) return;
       const int ch = (int)(tile / tok_tiles) * span + (int)rank * a.rows + quad * 32 + lane;
       const int t = (int)(tile % tok_tiles) * a.bn + et;
-      if (et < a.bn && t < a.M) xs = __ldg(a.x_scale + t);
+      if (et < a.bn && t < a.M) xs = load_in(a.x_scale + t);
       const bool live = quad * 32 + lane < a.rows && ch < a.N;
-      ws = live ? __ldg(a.w_scale + ch) : 0.f;
-      bias = live && a.bias ? __ldg(a.bias + ch) : 0.f;
+      ws = live ? load_in(a.w_scale + ch) : 0.f;
+      bias = live && a.bias ? load_in(a.bias + ch) : 0.f;
     };
     scales(worker);
     int n = 0;

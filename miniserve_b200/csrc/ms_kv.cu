@@ -73,7 +73,7 @@ struct KvRow {
 __device__ __forceinline__ KvRow kv_row(const KvArgs &p, int64_t t) {
   const ms_kv_append_args &a = p.a;
   KvRow r{0, 0, 0, MS_ROW_OK, false};
-  const int64_t slot = __ldg(a.slots + t);
+  const int64_t slot = load_in(a.slots + t);
   if (slot >= a.pages * a.page_size) {
     r.status |= MS_ROW_BAD_SLOT;
   } else if (slot >= 0) {
@@ -90,7 +90,7 @@ __device__ __forceinline__ KvRow kv_row(const KvArgs &p, int64_t t) {
     r.write = true;
   }
   if (a.rotary > 0) {
-    r.position = __ldg(a.positions + t);
+    r.position = load_in(a.positions + t);
     if (r.position < 0 || r.position >= a.table_rows) {
       r.status |= MS_ROW_BAD_POSITION;
       r.position = 0;
@@ -180,8 +180,8 @@ __global__ void __launch_bounds__(kKvThreads, 4) ms_kv_append_kernel(const __gri
       const float *row = a.table + r.position * a.rotary + j * kV;
 #pragma unroll
       for (int i = 0; i < kV; i += 4) {
-        *reinterpret_cast<float4 *>(c + i) = __ldg(reinterpret_cast<const float4 *>(row + i));
-        *reinterpret_cast<float4 *>(s + i) = __ldg(reinterpret_cast<const float4 *>(row + (a.rotary >> 1) + i));
+        *reinterpret_cast<float4 *>(c + i) = load_in(reinterpret_cast<const float4 *>(row + i));
+        *reinterpret_cast<float4 *>(s + i) = load_in(reinterpret_cast<const float4 *>(row + (a.rotary >> 1) + i));
       }
     }
     const int64_t dst_head = query ? a.q_out_head : key ? a.ck_head : a.cv_head;
@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(kKvThreads) ms_kv_append_any_kernel(const __gr
     if (rotates) {
       lo = kInterleaved ? 2 * j : j;
       hi = kInterleaved ? 2 * j + 1 : j + half;
-      c = __ldg(a.table + r.position * a.rotary + j);
-      s = __ldg(a.table + r.position * a.rotary + half + j);
+      c = load_in(a.table + r.position * a.rotary + j);
+      s = load_in(a.table + r.position * a.rotary + half + j);
     } else {
       lo = a.rotary + 2 * (j - half);
       hi = lo + 1;

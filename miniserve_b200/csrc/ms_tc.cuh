@@ -77,6 +77,15 @@ __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// A load of the caller's or of the grid before's data.  A grid launched so is
+// resident while the one before it still writes; only a coherent load is
+// certain to stay behind grid_wait.  (The read-only path, __ldg, is for memory
+// that nothing writes during the kernel's whole life.)
+template <typename T>
+__device__ __forceinline__ T load_in(const T *p) {
+  return *p;
+}
+
 // -------------------------------------------------------------------- TMA
 // By the one lane of a converged warp that has `leader` set.
 __device__ __forceinline__ void tma_load_2d(uint32_t leader, uint32_t dst, const void *map, uint32_t bar, int x, int y) {

@@ -23,3 +23,12 @@ def test_builds_and_exports_declared_symbols():
         assert n in _lib.SIGNATURES, n
     assert L.ms_version() >= 100
     assert L.ms_error_string(-1).decode().startswith("invalid")
+
+
+def test_dependent_grids_read_coherently():
+    """The decode-step kernels are launched while the grid before them may
+    still write what they read: none of them uses the read-only path."""
+    csrc = os.path.join(ROOT, "miniserve_b200", "csrc")
+    for name in ("ms_kv.cu", "ms_attn.cu", "ms_attn.cuh", "ms_int8.cu", "ms_tc.cuh"):
+        text = re.sub(r"//.*", "", open(os.path.join(csrc, name)).read())
+        assert not re.search(r"__ldg|ld\.global\.nc|__restrict__", text), name
