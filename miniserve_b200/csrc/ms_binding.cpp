@@ -77,6 +77,13 @@ void check_writable(const char *name, const at::Tensor &t) {
       refuse(PyExc_ValueError, name, " must not repeat its memory (an expanded tensor)");
 }
 
+// Whether two tensors of one shape lie alike: a dimension of one entry is never stepped along.
+bool same_strides(const at::Tensor &a, const at::Tensor &b) {
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+
 int half_code(const char *name, const at::Tensor &t) {
   if (t.scalar_type() == at::kBFloat16) return MS_DTYPE_BF16;
   if (t.scalar_type() == at::kHalf) return MS_DTYPE_F16;
@@ -180,7 +187,7 @@ PyObject *append_kv(PyObject *const *o) {
       q_out = tensor("q_out", o[9]);
       check("q_out", q_out, type, dev, q.sizes());
       check_writable("q_out", q_out);
-      if (q_out.const_data_ptr() == q.const_data_ptr() && q_out.strides() != q.strides())
+      if (q_out.const_data_ptr() == q.const_data_ptr() && !same_strides(q_out, q))
         refuse(PyExc_ValueError, "q_out in place of q must have q's strides");
     }
     a.heads = (int32_t)q.size(1);

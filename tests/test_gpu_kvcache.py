@@ -139,6 +139,30 @@ def test_in_place_and_unaligned(dim, offset):
 
 
 @gpu
+@pytest.mark.parametrize("T,H", [(1, 4), (3, 1), (1, 1)])
+def test_in_place_through_another_view(T, H):
+    """q's memory as q_out through a view that differs in the stride of a
+    dimension of one entry; views that lie otherwise are refused."""
+    from miniserve_b200.kvcache import append_kv, rope_table
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    qkv = torch.randn((T, H + 2, 64), generator=gen, device="cuda").bfloat16()
+    q, k, v = qkv[:, :H], qkv[:, H:H + 1], qkv[:, H + 1:]
+    ck, cv = (make_cache(gen, 4, 8, 1, 64, torch.bfloat16, "nhd") for _ in range(2))
+    slots = torch.arange(T, device="cuda")
+    rope = rope_table(T + 3, 64)
+    qq, (kk, kslack), vv = expect(ck, cv, q, k, v, slots, slots + 2, rope, False)
+    view = q.as_strided((T, H, 64), (q.stride(0) if T > 1 else 7, q.stride(1) if H > 1 else 9, 1))
+    out, status = append_kv(ck, cv, k, v, slots, q=q, positions=slots + 2, rope=rope, q_out=view)
+    assert out is view and not status.any()
+    close(q, *qq, torch.bfloat16)
+    close(ck, kk, kslack, torch.bfloat16)
+    if T * H > 1:
+        other = q.as_strided((T, H, 64), (64 * H, 64, 1) if T > 1 else (0, 32, 1))
+        with pytest.raises(ValueError):
+            append_kv(ck, cv, k, v, slots, q=q, positions=slots + 2, rope=rope, q_out=other)
+
+
+@gpu
 @pytest.mark.parametrize("dim", [64, 40])
 def test_bad_rows_are_flagged_and_write_nothing(dim):
     from miniserve_b200.kvcache import append_kv, rope_table
