@@ -167,9 +167,13 @@ def binding():
                 raise SamplerLibraryError(
                     f"{BINDING_PATH} is missing: build it with `python -m miniserve_b200.build`")
             loader = importlib.machinery.ExtensionFileLoader("miniserve_b200._binding", BINDING_PATH)
-            module = importlib.util.module_from_spec(
-                importlib.util.spec_from_file_location("miniserve_b200._binding", BINDING_PATH, loader=loader))
-            loader.exec_module(module)
+            try:
+                module = importlib.util.module_from_spec(
+                    importlib.util.spec_from_file_location("miniserve_b200._binding", BINDING_PATH, loader=loader))
+                loader.exec_module(module)
+            except ImportError as e:  # another torch's symbols, before the version could be compared
+                raise SamplerLibraryError(f"{BINDING_PATH} cannot be loaded with torch {torch.__version__}: build it "
+                                          f"again with `python -m miniserve_b200.build` ({e})") from e
             if module.torch_version != torch.__version__.split("+")[0]:
                 raise SamplerLibraryError(f"{BINDING_PATH} was built for torch {module.torch_version}, this is "
                                           f"{torch.__version__}: build it again")

@@ -1,6 +1,9 @@
 """The C-ABI library builds, loads and exports every symbol the header declares (no GPU)."""
 import os
 import re
+import subprocess
+
+import pytest
 
 from miniserve_b200 import _lib, build
 
@@ -23,6 +26,21 @@ def test_builds_and_exports_declared_symbols():
         assert n in _lib.SIGNATURES, n
     assert L.ms_version() >= 100
     assert L.ms_error_string(-1).decode().startswith("invalid")
+
+
+def test_binding_that_does_not_load_says_what_to_do(tmp_path, monkeypatch):
+    """An extension of another torch fails in the loader, on a missing symbol:
+    here one that needs a symbol that no library has."""
+    source, made = tmp_path / "binding.c", tmp_path / "_binding.so"
+    source.write_text("void *of_another_torch(void); void *PyInit__binding(void) { return of_another_torch(); }")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", made, source], check=True)
+    monkeypatch.setattr(_lib, "BINDING_PATH", str(made))
+    monkeypatch.setattr(_lib, "_binding", None)
+    with pytest.raises(_lib.SamplerLibraryError, match="build it again"):
+        _lib.binding()
+    made.unlink()
+    with pytest.raises(_lib.SamplerLibraryError, match="is missing"):
+        _lib.binding()
 
 
 def test_dependent_grids_read_coherently():
