@@ -12,11 +12,11 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <algorithm>
 #include <atomic>
 
 #include "../../include/mssample.h"
 #include "ms_host.h"
+#include "ms_int8_tiling.h"
 #include "ms_tc.cuh"
 
 namespace ms {
@@ -178,11 +178,6 @@ static cudaError_t launch_quantize(const void *x, int dtype, int64_t M, int64_t 
 // busy; 256 tiles over 74 pairs leave 13 % of the rounds idle).
 constexpr int kI8Epilogue = 8;  // warps: two for each 32 lanes of tensor memory, on alternate 16 columns
 constexpr int kI8Threads = 64 + 32 * kI8Epilogue + 32;
-constexpr int kI8Rows = 128;    // channels of a tile
-constexpr int kI8Step = 128;    // bytes of K of a stage
-constexpr int kI8MaxStages = 11;
-constexpr int kI8Cols = 256;    // columns of an accumulator
-constexpr int kI8Ring = 208 * 1024;
 
 struct I8Shared {
   uint64_t full[kI8MaxStages], empty[kI8MaxStages];
@@ -414,53 +409,6 @@ static cudaError_t i8_map(CUtensorMap *map, const void *p, int64_t rows, int64_t
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-// Tiles of a call: tokens (bn) and channels (rows) of one, and whether two SMs
-// share it, by the clocks that the busiest SM needs.
-struct I8Tiling {
-  int bn, rows;
-  bool pair;
-};
-
-static I8Tiling i8_tiling(int64_t M, int64_t N, int64_t K, int out_size, int sms) {
-  I8Tiling best{};
-  double least = 0;
-  const double steps = (double)((K + kI8Step - 1) / kI8Step);
-  for (int pair = 0; pair < 2; ++pair) {
-    const int ctas = pair + 1, grain = 16 * ctas;
-    const int64_t workers = sms / ctas, parts0 = (M + kI8Cols - 1) / kI8Cols;
-    int seen = 0;
-    for (int64_t parts = parts0; parts < parts0 + 12; ++parts) {
-      // equal token tiles, rounded up to what an N of the product, and half of it for a pair, allow
-      const int bn = (int)(((M + parts - 1) / parts + grain - 1) / grain * grain);
-      if (bn == seen) continue;
-      seen = bn;
-      const int64_t tok_tiles = (M + bn - 1) / bn;
-      // 128 channels, or the same rounds of tiles with the channels spread evenly over them
-      for (int spread = 0; spread < 2 - pair; ++spread) {
-        int64_t rows = kI8Rows;
-        int64_t tiles = (N + rows * ctas - 1) / (rows * ctas) * tok_tiles;
-        const int64_t rounds = (tiles + workers - 1) / workers;
-        if (spread) {
-          const int64_t most = rounds * workers / tok_tiles;
-          if (most < 1) continue;
-          rows = (N + most - 1) / most;
-          if (rows > kI8Rows) continue;
-        }
-        // a step of 128 bytes of K: the products (512 clocks for 256 tokens), the SM's reads (64 bytes a clock,
-        // 24 of them from HBM where no other tile uses the weights); the stores run under the next tile's
-        // steps, whole lines at 24 bytes a clock, others slower (512 x 896 x 151936: 102 us, 117 us with odd
-        // tiles); what is hidden still takes a part of the SM's way to L2
-        const double reads = (rows + bn / ctas) * 128 / 60.0, hbm = tok_tiles == 1 ? rows * 128 / 24.0 : 0;
-        const double step = std::max(2.0 * bn, std::max(reads, hbm));
-        const double store = (double)rows * std::min<int64_t>(bn, M) * out_size / (rows % 32 ? 16 : 24);
-        const double cost = rounds * (std::max(steps * step, store) + 0.3 * std::min(steps * step, store)) + store;
-        if (!best.bn || cost < least) best = {bn, (int)rows, pair != 0}, least = cost;
-      }
-    }
-  }
-  return best;
-}
-
 template <typename T, bool kPair>
 static cudaError_t launch_int8_as(I8Args &a, const int8_t *xq, int64_t ldx, const int8_t *wq, int64_t ldw, int sms,
                                   int dev, cudaStream_t s) {
@@ -473,11 +421,8 @@ static cudaError_t launch_int8_as(I8Args &a, const int8_t *xq, int64_t ldx, cons
     ready[dev].store(1, std::memory_order_release);
   }
   const int64_t tok_tiles = (a.M + (int64_t)a.bn - 1) / a.bn;
-  const int stage = (kI8Rows + a.bn / kCtas) * kI8Step;
-  a.stages = kI8Ring / stage < kI8MaxStages ? kI8Ring / stage : kI8MaxStages;
-  // few tokens: all SMs only stream weights, and six stages (108 KB) in flight on each do better than eleven
-  // (1 x 896 x 151936: 26.1 against 28.3 us; 4 x 5181 x 42138: 42.3 against 41.3)
-  if (a.bn <= 32 && a.stages > 6) a.stages = 6;
+  const int stage = i8_stage_bytes(a.bn, kPair);
+  a.stages = i8_stages(a.bn, kPair);
   const int64_t span = (int64_t)a.rows * kCtas;
   const int64_t tiles = (a.N + span - 1) / span * tok_tiles;
   CUtensorMap wmap, xmap;

@@ -175,6 +175,23 @@ def test_scale_and_strided_tensors(scale):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,H,Hkv,D,prefix", [(33, 6, 2, 64, 200), (130, 8, 1, 128, 130), (3, 6, 2, 72, 50),
+                                              (5, 40, 2, 80, 0)])
+@pytest.mark.parametrize("offset,gap", [(1, 0), (0, 3), (4, 4)])
+def test_queries_off_the_16_byte_grid(B, H, Hkv, D, prefix, offset, gap, dtype):
+    """A base, or strides, that 16-byte reads of the queries do not fit: the
+    prefix kernel (first two), a prefix of few rows and plain rows."""
+    p = Problem(B, H, Hkv, D, prefix, [(5 * i) % 77 for i in range(B)], 16, "nhd", dtype, seed=B + D)
+    flat = torch.full((offset + B * H * (D + gap),), math.nan, dtype=dtype, device="cuda")
+    view = flat[offset:].view(B, H, D + gap)[..., :D]
+    view.copy_(p.q)
+    p.q = view
+    assert view.data_ptr() % 16 or view.stride(1) % 8
+    p.check(*p.run())
+
+
+@gpu
 def test_keys_and_values_in_one_allocation_of_wide_slots():
     """K and V interleaved in one tensor (different bases, equal odd strides)."""
     p = Problem(17, 8, 4, 64, 90, [(11 * i) % 60 for i in range(17)], 16, "nhd", torch.float16, seed=6)

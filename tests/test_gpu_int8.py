@@ -97,6 +97,69 @@ def test_product_matches_definition(M, N, K, out_dtype):
     check_product(out, *quantized(x), wq, ws, bias)
 
 
+# M, N, K, out type, and what they are to run on 148 SMs: tokens and channels of a tile, two SMs a tile, stages of the
+# ring, rounds of tiles.  All have several steps of K and several rounds of tiles (a ring and an accumulator carried from
+# tile to tile), each in another form.
+TILINGS = [
+    (1, 151936, 896, torch.float32, (16, 115, False, 6, 9)),      # one row of an LM head
+    (5, 60000, 1001, torch.float32, (16, 102, False, 6, 4)),
+    (37, 21595, 1277, torch.float16, (48, 73, False, 9, 2)),      # a last round one tile short
+    (40, 70001, 1300, torch.float32, (32, 128, True, 6, 8)),
+    (77, 40003, 1001, torch.float32, (80, 91, False, 8, 3)),
+    (100, 64001, 1100, torch.bfloat16, (64, 128, True, 10, 7)),   # the longest ring
+    (129, 60001, 640, torch.float32, (144, 128, False, 6, 4)),
+    (155, 33765, 2650, torch.float16, (160, 115, False, 5, 2)),
+    (231, 48437, 1030, torch.bfloat16, (256, 128, True, 6, 3)),   # a token tile that is part full
+    (512, 40000, 896, torch.bfloat16, (256, 128, True, 6, 5)),
+    (513, 38001, 897, torch.float32, (192, 128, True, 7, 7)),     # a last token tile of 129, channels and K off the grid
+    (785, 8597, 262, torch.float16, (208, 128, False, 4, 2)),     # the shortest ring
+    (1401, 2337, 279, torch.float32, (176, 64, False, 5, 2)),
+    (2048, 8192, 1000, torch.bfloat16, (256, 128, True, 6, 4)),   # a prompt's projection
+]
+
+
+def test_the_tilings_that_the_shapes_are_to_run(tmp_path):
+    """The launch's own rule, compiled for the host."""
+    import ctypes
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc")
+    source, made = tmp_path / "tiling.cpp", tmp_path / "tiling.so"
+    source.write_text('''#include "ms_int8_tiling.h"
+        extern "C" void tiling(int64_t M, int64_t N, int64_t K, int size, int *out) {
+          const ms::I8Tiling t = ms::i8_tiling(M, N, K, size, 148);
+          out[0] = t.bn, out[1] = t.rows, out[2] = t.pair, out[3] = ms::i8_stages(t.bn, t.pair);
+        }''')
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", csrc, "-o", made, source], check=True)
+    rule = ctypes.CDLL(str(made)).tiling
+    rule.argtypes = [ctypes.c_int64] * 3 + [ctypes.c_int, ctypes.c_void_p]
+    forms = set()
+    for M, N, K, out_dtype, (bn, rows, pair, stages, rounds) in TILINGS:
+        got = (ctypes.c_int * 4)()
+        rule(M, N, K, out_dtype.itemsize, got)
+        assert tuple(got) == (bn, rows, pair, stages), (M, N, K)
+        each = 2 if pair else 1
+        tiles = -(-M // bn) * -(-N // (rows * each))
+        assert -(-tiles // (148 // each)) == rounds >= 2 and K > 256, (M, N, K)
+        forms.add((pair, stages))
+    assert {(False, 4), (False, 9), (True, 6), (True, 10)} <= forms
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K,out_dtype", [t[:4] for t in TILINGS], ids=str)
+def test_products_of_several_rounds_and_steps(M, N, K, out_dtype):
+    from miniserve_b200.int8 import Int8Linear
+    gen = torch.Generator(device="cuda").manual_seed(M + N + K)
+    x = torch.randn((M, K), generator=gen, device="cuda").bfloat16()
+    wq = torch.randint(-127, 128, (N, K), generator=gen, device="cuda").to(torch.int8)
+    ws = torch.rand(N, generator=gen, device="cuda") * 1e-3
+    bias = torch.randn(N, generator=gen, device="cuda") if N % 2 else None
+    room = torch.full((M + 1, N), 7.0, dtype=out_dtype, device="cuda")
+    out = Int8Linear(wq, ws, bias)(x, out=room[:M])
+    check_product(out, *quantized(x), wq, ws, bias)
+    assert bool((room[M] == 7.0).all())
+
+
 @gpu
 def test_extreme_integers_are_exact():
     """Every product 127 * 127 or -127 * 127, or int8's lowest value, up to the

@@ -70,7 +70,7 @@ CASES = [
     (50, 5, 5, 33, 10, 7, False, "nhd"),    # odd head size: single entries
     (50, 5, 5, 33, 32, 7, True, "hnd"),
     (129, 8, 8, 256, 256, 64, False, "nhd"),
-    (5000, 14, 2, 64, 64, 16, False, "nhd"),  # four heads a thread
+    (5000, 14, 2, 64, 64, 16, False, "nhd"),  # one head a thread still (LARGE has two)
     (2500, 9, 3, 96, 48, 16, True, "hnd"),
     (64, 0, 2, 64, 64, 16, False, "nhd"),   # keys and values only
     (64, 2, 2, 64, 0, 16, False, "nhd"),    # no rotation
@@ -103,6 +103,60 @@ def test_append_matches_definition(case, dtype):
         assert q_out is None
     close(ck, kk, kslack, dtype)
     assert torch.equal(cv.double(), vv)
+
+
+# Above this many entries a thread takes two heads.
+TWO_HEADS = 16 * 4 * 148 * 2048
+LARGE = [
+    # tokens, heads, kv_heads, dim, rotary, page, interleaved, order, a base's offset in entries: 16-byte pieces ...
+    (30011, 14, 2, 64, 64, 16, False, "nhd", 0),
+    (25000, 13, 3, 64, 64, 16, False, "hnd", 0),   # odd head counts: a thread without a second head
+    (25000, 13, 3, 64, 32, 24, True, "nhd", 0),
+    (24000, 11, 1, 64, 64, 16, False, "nhd", 0),   # one key head
+    (24000, 0, 7, 64, 64, 16, True, "nhd", 0),     # no queries
+    (11000, 9, 5, 96, 96, 64, True, "hnd", 0),
+    (20000, 13, 3, 80, 40, 16, False, "nhd", 0),   # 8-byte pieces
+    (20000, 13, 3, 80, 40, 7, True, "hnd", 0),
+    (25000, 13, 3, 64, 64, 16, False, "nhd", 4),
+    (30000, 13, 3, 35, 10, 16, False, "nhd", 0),   # single entries
+    (30000, 13, 3, 35, 34, 16, True, "hnd", 0),
+    (25000, 13, 3, 64, 64, 16, False, "nhd", 1),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", LARGE, ids=str)
+def test_append_of_prompts_matches_definition(case, dtype):
+    """Calls large enough for two heads a thread, in pieces of every size."""
+    from miniserve_b200.kvcache import append_kv, rope_table
+    T, H, Hkv, D, rotary, page, interleaved, order, offset = case
+    assert T * (H + 2 * Hkv) * D > TWO_HEADS
+    gen = torch.Generator(device="cuda").manual_seed(T + D)
+    pages = T // page + 3
+    ck, cv = (make_cache(gen, pages, page, Hkv, D, dtype, order) for _ in range(2))
+    flat = torch.randn(offset + T * (H + 2 * Hkv) * D, generator=gen, device="cuda").to(dtype)
+    qkv = flat[offset:].view(T, H + 2 * Hkv, D)
+    q, k, v = qkv[:, :H], qkv[:, H:H + Hkv], qkv[:, H + Hkv:]
+    slots = torch.randperm(pages * page, generator=gen, device="cuda")[:T].clone()
+    slots[::5] = -1
+    rope = rope_table(301, rotary)
+    positions = torch.randint(0, 301, (T,), generator=gen, device="cuda")
+    table = rope.reshape(301, -1)[positions]
+    kept = torch.nonzero(slots >= 0)[:, 0]
+    at = (torch.div(slots[kept], page, rounding_mode="floor"), slots[kept] % page)
+    kk, ks = turned(k, table, interleaved)
+    want_k, slack = ck.double(), torch.zeros(ck.shape, dtype=torch.float64, device="cuda")
+    want_k[at], slack[at] = kk[kept], ks[kept]
+    want_v = cv.clone()
+    want_v[at] = v[kept]
+    q_out, status = append_kv(ck, cv, k, v, slots, q=q if H else None, positions=positions, rope=rope,
+                              interleaved=interleaved)
+    assert not status.any()
+    if H:
+        close(q_out, *turned(q, table, interleaved), dtype)
+    close(ck, want_k, slack, dtype)
+    assert torch.equal(cv, want_v)
 
 
 @gpu
