@@ -422,7 +422,7 @@ static cudaError_t launch_int8_as(I8Args &a, const int8_t *xq, int64_t ldx, cons
   }
   const int64_t tok_tiles = (a.M + (int64_t)a.bn - 1) / a.bn;
   const int stage = i8_stage_bytes(a.bn, kPair);
-  a.stages = i8_stages(a.bn, kPair);
+  a.stages = i8_stages(a.M, a.K, a.bn, kPair);
   const int64_t span = (int64_t)a.rows * kCtas;
   const int64_t tiles = (a.N + span - 1) / span * tok_tiles;
   CUtensorMap wmap, xmap;

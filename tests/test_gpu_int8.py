@@ -104,7 +104,8 @@ TILINGS = [
     (1, 151936, 896, torch.float32, (16, 115, False, 6, 9)),      # one row of an LM head
     (5, 60000, 1001, torch.float32, (16, 102, False, 6, 4)),
     (37, 21595, 1277, torch.float16, (48, 73, False, 9, 2)),      # a last round one tile short
-    (40, 70001, 1300, torch.float32, (32, 128, True, 6, 8)),
+    (16, 30001, 8192, torch.bfloat16, (16, 102, False, 10, 2)),    # long rows: the whole ring for a few tokens
+    (40, 70001, 1300, torch.float32, (32, 128, True, 10, 8)),
     (77, 40003, 1001, torch.float32, (80, 91, False, 8, 3)),
     (100, 64001, 1100, torch.bfloat16, (64, 128, True, 10, 7)),   # the longest ring
     (129, 60001, 640, torch.float32, (144, 128, False, 6, 4)),
@@ -128,7 +129,7 @@ def test_the_tilings_that_the_shapes_are_to_run(tmp_path):
     source.write_text('''#include "ms_int8_tiling.h"
         extern "C" void tiling(int64_t M, int64_t N, int64_t K, int size, int *out) {
           const ms::I8Tiling t = ms::i8_tiling(M, N, K, size, 148);
-          out[0] = t.bn, out[1] = t.rows, out[2] = t.pair, out[3] = ms::i8_stages(t.bn, t.pair);
+          out[0] = t.bn, out[1] = t.rows, out[2] = t.pair, out[3] = ms::i8_stages(M, K, t.bn, t.pair);
         }''')
     subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", csrc, "-o", made, source], check=True)
     rule = ctypes.CDLL(str(made)).tiling
