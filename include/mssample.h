@@ -443,7 +443,8 @@ int ms_kv_append(const ms_kv_append_args *args, ms_stream_t stream);
  *   lse[b, h] = log sum_j exp(scale q[b, h] . k_j)
  *
  * in fp32, the weights rounded to the cache's type for their product with v
- * and out rounded once.  A row that sees no key has out 0 and lse -inf.  The
+ * (fp16's scaled up first, so that small ones keep their bits) and out rounded
+ * once.  A row that sees no key has out 0 and lse -inf.  The
  * cache past a row's keys is not used, whatever it holds (a part-full page,
  * table entries past ceil(lengths[b] / page_size)).  prefix_length 0 is plain
  * attention over the rows' own pages.

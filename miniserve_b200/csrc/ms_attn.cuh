@@ -1,5 +1,6 @@
 // Attention over a paged cache: arguments, the split kernel (rows' own keys,
-// and the prefix's where few rows share it) and the merge.
+// and the prefix's where few rows share it), the prefix kernel (where more
+// do) and the merge.
 #pragma once
 
 #include <cuda.h>
@@ -526,11 +527,13 @@ __global__ void __launch_bounds__(kSpWarps * 32, kCtas)
 // passes it by 2^8 (the weights then stay below 2^8, or 2^15 in fp16, see
 // at_reference): O is rescaled rarely.
 //
-// Bound by the exponentials (16 a clock and SM) and, with two CTAs, by the
-// latencies between them: 128 x 64 scores are 512 clocks of exponentials and
+// Bound by the latencies between a tile's steps (scores, maximum, exponentials,
+// weights stored, products), which two CTAs hide in part; the exponentials (16
+// a clock and SM) are the busiest pipe, 53 %: 128 x 64 scores are 512 clocks of exponentials and
 // take about 700 (two CTAs on an SM: 1400 each), their products of 64-entry
 // heads 64 each way.  512 rows of 14 / 2 heads of 64 behind 8192 keys: 29 us
-// (15.3 GFLOP; the exponentials alone 14 us, the products 9).  A quarter of the
+// (15.3 GFLOP; the exponentials alone 14 us, the products 9), 46 us with the
+// split kernel and the merge.  A quarter of the
 // exponentials as polynomials on the FMA pipe gained 1 % and is not done.
 constexpr int kPrThreads = 224;
 constexpr int kPrRows = 128;
@@ -552,7 +555,7 @@ struct PrShared {
   volatile int bad;   // a page of this part is outside the cache
 };
 
-// The largest of 64 values.
+// The largest of three values, and of 64.
 __device__ __forceinline__ float at_max3(float x, float y, float z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));

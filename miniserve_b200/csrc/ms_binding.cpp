@@ -5,8 +5,8 @@
 // few microseconds, about what the interpreter needs to look at one tensor's
 // type, device, shape and strides a few times over.  So the checks that the
 // kernels rely on, the allocations and the call of the C entry point are made
-// here, on the tensors themselves: an append of 8 tokens takes 5 us of host
-// time, 23 us with the same checks in Python.
+// here, on the tensors themselves: an append of 8 tokens takes 6.5 us of host
+// time, 22 us with the same checks in Python.
 //
 // The C entry points are those of libmssample.so, handed over by address
 // (bind); nothing here is a second path to the GPU.

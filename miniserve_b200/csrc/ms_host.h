@@ -14,8 +14,11 @@ constexpr int kMaxDevices = 64;
 __attribute__((visibility("hidden"))) int cuda_fail(cudaError_t e);
 
 // A launch that may be set up while the kernel before it in the stream still
-// runs (a programmatic dependent launch): the kernel waits (griddepcontrol.wait)
-// before it touches memory that an earlier one uses.
+// runs (a programmatic dependent launch).  A call's first kernel waits
+// (griddepcontrol.wait) before it touches memory and only then releases the
+// next one, so the call's later kernels find the caller's tensors complete and
+// their workspace free; they wait before they read what the call's own earlier
+// kernels write.
 template <typename... P, typename... A>
 cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, int shared, cudaStream_t s, const A &...args) {
   cudaLaunchConfig_t cfg = {};

@@ -172,10 +172,13 @@ static cudaError_t launch_quantize(const void *x, int dtype, int64_t M, int64_t 
 // tokens, 64 bytes a clock, the first CTA issues the products for both, and
 // each stores its own channels.
 //
-// With their quantisation: 1 x 896 x 151936 to fp32 26.1 us (137 MB of weights,
-// 5.3 TB/s); 512 x 896 x 151936 85 us (449 MB, 5.3 TB/s, 81 % of the measured
-// copy rate); 2048 x 4096 x 8192 to bf16 56 us (2.4 POP/s, tensor pipe 79 %
-// busy; 256 tiles over 74 pairs leave 13 % of the rounds idle).
+// With their quantisation, a few dozen calls on end: 1 x 896 x 151936 to fp32
+// 27.8 us (137 MB of weights, 4.9 TB/s; 25.5 us in a graph); 512 x 896 x 151936
+// 87.7 us (449 MB, 5.1 TB/s, 79 % of the measured copy rate); 2048 x 4096 x 8192
+// to bf16 56.7 us (2.4 POP/s, tensor pipe 79 % busy; 256 tiles over 74 pairs
+// leave 13 % of the rounds idle).  Calls that last a second or more meet the
+// GPU's power limit: the last two then take 102 us (1305 MHz) and 65 us (1590
+// MHz), in a graph as well.
 constexpr int kI8Epilogue = 8;  // warps: two for each 32 lanes of tensor memory, on alternate 16 columns
 constexpr int kI8Threads = 64 + 32 * kI8Epilogue + 32;
 

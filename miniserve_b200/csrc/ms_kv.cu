@@ -11,7 +11,7 @@
 // owns 16 entries of a head (two 16-byte loads and stores: eight pairs, or 16
 // copied entries), keeps its eight cosines and sines in registers and turns
 // one to kKvHeads heads with them.  30011 tokens of 14 + 2 + 2 heads of 64
-// (139 MB): 29 us, 4.8 TB/s, 74 % of the measured copy rate; issue slots are
+// (139 MB): 28.5 us, 4.9 TB/s, 75 % of the measured copy rate; issue slots are
 // 60 % busy (address arithmetic and conversions) with four CTAs an SM.  512
 // tokens of 32 + 8 + 8 heads of 128 (12.7 MB): 4.1 us.
 #include <cuda_bf16.h>
@@ -139,7 +139,9 @@ struct KvVec<4> {
 // are (chunk of 2 kV entries, head slot, token); a slot is up to kHeads heads
 // of one of q, k and v, so that a thread finds its addresses once and steps
 // along them.  Its loads are issued before anything that depends on the
-// token's slot, position and table row.
+// token's slot, position and table row.  8-byte pieces cost twice the threads,
+// each with its slot, position and addresses: 20000 tokens of 14 + 2 + 2 heads
+// of 80, 40 of them rotated (115 MB), take 30.7 us.
 template <typename T, bool kInterleaved, int kHeads, int kV>
 __global__ void __launch_bounds__(kKvThreads, 4) ms_kv_append_kernel(const __grid_constant__ KvArgs p) {
   grid_wait();
@@ -217,7 +219,8 @@ __global__ void __launch_bounds__(kKvThreads, 4) ms_kv_append_kernel(const __gri
 }
 
 // Any head_dim, rotary and stride: a thread owns one pair, or two copied
-// entries, of a head.
+// entries, of a head.  Bound by instructions, a load and a store for every two
+// bytes: 30000 tokens of 13 + 3 + 3 heads of 35 (80 MB) take 79 us.
 template <typename T, bool kInterleaved>
 __global__ void __launch_bounds__(kKvThreads) ms_kv_append_any_kernel(const __grid_constant__ KvArgs p) {
   grid_wait();
