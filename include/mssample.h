@@ -67,8 +67,9 @@ enum {
                                  of the row had not arrived when
                                  ms_exchange_merge gave up waiting; token -1 */
   /* decode-step operators */
-  MS_ROW_BAD_SLOT = 32,       /* ms_kv_append: slot past the cache; nothing is
-                                 written to the cache for the token */
+  MS_ROW_BAD_SLOT = 32,       /* ms_kv_append, ms_kv4_append: slot past the
+                                 cache; nothing is written to the cache for the
+                                 token (ms_kv4_read: it reads as zeros) */
   MS_ROW_BAD_POSITION = 64,   /* ms_kv_append: position outside the table;
                                  nothing is written to the cache, the
                                  token's q_out is zero */
@@ -77,10 +78,12 @@ enum {
                                  its lse -inf */
   MS_ROW_BAD_PAGE = 256,      /* ms_prefix_attention: a page that the row or
                                  the prefix uses is outside the cache; as above */
-  MS_ROW_WAIT_TIMEOUT = 512   /* ms_prefix_attention: a wait inside the kernel
+  MS_ROW_WAIT_TIMEOUT = 512,  /* ms_prefix_attention: a wait inside the kernel
                                  of the shared prefix was given up after 1 s;
                                  the heads concerned have output 0 and lse
                                  -inf */
+  MS_ROW_BAD_DRAFT = 1024     /* ms_verify_drafts: a drafted token outside the
+                                 vocabulary; every token of the row is -1 */
 };
 
 /*
@@ -523,6 +526,87 @@ int64_t ms_int8_workspace(int64_t M, int64_t K);
 int ms_int8_linear(const void *x, int dtype, int64_t ldx, int64_t M, const int8_t *wq, int64_t ldw,
                    const float *w_scale, int64_t N, int64_t K, const float *bias, void *out, int out_dtype,
                    int64_t ldo, void *workspace, ms_stream_t stream);
+
+/*
+ * A paged cache held in 4 bits.  A token's head of head_dim entries (a multiple
+ * of 16, at most 128) is stored as codes, padded to a multiple of 32 entries
+ * and at least 64, and as a scale and a middle for every 32 entries, whose
+ * count is padded to 2 or 4:
+ *
+ *   codes   [pages, kv_heads, page_size, padded / 2] bytes; byte j holds
+ *           entries 2j (its low four bits) and 2j + 1
+ *   params  [pages, kv_heads, page_size, groups, 2] fp16
+ *   entry i stands for  middle[i / 32] + scale[i / 32] (code[i] - 8)
+ *
+ * for the keys and the values each, contiguous, the bases 16-byte aligned
+ * (MS_E_UNSUPPORTED otherwise).  What lies behind a head's entries and its
+ * ceil(head_dim / 32) parameters is not used.
+ */
+typedef struct {
+  int32_t kv_heads, head_dim;
+  int64_t pages, page_size;
+  uint8_t *k_codes;
+  void *k_params;
+  uint8_t *v_codes;
+  void *v_params;
+} ms_kv4_cache;
+
+/*
+ * ms_kv_append into such a cache.  The entries y of a group, the keys rotated
+ * (in fp32, not rounded to the model's type), are held with
+ *
+ *   scale = (max y - min y) / 15,  middle = min y + 8 scale   (rounded to fp16)
+ *   code  = clamp(rint((y - middle) / scale) + 8, 0, 15)
+ *
+ * that is, to half a scale and the roundings of scale and middle.  A group that
+ * holds a NaN or an infinity, or whose scale or middle is past fp16's range,
+ * reads back as NaN, and its token is flagged MS_ROW_NONFINITE.  Slots of one
+ * call must differ: of two equal ones the slot may hold some of either token's.
+ * q_out may be q itself (the same strides).  The struct is read on the host
+ * during the call; strides count entries and the last dimension is contiguous.
+ */
+typedef struct {
+  int32_t dtype;        /* MS_DTYPE_BF16 or MS_DTYPE_F16: q, k and v */
+  int32_t heads;        /* query heads; 0: no queries (q and q_out are not read) */
+  int32_t rotary;       /* even, <= head_dim; 0: nothing is rotated */
+  int32_t interleaved;
+  int64_t tokens;
+  const void *q;        /* [tokens, heads, head_dim] */
+  int64_t q_token, q_head;
+  const void *k;        /* [tokens, kv_heads, head_dim] */
+  int64_t k_token, k_head;
+  const void *v;        /* [tokens, kv_heads, head_dim] */
+  int64_t v_token, v_head;
+  void *q_out;          /* [tokens, heads, head_dim] */
+  int64_t q_out_token, q_out_head;
+  ms_kv4_cache cache;
+  const int64_t *slots; /* [tokens]; negative: padding */
+  const int64_t *positions; /* [tokens]; not read when rotary is 0 */
+  const float *table;   /* [table_rows, rotary]: rotary/2 cosines, then rotary/2 sines */
+  int64_t table_rows;
+  int32_t *status;      /* [tokens] MS_ROW_* bits out, or NULL */
+} ms_kv4_append_args;
+
+int ms_kv4_append(const ms_kv4_append_args *args, ms_stream_t stream);
+
+/*
+ * What the cache stands for in the given slots, computed in fp32 and rounded
+ * once to dtype (fp16: entries past its range become its largest).  A negative
+ * slot (padding) and one past the cache (MS_ROW_BAD_SLOT) read as zeros.
+ */
+typedef struct {
+  int32_t dtype;        /* MS_DTYPE_BF16 or MS_DTYPE_F16: k_out and v_out */
+  int64_t tokens;
+  ms_kv4_cache cache;
+  const int64_t *slots; /* [tokens] */
+  void *k_out;          /* [tokens, kv_heads, head_dim] */
+  int64_t k_token, k_head;
+  void *v_out;
+  int64_t v_token, v_head;
+  int32_t *status;      /* [tokens] MS_ROW_* bits out, or NULL */
+} ms_kv4_read_args;
+
+int ms_kv4_read(const ms_kv4_read_args *args, ms_stream_t stream);
 
 /* Human-readable text for an MS_E_* code. */
 const char *ms_error_string(int code);

@@ -10,10 +10,15 @@ The rest of a decode step's hot path lies beside it:
     from miniserve_b200 import append_kv, rope_table      # keys and values into a paged cache, rotated
     from miniserve_b200 import prefix_attention            # attention over the cache, a shared prefix read once
     from miniserve_b200 import Int8Linear                  # projections and LM head in 8-bit integers
+
+and the parts of a drafted-token step over a cache held in 4 bits:
+
+    from miniserve_b200 import KvCache4, append_kv4, read_kv4   # quantised as it is written, and read back
 """
 from .attention import prefix_attention  # noqa: F401
 from .int8 import Int8Linear, int8_matmul, quantize_rows  # noqa: F401
 from .kvcache import append_kv, rope_table  # noqa: F401
+from .kvcache4 import KvCache4, append_kv4, read_kv4  # noqa: F401
 from .sampler import Sampler, uniform_for_seed  # noqa: F401
 
 __version__ = "0.1.0"

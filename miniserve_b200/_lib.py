@@ -28,6 +28,7 @@ MS_ROW_BAD_POSITION = 64
 MS_ROW_BAD_LENGTH = 128
 MS_ROW_BAD_PAGE = 256
 MS_ROW_WAIT_TIMEOUT = 512
+MS_ROW_BAD_DRAFT = 1024
 
 BINDING_PATH = os.path.join(HERE, "_binding.so")
 
@@ -61,6 +62,28 @@ class PrefixAttentionArgs(ctypes.Structure):
                 ("lengths", _P), ("prefix_pages", _P), ("prefix_length", _I64), ("scale", ctypes.c_float),
                 ("out", _P), ("out_row", _I64), ("out_head", _I64), ("lse", _P), ("status", _P), ("workspace", _P),
                 ("workspace_bytes", _I64)]
+
+
+class Kv4Cache(ctypes.Structure):
+    """ms_kv4_cache of include/mssample.h."""
+    _fields_ = [("kv_heads", _I32), ("head_dim", _I32), ("pages", _I64), ("page_size", _I64), ("k_codes", _P),
+                ("k_params", _P), ("v_codes", _P), ("v_params", _P)]
+
+
+class Kv4AppendArgs(ctypes.Structure):
+    """ms_kv4_append_args of include/mssample.h."""
+    _fields_ = [("dtype", _I32), ("heads", _I32), ("rotary", _I32), ("interleaved", _I32), ("tokens", _I64),
+                ("q", _P), ("q_token", _I64), ("q_head", _I64), ("k", _P), ("k_token", _I64), ("k_head", _I64),
+                ("v", _P), ("v_token", _I64), ("v_head", _I64), ("q_out", _P), ("q_out_token", _I64),
+                ("q_out_head", _I64), ("cache", Kv4Cache), ("slots", _P), ("positions", _P), ("table", _P),
+                ("table_rows", _I64), ("status", _P)]
+
+
+class Kv4ReadArgs(ctypes.Structure):
+    """ms_kv4_read_args of include/mssample.h."""
+    _fields_ = [("dtype", _I32), ("tokens", _I64), ("cache", Kv4Cache), ("slots", _P), ("k_out", _P),
+                ("k_token", _I64), ("k_head", _I64), ("v_out", _P), ("v_token", _I64), ("v_head", _I64),
+                ("status", _P)]
 
 
 # name -> (restype, argtypes); every function include/mssample.h declares
@@ -120,6 +143,8 @@ SIGNATURES = {
                                       _I64, _P, _P]),
     "ms_prefix_attention": (ctypes.c_int, [ctypes.POINTER(PrefixAttentionArgs), _P]),
     "ms_prefix_attention_workspace": (_I64, [_I64, _I32, _I32, _I32, _I64]),
+    "ms_kv4_append": (ctypes.c_int, [ctypes.POINTER(Kv4AppendArgs), _P]),
+    "ms_kv4_read": (ctypes.c_int, [ctypes.POINTER(Kv4ReadArgs), _P]),
     "ms_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ms_last_cuda_error": (ctypes.c_int, []),
     "ms_version": (ctypes.c_int, []),
@@ -179,7 +204,7 @@ def binding():
                                           f"{torch.__version__}: build it again")
             module.bind(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in (
                 "ms_kv_append", "ms_prefix_attention", "ms_prefix_attention_workspace", "ms_int8_linear",
-                "ms_int8_workspace")))
+                "ms_int8_workspace", "ms_kv4_append", "ms_kv4_read")))
             _binding = module
     return _binding
 

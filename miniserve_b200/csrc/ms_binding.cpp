@@ -1,5 +1,5 @@
 // Python entry points of the decode-step operators: append_kv,
-// prefix_attention and int8_linear.
+// prefix_attention, int8_linear, and append_kv4 and read_kv4 of the 4-bit cache.
 //
 // A decode step makes dozens of these calls and a small batch's kernels take a
 // few microseconds, about what the interpreter needs to look at one tensor's
@@ -22,6 +22,7 @@
 #include <torch/version.h>
 
 #include <cmath>
+#include <cstring>
 #include <sstream>
 #include <string>
 
@@ -35,6 +36,8 @@ struct Entries {
   decltype(&ms_prefix_attention_workspace) prefix_attention_workspace;
   decltype(&ms_int8_linear) int8_linear;
   decltype(&ms_int8_workspace) int8_workspace;
+  decltype(&ms_kv4_append) kv4_append;
+  decltype(&ms_kv4_read) kv4_read;
 } entries = {};
 
 // A refused argument: the Python exception and its message.
@@ -144,6 +147,29 @@ PyObject *pair(PyObject *a, PyObject *b, PyObject *c = nullptr) {
   return t;
 }
 
+const at::Tensor &check_rope(PyObject *o, at::Device dev, int64_t dim) {
+  const at::Tensor &rope = tensor("rope", o);
+  check("rope", rope, at::kFloat, dev, {-1, 2, -1});
+  if (!rope.is_contiguous())
+    refuse(PyExc_ValueError, "rope must be a contiguous [positions, 2, rotary / 2] table (rope_table)");
+  if (rope.size(0) < 1 || rope.size(2) < 1 || 2 * rope.size(2) > dim)
+    refuse(PyExc_ValueError, "rope rotates ", 2 * rope.size(2), " entries of heads of ", dim, ", at ", rope.size(0),
+           " positions");
+  return rope;
+}
+
+// The rotated queries' tensor: q_out as given, or a new one.
+at::Tensor check_queries(const at::Tensor &q, PyObject *o, at::ScalarType type, at::Device dev, int64_t T, int64_t dim) {
+  check("q", q, type, dev, {T, -1, dim});
+  if (o == Py_None) return make(q.sizes(), type, dev);
+  const at::Tensor &q_out = tensor("q_out", o);
+  check("q_out", q_out, type, dev, q.sizes());
+  check_writable("q_out", q_out);
+  if (q_out.const_data_ptr() == q.const_data_ptr() && !same_strides(q_out, q))
+    refuse(PyExc_ValueError, "q_out in place of q must have q's strides");
+  return q_out;
+}
+
 // (cache_k, cache_v, k, v, slots, q, positions, rope, interleaved, q_out)
 PyObject *append_kv(PyObject *const *o) {
   const at::Tensor &ck = cuda_tensor("cache_k", o[0]), &cv = tensor("cache_v", o[1]);
@@ -163,13 +189,7 @@ PyObject *append_kv(PyObject *const *o) {
   if (interleaved < 0) return nullptr;
   a.interleaved = interleaved;
   if (o[7] != Py_None) {
-    const at::Tensor &rope = tensor("rope", o[7]);
-    check("rope", rope, at::kFloat, dev, {-1, 2, -1});
-    if (!rope.is_contiguous())
-      refuse(PyExc_ValueError, "rope must be a contiguous [positions, 2, rotary / 2] table (rope_table)");
-    if (rope.size(0) < 1 || rope.size(2) < 1 || 2 * rope.size(2) > dim)
-      refuse(PyExc_ValueError, "rope rotates ", 2 * rope.size(2), " entries of heads of ", dim, ", at ", rope.size(0),
-             " positions");
+    const at::Tensor &rope = check_rope(o[7], dev, dim);
     if (o[6] == Py_None) refuse(PyExc_ValueError, "rope needs positions");
     const at::Tensor &positions = tensor("positions", o[6]);
     check("positions", positions, at::kLong, dev, {T});
@@ -180,16 +200,7 @@ PyObject *append_kv(PyObject *const *o) {
   at::Tensor q_out;
   if (o[5] != Py_None) {
     const at::Tensor &q = tensor("q", o[5]);
-    check("q", q, type, dev, {T, -1, dim});
-    if (o[9] == Py_None) {
-      q_out = make(q.sizes(), type, dev);
-    } else {
-      q_out = tensor("q_out", o[9]);
-      check("q_out", q_out, type, dev, q.sizes());
-      check_writable("q_out", q_out);
-      if (q_out.const_data_ptr() == q.const_data_ptr() && !same_strides(q_out, q))
-        refuse(PyExc_ValueError, "q_out in place of q must have q's strides");
-    }
+    q_out = check_queries(q, o[9], type, dev, T, dim);
     a.heads = (int32_t)q.size(1);
     a.q = q.const_data_ptr(), a.q_token = q.stride(0), a.q_head = q.stride(1);
     a.q_out = q_out.data_ptr(), a.q_out_token = q_out.stride(0), a.q_out_head = q_out.stride(1);
@@ -334,6 +345,121 @@ PyObject *int8_linear(PyObject *const *o) {
   return o[5] != Py_None ? Py_NewRef(o[5]) : THPVariable_Wrap(out);
 }
 
+// A KvCache4 as its wrapper hands it over: (k_codes, k_params, v_codes, v_params, head_dim, dtype).
+constexpr int kCache4 = 6;
+struct Cache4 {
+  ms_kv4_cache c = {};
+  at::ScalarType type;
+  at::Device device;
+};
+Cache4 cache4(PyObject *const *o) {
+  const at::Tensor &kc = cuda_tensor("k_codes", o[0]), &kp = tensor("k_params", o[1]), &vc = tensor("v_codes", o[2]),
+                   &vp = tensor("v_params", o[3]);
+  Cache4 r{{}, at::kBFloat16, kc.device()};
+  if (!THPDtype_Check(o[5])) refuse(PyExc_TypeError, "the cache's dtype must be a torch.dtype");
+  r.type = reinterpret_cast<THPDtype *>(o[5])->scalar_type;
+  if (r.type != at::kBFloat16 && r.type != at::kHalf)
+    refuse(PyExc_TypeError, "the cache's dtype is ", r.type, ", expected bfloat16 or float16");
+  const int64_t dim = integer("head_dim", o[4]);
+  if (dim < 16 || dim % 16 || dim > 128) refuse(PyExc_ValueError, "head_dim ", dim, " is not a multiple of 16 up to 128");
+  const int64_t used = (dim + 31) / 32, stored = used < 2 ? 2 : used, groups = stored == 3 ? 4 : stored;
+  check("k_codes", kc, at::kByte, r.device, {-1, -1, -1, stored * 16});
+  check("k_params", kp, at::kHalf, r.device, {kc.size(0), kc.size(1), kc.size(2), groups, 2});
+  check("v_codes", vc, at::kByte, r.device, kc.sizes());
+  check("v_params", vp, at::kHalf, r.device, kp.sizes());
+  if (kc.numel() == 0) refuse(PyExc_ValueError, "the cache is empty");
+  uintptr_t bases = 0;
+  for (const at::Tensor *t : {&kc, &kp, &vc, &vp}) {
+    if (!t->is_contiguous()) refuse(PyExc_ValueError, "the cache's tensors must be contiguous");
+    bases |= reinterpret_cast<uintptr_t>(t->const_data_ptr());
+  }
+  if (bases & 15) refuse(PyExc_ValueError, "the cache's tensors must start 16-byte aligned");
+  r.c.pages = kc.size(0), r.c.kv_heads = (int32_t)kc.size(1), r.c.page_size = kc.size(2), r.c.head_dim = (int32_t)dim;
+  r.c.k_codes = static_cast<uint8_t *>(kc.data_ptr()), r.c.k_params = kp.data_ptr();
+  r.c.v_codes = static_cast<uint8_t *>(vc.data_ptr()), r.c.v_params = vp.data_ptr();
+  return r;
+}
+
+// (KvCache4, k, v, slots, q, positions, rope, interleaved, q_out)
+PyObject *append_kv4(PyObject *const *o) {
+  const Cache4 cache = cache4(o);
+  o += kCache4;
+  const at::ScalarType type = cache.type;
+  const at::Device dev = cache.device;
+  const int64_t heads = cache.c.kv_heads, dim = cache.c.head_dim;
+  const at::Tensor &k = tensor("k", o[0]), &v = tensor("v", o[1]), &slots = tensor("slots", o[2]);
+  check("k", k, type, dev, {-1, heads, dim});
+  const int64_t T = k.size(0);
+  check("v", v, type, dev, {T, heads, dim});
+  check("slots", slots, at::kLong, dev, {T});
+  ms_kv4_append_args a = {};
+  a.dtype = type == at::kHalf ? MS_DTYPE_F16 : MS_DTYPE_BF16;
+  a.tokens = T, a.cache = cache.c;
+  const int interleaved = PyObject_IsTrue(o[6]);
+  if (interleaved < 0) return nullptr;
+  a.interleaved = interleaved;
+  if (o[5] != Py_None) {
+    const at::Tensor &rope = check_rope(o[5], dev, dim);
+    if (o[4] == Py_None) refuse(PyExc_ValueError, "rope needs positions");
+    const at::Tensor &positions = tensor("positions", o[4]);
+    check("positions", positions, at::kLong, dev, {T});
+    a.rotary = (int32_t)(2 * rope.size(2));
+    a.positions = positions.const_data_ptr<int64_t>();
+    a.table = rope.const_data_ptr<float>(), a.table_rows = rope.size(0);
+  }
+  at::Tensor q_out;
+  if (o[3] != Py_None) {
+    const at::Tensor &q = tensor("q", o[3]);
+    q_out = check_queries(q, o[7], type, dev, T, dim);
+    a.heads = (int32_t)q.size(1);
+    a.q = q.const_data_ptr(), a.q_token = q.stride(0), a.q_head = q.stride(1);
+    a.q_out = q_out.data_ptr(), a.q_out_token = q_out.stride(0), a.q_out_head = q_out.stride(1);
+  } else if (o[7] != Py_None) {
+    refuse(PyExc_ValueError, "q_out needs q");
+  }
+  a.k = k.const_data_ptr(), a.k_token = k.stride(0), a.k_head = k.stride(1);
+  a.v = v.const_data_ptr(), a.v_token = v.stride(0), a.v_head = v.stride(1);
+  a.slots = slots.const_data_ptr<int64_t>();
+  at::Tensor status = make({T}, at::kInt, dev);
+  a.status = status.data_ptr<int32_t>();
+  call(dev, [&](ms_stream_t s) { return entries.kv4_append(&a, s); });
+  PyObject *first = q_out.defined() ? (o[7] != Py_None ? Py_NewRef(o[7]) : THPVariable_Wrap(q_out)) : Py_NewRef(Py_None);
+  return pair(first, THPVariable_Wrap(status));
+}
+
+// (KvCache4, slots, k_out, v_out)
+PyObject *read_kv4(PyObject *const *o) {
+  const Cache4 cache = cache4(o);
+  o += kCache4;
+  const at::Device dev = cache.device;
+  const at::Tensor &slots = tensor("slots", o[0]);
+  check("slots", slots, at::kLong, dev, {-1});
+  const int64_t T = slots.size(0), heads = cache.c.kv_heads, dim = cache.c.head_dim;
+  at::Tensor out[2];
+  for (int i = 0; i < 2; ++i) {
+    const char *name = i ? "v_out" : "k_out";
+    if (o[1 + i] == Py_None) {
+      out[i] = make({T, heads, dim}, cache.type, dev);
+    } else {
+      out[i] = tensor(name, o[1 + i]);
+      check(name, out[i], cache.type, dev, {T, heads, dim});
+      check_writable(name, out[i]);
+    }
+  }
+  if (out[0].numel() > 0 && out[0].const_data_ptr() == out[1].const_data_ptr())
+    refuse(PyExc_ValueError, "k_out and v_out are the same memory");
+  at::Tensor status = make({T}, at::kInt, dev);
+  ms_kv4_read_args a = {};
+  a.dtype = cache.type == at::kHalf ? MS_DTYPE_F16 : MS_DTYPE_BF16;
+  a.tokens = T, a.cache = cache.c, a.slots = slots.const_data_ptr<int64_t>();
+  a.k_out = out[0].data_ptr(), a.k_token = out[0].stride(0), a.k_head = out[0].stride(1);
+  a.v_out = out[1].data_ptr(), a.v_token = out[1].stride(0), a.v_head = out[1].stride(1);
+  a.status = status.data_ptr<int32_t>();
+  call(dev, [&](ms_stream_t s) { return entries.kv4_read(&a, s); });
+  return pair(o[1] != Py_None ? Py_NewRef(o[1]) : THPVariable_Wrap(out[0]),
+              o[2] != Py_None ? Py_NewRef(o[2]) : THPVariable_Wrap(out[1]), THPVariable_Wrap(status));
+}
+
 // Arguments counted, exceptions turned into Python's: (type, text) of a
 // refusal, (None, code) of an entry point's return.
 template <int kCount, PyObject *(*kRun)(PyObject *const *)>
@@ -370,15 +496,19 @@ PyObject *entry(PyObject *self, PyObject *const *args, Py_ssize_t n) {
   return nullptr;
 }
 
-// bind(address of ms_kv_append, ms_prefix_attention, ms_prefix_attention_workspace, ms_int8_linear, ms_int8_workspace)
+// bind(addresses of the entry points, in the order of Entries)
 PyObject *bind(PyObject *, PyObject *args) {
-  unsigned long long p[5];
-  if (!PyArg_ParseTuple(args, "KKKKK", &p[0], &p[1], &p[2], &p[3], &p[4])) return nullptr;
-  entries.prefix_attention = reinterpret_cast<decltype(entries.prefix_attention)>(p[1]);
-  entries.prefix_attention_workspace = reinterpret_cast<decltype(entries.prefix_attention_workspace)>(p[2]);
-  entries.int8_linear = reinterpret_cast<decltype(entries.int8_linear)>(p[3]);
-  entries.int8_workspace = reinterpret_cast<decltype(entries.int8_workspace)>(p[4]);
-  entries.kv_append = reinterpret_cast<decltype(entries.kv_append)>(p[0]);
+  constexpr Py_ssize_t kEntries = sizeof(Entries) / sizeof(void *);
+  if (PyTuple_GET_SIZE(args) != kEntries) {
+    PyErr_Format(PyExc_TypeError, "bind takes %zd addresses", kEntries);
+    return nullptr;
+  }
+  void *p[kEntries];
+  for (Py_ssize_t i = 0; i < kEntries; ++i) {
+    p[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(args, i));
+    if (!p[i] && PyErr_Occurred()) return nullptr;
+  }
+  std::memcpy(&entries, p, sizeof(entries));
   Py_RETURN_NONE;
 }
 
@@ -392,6 +522,8 @@ PyMethodDef methods[] = {
     {"append_kv", fast<10, append_kv>(), METH_FASTCALL, "see miniserve_b200.kvcache.append_kv"},
     {"prefix_attention", fast<9, prefix_attention>(), METH_FASTCALL, "see miniserve_b200.attention.prefix_attention"},
     {"int8_linear", fast<6, int8_linear>(), METH_FASTCALL, "see miniserve_b200.int8.Int8Linear"},
+    {"append_kv4", fast<kCache4 + 8, append_kv4>(), METH_FASTCALL, "see miniserve_b200.kvcache4.append_kv4"},
+    {"read_kv4", fast<kCache4 + 3, read_kv4>(), METH_FASTCALL, "see miniserve_b200.kvcache4.read_kv4"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", "Checked entry points of the decode-step operators.", -1,

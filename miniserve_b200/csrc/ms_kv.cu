@@ -20,36 +20,10 @@
 
 #include "../../include/mssample.h"
 #include "ms_host.h"
+#include "ms_kv.cuh"
 #include "ms_tc.cuh"
 
 namespace ms {
-
-template <typename T>
-__device__ __forceinline__ float2 kv_widen(uint32_t u);
-template <>
-__device__ __forceinline__ float2 kv_widen<__nv_bfloat16>(uint32_t u) {
-  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
-}
-template <>
-__device__ __forceinline__ float2 kv_widen<__half>(uint32_t u) {
-  return __half22float2(*reinterpret_cast<const __half2 *>(&u));
-}
-template <typename T>
-__device__ __forceinline__ uint32_t kv_narrow(float x, float y);
-template <>
-__device__ __forceinline__ uint32_t kv_narrow<__nv_bfloat16>(float x, float y) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t kv_narrow<__half>(float x, float y) {
-  const __half2 h = __floats2half2_rn(x, y);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float kv_to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float kv_to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ void kv_from_float(float x, __nv_bfloat16 &y) { y = __float2bfloat16_rn(x); }
-__device__ __forceinline__ void kv_from_float(float x, __half &y) { y = __float2half_rn(x); }
 
 struct KvArgs {
   ms_kv_append_args a;
@@ -77,16 +51,7 @@ __device__ __forceinline__ KvRow kv_row(const KvArgs &p, int64_t t) {
   if (slot >= a.pages * a.page_size) {
     r.status |= MS_ROW_BAD_SLOT;
   } else if (slot >= 0) {
-    if (p.page_shift >= 0) {
-      r.page = slot >> p.page_shift;
-      r.offset = slot & (a.page_size - 1);
-    } else if (slot < (1ll << 32)) {
-      r.page = (uint32_t)slot / (uint32_t)a.page_size;
-      r.offset = (uint32_t)slot - (uint32_t)r.page * (uint32_t)a.page_size;
-    } else {
-      r.page = slot / a.page_size;
-      r.offset = slot - r.page * a.page_size;
-    }
+    kv_place(slot, a.page_size, p.page_shift, r.page, r.offset);
     r.write = true;
   }
   if (a.rotary > 0) {
@@ -326,9 +291,7 @@ extern "C" int ms_kv_append(const ms_kv_append_args *args, ms_stream_t stream) {
   uint64_t bases = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
                    reinterpret_cast<uintptr_t>(a.cache_k) | reinterpret_cast<uintptr_t>(a.cache_v);
   if (a.heads > 0) bases |= reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out);
-  p.page_shift = -1;
-  for (int i = 0; i < 31; ++i)
-    if (a.page_size == 1ll << i) p.page_shift = i;
+  p.page_shift = ms::kv_page_shift(a.page_size);
   int64_t strides = a.k_token | a.k_head | a.v_token | a.v_head | a.ck_page | a.ck_token | a.ck_head | a.cv_page |
                     a.cv_token | a.cv_head;
   if (a.heads > 0) strides |= a.q_token | a.q_head | a.q_out_token | a.q_out_head;
