@@ -608,6 +608,54 @@ typedef struct {
 
 int ms_kv4_read(const ms_kv4_read_args *args, ms_stream_t stream);
 
+/*
+ * Attention over a cache held in 4 bits: `tokens` query tokens of every row
+ * over the row's own pages.  Token t of row b sees keys 0..lengths[b, t]-1
+ * (pages table[b, j / page_size]); query head h sees key head
+ * h / (heads / kv_heads):
+ *
+ *   out[b, t, h] = sum_j softmax_j(scale q[b, t, h] . k_j) v_j
+ *   lse[b, t, h] = log sum_j exp(scale q[b, t, h] . k_j)
+ *
+ * k_j and v_j being what the cache stands for, not rounded; scores and sums in
+ * fp32, the weights (times the values' scales) rounded to fp16 for their
+ * product with the codes, out rounded once.  A token that sees no key has out
+ * 0 and lse -inf.  What the cache holds past the keys that a token sees is not
+ * used for it, NaN and infinities included.  A row with a length below 0 or
+ * past its pages has out 0 and lse -inf for all its tokens and is flagged
+ * MS_ROW_BAD_LENGTH; one that uses a page outside the cache has so for the
+ * heads concerned and is flagged MS_ROW_BAD_PAGE.
+ *
+ * tokens is at most 1024; scale is positive, at most 2e38.  The struct is read
+ * on the host during the call.  workspace: ms_kv4_attention_workspace(...)
+ * bytes of the current device, 256-byte aligned, this call's until it has
+ * finished.
+ */
+typedef struct {
+  int32_t dtype;        /* MS_DTYPE_BF16 or MS_DTYPE_F16: q and out */
+  int32_t tokens;       /* query tokens of a row */
+  int32_t heads;        /* query heads, a multiple of the cache's */
+  int64_t rows;
+  const void *q;        /* [rows, tokens, heads, head_dim] */
+  int64_t q_row, q_token, q_head;
+  ms_kv4_cache cache;
+  const int32_t *table; /* [rows, table_width] pages, rows table_row entries apart */
+  int64_t table_width, table_row;
+  const int32_t *lengths; /* [rows, tokens], rows length_row entries apart */
+  int64_t length_row;
+  float scale;
+  void *out;            /* [rows, tokens, heads, head_dim] */
+  int64_t out_row, out_token, out_head;
+  float *lse;           /* [rows, tokens, heads] */
+  int32_t *status;      /* [rows] MS_ROW_* bits */
+  void *workspace;
+  int64_t workspace_bytes;
+} ms_kv4_attention_args;
+
+int ms_kv4_attention(const ms_kv4_attention_args *args, ms_stream_t stream);
+
+int64_t ms_kv4_attention_workspace(int64_t rows, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim);
+
 /* Human-readable text for an MS_E_* code. */
 const char *ms_error_string(int code);
 

@@ -86,6 +86,15 @@ class Kv4ReadArgs(ctypes.Structure):
                 ("status", _P)]
 
 
+class Kv4AttentionArgs(ctypes.Structure):
+    """ms_kv4_attention_args of include/mssample.h."""
+    _fields_ = [("dtype", _I32), ("tokens", _I32), ("heads", _I32), ("rows", _I64), ("q", _P), ("q_row", _I64),
+                ("q_token", _I64), ("q_head", _I64), ("cache", Kv4Cache), ("table", _P), ("table_width", _I64),
+                ("table_row", _I64), ("lengths", _P), ("length_row", _I64), ("scale", ctypes.c_float), ("out", _P),
+                ("out_row", _I64), ("out_token", _I64), ("out_head", _I64), ("lse", _P), ("status", _P),
+                ("workspace", _P), ("workspace_bytes", _I64)]
+
+
 # name -> (restype, argtypes); every function include/mssample.h declares
 SIGNATURES = {
     "ms_sample": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64,
@@ -145,6 +154,8 @@ SIGNATURES = {
     "ms_prefix_attention_workspace": (_I64, [_I64, _I32, _I32, _I32, _I64]),
     "ms_kv4_append": (ctypes.c_int, [ctypes.POINTER(Kv4AppendArgs), _P]),
     "ms_kv4_read": (ctypes.c_int, [ctypes.POINTER(Kv4ReadArgs), _P]),
+    "ms_kv4_attention": (ctypes.c_int, [ctypes.POINTER(Kv4AttentionArgs), _P]),
+    "ms_kv4_attention_workspace": (_I64, [_I64, _I32, _I32, _I32, _I32]),
     "ms_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ms_last_cuda_error": (ctypes.c_int, []),
     "ms_version": (ctypes.c_int, []),
@@ -204,7 +215,8 @@ def binding():
                                           f"{torch.__version__}: build it again")
             module.bind(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in (
                 "ms_kv_append", "ms_prefix_attention", "ms_prefix_attention_workspace", "ms_int8_linear",
-                "ms_int8_workspace", "ms_kv4_append", "ms_kv4_read")))
+                "ms_int8_workspace", "ms_kv4_append", "ms_kv4_read", "ms_kv4_attention",
+                "ms_kv4_attention_workspace")))
             _binding = module
     return _binding
 

@@ -1,5 +1,6 @@
 // Python entry points of the decode-step operators: append_kv,
-// prefix_attention, int8_linear, and append_kv4 and read_kv4 of the 4-bit cache.
+// prefix_attention, int8_linear, and append_kv4, read_kv4 and attention_kv4 of
+// the 4-bit cache.
 //
 // A decode step makes dozens of these calls and a small batch's kernels take a
 // few microseconds, about what the interpreter needs to look at one tensor's
@@ -38,6 +39,8 @@ struct Entries {
   decltype(&ms_int8_workspace) int8_workspace;
   decltype(&ms_kv4_append) kv4_append;
   decltype(&ms_kv4_read) kv4_read;
+  decltype(&ms_kv4_attention) kv4_attention;
+  decltype(&ms_kv4_attention_workspace) kv4_attention_workspace;
 } entries = {};
 
 // A refused argument: the Python exception and its message.
@@ -460,6 +463,61 @@ PyObject *read_kv4(PyObject *const *o) {
               o[2] != Py_None ? Py_NewRef(o[2]) : THPVariable_Wrap(out[1]), THPVariable_Wrap(status));
 }
 
+// (KvCache4, q, pages, lengths, scale, out)
+PyObject *attention_kv4(PyObject *const *o) {
+  const Cache4 cache = cache4(o);
+  o += kCache4;
+  const at::Device dev = cache.device;
+  const int64_t kv_heads = cache.c.kv_heads, dim = cache.c.head_dim;
+  const at::Tensor &q = tensor("q", o[0]), &pages = tensor("pages", o[1]), &lengths = tensor("lengths", o[2]);
+  const bool several = q.dim() == 4;
+  if (several) check("q", q, cache.type, dev, {-1, -1, -1, dim});
+  else check("q", q, cache.type, dev, {-1, -1, dim});
+  const int64_t B = q.size(0), T = several ? q.size(1) : 1, heads = q.size(several ? 2 : 1);
+  if (heads < 1 || heads % kv_heads)
+    refuse(PyExc_ValueError, "q has ", heads, " heads, expected a multiple of the cache's ", kv_heads);
+  if (T < 1 || T > 1024) refuse(PyExc_ValueError, "q has ", T, " tokens a row, expected 1 to 1024");
+  check("pages", pages, at::kInt, dev, {B, -1});
+  if (several) check("lengths", lengths, at::kInt, dev, {B, T});
+  else check("lengths", lengths, at::kInt, dev, {B});
+  double scale = 1.0 / std::sqrt((double)dim);
+  if (o[3] != Py_None) {
+    scale = PyFloat_AsDouble(o[3]);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    if (!((float)scale > 0.f) || !std::isfinite((float)scale))
+      refuse(PyExc_ValueError, "scale must be positive and finite");
+  }
+  at::Tensor out;
+  if (o[4] == Py_None) {
+    out = make(q.sizes(), cache.type, dev);
+  } else {
+    out = tensor("out", o[4]);
+    check("out", out, cache.type, dev, q.sizes());
+    check_writable("out", out);
+  }
+  at::Tensor lse = make(q.sizes().slice(0, q.dim() - 1), at::kFloat, dev), status = make({B}, at::kInt, dev);
+  ms_kv4_attention_args a = {};
+  a.dtype = cache.type == at::kHalf ? MS_DTYPE_F16 : MS_DTYPE_BF16;
+  a.tokens = (int32_t)T, a.heads = (int32_t)heads, a.rows = B, a.cache = cache.c;
+  a.q = q.const_data_ptr(), a.q_row = q.stride(0), a.q_token = several ? q.stride(1) : 0, a.q_head = q.stride(-2);
+  a.table = pages.const_data_ptr<int32_t>(), a.table_width = pages.size(1);
+  a.table_row = B > 1 ? pages.stride(0) : pages.size(1);
+  a.lengths = lengths.const_data_ptr<int32_t>(), a.length_row = B > 1 ? lengths.stride(0) : T;
+  a.scale = (float)scale;
+  a.out = out.data_ptr(), a.out_row = out.stride(0), a.out_token = several ? out.stride(1) : 0, a.out_head = out.stride(-2);
+  a.lse = lse.data_ptr<float>(), a.status = status.data_ptr<int32_t>();
+  at::Tensor workspace;
+  {
+    const c10::cuda::CUDAGuard guard(dev);
+    a.workspace_bytes = entries.kv4_attention_workspace(B, a.tokens, a.heads, a.cache.kv_heads, a.cache.head_dim);
+    workspace = make({a.workspace_bytes}, at::kByte, dev);
+  }
+  a.workspace = workspace.data_ptr();
+  call(dev, [&](ms_stream_t s) { return entries.kv4_attention(&a, s); });
+  return pair(o[4] != Py_None ? Py_NewRef(o[4]) : THPVariable_Wrap(out), THPVariable_Wrap(lse),
+              THPVariable_Wrap(status));
+}
+
 // Arguments counted, exceptions turned into Python's: (type, text) of a
 // refusal, (None, code) of an entry point's return.
 template <int kCount, PyObject *(*kRun)(PyObject *const *)>
@@ -524,6 +582,7 @@ PyMethodDef methods[] = {
     {"int8_linear", fast<6, int8_linear>(), METH_FASTCALL, "see miniserve_b200.int8.Int8Linear"},
     {"append_kv4", fast<kCache4 + 8, append_kv4>(), METH_FASTCALL, "see miniserve_b200.kvcache4.append_kv4"},
     {"read_kv4", fast<kCache4 + 3, read_kv4>(), METH_FASTCALL, "see miniserve_b200.kvcache4.read_kv4"},
+    {"attention_kv4", fast<kCache4 + 5, attention_kv4>(), METH_FASTCALL, "see miniserve_b200.attention4.attention_kv4"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", "Checked entry points of the decode-step operators.", -1,
