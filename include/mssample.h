@@ -656,6 +656,64 @@ int ms_kv4_attention(const ms_kv4_attention_args *args, ms_stream_t stream);
 
 int64_t ms_kv4_attention_workspace(int64_t rows, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim);
 
+/*
+ * Verification of drafted tokens against a target model's logits, from given
+ * uniforms.  Row b's drafts d_0, d_1, ... are draft_tokens[b] up to its first
+ * negative entry, n of them.  With p_i = softmax(logits[b, i] / temperature[b])
+ * and q_i = draft_probs[b, i] (what d_i was drawn from):
+ *
+ *   d_i is accepted when  u[b, i] q_i(d_i) < p_i(d_i),  one after the other;
+ *   at the first i that is not, a token is drawn from max(p_i - q_i, 0);
+ *   where all are accepted, one is drawn from p_n.
+ *
+ * The drawn token is the first, in index order, whose running mass passes
+ * u[b, drafts] times the whole mass.  draft_probs NULL: drafts that come from no
+ * distribution (looked up); q_i is 1 at d_i, 0 elsewhere.  Temperature 0: p_i is
+ * 1 at the first largest logit, draft_probs is not used.  Tokens that a filter
+ * or grammar forbids have logits -inf (the logits-processor convention,
+ * miniserve/model_runner.py:214-216).
+ *
+ *   tokens [rows, drafts + 1]: the accepted drafts, the drawn token, then -1;
+ *   probs the same places: p_i of the token (0 behind the last);
+ *   counts [rows]: how many tokens that is, 1 to n + 1.
+ *
+ * row_status: MS_ROW_BAD_TEMPERATURE (negative, NaN, infinite), MS_ROW_BAD_DRAFT
+ * (a draft >= vocab), MS_ROW_ALL_MASKED (every logit of the position drawn from
+ * is -inf, temperature > 0): tokens -1, probs 0, count 0.  MS_ROW_NONFINITE: a
+ * position up to the one drawn from holds a NaN logit (read as -inf) or +inf
+ * (such tokens share the probability), or the draft's probabilities that were
+ * subtracted an infinity, a negative entry or a NaN (read as 0).
+ *
+ * Acceptance is decided with sums of fp32 weights (within 1e-6 of p), draws
+ * with fp64 weights and sums.  drafts is at most 255.  The struct is read on the host
+ * during the call; strides count entries.  workspace: ms_verify_workspace(...)
+ * bytes, 16-byte aligned, this call's until it has finished.
+ */
+typedef struct {
+  int32_t dtype;        /* MS_DTYPE_F32, _BF16 or _F16: logits */
+  int32_t drafts;       /* drafted tokens of a row, at most */
+  int64_t rows, vocab;
+  const void *logits;   /* [rows, drafts + 1, vocab], the last dimension contiguous */
+  int64_t logits_row, logits_pos;
+  const int64_t *draft_tokens; /* [rows, drafts], rows draft_row entries apart */
+  int64_t draft_row;
+  const float *draft_probs;    /* [rows, drafts, vocab], or NULL */
+  int64_t probs_row, probs_pos;
+  const double *uniforms;      /* [rows, drafts + 1] in [0, 1), rows uniform_row entries apart */
+  int64_t uniform_row;
+  const double *temperature;   /* [rows] */
+  int64_t *tokens;      /* [rows, drafts + 1] */
+  float *probs;         /* [rows, drafts + 1] */
+  int32_t *counts;      /* [rows] */
+  int32_t *status;      /* [rows] MS_ROW_* bits */
+  void *workspace;
+  int64_t workspace_bytes;
+} ms_verify_args;
+
+int ms_verify_drafts(const ms_verify_args *args, ms_stream_t stream);
+
+int64_t ms_verify_workspace(int64_t rows, int32_t drafts, int64_t vocab);
+
 /* Human-readable text for an MS_E_* code. */
 const char *ms_error_string(int code);
 

@@ -15,6 +15,7 @@ and the parts of a drafted-token step over a cache held in 4 bits:
 
     from miniserve_b200 import KvCache4, append_kv4, read_kv4   # quantised as it is written, and read back
     from miniserve_b200 import attention_kv4                    # one or several tokens a row over it
+    from miniserve_b200 import verify_drafts                    # drafted tokens against the target's logits
 """
 from .attention import prefix_attention  # noqa: F401
 from .attention4 import attention_kv4  # noqa: F401
@@ -22,5 +23,6 @@ from .int8 import Int8Linear, int8_matmul, quantize_rows  # noqa: F401
 from .kvcache import append_kv, rope_table  # noqa: F401
 from .kvcache4 import KvCache4, append_kv4, read_kv4  # noqa: F401
 from .sampler import Sampler, uniform_for_seed  # noqa: F401
+from .verify import verify_drafts  # noqa: F401
 
 __version__ = "0.1.0"

@@ -95,6 +95,15 @@ class Kv4AttentionArgs(ctypes.Structure):
                 ("workspace", _P), ("workspace_bytes", _I64)]
 
 
+class VerifyArgs(ctypes.Structure):
+    """ms_verify_args of include/mssample.h."""
+    _fields_ = [("dtype", _I32), ("drafts", _I32), ("rows", _I64), ("vocab", _I64), ("logits", _P),
+                ("logits_row", _I64), ("logits_pos", _I64), ("draft_tokens", _P), ("draft_row", _I64),
+                ("draft_probs", _P), ("probs_row", _I64), ("probs_pos", _I64), ("uniforms", _P),
+                ("uniform_row", _I64), ("temperature", _P), ("tokens", _P), ("probs", _P), ("counts", _P),
+                ("status", _P), ("workspace", _P), ("workspace_bytes", _I64)]
+
+
 # name -> (restype, argtypes); every function include/mssample.h declares
 SIGNATURES = {
     "ms_sample": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64,
@@ -156,6 +165,8 @@ SIGNATURES = {
     "ms_kv4_read": (ctypes.c_int, [ctypes.POINTER(Kv4ReadArgs), _P]),
     "ms_kv4_attention": (ctypes.c_int, [ctypes.POINTER(Kv4AttentionArgs), _P]),
     "ms_kv4_attention_workspace": (_I64, [_I64, _I32, _I32, _I32, _I32]),
+    "ms_verify_drafts": (ctypes.c_int, [ctypes.POINTER(VerifyArgs), _P]),
+    "ms_verify_workspace": (_I64, [_I64, _I32, _I64]),
     "ms_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ms_last_cuda_error": (ctypes.c_int, []),
     "ms_version": (ctypes.c_int, []),
@@ -216,7 +227,7 @@ def binding():
             module.bind(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in (
                 "ms_kv_append", "ms_prefix_attention", "ms_prefix_attention_workspace", "ms_int8_linear",
                 "ms_int8_workspace", "ms_kv4_append", "ms_kv4_read", "ms_kv4_attention",
-                "ms_kv4_attention_workspace")))
+                "ms_kv4_attention_workspace", "ms_verify_drafts", "ms_verify_workspace")))
             _binding = module
     return _binding
 

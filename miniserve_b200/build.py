@@ -19,7 +19,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmssample.so")
 BINDING = os.path.join(HERE, "_binding.so")
-SOURCES = ["ms_sample.cu", "ms_kv.cu", "ms_kv4.cu", "ms_attn.cu", "ms_attn4.cu", "ms_int8.cu"]
+SOURCES = ["ms_sample.cu", "ms_kv.cu", "ms_kv4.cu", "ms_attn.cu", "ms_attn4.cu", "ms_int8.cu",
+           "ms_verify.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

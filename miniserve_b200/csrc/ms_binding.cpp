@@ -1,6 +1,6 @@
 // Python entry points of the decode-step operators: append_kv,
-// prefix_attention, int8_linear, and append_kv4, read_kv4 and attention_kv4 of
-// the 4-bit cache.
+// prefix_attention, int8_linear, append_kv4, read_kv4 and attention_kv4 of the
+// 4-bit cache, and verify_drafts.
 //
 // A decode step makes dozens of these calls and a small batch's kernels take a
 // few microseconds, about what the interpreter needs to look at one tensor's
@@ -41,6 +41,8 @@ struct Entries {
   decltype(&ms_kv4_read) kv4_read;
   decltype(&ms_kv4_attention) kv4_attention;
   decltype(&ms_kv4_attention_workspace) kv4_attention_workspace;
+  decltype(&ms_verify_drafts) verify_drafts;
+  decltype(&ms_verify_workspace) verify_workspace;
 } entries = {};
 
 // A refused argument: the Python exception and its message.
@@ -518,6 +520,47 @@ PyObject *attention_kv4(PyObject *const *o) {
               THPVariable_Wrap(status));
 }
 
+// (logits, drafts, uniforms, draft_probs, temperature)
+PyObject *verify_drafts(PyObject *const *o) {
+  const at::Tensor &logits = cuda_tensor("logits", o[0]), &drafts = tensor("drafts", o[1]), &uniforms = tensor("uniforms", o[2]),
+                   &heat = tensor("temperature", o[4]);
+  const at::Device dev = logits.device();
+  ms_verify_args a = {};
+  a.dtype = float_code("logits'", logits.scalar_type());
+  check("logits", logits, logits.scalar_type(), dev, {-1, -1, -1});
+  const int64_t B = logits.size(0), n = logits.size(1) - 1, V = logits.size(2);
+  if (n < 0 || n > 255) refuse(PyExc_ValueError, "logits has ", n + 1, " positions a row, expected 1 to 256");
+  if (V < 1) refuse(PyExc_ValueError, "logits has no vocabulary");
+  check("drafts", drafts, at::kLong, dev, {B, n});
+  check("uniforms", uniforms, at::kDouble, dev, {B, n + 1});
+  check("temperature", heat, at::kDouble, dev, {B});
+  if (o[3] != Py_None) {
+    const at::Tensor &q = tensor("draft_probs", o[3]);
+    check("draft_probs", q, at::kFloat, dev, {B, n, V});
+    a.draft_probs = q.const_data_ptr<float>(), a.probs_row = q.stride(0), a.probs_pos = q.stride(1);
+  }
+  a.drafts = (int32_t)n, a.rows = B, a.vocab = V;
+  a.logits = logits.const_data_ptr(), a.logits_row = logits.stride(0), a.logits_pos = logits.stride(1);
+  a.draft_tokens = drafts.const_data_ptr<int64_t>(), a.draft_row = drafts.stride(0);
+  a.uniforms = uniforms.const_data_ptr<double>(), a.uniform_row = uniforms.stride(0);
+  a.temperature = heat.const_data_ptr<double>();
+  at::Tensor tokens = make({B, n + 1}, at::kLong, dev), probs = make({B, n + 1}, at::kFloat, dev),
+             counts = make({B}, at::kInt, dev), status = make({B}, at::kInt, dev);
+  a.tokens = tokens.data_ptr<int64_t>(), a.probs = probs.data_ptr<float>();
+  a.counts = counts.data_ptr<int32_t>(), a.status = status.data_ptr<int32_t>();
+  a.workspace_bytes = entries.verify_workspace(B, a.drafts, V);
+  at::Tensor workspace = make({a.workspace_bytes}, at::kByte, dev);
+  a.workspace = workspace.data_ptr();
+  call(dev, [&](ms_stream_t s) { return entries.verify_drafts(&a, s); });
+  PyObject *parts[4] = {THPVariable_Wrap(tokens), THPVariable_Wrap(probs), THPVariable_Wrap(counts), THPVariable_Wrap(status)};
+  PyObject *all = PyTuple_New(4);
+  for (int i = 0; i < 4; ++i) {
+    if (all && parts[i]) PyTuple_SET_ITEM(all, i, parts[i]);
+    else return nullptr;
+  }
+  return all;
+}
+
 // Arguments counted, exceptions turned into Python's: (type, text) of a
 // refusal, (None, code) of an entry point's return.
 template <int kCount, PyObject *(*kRun)(PyObject *const *)>
@@ -583,6 +626,7 @@ PyMethodDef methods[] = {
     {"append_kv4", fast<kCache4 + 8, append_kv4>(), METH_FASTCALL, "see miniserve_b200.kvcache4.append_kv4"},
     {"read_kv4", fast<kCache4 + 3, read_kv4>(), METH_FASTCALL, "see miniserve_b200.kvcache4.read_kv4"},
     {"attention_kv4", fast<kCache4 + 5, attention_kv4>(), METH_FASTCALL, "see miniserve_b200.attention4.attention_kv4"},
+    {"verify_drafts", fast<5, verify_drafts>(), METH_FASTCALL, "see miniserve_b200.verify.verify_drafts"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", "Checked entry points of the decode-step operators.", -1,
