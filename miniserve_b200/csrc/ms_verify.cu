@@ -7,17 +7,19 @@
 // the tokens are distributed as if each had been drawn from p_i.  Draws run in
 // index order: the first token whose running mass passes u times the whole.
 //
-// Two kernels: the statistics of every position's logits (largest value, sum of
-// weights; read once, bound by bytes), then one cluster of CTAs a row that
-// decides and draws from one position.  Decisions compare numbers that are
-// 1e-7 off at worst in 2^-24 of all cases; a draw compares with a running mass
-// at every one of the vocabulary's borders, so that its weights and sums are in
-// 64 bits: with 32 about one draw in a thousand would land beside its token.
+// Two kernels.  The first reads every position's logits once, for their largest
+// values and the sums of their weights in fp32 (bound by bytes): what the
+// decisions compare with is off by 1e-7, which decides one case in ten million
+// otherwise.  The second, a cluster of CTAs a row, decides and draws from one
+// position.  A draw compares with the running mass at every one of the
+// vocabulary's borders, so that its weights and sums are in 64 bits: with 32
+// about one draw in a thousand would land beside its token.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/mssample.h"
 #include "ms_host.h"
@@ -25,25 +27,26 @@
 
 namespace ms {
 
-constexpr int kVfThreads = 256;
-constexpr int kVfWarps = kVfThreads / 32;
-constexpr int kVfCluster = 8;     // CTAs of a row's draw
+constexpr int kVfThreads = 128;   // of a CTA that sums slices
+constexpr int kVfSums = 8;        // such CTAs of an SM
+constexpr int kVfCluster = 8;     // CTAs of a row's draw, at most
 constexpr int kVfMaxDrafts = 255;
-constexpr int64_t kVfMaxVocab = 0x7FFFFFFFll - 4096;
+constexpr int64_t kVfMaxVocab = 0x7FFFFFFFll - 65536;
 
 // Of a slice of one position's logits.
 struct VfRecord {
-  double sum;   // of exp2((x - top) c)
-  float top;    // largest value
-  int index;    // its first place
-  int flags;    // MS_ROW_NONFINITE
+  double sum;  // of the weights, relative to the largest value's
+  float top;   // largest value
+  int index;   // its first place
+  int flags;   // MS_ROW_NONFINITE
 };
 
 struct VfArgs {
   ms_verify_args x;
   VfRecord *records;  // [rows][drafts + 1][slices]
   int slices;
-  int64_t slice;      // entries of a slice
+  int slice;          // entries of a slice
+  int ranks;          // CTAs of a row's draw
 };
 
 template <int DT>
@@ -83,17 +86,6 @@ struct VfType<MS_DTYPE_F16> {
   static __device__ __forceinline__ float one(const T *p) { return __half2float(load_in(p)); }
 };
 
-__device__ __forceinline__ float vf_max_nan(float x, float y, float z) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
-  return r;
-}
-__device__ __forceinline__ float vf_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Drafts of a row, at most `most`: those before the first negative one.  By a
 // whole warp.
 __device__ __forceinline__ int vf_drafts(const ms_verify_args &x, int64_t b, int most) {
@@ -108,114 +100,228 @@ __device__ __forceinline__ int vf_drafts(const ms_verify_args &x, int64_t b, int
 // A temperature that rows can be drawn at.
 __device__ __forceinline__ bool vf_heat(double t) { return t >= 0.0 && t <= 1.7976931348623157e308; }
 
-// Statistics: a CTA takes a slice of one position.  The maximum moves with the
-// values; weights are fp32, their sums of one step go into fp64.
-template <int DT>
-__global__ void __launch_bounds__(kVfThreads) ms_verify_stats_kernel(const __grid_constant__ VfArgs a) {
-  using V = VfType<DT>;
-  constexpr int kVec = V::kVec, kSteps = 16 / kVec * 2;  // 16-byte loads in flight: 32 values
+__device__ __forceinline__ float vf_max_nan(float x, float y, float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+__device__ __forceinline__ float vf_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 vf_add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+  return *reinterpret_cast<float2 *>(&d);
+}
+__device__ __forceinline__ float2 vf_mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+  return *reinterpret_cast<float2 *>(&d);
+}
+// A unit of logit in units of log2: finite and not 0, so that it makes neither
+// a number of 0 times infinity.
+__device__ __forceinline__ float vf_unit(double heat) {
+  return heat == 0.0 ? 1.f : (float)fmin(fmax(1.4426950408889634 / heat, 1e-37), 3e38);
+}
+// A sum of weights relative to `from`, as one relative to `to`, which is not below it.
+__device__ __forceinline__ double vf_moved(double sum, float from, float to, float unit) {
+  return from == to || sum == 0.0 ? sum : sum * (double)vf_exp2((from - to) * unit);
+}
+
+// A thread's values so far.
+struct VfSum {
+  float top;
+  double sum;  // of the weights, relative to top's
+  int index, flags;
+};
+
+// One more batch of values, piece s's at s * 32 pieces from place `first` on.
+template <int kPieces, int kVec>
+__device__ __forceinline__ void vf_add(VfSum &a, float (&v)[kPieces][kVec], int first, bool greedy, float unit) {
   const float kNone = __uint_as_float(0xFF800000u), kInf = __uint_as_float(0x7F800000u);
+  float most = kNone;
+#pragma unroll
+  for (int s = 0; s < kPieces; ++s)
+#pragma unroll
+    for (int k = 0; k < kVec; k += 2) most = vf_max_nan(most, v[s][k], v[s][k + 1]);
+  if (!(most < kInf)) {  // NaN reads as -inf
+    a.flags = MS_ROW_NONFINITE;
+    most = kNone;
+#pragma unroll
+    for (int s = 0; s < kPieces; ++s)
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        if (v[s][k] != v[s][k]) v[s][k] = kNone;
+        most = fmaxf(most, v[s][k]);
+      }
+  }
+  if (most > a.top) {
+    a.sum = vf_moved(a.sum, a.top, most, unit);
+    a.top = most;
+    if (greedy) {
+      a.index = 0x7FFFFFFF;
+#pragma unroll
+      for (int s = kPieces - 1; s >= 0; --s)
+#pragma unroll
+        for (int k = kVec - 1; k >= 0; --k)
+          if (v[s][k] == most) a.index = first + s * 32 * kVec + k;
+    }
+  }
+  if (greedy || a.top == kNone) return;
+  float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  if (a.top < kInf) {
+    const float2 from = make_float2(-a.top, -a.top), by = make_float2(unit, unit);
+#pragma unroll
+    for (int s = 0; s < kPieces; ++s)
+#pragma unroll
+      for (int k = 0; k < kVec; k += 2) {
+        const float2 t = vf_mul2(vf_add2(make_float2(v[s][k], v[s][k + 1]), from), by);
+        part[(k >> 1) & 1] = vf_add2(part[(k >> 1) & 1], make_float2(vf_exp2(t.x), vf_exp2(t.y)));
+      }
+  } else {  // infinite values share the weight
+#pragma unroll
+    for (int s = 0; s < kPieces; ++s)
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) part[0].x += v[s][k] == kInf ? 1.f : 0.f;
+  }
+  a.sum += (double)((part[0].x + part[0].y) + (part[1].x + part[1].y));
+}
+
+// Sums: a warp takes a slice of a position, the next values on their way while
+// it weighs the last ones.  CTAs are small and many: positions behind a row's
+// drafts have none, and what a slice costs varies.
+template <int DT>
+__global__ void __launch_bounds__(kVfThreads, kVfSums) ms_verify_sums_kernel(const __grid_constant__ VfArgs a) {
+  using V = VfType<DT>;
+  constexpr int kVec = V::kVec, kPieces = kVec == 4 ? 4 : 2;  // of a lane's batch: 16 values
+  const float kNone = __uint_as_float(0xFF800000u);
   grid_wait();
   grid_release();
   const ms_verify_args &x = a.x;
-  const int slice = blockIdx.x % a.slices;
-  const int64_t at = blockIdx.x / a.slices, b = at / (x.drafts + 1);
-  const int i = (int)(at - b * (x.drafts + 1));
-  if (vf_drafts(x, b, i) < i) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * (kVfThreads / 32) + (threadIdx.x >> 5);
+  if (item >= x.rows * (x.drafts + 1) * a.slices) return;
+  const int64_t at = item / a.slices, b = at / (x.drafts + 1);
+  const int slice = (int)(item - at * a.slices), i = (int)(at - b * (x.drafts + 1));
   const double heat = load_in(x.temperature + b);
+  if (vf_drafts(x, b, i) < i || !vf_heat(heat)) return;
   const bool greedy = heat == 0.0;
-  // finite and not 0, so that it makes neither a number of 0 times infinity
-  const float c = greedy ? 1.f : (float)fmin(fmax(1.4426950408889634 / heat, 1e-37), 3e38);
+  const float unit = vf_unit(heat);
   const typename V::T *row = static_cast<const typename V::T *>(x.logits) + b * x.logits_row + i * x.logits_pos;
-  // 16-byte pieces: the first one starts before the row where the row does not start on one
+  // 16-byte pieces: the first one starts before the row where the row does not start on one.  Pieces `inner` .. `outer`
+  // - 1 lie in the row as a whole.
   const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename V::T));
-  const int64_t pieces = (x.vocab + skew + kVec - 1) / kVec;
-  const int64_t each = a.slice / kVec, first = slice * each, last = min(pieces, first + each);
-  float top = kNone;
-  double sum = 0.0;
-  int index = 0x7FFFFFFF, flags = 0;
-  for (int64_t p0 = first + threadIdx.x; p0 < last; p0 += kSteps * kVfThreads) {
-    float v[kSteps][kVec];
+  const int vocab = (int)x.vocab;
+  const int first = slice * (a.slice / kVec), last = min((vocab + skew + kVec - 1) / kVec, first + a.slice / kVec);
+  const int inner = skew ? 1 : 0, outer = min((vocab + skew) / kVec, last);
+  const uint4 *base = reinterpret_cast<const uint4 *>(row - skew);
+  VfSum mine{kNone, 0.0, 0x7FFFFFFF, 0};
+  uint4 u[kPieces];
+  auto fetch = [&](int p0) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int64_t e = (p0 + s * kVfThreads) * kVec - skew;
-      if (p0 + s * kVfThreads >= last) {
-#pragma unroll
-        for (int k = 0; k < kVec; ++k) v[s][k] = kNone;
-      } else if (e >= 0 && e + kVec <= x.vocab) {
-        V::wide(load_in(reinterpret_cast<const uint4 *>(row + e)), v[s]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < kVec; ++k) v[s][k] = e + k >= 0 && e + k < x.vocab ? V::one(row + e + k) : kNone;
-      }
+    for (int s = 0; s < kPieces; ++s) {
+      const int p = p0 + s * 32;
+      if (p >= inner && p < outer) u[s] = load_in(base + p);
     }
-    float most = kNone;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-      for (int k = 0; k < kVec; k += 2) most = vf_max_nan(most, v[s][k], v[s][k + 1]);
-    if (!(most < kInf)) {  // NaN reads as -inf
-      flags = MS_ROW_NONFINITE;
-      most = kNone;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-        for (int k = 0; k < kVec; ++k) {
-          if (v[s][k] != v[s][k]) v[s][k] = kNone;
-          most = fmaxf(most, v[s][k]);
-        }
-    }
-    if (most > top) {
-      sum = sum == 0.0 ? 0.0 : sum * (double)vf_exp2((top - most) * c);
-      top = most;
-      if (greedy) {
-        index = 0x7FFFFFFF;
-#pragma unroll
-        for (int s = kSteps - 1; s >= 0; --s)
-#pragma unroll
-          for (int k = kVec - 1; k >= 0; --k)
-            if (v[s][k] == top) index = (int)((p0 + s * kVfThreads) * kVec - skew + k);
-      }
-    }
-    if (!greedy && top > kNone) {
-      float part = 0.f;
-      if (top < kInf) {
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-          for (int k = 0; k < kVec; ++k) part += vf_exp2((v[s][k] - top) * c);
-      } else {  // infinite values share the weight
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-          for (int k = 0; k < kVec; ++k) part += v[s][k] == kInf ? 1.f : 0.f;
-      }
-      sum += (double)part;
-    }
-  }
-  __shared__ VfRecord part[kVfWarps];
-  auto join = [&](float t, double s, int k, int f) {
-    const float next = fmaxf(top, t);
-    if (top < next) sum = sum == 0.0 ? 0.0 : sum * (double)vf_exp2((top - next) * c);
-    if (t < next) s = s == 0.0 ? 0.0 : s * (double)vf_exp2((t - next) * c);
-    index = t > top ? k : t < top ? index : min(index, k);
-    top = next;
-    sum += s;
-    flags |= f;
   };
+  fetch(first + lane);
+  for (int p0 = first + lane; p0 - lane < last; p0 += 32 * kPieces) {
+    float v[kPieces][kVec];
+#pragma unroll
+    for (int s = 0; s < kPieces; ++s) V::wide(u[s], v[s]);
+    if (p0 - lane < inner || p0 - lane + 32 * kPieces > outer) {  // the row's ends
+#pragma unroll
+      for (int s = 0; s < kPieces; ++s) {
+        const int p = p0 + s * 32;
+        if (p < inner || p >= outer) {
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) {
+            const int e = p * kVec - skew + k;
+            v[s][k] = p < last && e >= 0 && e < vocab ? V::one(row + e) : kNone;
+          }
+        }
+      }
+    }
+    fetch(p0 + 32 * kPieces);
+    vf_add<kPieces, kVec>(mine, v, p0 * kVec - skew, greedy, unit);
+  }
+  // the lanes' sums, relative to the slice's largest value
+  float top = mine.top;
+  int index = mine.index;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float t = __shfl_xor_sync(0xFFFFFFFFu, top, o);
-    const double s = __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    const int k = __shfl_xor_sync(0xFFFFFFFFu, index, o), f = __shfl_xor_sync(0xFFFFFFFFu, flags, o);
-    join(t, s, k, f);
+    const int k = __shfl_xor_sync(0xFFFFFFFFu, index, o);
+    if (t > top) top = t, index = k;
+    else if (t == top) index = min(index, k);
   }
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = VfRecord{sum, top, index, flags};
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kVfWarps; ++w) join(part[w].top, part[w].sum, part[w].index, part[w].flags);
-    a.records[at * a.slices + slice] = VfRecord{sum, top, index, flags};
+  double sum = vf_moved(mine.sum, mine.top, top, unit);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  const int flags = __reduce_or_sync(0xFFFFFFFFu, mine.flags);
+  if (lane == 0) a.records[item] = VfRecord{sum, top, index, flags};
+}
+
+// Weights in 64 bits.  2^(t / 128) for t = v c - R, c = 128 log2(e) /
+// temperature: the nearest whole number k of t gives the power of two (k / 128
+// rounded down) and a table's place; the rest r of at most a half is a power
+// series of three terms, (r ln 2 / 128)^4 / 24 < 2^-38 off.  R is a multiple of
+// 128 near the largest value's t.  The table is there sixteen times, a copy for
+// each pair of lanes, so that no two copies share a bank; its high words have
+// the place's bits taken off, so that k 2^13 added to one is the scaled power.
+constexpr int kVfSteps = 128, kVfCopies = 16;
+struct VfPowers {
+  double of[kVfSteps];  // 2^(i / 128), by its power series
+  constexpr VfPowers() : of() {
+    for (int i = 0; i < kVfSteps; ++i) {
+      const double x = 0.69314718055994530942 * i / kVfSteps;
+      double sum = 1.0;
+      for (int k = 24; k > 0; --k) sum = 1.0 + sum * x / k;
+      of[i] = sum;
+    }
   }
+};
+__device__ const VfPowers vf_powers{};
+
+constexpr double kVfMagic = 6755399441055744.0;  // 1.5 * 2^52: the low word of a sum with it is a whole number
+constexpr double kVfLeast = 1000.0;              // weights below 2^-1000 count as 0
+
+struct VfScale {
+  double c;     // steps of a unit of logit
+  double base;  // kVfMagic - R
+  float top;
+  float least;  // values below it weigh nothing
+  // v c is far inside whole numbers' range.  Where it is not (temperatures so small that neighbouring values are 2^21
+  // steps apart, or an infinite value), the largest value weighs 1 and all others nothing.
+  bool plain;
+};
+__device__ __forceinline__ VfScale vf_scale(double heat, float top) {
+  VfScale s;
+  s.c = 1.4426950408889634 * kVfSteps / heat, s.top = top;
+  s.plain = fabs((double)top) * s.c < 35184372088832.0 && s.c < 1e290;  // 2^45
+  s.base = kVfMagic - (s.plain ? kVfSteps * ceil((double)top * s.c / kVfSteps) : 0.0);
+  s.least = s.plain ? (float)fmax((double)top - kVfLeast * kVfSteps / s.c, -3.4e38) : top;
+  return s;
+}
+// Relative to 2^(R / 128) or, of scales that are not plain, to the largest
+// value's; for values from `least` on.
+__device__ __forceinline__ double vf_power(const VfScale &s, float v, const double *power) {
+  const double x = (double)v, shifted = fma(x, s.c, s.base), r = fma(x, s.c, s.base - shifted);
+  const int k = __double2loint(shifted);
+  const double g = power[(k & (kVfSteps - 1)) * kVfCopies + (threadIdx.x & (kVfCopies - 1))];
+  const double f = __hiloint2double(__double2hiint(g) + (k << 13), __double2loint(g));
+  constexpr double ln = 0.69314718055994530942 / kVfSteps;
+  return s.plain ? fma(f, r * fma(r, fma(r, ln * ln * ln / 6.0, ln * ln / 2.0), ln), f) : 1.0;
+}
+__device__ __forceinline__ double vf_weight(const VfScale &s, float v, const double *power) {
+  return v >= s.least ? vf_power(s, v, power) : 0.0;  // a NaN is not
 }
 
 __device__ __forceinline__ uint32_t vf_remote(const void *p, int rank) {
@@ -226,33 +332,80 @@ __device__ __forceinline__ uint32_t vf_remote(const void *p, int rank) {
 __device__ __forceinline__ void vf_send(uint32_t to, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(v) : "memory");
 }
+__device__ __forceinline__ double vf_warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+// Running sums over a warp's lanes.
+__device__ __forceinline__ double vf_warp_run(double v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double e = __shfl_up_sync(0xFFFFFFFFu, v, o);
+    if (lane >= o) v += e;
+  }
+  return v;
+}
+// The first lane whose running mass, on top of `before`, passes r, or by rounding the last one with mass; `before`
+// becomes the mass up to it.  False where no lane has mass, or, unless `end`, none passes r: `before` then has all lanes'.
+__device__ __forceinline__ bool vf_find(double mass, double r, bool end, double &before, int &found) {
+  const double run = vf_warp_run(mass);
+  const uint32_t some = __ballot_sync(0xFFFFFFFFu, mass > 0.0);
+  const uint32_t past = __ballot_sync(0xFFFFFFFFu, mass > 0.0 && before + run > r);
+  const bool here = past || (end && some);
+  found = past ? __ffs(past) - 1 : 31 - __clz(some | 1);
+  before += __shfl_sync(0xFFFFFFFFu, here ? run - mass : run, here ? found : 31);
+  return here;
+}
 
+// What a part's sums are of: the weights, of all entries or of all but a draft;
+// the weights, and the draft's probabilities, of entries that have more weight
+// than the draft gave them; what is left of those entries.
+enum { kVfAll, kVfMore, kVfTaken, kVfRest, kVfKinds };
+
+template <int kThreads>
 struct VfShared {
-  double mass[2][kVfCluster * kVfWarps];  // of the cluster's warps, in index order
-  double odd[kVfCluster];                 // CTAs that met a draft probability that is none
-  double accepted[kVfMaxDrafts + 1];      // p_i(d_i)
-  double scan[kVfWarps];
-  double z;
-  float top;
-  int index, flags, stop, drafts, status;
-  int owner, last;
+  double power[kVfSteps * kVfCopies];
+  double sum[kVfKinds][kThreads / 32];       // of the CTA's warps
+  double mass[kVfKinds][kVfCluster];         // of the cluster's CTAs, in index order
+  double odd[kVfCluster];                    // CTAs that met a draft probability that is none
+  double accepted[kVfMaxDrafts + 1];         // p_i(d_i)
+  double whole[kVfMaxDrafts + 1];            // sums of the positions' weights, relative to their largest values
+  float top[kVfMaxDrafts + 1];
+  int index[kVfMaxDrafts + 1], flags[kVfMaxDrafts + 1];
+  int stop, drafts, status;
 };
 
-// Decision and draw: a cluster of eight CTAs takes a row.  Every CTA joins the
-// row's records and decides, alike; then each sums its eighth of the position
-// that is drawn from, warp by warp, the warps' sums are sent to all CTAs, and
-// the CTA that holds the drawn place looks for it.
-template <int DT>
-__global__ void __launch_bounds__(kVfThreads) ms_verify_draw_kernel(const __grid_constant__ VfArgs a) {
+// Decision and draw: a cluster of CTAs takes a row.  Every CTA joins the row's
+// records and decides, alike; then each sums its part of the position that is
+// drawn from, the sums are sent to all CTAs, and the CTA that holds the drawn
+// place looks for it: in its warps' sums, in the warps' parts of that warp's
+// entries, and in those 32 at a time.
+//
+// What the draft's probabilities leave, max(w / z - q, 0), needs the whole z of
+// the weights w first.  One pass is enough all the same: the first kernel's z is
+// known to 1e-7, and the entries that it puts on the wrong side of w / z = q are
+// those where next to nothing is left, so that sum w / z - sum q over the others'
+// side is the sum to 1e-13.  Where all that is left is itself small (a draft
+// model that is the target, nearly), a second pass takes the exact z.
+//
+// fp64 operations take tens of cycles one after the other: 32-wide scans stand
+// where a loop over eight sums would do.
+template <int DT, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kernel(const __grid_constant__ VfArgs a) {
   using V = VfType<DT>;
+  constexpr int kWarps = kThreads / 32;
   const float kNone = __uint_as_float(0xFF800000u);
-  __shared__ VfShared sh;
+  __shared__ VfShared<kThreads> sh;
   const ms_verify_args &x = a.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = (int)cluster_rank();
-  const int64_t b = blockIdx.x / kVfCluster;
+  const int rank = (int)cluster_rank(), ranks = a.ranks;
+  const int64_t b = blockIdx.x / ranks;
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for before a CTA writes to another
+  const double entry = vf_powers.of[(tid >> 1) % kVfSteps];
   grid_wait();
-  const double heat = load_in(x.temperature + b), inv = 1.0 / heat;
+  const double heat = load_in(x.temperature + b);
   const bool greedy = heat == 0.0;
   if (warp == 0) {
     const int n = vf_drafts(x, b, x.drafts);
@@ -263,13 +416,19 @@ __global__ void __launch_bounds__(kVfThreads) ms_verify_draw_kernel(const __grid
       sh.drafts = n;
       sh.status = (vf_heat(heat) ? MS_ROW_OK : MS_ROW_BAD_TEMPERATURE) | (bad ? MS_ROW_BAD_DRAFT : MS_ROW_OK);
       sh.stop = n;
-      sh.flags = 0;
     }
+  }
+  if (tid < 2 * kVfSteps) {
+    const int step = tid >> 1;
+    const double g = __hiloint2double(__double2hiint(entry) - (step << 13), __double2loint(entry));
+#pragma unroll
+    for (int i = 0; i < kVfCopies / 2; ++i) sh.power[step * kVfCopies + (tid & 1) * (kVfCopies / 2) + i] = g;
   }
   __syncthreads();
   const int n = sh.drafts;
+  auto meet = [&]() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); };
   auto give_up = [&](int status) {  // by the first CTA
-    for (int i = tid; i <= x.drafts; i += kVfThreads) {
+    for (int i = tid; i <= x.drafts; i += kThreads) {
       x.tokens[b * (x.drafts + 1) + i] = -1;
       x.probs[b * (x.drafts + 1) + i] = 0.f;
     }
@@ -277,67 +436,64 @@ __global__ void __launch_bounds__(kVfThreads) ms_verify_draw_kernel(const __grid
   };
   if (sh.status != MS_ROW_OK) {
     if (rank == 0) give_up(sh.status);
+    __syncwarp();
+    meet();
     return;
   }
-  // weight of a value relative to the position's largest
-  auto weigh = [&](float v, float top) { return v == top ? 1.0 : v == v ? exp(((double)v - (double)top) * inv) : 0.0; };
+  const float unit = vf_unit(heat);
   auto logits = [&](int i) { return static_cast<const typename V::T *>(x.logits) + b * x.logits_row + i * x.logits_pos; };
-
-  struct Whole {
-    float top;
-    double z;
-    int index, flags;
-  };
-  auto join = [&](int i) {  // by a warp: position i's records
-    Whole w{kNone, 0.0, 0x7FFFFFFF, 0};
-    const VfRecord *r = a.records + (b * (x.drafts + 1) + i) * a.slices;
-    for (int s = lane; s < a.slices; s += 32) {
-      const VfRecord &v = r[s];
-      w.flags |= v.flags;
-      if (v.top > w.top) w.top = v.top, w.index = v.index;
-      else if (v.top == w.top) w.index = min(w.index, v.index);
+  for (int i = warp; i <= n; i += kWarps) {  // the positions' records
+    int64_t d = 0;
+    double u = 0.0, q = 1.0;
+    float v = kNone;
+    if (i < n && lane == 0) {
+      d = load_in(x.draft_tokens + b * x.draft_row + i);
+      u = load_in(x.uniforms + b * x.uniform_row + i);
+      v = V::one(logits(i) + d);
+      if (x.draft_probs && !greedy) q = load_in(x.draft_probs + b * x.probs_row + i * x.probs_pos + d);
     }
+    const VfRecord *r = a.records + (b * (x.drafts + 1) + i) * a.slices;
+    VfSum all{kNone, 0.0, 0x7FFFFFFF, 0};
+    for (int s = lane; s < a.slices; s += 32) {
+      const VfRecord e = r[s];
+      const float next = fmaxf(all.top, e.top);
+      all.sum = vf_moved(all.sum, all.top, next, unit) + vf_moved(e.sum, e.top, next, unit);
+      all.index = e.top > all.top ? e.index : e.top < all.top ? all.index : min(all.index, e.index);
+      all.top = next;
+      all.flags |= e.flags;
+    }
+    float top = all.top;
+    int index = all.index;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      const float t = __shfl_xor_sync(0xFFFFFFFFu, w.top, o);
-      const int k = __shfl_xor_sync(0xFFFFFFFFu, w.index, o);
-      if (t > w.top) w.top = t, w.index = k;
-      else if (t == w.top) w.index = min(w.index, k);
+      const float t = __shfl_xor_sync(0xFFFFFFFFu, top, o);
+      const int k = __shfl_xor_sync(0xFFFFFFFFu, index, o);
+      if (t > top) top = t, index = k;
+      else if (t == top) index = min(index, k);
     }
-    w.flags = __reduce_or_sync(0xFFFFFFFFu, w.flags);
-    for (int s = lane; s < a.slices; s += 32) w.z += r[s].sum * weigh(r[s].top, w.top);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) w.z += __shfl_xor_sync(0xFFFFFFFFu, w.z, o);
-    return w;
-  };
-  for (int i = warp; i < n; i += kVfWarps) {
-    const Whole w = join(i);
+    const int flags = __reduce_or_sync(0xFFFFFFFFu, all.flags);
+    const double z = vf_warp_sum(vf_moved(all.sum, all.top, top, unit));
     if (lane == 0) {
-      const int64_t d = load_in(x.draft_tokens + b * x.draft_row + i);
-      const double u = load_in(x.uniforms + b * x.uniform_row + i);
-      const float v = V::one(logits(i) + d);
-      const double p = greedy ? (d == w.index ? 1.0 : 0.0) : w.top > kNone ? weigh(v, w.top) / w.z : 0.0;
-      const double q = x.draft_probs && !greedy ? (double)load_in(x.draft_probs + b * x.probs_row + i * x.probs_pos + d) : 1.0;
-      sh.accepted[i] = p;
-      if (!(u * q < p)) atomicMin(&sh.stop, i);
+      sh.top[i] = top, sh.whole[i] = z, sh.index[i] = index, sh.flags[i] = flags;
+      if (i < n) {
+        double p = 0.0;
+        if (greedy) {
+          p = d == index ? 1.0 : 0.0;
+        } else if (top > kNone) {
+          const VfScale s = vf_scale(heat, top);
+          p = vf_weight(s, v, sh.power) / (vf_power(s, top, sh.power) * z);
+        }
+        sh.accepted[i] = p;
+        if (!(u * q < p)) atomicMin(&sh.stop, i);
+      }
     }
   }
   __syncthreads();
   const int f = sh.stop;
-  for (int i = warp; i <= f; i += kVfWarps) {  // what the positions up to the one that is drawn from hold
-    const Whole w = join(i);
-    if (lane == 0) {
-      if (w.flags) atomicOr(&sh.flags, w.flags);
-      if (i == f) sh.top = w.top, sh.index = w.index;
-    }
-  }
-  __syncthreads();
-  const float top = sh.top;
-  if (!greedy && top == kNone) {
-    if (rank == 0) give_up(MS_ROW_ALL_MASKED | sh.flags);
-    return;
-  }
-  auto finish = [&](int64_t token, double p, int flags) {  // by a warp
+  int flags = 0;
+  for (int i = 0; i <= f; ++i) flags |= sh.flags[i];
+  const float top = sh.top[f];
+  auto finish = [&](int64_t token, double p) {  // by a warp
     for (int i = lane; i <= x.drafts; i += 32) {
       const int64_t o = b * (x.drafts + 1) + i;
       x.tokens[o] = i < f ? load_in(x.draft_tokens + b * x.draft_row + i) : i == f ? token : -1;
@@ -345,150 +501,182 @@ __global__ void __launch_bounds__(kVfThreads) ms_verify_draw_kernel(const __grid
     }
     if (lane == 0) x.counts[b] = f + 1, x.status[b] = flags;
   };
-  if (greedy) {
-    if (rank == 0 && warp == 0) finish(top == kNone ? 0 : sh.index, 1.0, sh.flags);
+  if (greedy || top == kNone) {
+    if (rank == 0 && !greedy) give_up(MS_ROW_ALL_MASKED | flags);
+    if (rank == 0 && greedy && warp == 0) finish(top == kNone ? 0 : sh.index[f], 1.0);
+    __syncwarp();
+    meet();
     return;
   }
-  __syncwarp();
-  cluster_sync();  // the others have started
   const typename V::T *row = logits(f);
   const bool refused = f < n;
   const float *q = refused && x.draft_probs ? x.draft_probs + b * x.probs_row + f * x.probs_pos : nullptr;
-  const int64_t without = refused && !q ? load_in(x.draft_tokens + b * x.draft_row + f) : -1;
-  // the warp's part of the vocabulary
-  const int64_t per = ((x.vocab + kVfCluster * kVfWarps - 1) / (kVfCluster * kVfWarps) + 31) / 32 * 32;
-  const int part = rank * kVfWarps + warp;
-  const int64_t lo = min(x.vocab, part * per), hi = min(x.vocab, lo + per);
-  int odd = 0;
-  // mass of entry j: of p alone, or of what is left of it
-  enum { kWhole, kRest };
-  double z_inv = 0.0;
-  auto mass = [&](int64_t j, int kind) {
-    const double w = weigh(V::one(row + j), top);
-    if (kind == kWhole) return w;
-    if (!q) return j == without ? 0.0 : w;
-    const float d = load_in(q + j);
-    if (!(d >= 0.f && d <= 3.402823466e38f)) odd = 1;
-    return fmax(w * z_inv - fmax((double)d, 0.0), 0.0);  // a NaN reads as 0
-  };
-  auto sums = [&](int kind, int buffer) {
-    double s[4] = {0.0, 0.0, 0.0, 0.0};
-    int64_t j = lo + lane;
-    for (; j + 96 < hi; j += 128) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) s[k] += mass(j + 32 * k, kind);
+  int without = refused && !q ? (int)load_in(x.draft_tokens + b * x.draft_row + f) : -1;
+  const double u = load_in(x.uniforms + b * x.uniform_row + x.drafts);
+  const VfScale scale = vf_scale(heat, top);
+  double share = 1.0 / (vf_power(scale, top, sh.power) * sh.whole[f]);  // 1 / z
+  uint32_t odd = 0;  // the largest bit pattern of the draft's probabilities: those past the finite ones are none
+  // a warp's part of the vocabulary, of one CTA after the other
+  const int64_t per = ((x.vocab + ranks * kWarps - 1) / (ranks * kWarps) + 31) / 32 * 32;
+  constexpr std::integral_constant<int, kVfAll> kAll{};
+  constexpr std::integral_constant<int, kVfMore> kMore{};
+  constexpr std::integral_constant<int, kVfRest> kRest{};
+  // an entry's part in the sums s of a kind
+  auto add = [&](double (&s)[3], float v, float d, bool in, auto kind) {
+    const double w = vf_power(scale, v, sh.power);
+    const bool some = in && v >= scale.least;  // a NaN is not
+    if constexpr (kind.value == kVfAll) {
+      if (some) s[0] += w;
+    } else {
+      d += 0.f;  // no -0
+      odd = max(odd, __float_as_uint(d));
+      const double taken = (double)fmaxf(d, 0.f);  // a NaN reads as 0
+      const double rest = fma(w, share, -taken);
+      if constexpr (kind.value == kVfMore) {
+        if (some) s[0] += w;
+        if (some && rest > 0.0) s[1] += w, s[2] += taken;
+      } else {
+        if (some && rest > 0.0) s[0] += rest;
+      }
     }
-    for (; j < hi; j += 32) s[0] += mass(j, kind);
-    double t = (s[0] + s[1]) + (s[2] + s[3]);
+  };
+  // entries lo .. hi - 1 by a warp
+  auto part = [&](int64_t lo, int64_t hi, double (&s)[3], auto kind) {
+    constexpr int kBatch = 8;
+    constexpr bool kTakes = kind.value != kVfAll;
+    double t[2][3] = {};
+    int j = (int)lo + lane;
+    for (; j - lane + 32 * kBatch <= (int)hi; j += 32 * kBatch) {
+      const typename V::T *at = row + j;
+      const float *taken = q + j;
+      float v[kBatch], d[kBatch];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
-    if (lane < kVfCluster) vf_send(vf_remote(&sh.mass[buffer][part], lane), t);
-    if (kind == kRest && q) {
-      const int any = __syncthreads_or(odd);
-      if (tid < kVfCluster) vf_send(vf_remote(&sh.odd[rank], tid), (double)any);
+      for (int k = 0; k < kBatch; ++k) v[k] = V::one(at + 32 * k), d[k] = kTakes ? load_in(taken + 32 * k) : 0.f;
+      if (!kTakes && (unsigned)(without - (j - lane)) < 32 * kBatch) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) add(t[k & 1], v[k], d[k], j + 32 * k != without, kind);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) add(t[k & 1], v[k], d[k], true, kind);
+      }
+    }
+    for (; j - lane < (int)hi; j += 32)
+      add(t[0], j < (int)hi ? V::one(row + j) : kNone, kTakes && j < (int)hi ? load_in(q + j) : 0.f, j != without, kind);
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i == 0 || kind.value == kVfMore) s[i] = vf_warp_sum(t[0][i] + t[1][i]);
+  };
+  // Every CTA's sums of its part to all of them, at places `slot` on.
+  bool met = false;
+  auto sums = [&](int slot, auto kind) {
+    constexpr int kSums = kind.value == kVfMore ? 3 : 1;
+    const int64_t lo = min(x.vocab, (rank * kWarps + warp) * per), hi = min(x.vocab, lo + per);
+    double s[3];
+    part(lo, hi, s, kind);
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < kSums; ++i) sh.sum[slot + i][warp] = s[i];
+    }
+    const int any = __syncthreads_or(odd > 0x7F7FFFFFu);
+    if (!met) {
+      __syncwarp();
+      meet();
+      met = true;
+    }
+    if (warp < kSums) {
+      const double all = vf_warp_sum(lane < kWarps ? sh.sum[slot + warp][lane] : 0.0);
+      if (lane < ranks) {
+        vf_send(vf_remote(&sh.mass[slot + warp][rank], lane), all);
+        if (warp == 0) vf_send(vf_remote(&sh.odd[rank], lane), (double)any);
+      }
     }
     __syncwarp();
     cluster_sync();
   };
-  auto total = [&](int buffer) {
-    double t = 0.0;
-    for (int i = 0; i < kVfCluster * kVfWarps; ++i) t += sh.mass[buffer][i];
-    return t;
+  // A lane's part of the row, of CTAs or of warps, as the draw sees it.  What is left of a part is the difference of two
+  // sums: nothing where it is within their rounding.
+  int slot = kVfAll;
+  auto mass = [&](const double *of, int pitch, int count) {
+    if (lane >= count) return 0.0;
+    if (slot != kVfMore) return of[slot * pitch + lane];
+    const double more = of[kVfMore * pitch + lane] * share, rest = more - of[kVfTaken * pitch + lane];
+    return rest > 1e-13 * more ? rest : 0.0;
   };
-  double z = 0.0;
-  int kind = kWhole, buffer = 0;
-  if (q) {
-    sums(kWhole, 0);
-    z = total(0);
-    z_inv = 1.0 / z;
-  }
-  int flags = sh.flags;
-  if (refused) {
-    kind = kRest, buffer = 1;
-    sums(kRest, 1);
-    if (q)
-      for (int i = 0; i < kVfCluster; ++i) flags |= sh.odd[i] != 0.0 ? MS_ROW_NONFINITE : 0;
+  auto whole = [&]() { return vf_warp_sum(mass(&sh.mass[0][0], kVfCluster, ranks)); };
+  double all;
+  if (!q) {
+    sums(kVfAll, kAll);
+    all = whole();
+    const double z = all + (refused ? vf_weight(scale, V::one(row + without), sh.power) : 0.0);
+    share = 1.0 / z;
+    if (!(all > 0.0)) {  // nothing left: from p as it is
+      without = -1;
+      slot = kVfRest;  // not where others may still read
+      sums(kVfRest, kAll);
+      all = whole();
+    }
   } else {
-    sums(kWhole, 0);
-    z = total(0);
+    sums(kVfAll, kMore);
+    share = 1.0 / whole();
+    slot = kVfMore;
+    all = whole();
+    if (!(all > 1e-3)) {
+      slot = kVfRest;
+      sums(kVfRest, kRest);
+      all = whole();
+    }
+    if (__any_sync(0xFFFFFFFFu, lane < ranks && sh.odd[lane] != 0.0)) flags |= MS_ROW_NONFINITE;
+    if (!(all > 0.0)) {
+      slot = kVfAll;
+      all = whole();
+    }
   }
-  double all = total(buffer);
-  if (refused && !(all > 0.0)) {  // nothing left: from p as it is
-    kind = kWhole, buffer = 0;
-    if (!q) sums(kWhole, 0), z = total(0);
-    all = z;
-  } else if (refused && !q) {
-    z = all + weigh(V::one(row + without), top);
-  }
-  // the warp's part that holds the drawn place
-  const double r = load_in(x.uniforms + b * x.uniform_row + x.drafts) * all;
+  const bool rest = q && slot != kVfAll;
+  const double r = u * all;
   double before = 0.0;
-  int found = -1, nonzero = 0;
+  int found;
+  vf_find(mass(&sh.mass[0][0], kVfCluster, ranks), r, true, before, found);
+  if (found != rank) return;
+  vf_find(mass(&sh.sum[0][0], kWarps, kWarps), r, true, before, found);
+  const int64_t begin = min(x.vocab, (rank * kWarps + found) * per), end = min(x.vocab, begin + per);
+  // that warp's entries, a part for each warp
+  const int64_t step = ((end - begin + kWarps - 1) / kWarps + 31) / 32 * 32;
+  const int64_t lo = min(end, begin + warp * step), hi = min(end, lo + step);
   {
-    double run = 0.0;
-    for (int i = 0; i < kVfCluster * kVfWarps; ++i) {
-      const double s = sh.mass[buffer][i];
-      if (found < 0 && s > 0.0) {
-        nonzero = i;
-        before = run;
-        if (run + s > r) found = i;
-      }
-      run += s;
+    double s[3];
+    if (rest) part(lo, hi, s, kRest);
+    else part(lo, hi, s, kAll);
+    __syncthreads();  // the sums above have been read
+    if (lane == 0) sh.sum[0][warp] = s[0];
+    __syncthreads();
+  }
+  vf_find(lane < kWarps ? sh.sum[0][lane] : 0.0, r, true, before, found);
+  if (found != warp) return;
+  int64_t token = lo;
+  for (int64_t j0 = lo; j0 < hi; j0 += 32) {
+    const int64_t j = j0 + lane;
+    double s[3] = {0.0, 0.0, 0.0};
+    if (j < hi) {
+      if (rest) add(s, V::one(row + j), load_in(q + j), true, kRest);
+      else add(s, V::one(row + j), 0.f, (int)j != without, kAll);
     }
-    if (found < 0) found = nonzero;  // rounding: the last part with mass
-  }
-  if (found / kVfWarps != rank) return;
-  // all threads of this CTA look through it, each a run of entries
-  const int64_t from = min(x.vocab, found * per), to = min(x.vocab, from + per);
-  const int run = (int)((to - from + kVfThreads - 1) / kVfThreads);
-  const int64_t t0 = min(to, from + (int64_t)tid * run), t1 = min(to, t0 + run);
-  if (tid == 0) sh.owner = 0x7FFFFFFF, sh.last = -1;
-  double s = 0.0;
-  for (int64_t j = t0; j < t1; ++j) s += mass(j, kind);
-  double incl = s;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) sh.scan[warp] = incl;
-  __syncthreads();
-  double base = before;
-  for (int i = 0; i < warp; ++i) base += sh.scan[i];
-  if (s > 0.0) {
-    if (base + incl > r) atomicMin(&sh.owner, tid);
-    atomicMax(&sh.last, tid);
-  }
-  __syncthreads();
-  const int owner = sh.owner != 0x7FFFFFFF ? sh.owner : sh.last;
-  if (tid / 32 != owner / 32) return;
-  int64_t token = 0;
-  double p = 0.0;
-  if (tid == owner) {
-    double at = base + (incl - s);
-    for (int64_t j = t0; j < t1; ++j) {
-      const double v = mass(j, kind);
-      if (v > 0.0) {
-        token = j;
-        at += v;
-        if (at > r) break;
-      }
+    const uint32_t some = __ballot_sync(0xFFFFFFFFu, s[0] > 0.0);
+    if (some) token = j0 + 31 - __clz(some);  // the last one so far, should none pass r by rounding
+    if (vf_find(s[0], r, false, before, found)) {
+      token = j0 + found;
+      break;
     }
-    p = weigh(V::one(row + token), top) / z;
   }
-  token = __shfl_sync(0xFFFFFFFFu, token, owner & 31);
-  p = __shfl_sync(0xFFFFFFFFu, p, owner & 31);
-  finish(token, p, flags);
+  finish(token, vf_weight(scale, V::one(row + token), sh.power) * share);
 }
 
-// Slices of a position: so many that the positions fill the GPU, of 2048
-// entries at least.
-static void vf_slices(int64_t positions, int64_t vocab, int *slices, int64_t *slice) {
-  const int64_t want = std::max<int64_t>(1, (148 * 8 + positions - 1) / positions);
-  int64_t each = (vocab + want - 1) / want;
-  each = std::max<int64_t>(2048, (each + 2047) / 2048 * 2048);
-  *slice = each;
-  *slices = (int)((vocab + 8 + each - 1) / each);  // 8: a row may start inside a piece
+// Entries of a slice: about three slices for each warp that an SM has room for,
+// of 1024 entries at least.
+static void vf_slices(int64_t positions, int64_t vocab, int *slices, int *slice) {
+  const int64_t warps = 148ll * kVfSums * (kVfThreads / 32) * 3;
+  const int64_t want = std::max<int64_t>(1, (warps + positions - 1) / positions);
+  *slice = (int)std::max<int64_t>(1024, ((vocab + want - 1) / want + 1023) / 1024 * 1024);
+  *slices = (int)((vocab + 8 + *slice - 1) / *slice);  // 8: a row may start inside a piece
 }
 
 static bool vf_sizes(int64_t rows, int32_t drafts, int64_t vocab) {
@@ -496,25 +684,31 @@ static bool vf_sizes(int64_t rows, int32_t drafts, int64_t vocab) {
          vocab <= kVfMaxVocab;
 }
 
-template <int DT>
-static cudaError_t vf_run(const VfArgs &a, cudaStream_t s) {
-  const int64_t positions = a.x.rows * (a.x.drafts + 1);
-  cudaError_t e = launch_dependent(ms_verify_stats_kernel<DT>, (unsigned)(positions * a.slices), kVfThreads, 0, s, a);
-  if (e != cudaSuccess) return e;
+template <int DT, int kThreads>
+static cudaError_t vf_draw(const VfArgs &a, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.x.rows * kVfCluster));
-  cfg.blockDim = dim3(kVfThreads);
+  cfg.gridDim = dim3((unsigned)(a.x.rows * a.ranks));
+  cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = kVfCluster;
+  attr[1].val.clusterDim.x = a.ranks;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, ms_verify_draw_kernel<DT>, a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, ms_verify_draw_kernel<DT, kThreads>, a);
   return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <int DT>
+static cudaError_t vf_run(const VfArgs &a, cudaStream_t s) {
+  const int64_t items = a.x.rows * (a.x.drafts + 1) * a.slices;
+  const unsigned blocks = (unsigned)((items + kVfThreads / 32 - 1) / (kVfThreads / 32));
+  cudaError_t e = launch_dependent(ms_verify_sums_kernel<DT>, blocks, kVfThreads, 0, s, a);
+  if (e != cudaSuccess) return e;
+  return a.x.rows * kVfCluster <= 148 ? vf_draw<DT, 1024>(a, s) : vf_draw<DT, 256>(a, s);
 }
 
 }  // namespace ms
@@ -523,8 +717,7 @@ extern "C" {
 
 int64_t ms_verify_workspace(int64_t rows, int32_t drafts, int64_t vocab) {
   if (!ms::vf_sizes(rows, drafts, vocab) || rows == 0) return 0;
-  int slices;
-  int64_t slice;
+  int slices, slice;
   ms::vf_slices(rows * (drafts + 1), vocab, &slices, &slice);
   return rows * (drafts + 1) * slices * (int64_t)sizeof(ms::VfRecord);
 }
@@ -544,6 +737,9 @@ int ms_verify_drafts(const ms_verify_args *args, ms_stream_t stream) {
   a.records = static_cast<ms::VfRecord *>(x.workspace);
   ms::vf_slices(x.rows * (x.drafts + 1), x.vocab, &a.slices, &a.slice);
   if (x.rows * (x.drafts + 1) > 0x7FFFFFFFll / a.slices) return MS_E_INVALID;
+  // CTAs of a row: as many as one wave has room for (four of 256 threads an SM), so that every row's draw runs at once
+  a.ranks = ms::kVfCluster;
+  while (a.ranks > 1 && x.rows * a.ranks > 148 * 4) a.ranks >>= 1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = x.dtype == MS_DTYPE_F32    ? ms::vf_run<MS_DTYPE_F32>(a, s)
                   : x.dtype == MS_DTYPE_BF16 ? ms::vf_run<MS_DTYPE_BF16>(a, s)
