@@ -28,7 +28,9 @@
 namespace ms {
 
 constexpr int kVfThreads = 128;   // of a CTA that sums slices
-constexpr int kVfSums = 8;        // such CTAs of an SM
+constexpr int kVfSums = 7;        // such CTAs of an SM
+constexpr int kVfPieces = 4;      // 16-byte pieces of a lane's batch of values
+constexpr int kVfStages = 4;      // batches of a warp's ring
 constexpr int kVfCluster = 8;     // CTAs of a row's draw, at most
 constexpr int kVfMaxDrafts = 255;
 constexpr int64_t kVfMaxVocab = 0x7FFFFFFFll - 65536;
@@ -194,22 +196,26 @@ __device__ __forceinline__ void vf_add(VfSum &a, float (&v)[kPieces][kVec], int 
   a.sum += (double)((part[0].x + part[0].y) + (part[1].x + part[1].y));
 }
 
-// Sums: a warp takes a slice of a position, the next values on their way while
-// it weighs the last ones.  CTAs are small and many: positions behind a row's
-// drafts have none, and what a slice costs varies.
+// Sums: a warp takes a slice of a position; a ring of asynchronous copies, each
+// lane's pieces for itself, keeps three batches on their way while it weighs the
+// fourth.  CTAs are small and many: positions behind a row's drafts have none,
+// and what a slice costs varies.
 template <int DT>
 __global__ void __launch_bounds__(kVfThreads, kVfSums) ms_verify_sums_kernel(const __grid_constant__ VfArgs a) {
   using V = VfType<DT>;
-  constexpr int kVec = V::kVec, kPieces = kVec == 4 ? 4 : 2;  // of a lane's batch: 16 values
+  constexpr int kVec = V::kVec, kPieces = kVfPieces;
   const float kNone = __uint_as_float(0xFF800000u);
+  __shared__ uint4 ring[kVfThreads / 32][kVfStages][kPieces][32];
   grid_wait();
   grid_release();
   const ms_verify_args &x = a.x;
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * (kVfThreads / 32) + (threadIdx.x >> 5);
-  if (item >= x.rows * (x.drafts + 1) * a.slices) return;
-  const int64_t at = item / a.slices, b = at / (x.drafts + 1);
-  const int slice = (int)(item - at * a.slices), i = (int)(at - b * (x.drafts + 1));
+  // fewer than 2^31 items (the host's check): divisions in 32 bits
+  const uint32_t item = blockIdx.x * (kVfThreads / 32) + (threadIdx.x >> 5);
+  const uint32_t at = item / (uint32_t)a.slices, row_at = at / (uint32_t)(x.drafts + 1);
+  const int slice = (int)(item - at * a.slices), i = (int)(at - row_at * (x.drafts + 1));
+  const int64_t b = row_at;
+  if (b >= x.rows) return;
   const double heat = load_in(x.temperature + b);
   if (vf_drafts(x, b, i) < i || !vf_heat(heat)) return;
   const bool greedy = heat == 0.0;
@@ -223,20 +229,30 @@ __global__ void __launch_bounds__(kVfThreads, kVfSums) ms_verify_sums_kernel(con
   const int inner = skew ? 1 : 0, outer = min((vocab + skew) / kVec, last);
   const uint4 *base = reinterpret_cast<const uint4 *>(row - skew);
   VfSum mine{kNone, 0.0, 0x7FFFFFFF, 0};
-  uint4 u[kPieces];
-  auto fetch = [&](int p0) {
+  uint4 (*mine_ring)[kPieces][32] = ring[threadIdx.x >> 5];
+  auto fetch = [&](int p0, int stage) {
 #pragma unroll
     for (int s = 0; s < kPieces; ++s) {
       const int p = p0 + s * 32;
-      if (p >= inner && p < outer) u[s] = load_in(base + p);
+      const bool in = p >= inner && p < outer;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(&mine_ring[stage][s][lane])),
+                   "l"(in ? base + p : reinterpret_cast<const uint4 *>(a.records)), "r"(in ? 16 : 0)
+                   : "memory");
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  fetch(first + lane);
-  for (int p0 = first + lane; p0 - lane < last; p0 += 32 * kPieces) {
+  constexpr int kStep = 32 * kPieces;
+#pragma unroll
+  for (int s = 0; s < kVfStages - 1; ++s) fetch(first + lane + s * kStep, s);
+  int stage = 0;
+  for (int p0 = first + lane; p0 - lane < last; p0 += kStep) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kVfStages - 2) : "memory");
     float v[kPieces][kVec];
 #pragma unroll
-    for (int s = 0; s < kPieces; ++s) V::wide(u[s], v[s]);
-    if (p0 - lane < inner || p0 - lane + 32 * kPieces > outer) {  // the row's ends
+    for (int s = 0; s < kPieces; ++s) V::wide(mine_ring[stage][s][lane], v[s]);
+    fetch(p0 + (kVfStages - 1) * kStep, stage == 0 ? kVfStages - 1 : stage - 1);
+    if (++stage == kVfStages) stage = 0;
+    if (p0 - lane < inner || p0 - lane + kStep > outer) {  // the row's ends
 #pragma unroll
       for (int s = 0; s < kPieces; ++s) {
         const int p = p0 + s * 32;
@@ -249,9 +265,9 @@ __global__ void __launch_bounds__(kVfThreads, kVfSums) ms_verify_sums_kernel(con
         }
       }
     }
-    fetch(p0 + 32 * kPieces);
     vf_add<kPieces, kVec>(mine, v, p0 * kVec - skew, greedy, unit);
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   // the lanes' sums, relative to the slice's largest value
   float top = mine.top;
   int index = mine.index;
@@ -296,18 +312,18 @@ constexpr double kVfLeast = 1000.0;              // weights below 2^-1000 count 
 struct VfScale {
   double c;     // steps of a unit of logit
   double base;  // kVfMagic - R
-  float top;
   float least;  // values below it weigh nothing
   // v c is far inside whole numbers' range.  Where it is not (temperatures so small that neighbouring values are 2^21
   // steps apart, or an infinite value), the largest value weighs 1 and all others nothing.
   bool plain;
 };
-__device__ __forceinline__ VfScale vf_scale(double heat, float top) {
+// Of the steps c of a unit of logit at a temperature, for a largest value that is not -inf.
+__device__ __forceinline__ VfScale vf_scale(double c, double heat, float top) {
   VfScale s;
-  s.c = 1.4426950408889634 * kVfSteps / heat, s.top = top;
-  s.plain = fabs((double)top) * s.c < 35184372088832.0 && s.c < 1e290;  // 2^45
-  s.base = kVfMagic - (s.plain ? kVfSteps * ceil((double)top * s.c / kVfSteps) : 0.0);
-  s.least = s.plain ? (float)fmax((double)top - kVfLeast * kVfSteps / s.c, -3.4e38) : top;
+  s.c = c;
+  s.plain = fabs((double)top) * c < 35184372088832.0 && c < 1e290;  // 2^45
+  s.base = kVfMagic - (s.plain ? kVfSteps * ceil((double)top * c * (1.0 / kVfSteps)) : 0.0);
+  s.least = s.plain ? (float)fmax((double)top - kVfLeast * 0.69314718055994530942 * heat, -3.4e38) : top;
   return s;
 }
 // Relative to 2^(R / 128) or, of scales that are not plain, to the largest
@@ -360,8 +376,8 @@ __device__ __forceinline__ bool vf_find(double mass, double r, bool end, double 
 }
 
 // What a part's sums are of: the weights, of all entries or of all but a draft;
-// the weights, and the draft's probabilities, of entries that have more weight
-// than the draft gave them; what is left of those entries.
+// what is left, by the first kernel's z, of the entries that have more weight
+// than the draft gave them, and what it gave those; what is left by the exact z.
 enum { kVfAll, kVfMore, kVfTaken, kVfRest, kVfKinds };
 
 template <int kThreads>
@@ -370,10 +386,14 @@ struct VfShared {
   double sum[kVfKinds][kThreads / 32];       // of the CTA's warps
   double mass[kVfKinds][kVfCluster];         // of the cluster's CTAs, in index order
   double odd[kVfCluster];                    // CTAs that met a draft probability that is none
-  double accepted[kVfMaxDrafts + 1];         // p_i(d_i)
-  double whole[kVfMaxDrafts + 1];            // sums of the positions' weights, relative to their largest values
-  float top[kVfMaxDrafts + 1];
+  double share[kVfMaxDrafts + 1];            // 1 over the sum of a position's weights
+  VfScale scale[kVfMaxDrafts + 1];
+  float accepted[kVfMaxDrafts + 1];          // p_i(d_i)
+  int draft[kVfMaxDrafts + 1];
   int index[kVfMaxDrafts + 1], flags[kVfMaxDrafts + 1];
+  bool none[kVfMaxDrafts + 1];               // all values are -inf
+  double c, heat;
+  float unit;
   int stop, drafts, status;
 };
 
@@ -386,12 +406,14 @@ struct VfShared {
 // What the draft's probabilities leave, max(w / z - q, 0), needs the whole z of
 // the weights w first.  One pass is enough all the same: the first kernel's z is
 // known to 1e-7, and the entries that it puts on the wrong side of w / z = q are
-// those where next to nothing is left, so that sum w / z - sum q over the others'
-// side is the sum to 1e-13.  Where all that is left is itself small (a draft
-// model that is the target, nearly), a second pass takes the exact z.
+// those where next to nothing is left, so that the sum over its side, S = sum (w
+// / z - q) and Q = sum q, is S + (S + Q) (z / z' - 1) for the exact z' to 1e-13,
+// with Q to 1e-6.  Where all that is left is itself small (a draft model that is
+// the target, nearly), a second pass takes the exact z.
 //
-// fp64 operations take tens of cycles one after the other: 32-wide scans stand
-// where a loop over eight sums would do.
+// fp64 operations take some 40 cycles one after the other, and divisions several
+// hundred: one thread makes a position's scale, and 32-wide scans stand where a
+// loop over eight sums would do.
 template <int DT, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kernel(const __grid_constant__ VfArgs a) {
   using V = VfType<DT>;
@@ -405,17 +427,23 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for before a CTA writes to another
   const double entry = vf_powers.of[(tid >> 1) % kVfSteps];
   grid_wait();
-  const double heat = load_in(x.temperature + b);
-  const bool greedy = heat == 0.0;
+  const double u = load_in(x.uniforms + b * x.uniform_row + x.drafts);  // the draw's
   if (warp == 0) {
+    const double heat = load_in(x.temperature + b);
     const int n = vf_drafts(x, b, x.drafts);
     bool bad = false;
-    for (int i = lane; i < n; i += 32) bad = bad || load_in(x.draft_tokens + b * x.draft_row + i) >= x.vocab;
+    for (int i = lane; i < n; i += 32) {
+      const int64_t d = load_in(x.draft_tokens + b * x.draft_row + i);
+      bad = bad || d >= x.vocab;
+      sh.draft[i] = (int)d;
+    }
     bad = __any_sync(0xFFFFFFFFu, bad);
     if (lane == 0) {
-      sh.drafts = n;
+      sh.drafts = sh.stop = n;
       sh.status = (vf_heat(heat) ? MS_ROW_OK : MS_ROW_BAD_TEMPERATURE) | (bad ? MS_ROW_BAD_DRAFT : MS_ROW_OK);
-      sh.stop = n;
+      sh.heat = heat;
+      sh.c = 1.4426950408889634 * kVfSteps / heat;
+      sh.unit = vf_unit(heat);
     }
   }
   if (tid < 2 * kVfSteps) {
@@ -440,15 +468,15 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
     meet();
     return;
   }
-  const float unit = vf_unit(heat);
+  const float unit = sh.unit;
+  const bool greedy = sh.heat == 0.0;
   auto logits = [&](int i) { return static_cast<const typename V::T *>(x.logits) + b * x.logits_row + i * x.logits_pos; };
   for (int i = warp; i <= n; i += kWarps) {  // the positions' records
-    int64_t d = 0;
-    double u = 0.0, q = 1.0;
+    const int d = i < n ? sh.draft[i] : 0;
+    double chance = 0.0, q = 1.0;
     float v = kNone;
     if (i < n && lane == 0) {
-      d = load_in(x.draft_tokens + b * x.draft_row + i);
-      u = load_in(x.uniforms + b * x.uniform_row + i);
+      chance = load_in(x.uniforms + b * x.uniform_row + i);
       v = V::one(logits(i) + d);
       if (x.draft_probs && !greedy) q = load_in(x.draft_probs + b * x.probs_row + i * x.probs_pos + d);
     }
@@ -474,17 +502,19 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
     const int flags = __reduce_or_sync(0xFFFFFFFFu, all.flags);
     const double z = vf_warp_sum(vf_moved(all.sum, all.top, top, unit));
     if (lane == 0) {
-      sh.top[i] = top, sh.whole[i] = z, sh.index[i] = index, sh.flags[i] = flags;
+      sh.index[i] = index, sh.flags[i] = flags, sh.none[i] = top == kNone;
+      double p = 0.0;
+      if (greedy) {
+        p = d == index ? 1.0 : 0.0;
+      } else if (top > kNone) {
+        const VfScale s = vf_scale(sh.c, sh.heat, top);
+        const double share = 1.0 / (vf_power(s, top, sh.power) * z);
+        p = vf_weight(s, v, sh.power) * share;
+        sh.scale[i] = s, sh.share[i] = share;
+      }
       if (i < n) {
-        double p = 0.0;
-        if (greedy) {
-          p = d == index ? 1.0 : 0.0;
-        } else if (top > kNone) {
-          const VfScale s = vf_scale(heat, top);
-          p = vf_weight(s, v, sh.power) / (vf_power(s, top, sh.power) * z);
-        }
-        sh.accepted[i] = p;
-        if (!(u * q < p)) atomicMin(&sh.stop, i);
+        sh.accepted[i] = (float)p;
+        if (!(chance * q < p)) atomicMin(&sh.stop, i);
       }
     }
   }
@@ -492,18 +522,18 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
   const int f = sh.stop;
   int flags = 0;
   for (int i = 0; i <= f; ++i) flags |= sh.flags[i];
-  const float top = sh.top[f];
+  const bool none = sh.none[f];
   auto finish = [&](int64_t token, double p) {  // by a warp
     for (int i = lane; i <= x.drafts; i += 32) {
       const int64_t o = b * (x.drafts + 1) + i;
-      x.tokens[o] = i < f ? load_in(x.draft_tokens + b * x.draft_row + i) : i == f ? token : -1;
-      x.probs[o] = i < f ? (float)sh.accepted[i] : i == f ? (float)p : 0.f;
+      x.tokens[o] = i < f ? sh.draft[i] : i == f ? token : -1;
+      x.probs[o] = i < f ? sh.accepted[i] : i == f ? (float)p : 0.f;
     }
     if (lane == 0) x.counts[b] = f + 1, x.status[b] = flags;
   };
-  if (greedy || top == kNone) {
+  if (greedy || none) {
     if (rank == 0 && !greedy) give_up(MS_ROW_ALL_MASKED | flags);
-    if (rank == 0 && greedy && warp == 0) finish(top == kNone ? 0 : sh.index[f], 1.0);
+    if (rank == 0 && greedy && warp == 0) finish(none ? 0 : sh.index[f], 1.0);
     __syncwarp();
     meet();
     return;
@@ -511,18 +541,26 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
   const typename V::T *row = logits(f);
   const bool refused = f < n;
   const float *q = refused && x.draft_probs ? x.draft_probs + b * x.probs_row + f * x.probs_pos : nullptr;
-  int without = refused && !q ? (int)load_in(x.draft_tokens + b * x.draft_row + f) : -1;
-  const double u = load_in(x.uniforms + b * x.uniform_row + x.drafts);
-  const VfScale scale = vf_scale(heat, top);
-  double share = 1.0 / (vf_power(scale, top, sh.power) * sh.whole[f]);  // 1 / z
+  int without = refused && !q ? sh.draft[f] : -1;
+  const VfScale scale = sh.scale[f];
+  const double first_share = sh.share[f];
+  double share = first_share;  // 1 / z
   uint32_t odd = 0;  // the largest bit pattern of the draft's probabilities: those past the finite ones are none
   // a warp's part of the vocabulary, of one CTA after the other
   const int64_t per = ((x.vocab + ranks * kWarps - 1) / (ranks * kWarps) + 31) / 32 * 32;
+  {  // the CTA's entries on their way to L2
+    const int64_t from = min(x.vocab, rank * kWarps * per), to = min(x.vocab, from + kWarps * per);
+    auto touch = [&](const char *p, const char *end) {
+      for (p += tid * 128; p < end; p += kThreads * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+    };
+    touch(reinterpret_cast<const char *>(row + from), reinterpret_cast<const char *>(row + to));
+    if (q) touch(reinterpret_cast<const char *>(q + from), reinterpret_cast<const char *>(q + to));
+  }
   constexpr std::integral_constant<int, kVfAll> kAll{};
   constexpr std::integral_constant<int, kVfMore> kMore{};
   constexpr std::integral_constant<int, kVfRest> kRest{};
   // an entry's part in the sums s of a kind
-  auto add = [&](double (&s)[3], float v, float d, bool in, auto kind) {
+  auto add = [&](double (&s)[2], float &given, float v, float d, bool in, auto kind) {
     const double w = vf_power(scale, v, sh.power);
     const bool some = in && v >= scale.least;  // a NaN is not
     if constexpr (kind.value == kVfAll) {
@@ -532,11 +570,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
       odd = max(odd, __float_as_uint(d));
       const double taken = (double)fmaxf(d, 0.f);  // a NaN reads as 0
       const double rest = fma(w, share, -taken);
+      const bool more = some && __double2hiint(rest) > 0;  // above 2^-1023, that is
       if constexpr (kind.value == kVfMore) {
         if (some) s[0] += w;
-        if (some && rest > 0.0) s[1] += w, s[2] += taken;
+        if (more) s[1] += rest, given += fmaxf(d, 0.f);
       } else {
-        if (some && rest > 0.0) s[0] += rest;
+        if (more) s[0] += rest;
       }
     }
   };
@@ -544,27 +583,36 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
   auto part = [&](int64_t lo, int64_t hi, double (&s)[3], auto kind) {
     constexpr int kBatch = 8;
     constexpr bool kTakes = kind.value != kVfAll;
-    double t[2][3] = {};
-    int j = (int)lo + lane;
-    for (; j - lane + 32 * kBatch <= (int)hi; j += 32 * kBatch) {
+    double t[2][2] = {};
+    float given[2] = {0.f, 0.f};
+    const int end = (int)hi;
+    for (int j0 = (int)lo; j0 < end; j0 += 32 * kBatch) {
+      const int j = j0 + lane;
       const typename V::T *at = row + j;
       const float *taken = q + j;
       float v[kBatch], d[kBatch];
+      if (j0 + 32 * kBatch <= end && (kTakes || (unsigned)(without - j0) >= 32 * kBatch)) {
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) v[k] = V::one(at + 32 * k), d[k] = kTakes ? load_in(taken + 32 * k) : 0.f;
-      if (!kTakes && (unsigned)(without - (j - lane)) < 32 * kBatch) {
+        for (int k = 0; k < kBatch; ++k) v[k] = V::one(at + 32 * k), d[k] = kTakes ? load_in(taken + 32 * k) : 0.f;
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) add(t[k & 1], v[k], d[k], j + 32 * k != without, kind);
+        for (int k = 0; k < kBatch; ++k) add(t[k & 1], given[k & 1], v[k], d[k], true, kind);
       } else {
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) add(t[k & 1], v[k], d[k], true, kind);
+        for (int k = 0; k < kBatch; ++k) {
+          const bool in = j + 32 * k < end;
+          v[k] = in ? V::one(at + 32 * k) : kNone;
+          d[k] = in && kTakes ? load_in(taken + 32 * k) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          if (j0 + 32 * k < end) add(t[k & 1], given[k & 1], v[k], d[k], j + 32 * k != without, kind);
       }
     }
-    for (; j - lane < (int)hi; j += 32)
-      add(t[0], j < (int)hi ? V::one(row + j) : kNone, kTakes && j < (int)hi ? load_in(q + j) : 0.f, j != without, kind);
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (i == 0 || kind.value == kVfMore) s[i] = vf_warp_sum(t[0][i] + t[1][i]);
+    s[0] = vf_warp_sum(t[0][0] + t[1][0]);
+    if constexpr (kind.value == kVfMore) {
+      s[1] = vf_warp_sum(t[0][1] + t[1][1]);
+      s[2] = vf_warp_sum((double)(given[0] + given[1]));
+    }
   };
   // Every CTA's sums of its part to all of them, at places `slot` on.
   bool met = false;
@@ -593,14 +641,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
     __syncwarp();
     cluster_sync();
   };
-  // A lane's part of the row, of CTAs or of warps, as the draw sees it.  What is left of a part is the difference of two
-  // sums: nothing where it is within their rounding.
+  // A lane's part of the row, of CTAs or of warps, as the draw sees it: nothing where what is left of a part is within
+  // the rounding of its sums.
   int slot = kVfAll;
+  double moved = 0.0;  // by the exact z, over the first kernel's: its share less 1
   auto mass = [&](const double *of, int pitch, int count) {
     if (lane >= count) return 0.0;
     if (slot != kVfMore) return of[slot * pitch + lane];
-    const double more = of[kVfMore * pitch + lane] * share, rest = more - of[kVfTaken * pitch + lane];
-    return rest > 1e-13 * more ? rest : 0.0;
+    const double left = of[kVfMore * pitch + lane], all = left + of[kVfTaken * pitch + lane];
+    const double rest = fma(all, moved, left);
+    return rest > 1e-13 * all ? rest : 0.0;
   };
   auto whole = [&]() { return vf_warp_sum(mass(&sh.mass[0][0], kVfCluster, ranks)); };
   double all;
@@ -618,6 +668,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
   } else {
     sums(kVfAll, kMore);
     share = 1.0 / whole();
+    moved = (share - first_share) / first_share;
     slot = kVfMore;
     all = whole();
     if (!(all > 1e-3)) {
@@ -652,17 +703,27 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
   }
   vf_find(lane < kWarps ? sh.sum[0][lane] : 0.0, r, true, before, found);
   if (found != warp) return;
-  int64_t token = lo;
-  for (int64_t j0 = lo; j0 < hi; j0 += 32) {
-    const int64_t j = j0 + lane;
-    double s[3] = {0.0, 0.0, 0.0};
-    if (j < hi) {
-      if (rest) add(s, V::one(row + j), load_in(q + j), true, kRest);
-      else add(s, V::one(row + j), 0.f, (int)j != without, kAll);
-    }
-    const uint32_t some = __ballot_sync(0xFFFFFFFFu, s[0] > 0.0);
+  // the warp's entries, a run for each lane; then the entries of the lane that is found
+  auto mass_at = [&](int64_t j) {
+    double s[2] = {0.0, 0.0};
+    float given = 0.f;
+    if (rest) add(s, given, V::one(row + j), load_in(q + j), true, kRest);
+    else add(s, given, V::one(row + j), 0.f, (int)j != without, kAll);
+    return s[0];
+  };
+  const int64_t run = (hi - lo + 31) / 32;
+  int64_t token = lo, from = min(hi, lo + lane * run);
+  if (run > 1) {
+    double s = 0.0;
+    for (int64_t j = from; j < min(hi, from + run); ++j) s += mass_at(j);
+    vf_find(s, r, true, before, found);
+    token = lo + found * run;
+  }
+  for (int64_t end = run > 1 ? min(hi, token + run) : hi, j0 = token; j0 < end; j0 += 32) {
+    const double m = j0 + lane < end ? mass_at(j0 + lane) : 0.0;
+    const uint32_t some = __ballot_sync(0xFFFFFFFFu, m > 0.0);
     if (some) token = j0 + 31 - __clz(some);  // the last one so far, should none pass r by rounding
-    if (vf_find(s[0], r, false, before, found)) {
+    if (vf_find(m, r, false, before, found)) {
       token = j0 + found;
       break;
     }
@@ -671,11 +732,15 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
 }
 
 // Entries of a slice: about three slices for each warp that an SM has room for,
-// of 1024 entries at least.
+// but 4096 entries (what a slice costs besides its entries is that of 1000), or
+// what fills the GPU once, of 1024 entries at least.
 static void vf_slices(int64_t positions, int64_t vocab, int *slices, int *slice) {
-  const int64_t warps = 148ll * kVfSums * (kVfThreads / 32) * 3;
-  const int64_t want = std::max<int64_t>(1, (warps + positions - 1) / positions);
-  *slice = (int)std::max<int64_t>(1024, ((vocab + want - 1) / want + 1023) / 1024 * 1024);
+  const int64_t warps = 148ll * kVfSums * (kVfThreads / 32);
+  auto each = [&](int64_t all) {
+    const int64_t want = std::max<int64_t>(1, (all + positions - 1) / positions);
+    return ((vocab + want - 1) / want + 1023) / 1024 * 1024;
+  };
+  *slice = (int)std::max(each(3 * warps), std::min<int64_t>(4096, each(warps)));
   *slices = (int)((vocab + 8 + *slice - 1) / *slice);  // 8: a row may start inside a piece
 }
 
