@@ -27,7 +27,10 @@ struct A4Plan {
 
 // CTAs of an SM that the kernel of these sizes is built for.
 static int a4_ctas(int groups, int eights) {
-  if (groups <= 2) return eights == 1 ? kA4Ctas<2, 1> : eights == 2 ? kA4Ctas<2, 2> : eights == 3 ? kA4Ctas<2, 3> : kA4Ctas<2, 4>;
+  if (groups <= 2) {
+    constexpr int ctas[5] = {kA4Ctas<2, 1>, kA4Ctas<2, 2>, kA4Ctas<2, 3>, kA4Ctas<2, 4>, kA4Ctas<2, 5>};
+    return ctas[eights - 1];
+  }
   return eights == 1 ? kA4Ctas<4, 1> : kA4Ctas<4, 2>;
 }
 
@@ -68,11 +71,11 @@ static cudaError_t a4_split(const A4Args &a, int dev, cudaStream_t s) {
   if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
   auto *kernel = ms_attn4_split_kernel<NG, NQ, kWhole>;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kA4Shared<NG>);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kA4Shared<NG, NQ>);
     if (e != cudaSuccess) return e;
     ready[dev].store(1, std::memory_order_release);
   }
-  return launch_dependent(kernel, (unsigned)(a.split_warps / kA4Warps), kA4Warps * 32, kA4Shared<NG>, s, a);
+  return launch_dependent(kernel, (unsigned)(a.split_warps / kA4Warps), kA4Warps * 32, kA4Shared<NG, NQ>, s, a);
 }
 template <int NG>
 static cudaError_t a4_split_as(const A4Args &a, int eights, int dev, cudaStream_t s) {
@@ -81,6 +84,7 @@ static cudaError_t a4_split_as(const A4Args &a, int eights, int dev, cudaStream_
   if (eights == 2) return whole ? a4_split<NG, 2, true>(a, dev, s) : a4_split<NG, 2, false>(a, dev, s);
   if constexpr (NG <= 2) {
     if (eights == 3) return whole ? a4_split<NG, 3, true>(a, dev, s) : a4_split<NG, 3, false>(a, dev, s);
+    if (eights == 5) return whole ? a4_split<NG, 5, true>(a, dev, s) : a4_split<NG, 5, false>(a, dev, s);
     if (eights == 4) return whole ? a4_split<NG, 4, true>(a, dev, s) : a4_split<NG, 4, false>(a, dev, s);
   }
   return cudaErrorInvalidValue;

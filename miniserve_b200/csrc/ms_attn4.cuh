@@ -18,6 +18,7 @@ constexpr int kA4Warps = 4;                // warps of a split CTA
 constexpr int kA4Tile = 16;                // keys of a tile: the M of the score products, the K of the output's
 constexpr int kA4Item = 2;                 // cost of an item's queries and record, in tiles
 constexpr int kA4Stages = 4;               // tiles of a warp's ring
+constexpr float kA4Least = -3e38f;         // refers to nothing yet: every score is far above it
 constexpr int64_t kA4MaxRows = 1 << 20;
 constexpr int kA4MaxTokens = 1024;         // of a row
 // Bytes of a token's codes in the ring: an odd multiple of 16, so that eight
@@ -26,13 +27,19 @@ template <int NG>
 constexpr int kA4Pitch = NG <= 3 ? 48 : 80;
 template <int NG>
 constexpr int kA4Stage = 2 * kA4Tile * kA4Pitch<NG> + 2 * kA4Tile * 16;  // K and V codes, K and V parameters
-template <int NG>
-constexpr int kA4Shared = kA4Warps * kA4Stages * kA4Stage<NG>;
+// Queries of more than four fragments a lane stay in shared memory: registers
+// are for the output's.
+template <int NG, int NQ>
+constexpr bool kA4QShared = NG * NQ > 4;
+template <int NG, int NQ>
+constexpr int kA4Queries = kA4QShared<NG, NQ> ? NG * NQ * 32 * 24 : 0;  // bytes of a warp's
+template <int NG, int NQ>
+constexpr int kA4Shared = kA4Warps * (kA4Stages * kA4Stage<NG> + kA4Queries<NG, NQ>);
 // Split CTAs of an SM, by what their registers allow.
 template <int NG, int NQ>
-constexpr int kA4Ctas = NG <= 2 ? (NQ <= 1 ? 4 : NQ <= 2 ? 3 : 2) : (NQ <= 1 ? 3 : 2);
+constexpr int kA4Ctas = NG <= 2 ? (NQ <= 1 ? 4 : NQ <= 3 ? 3 : 2) : (NQ <= 1 ? 3 : 2);
 // Query rows of an item, at most: eights that registers have room for.
-__host__ __device__ constexpr int a4_most(int groups) { return groups <= 2 ? 32 : 16; }
+__host__ __device__ constexpr int a4_most(int groups) { return groups <= 2 ? 40 : 16; }
 
 struct A4Header {
   int64_t share;  // units of one split warp
@@ -73,16 +80,13 @@ __device__ __forceinline__ int64_t a4_units(int keys) {
 }
 
 // Walks over a warp's tiles: the split kernel's sequence is rows' items (key
-// head and chunk) in order, each of kA4Item units and one unit a tile.
+// head and chunk) in order, each of kA4Item units and one unit a tile.  A warp's
+// share is far below 2^31 units (the kernel would run for days).
 struct A4Walk {
-  int64_t b, left;  // left: units of the share past this item
-  int hc, tile, end, tiles, keys;
+  int b, left;  // left: units of the share past this item
+  int hc, tile, end, keys;
 };
-__device__ __forceinline__ void a4_row(const A4Args &a, A4Walk &w) {
-  bool bad;
-  w.keys = a4_keys(a.x, w.b, bad);
-  w.tiles = (w.keys + kA4Tile - 1) / kA4Tile;
-}
+__device__ __forceinline__ int a4_tiles(int keys) { return (keys + kA4Tile - 1) / kA4Tile; }
 // The next item's tiles within the share; tile == end where none are left.
 __device__ __forceinline__ void a4_item_next(const A4Args &a, A4Walk &w) {
   w.tile = w.end = 0;
@@ -90,16 +94,13 @@ __device__ __forceinline__ void a4_item_next(const A4Args &a, A4Walk &w) {
   if (++w.hc >= a.x.cache.kv_heads * a.chunks) {
     w.hc = 0;
     do {  // a later row has keys: units are left
-      ++w.b;
-      a4_row(a, w);
-    } while (w.tiles == 0);
+      bool bad;
+      w.keys = a4_keys(a.x, ++w.b, bad);
+    } while (w.keys == 0);
   }
-  const int64_t take = min(w.left, (int64_t)w.tiles + kA4Item);
+  const int take = min(w.left, a4_tiles(w.keys) + kA4Item);
   w.left -= take;
-  w.end = (int)take - kA4Item;
-}
-__device__ __forceinline__ void a4_next(const A4Args &a, A4Walk &w) {
-  if (++w.tile >= w.end) a4_item_next(a, w);
+  w.end = take - kA4Item;
 }
 
 __device__ __forceinline__ void copy8(uint32_t dst, const void *src, bool live) {
@@ -128,6 +129,15 @@ __device__ __forceinline__ void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The upper eight rows of the product, of an A whose lower ones are zero.
+__device__ __forceinline__ void a4_mma_top(float (&d)[2], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
+  float none0, none1;
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
+      : "+f"(d[0]), "+f"(d[1]), "=f"(none0), "=f"(none1)
+      : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+  (void)none0, (void)none1;
 }
 __device__ __forceinline__ uint32_t a4_pack(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
@@ -161,10 +171,10 @@ __device__ __forceinline__ float a4_low(uint32_t u) { return __low2float(*reinte
 //
 // Queries enter as fp16, scaled by a power of two that puts a row's largest in
 // [2^9, 2^10): entries down to 2^-23 of it are exact.  Weights are at most 2^8
-// of the running maximum's (it moves only when a score passes it by 2^8),
-// scaled up by 2^7, and by the power of two below 1 over the largest value
-// scale met, so that fp16 holds them with 2^-21 and less of the largest at
-// full precision.
+// of what they refer to (it moves only when a score passes it by 2^8), scaled up
+// by 2^7 (and up to 2^0.5: references are whole numbers), and by the power of two
+// below 1 over the largest value scale met, so that fp16 holds them with 2^-21
+// and less of the largest at full precision.
 template <int NG, int NQ, bool kWhole>
 __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
     ms_attn4_split_kernel(const __grid_constant__ A4Args a) {
@@ -226,114 +236,166 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
       if (sums[mid + 1] * hcs > u0) hi = mid;
       else lo = mid + 1;
     }
-    load.b = min(rows, lo * run);
+    load.b = (int)min(rows, lo * run);
     int64_t first = sums[lo] * hcs;
-    a4_row(a, load);
+    load.keys = a4_keys(x, load.b, bad);
     while (first + a4_units(load.keys) * hcs <= u0) {
       first += a4_units(load.keys) * hcs;
-      ++load.b;
-      a4_row(a, load);
+      load.keys = a4_keys(x, ++load.b, bad);
     }
-    const int64_t units = load.tiles + kA4Item;
+    const int64_t units = a4_units(load.keys);
     load.hc = (int)((u0 - first) / units);
     const int64_t at = u0 - first - load.hc * units, take = min(u1 - u0, units - at);
-    load.left = u1 - u0 - take;
+    load.left = (int)(u1 - u0 - take);
     load.tile = (int)max((int64_t)0, at - kA4Item);
     load.end = (int)(at + take) - kA4Item;
     if (load.end <= load.tile) a4_item_next(a, load);
   }
   A4Walk now = load;
-  const uint32_t ring = smem_addr(a4_ring) + warp * kStages * kStage;
+  unsigned char *mine = a4_ring + warp * kStages * kStage;
+  const uint32_t ring = smem_addr(mine);
   constexpr int kV = kA4Tile * kPitch, kKp = 2 * kV, kVp = kKp + kA4Tile * 16;  // of a stage
   if (kPairs == 2) {  // the parameters' rows are 16 bytes there too: what lies behind the two pairs stays zero
-    unsigned char *mine = a4_ring + warp * kStages * kStage;
     for (int s = 0; s < kStages; ++s)
       *reinterpret_cast<uint4 *>(mine + s * kStage + kKp + lane * 16) = make_uint4(0, 0, 0, 0);
     __syncwarp();
   }
   const int page_size = (int)x.cache.page_size;
 
-  // One page for all lanes where tiles lie in one; else lanes 0-15 (and 16-31
-  // again) look up the tile's keys.
-  int64_t from = -1;  // the row (of codes and parameters) of the tile's first key, or of the lane's
-  int live_keys = 0;
-  uint32_t met = 0;  // bit i: the tile issued i tiles ago met a bad page
-  bool wrong = false;
-  auto look = [&]() {
-    from = -1;
+  // Copies.  Where tiles lie in one page each, a lane's places in the cache are
+  // stepped along the page; a new page's id is loaded a tile ahead of its use.
+  // Else lanes 0-15 (and 16-31 again) look up the tile's keys.
+  int page = -1;         // loaded, of the next tile (or the lane's key of it)
+  int fresh_page = 1;    // it is a new page, or every tile's keys are looked up
+  int offset = 0;        // in it
+  int room = 0;          // tokens of the page from the next tile on
+  int head = 0;          // of the next tile
+  int live_keys = 0;     // of the next tile; 0 where none is left
+  int64_t code_at = 0, param_at = 0;  // the lane's, of the tile copied last
+  bool good = false;     // its page is one
+  uint32_t met = 0;      // bit i: the tile issued i tiles ago met a bad page
+  auto look = [&](bool item) {  // at tile load.tile, the first of an item's or the one after the last
     live_keys = 0;
-    wrong = false;
-    if (load.tile < load.end) {
-      const int j = load.tile * kA4Tile + (kWhole ? 0 : lane & 15);
-      live_keys = load.keys - load.tile * kA4Tile;
+    if (load.tile >= load.end) return;
+    if (item) head = load.hc / a.chunks;
+    live_keys = load.keys - load.tile * kA4Tile;
+    if (kWhole) {
+      room -= kA4Tile;
+      fresh_page = item || room <= 0;
+      if (fresh_page) {
+        const int j = load.tile * kA4Tile, p = a.page_shift >= 0 ? j >> a.page_shift : j / page_size;
+        offset = j - p * page_size;
+        room = page_size - offset;
+        page = load_in(x.table + load.b * x.table_row + p);
+      }
+    } else {
+      const int j = load.tile * kA4Tile + (lane & 15);
+      page = 0, offset = 0;
       if (j < load.keys) {
         const int p = a.page_shift >= 0 ? j >> a.page_shift : j / page_size;
-        const int page = load_in(x.table + load.b * x.table_row + p);
-        if (page >= 0 && page < x.cache.pages)
-          from = ((int64_t)page * x.cache.kv_heads + load.hc / a.chunks) * page_size + (j - p * page_size);
-        else
-          wrong = true;
+        offset = j - p * page_size;
+        page = load_in(x.table + load.b * x.table_row + p);
       }
-      a4_next(a, load);
     }
   };
+  auto step = [&]() {
+    if (load.tile >= load.end) return;  // none is left
+    bool item = ++load.tile >= load.end;
+    if (item) a4_item_next(a, load);
+    look(item);
+  };
+  constexpr int kCopies = (kA4Tile * kPieces + 31) / 32;  // of a tile's codes of the keys
   auto issue = [&](int stage) {
     const uint32_t dst = ring + stage * kStage;
-    met = (met << 1) | (kWhole ? wrong : __any_sync(0xFFFFFFFFu, wrong));
-#pragma unroll
-    for (int i = 0; i < (kA4Tile * kPieces + 31) / 32; ++i) {
-      const int at = i * 32 + lane, r = at / kPieces, piece = at - r * kPieces;
-      const int64_t row = kWhole ? from + r : __shfl_sync(0xFFFFFFFFu, from, r & 15);
-      const bool live = (kWhole ? from >= 0 : row >= 0) && r < live_keys && r < kA4Tile;
-      const int64_t off = live ? row * kRow + piece * 16 : 0;
-      if (kA4Tile * kPieces % 32 == 0 || r < kA4Tile) {
-        copy16(dst + r * kPitch + piece * 16, x.cache.k_codes + off, live);
-        copy16(dst + kV + r * kPitch + piece * 16, x.cache.v_codes + off, live);
+    if (kWhole) {
+      if (fresh_page) {
+        good = page >= 0 && page < x.cache.pages;
+        const int64_t row = ((int64_t)page * x.cache.kv_heads + head) * page_size + offset;
+        code_at = good ? row * kRow + lane * 16 : 0;
+        param_at = good ? (row + (lane & 15)) * (kPairs * 4) : 0;
+      } else if (good) {
+        code_at += kA4Tile * kRow;
+        param_at += kA4Tile * kPairs * 4;
       }
-    }
-    {
-      const int r = lane & 15;
-      const int64_t row = kWhole ? from + r : from;
-      const bool live = from >= 0 && r < live_keys;
-      const char *src = static_cast<const char *>(lane < 16 ? x.cache.k_params : x.cache.v_params) + (live ? row * (kPairs * 4) : 0);
-      if (kPairs == 4) copy16(dst + kKp + lane * 16, src, live);
-      else copy8(dst + kKp + lane * 16, src, live);
+      met = (met << 1) | (live_keys > 0 && !good);
+      const unsigned char *ks = x.cache.k_codes + code_at, *vs = x.cache.v_codes + code_at;
+      const char *ps = static_cast<const char *>(lane < 16 ? x.cache.k_params : x.cache.v_params) + param_at;
+      const int rows_here = good ? live_keys : 0;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int at = i * 32 + lane, r = at / kPieces, piece = at - r * kPieces;
+        const bool live = rows_here >= kA4Tile || r < rows_here;
+        if (kA4Tile * kPieces % 32 == 0 || r < kA4Tile) {
+          copy16(dst + r * kPitch + piece * 16, live ? ks + i * 512 : x.cache.k_codes, live);
+          copy16(dst + kV + r * kPitch + piece * 16, live ? vs + i * 512 : x.cache.v_codes, live);
+        }
+      }
+      const bool live = (lane & 15) < rows_here;
+      if (kPairs == 4) copy16(dst + kKp + lane * 16, live ? ps : x.cache.k_params, live);
+      else copy8(dst + kKp + lane * 16, live ? ps : x.cache.k_params, live);
+    } else {
+      const bool mine_live = (lane & 15) < live_keys, fine = page >= 0 && page < x.cache.pages;
+      met = (met << 1) | __any_sync(0xFFFFFFFFu, mine_live && !fine);
+      const int64_t row = mine_live && fine ? ((int64_t)page * x.cache.kv_heads + head) * page_size + offset : -1;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int at = i * 32 + lane, r = at / kPieces, piece = at - r * kPieces;
+        const int64_t from = __shfl_sync(0xFFFFFFFFu, row, r & 15);
+        const bool live = from >= 0 && r < kA4Tile;
+        const int64_t off = live ? from * kRow + piece * 16 : 0;
+        if (kA4Tile * kPieces % 32 == 0 || r < kA4Tile) {
+          copy16(dst + r * kPitch + piece * 16, x.cache.k_codes + off, live);
+          copy16(dst + kV + r * kPitch + piece * 16, x.cache.v_codes + off, live);
+        }
+      }
+      const char *src = static_cast<const char *>(lane < 16 ? x.cache.k_params : x.cache.v_params) + (row >= 0 ? row * (kPairs * 4) : 0);
+      if (kPairs == 4) copy16(dst + kKp + lane * 16, src, row >= 0);
+      else copy8(dst + kKp + lane * 16, src, row >= 0);
     }
   };
 
-  look();
+  look(true);
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
     issue(s);
-    look();
+    step();
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  uint32_t qf[NQ][NG][4];      // queries as B: pairs of entries (8c, 8c + 4), (8c + 1, 8c + 5) 2^-4, ...
+  // Queries as B: pairs of entries (8c, 8c + 4), (8c + 1, 8c + 5) 2^-4, ... of a group, and -8 2^-24 times the groups'
+  // sums of queries 2c and 2c + 1.
+  constexpr bool kQShared = kA4QShared<NG, NQ>;
+  uint32_t qf[kQShared ? 1 : NQ][NG][4];
+  float q8[kQShared ? 1 : NQ][NG][2];
+  unsigned char *q_shared = a4_ring + kA4Warps * kStages * kStage + warp * kA4Queries<NG, NQ> + lane * 16;
   uint32_t qs[NQ][2];          // (0, sum of group c) in two halves
-  float q8[NQ][NG][2];         // -8 2^-24 times the groups' sums, of queries 2c and 2c + 1
   float o[NQ][2 * NG][4];      // entries 32 g + 4 r + 2 i (0, 1) and the next (2, 3), of queries 2c and 2c + 1
-  float z[NQ][4];              // the middles' part: row r is parameter r of a key
-  float m[NQ][2], l[NQ][2], unit[NQ][2];  // unit: a score of 1 in units of log2
-  int len[NQ][2];              // keys that queries 2c and 2c + 1 see
-  int least = 0;               // that every query of the item sees
+  float z[NQ][2];              // the middles' part: row r is parameter r of a key
+  // of queries 2c and 2c + 1: what a score of 1 is in units of log2, the score that weights refer to, the one past which
+  // they do no longer, the sum of weights, and the keys that they see
+  float unit[NQ][2], m[NQ][2], lim[NQ][2], l[NQ][2];
+  float base[NQ][2];           // 7 less the whole number nearest to m in units of log2
+  int len[NQ][2];
+  int least = 0;               // keys that every query of the item sees
+  int n = 0;                   // queries of the item
   float v_unit = 1.f;          // weights are multiplied by it and the value's scale
   float v_most = 0.f;          // largest value scale that fits it
+  bool far = false;            // m unit is so large that its rounding matters
   bool fresh = true, broken = false;
   int stage = 0;
   const int r = lane >> 2, c = lane & 3;
   while (now.tile < now.end) {
     issue(stage == 0 ? kStages - 1 : stage - 1);
-    look();
+    step();
     asm volatile("cp.async.commit_group;" ::: "memory");
-    const int h = now.hc / a.chunks, first = (now.hc - h * a.chunks) * a.chunk_rows;
-    const int n = min(a.chunk_rows, a.queries - first);
     if (fresh) {
+      const int h = now.hc / a.chunks, first = (now.hc - h * a.chunks) * a.chunk_rows;
+      n = min(a.chunk_rows, a.queries - first);
       least = 0x7FFFFFFF;
 #pragma unroll
       for (int t = 0; t < NQ; ++t) {
         const int g = t * 8 + r;
-        const int token = (first + (g < n ? g : 0)) / a.group, head = h * a.group + (first + (g < n ? g : 0)) - token * a.group;
-        const int64_t at = now.b * x.q_row + token * x.q_token + head * x.q_head + c * 8;
+        const int token = (first + (g < n ? g : 0)) / a.group, q_head = h * a.group + (first + (g < n ? g : 0)) - token * a.group;
+        const int64_t at = now.b * x.q_row + token * x.q_token + q_head * x.q_head + c * 8;
         float most = 0.f;
         float e[NG][8];
 #pragma unroll
@@ -371,47 +433,58 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
             e[k][i] = __half2float(__float2half_rn(e[k][i] * up));
             sum[k] += e[k][i];
           }
+          uint32_t f[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float f = i & 1 ? 0.0625f : 1.f;
-            qf[t][k][i] = a4_pack(e[k][i] * f, e[k][i + 4] * f);
+            const float down4 = i & 1 ? 0.0625f : 1.f;
+            f[i] = a4_pack(e[k][i] * down4, e[k][i + 4] * down4);
           }
           sum[k] += __shfl_xor_sync(0xFFFFFFFFu, sum[k], 1);
           sum[k] += __shfl_xor_sync(0xFFFFFFFFu, sum[k], 2);
+          const float s0 = -0x1p-21f * __shfl_sync(0xFFFFFFFFu, sum[k], 8 * c),
+                      s1 = -0x1p-21f * __shfl_sync(0xFFFFFFFFu, sum[k], 8 * c + 4);
+          if constexpr (kQShared) {
+            *reinterpret_cast<uint4 *>(q_shared + (t * NG + k) * 512) = make_uint4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float2 *>(q_shared - lane * 8 + NQ * NG * 512 + (t * NG + k) * 256) = make_float2(s0, s1);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qf[t][k][i] = f[i];
+            q8[t][k][0] = s0, q8[t][k][1] = s1;
+          }
         }
-        float mine = 0.f;
+        float own = 0.f;
 #pragma unroll
         for (int k = 0; k < NG; ++k)
-          if (c == k) mine = sum[k];
-        const float high = __half2float(__float2half_rn(mine));
+          if (c == k) own = sum[k];
+        const float high = __half2float(__float2half_rn(own));
         qs[t][0] = a4_pack(0.f, high);
-        qs[t][1] = a4_pack(0.f, mine - high);
+        qs[t][1] = a4_pack(0.f, own - high);
         // of the queries that this lane's columns of a product are
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int source = (2 * c + i) * 4;
-#pragma unroll
-          for (int k = 0; k < NG; ++k) q8[t][k][i] = -0x1p-21f * __shfl_sync(0xFFFFFFFFu, sum[k], source);
-          unit[t][i] = fmaxf(a.scale_log2 * __shfl_sync(0xFFFFFFFFu, down, source), 1e-38f);  // 0 times -inf is no number
+          unit[t][i] = fmaxf(a.scale_log2 * __shfl_sync(0xFFFFFFFFu, down, 8 * c + 4 * i), 1e-38f);  // 0 times -inf is no number
           const int g2 = t * 8 + 2 * c + i;
           len[t][i] = g2 < n ? load_in(x.lengths + now.b * x.length_row + (first + g2) / a.group) : 0x7FFFFFFF;
           least = min(least, len[t][i]);
-          m[t][i] = kNone;
-          l[t][i] = 0.f;
+          len[t][i] = min(len[t][i], now.keys);
+          m[t][i] = kA4Least;
+          lim[t][i] = kA4Least;
+          base[t][i] = 0.f;
+          l[t][i] = z[t][i] = 0.f;
         }
 #pragma unroll
         for (int i = 0; i < 2 * NG; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
-        z[t][0] = z[t][1] = z[t][2] = z[t][3] = 0.f;
       }
       least = __reduce_min_sync(0xFFFFFFFFu, least);
       v_unit = 1.f, v_most = 0.f;
+      far = true;  // nothing is referred to yet
       fresh = broken = false;
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     __syncwarp();
     broken |= (met >> (kStages - 1)) & 1;
     const uint32_t kst = ring + stage * kStage;
-    unsigned char *here = a4_ring + (warp * kStages + stage) * kStage;
+    unsigned char *here = mine + stage * kStage;
     // rows of the matrices that ldmatrix takes: keys 0-7 and 8-15 of a group, then of the next
     const uint32_t mat = (uint32_t)((lane & 15) * kPitch + (lane >> 4) * 16);
     float sc[NQ][4];
@@ -436,10 +509,18 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
         const float s0 = a4_low(pr[0][g]) * 0x1p24f, s1 = a4_low(pr[1][g]) * 0x1p24f;
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
+          uint4 b;
+          float2 from;
+          if constexpr (kQShared) {
+            b = *reinterpret_cast<const uint4 *>(q_shared + (t * NG + g) * 512);
+            from = *reinterpret_cast<const float2 *>(q_shared - lane * 8 + NQ * NG * 512 + (t * NG + g) * 256);
+          } else {
+            b = make_uint4(qf[t][g][0], qf[t][g][1], qf[t][g][2], qf[t][g][3]);
+            from = make_float2(q8[t][g][0], q8[t][g][1]);
+          }
           float d[4];
-          a4_mma(d, w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[t][g][0], qf[t][g][1],
-                 q8[t][g][0], q8[t][g][1]);
-          a4_mma(d, w2 & 0x000F000Fu, w3 & 0x000F000Fu, w2 & 0x00F000F0u, w3 & 0x00F000F0u, qf[t][g][2], qf[t][g][3]);
+          a4_mma(d, w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, b.x, b.y, from.x, from.y);
+          a4_mma(d, w2 & 0x000F000Fu, w3 & 0x000F000Fu, w2 & 0x00F000F0u, w3 & 0x00F000F0u, b.z, b.w);
           sc[t][0] = fmaf(s0, d[0], sc[t][0]);
           sc[t][1] = fmaf(s0, d[1], sc[t][1]);
           sc[t][2] = fmaf(s1, d[2], sc[t][2]);
@@ -451,12 +532,12 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
     const bool partial = j0 + kA4Tile > least;  // some query does not see some key
     if (partial) {
 #pragma unroll
-      for (int t = 0; t < NQ; ++t) {
-        if (j0 + r >= min(len[t][0], now.keys)) sc[t][0] = kNone;
-        if (j0 + r >= min(len[t][1], now.keys)) sc[t][1] = kNone;
-        if (j0 + r + 8 >= min(len[t][0], now.keys)) sc[t][2] = kNone;
-        if (j0 + r + 8 >= min(len[t][1], now.keys)) sc[t][3] = kNone;
-      }
+      for (int t = 0; t < NQ; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (j0 + r >= len[t][i]) sc[t][i] = kNone;
+          if (j0 + r + 8 >= len[t][i]) sc[t][2 + i] = kNone;
+        }
     }
     // the values' parameters
     uint32_t vr[2][4];
@@ -478,13 +559,10 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
       if (__any_sync(0xFFFFFFFFu, none[0] | none[1])) {
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (sc[t][0] != kNone) lost[t] |= none[0];
-            if (sc[t][1] != kNone) lost[t] |= none[0] << 8;
-            if (sc[t][2] != kNone) lost[t] |= none[1];
-            if (sc[t][3] != kNone) lost[t] |= none[1] << 8;
-          }
+          if (sc[t][0] != kNone) lost[t] |= none[0];
+          if (sc[t][1] != kNone) lost[t] |= none[0] << 8;
+          if (sc[t][2] != kNone) lost[t] |= none[1];
+          if (sc[t][3] != kNone) lost[t] |= none[1] << 8;
 #pragma unroll
           for (int s = 4; s < 32; s <<= 1) lost[t] |= __shfl_xor_sync(0xFFFFFFFFu, lost[t], s);
         }
@@ -509,8 +587,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
 #pragma unroll
     for (int t = 0; t < NQ; ++t)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        moves = moves || (fmaxf(sc[t][i], sc[t][2 + i]) - m[t][i]) * unit[t][i] > 8.f;
+      for (int i = 0; i < 2; ++i) moves = moves || fmaxf(sc[t][i], sc[t][2 + i]) > lim[t][i];
     if (__any_sync(0xFFFFFFFFu, moves)) {
       if (most > 65504.f) {  // an infinite scale spoils its own group alone
         most = 0.f;
@@ -528,16 +605,32 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
         v_unit = next;
         v_most = __uint_as_float((uint32_t)(127 + e) << 23);
       }
+      float top[NQ][2], whole[NQ][2];
+      bool next_far = false;
 #pragma unroll
       for (int t = 0; t < NQ; ++t) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float top = fmaxf(sc[t][i], sc[t][2 + i]);
+          top[t][i] = fmaxf(sc[t][i], sc[t][2 + i]);
 #pragma unroll
-          for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
-          top = fmaxf(top, m[t][i]);
-          const float f = m[t][i] == top ? 1.f : at_exp2((m[t][i] - top) * unit[t][i]);
-          m[t][i] = top;
+          for (int s = 4; s < 32; s <<= 1) top[t][i] = fmaxf(top[t][i], __shfl_xor_sync(0xFFFFFFFFu, top[t][i], s));
+          top[t][i] = fmaxf(top[t][i], m[t][i]);
+          whole[t][i] = rintf(top[t][i] * unit[t][i]);
+          next_far = next_far || !(fabsf(whole[t][i]) < kAtFar);
+        }
+      }
+      next_far = __any_sync(0xFFFFFFFFu, next_far);
+#pragma unroll
+      for (int t = 0; t < NQ; ++t) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // from what the weights referred to: m unit itself where far, else the whole number nearest to it
+          const float old = 7.f - base[t][i];
+          const float f = at_exp2(far ? (next_far ? (m[t][i] - top[t][i]) * unit[t][i] : fmaf(m[t][i], unit[t][i], -whole[t][i]))
+                                      : (next_far ? fmaf(-top[t][i], unit[t][i], old) : old - whole[t][i]));
+          m[t][i] = top[t][i];
+          lim[t][i] = top[t][i] == kA4Least ? kA4Least : top[t][i] + 8.f / unit[t][i];
+          base[t][i] = 7.f - whole[t][i];
           l[t][i] *= f;
           z[t][i] *= f;
           const float fo = f * v_factor;
@@ -545,28 +638,36 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
           for (int k = 0; k < 2 * NG; ++k) o[t][k][i] *= fo, o[t][k][2 + i] *= fo;
         }
       }
+      far = next_far;
     }
     uint32_t vp[2];
     ldmatrix2t(vp, kst + kVp + (lane & 15) * 16);
     uint32_t pw[NQ][NG][2];  // weights times the groups' scales as B: keys 2c and 2c + 1 of query r, then keys + 8
 #pragma unroll
-    for (int t = 0; t < NQ; ++t) {
-      float w[4];
+    for (int g = 0; g < NG; ++g) vs[0][g] *= v_unit, vs[1][g] *= v_unit;
+    if (far) {  // the difference from m, which is exact near it; the base's rounding would be whole units
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float base = m[t][i] == kNone ? 0.f : m[t][i];  // a score of -inf has weight 0 whatever the maximum
-        w[i] = at_exp2(fmaf(sc[t][i] - base, unit[t][i], 7.f));
-        w[2 + i] = at_exp2(fmaf(sc[t][2 + i] - base, unit[t][i], 7.f));
-        l[t][i] += w[i] + w[2 + i];
-      }
-      a4_mma(z[t], vp[0], 0, vp[1], 0, movmatrix(a4_pack(w[0], w[1])), movmatrix(a4_pack(w[2], w[3])));
+      for (int t = 0; t < NQ; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[t][i] = at_exp2(fmaf(sc[t][i] - m[t][i & 1], unit[t][i & 1], 7.f));
+    } else {
+#pragma unroll
+      for (int t = 0; t < NQ; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[t][i] = at_exp2(fmaf(sc[t][i], unit[t][i & 1], base[t][i & 1]));
+    }
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+      const float(&w)[4] = sc[t];
+      l[t][0] += w[0] + w[2];
+      l[t][1] += w[1] + w[3];
+      a4_mma_top(z[t], vp[0], vp[1], movmatrix(a4_pack(w[0], w[1])), movmatrix(a4_pack(w[2], w[3])));
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const float s0 = vs[0][g] * v_unit, s1 = vs[1][g] * v_unit;
-        pw[t][g][0] = movmatrix(a4_pack(w[0] * s0, w[1] * s0));
-        pw[t][g][1] = movmatrix(a4_pack(w[2] * s1, w[3] * s1));
+        pw[t][g][0] = movmatrix(a4_pack(w[0] * vs[0][g], w[1] * vs[0][g]));
+        pw[t][g][1] = movmatrix(a4_pack(w[2] * vs[1][g], w[3] * vs[1][g]));
       }
-      if (lost[t]) {
+      if (partial && lost[t]) {
         const float nan = __uint_as_float(0x7FFFFFFFu);
         if ((r & 1) && (lost[t] >> (r >> 1)) & 1) z[t][0] = nan;
         if ((r & 1) && (lost[t] >> (8 + (r >> 1))) & 1) z[t][1] = nan;
@@ -590,34 +691,34 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
       }
     }
     __syncwarp();  // the stage is read: the next round's copies may overwrite it
-    if (now.tile + 1 == now.end) {
-      const int64_t piece = now.b * hcs + now.hc + wid;
-      const float low = 0x1p17f / v_unit, high = 0x1p13f / v_unit;  // 2^24 and 2^20 without the weights' 2^7
+    if (++stage == kStages) stage = 0;
+    if (++now.tile < now.end) continue;
+    const int64_t piece = (int64_t)now.b * hcs + now.hc + wid;
+    const float low = 0x1p17f / v_unit, high = 0x1p13f / v_unit;  // 2^24 and 2^20 without the weights' 2^7
 #pragma unroll
-      for (int t = 0; t < NQ; ++t) {
+    for (int t = 0; t < NQ; ++t) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-          for (int s = 4; s < 32; s <<= 1) l[t][i] += __shfl_xor_sync(0xFFFFFFFFu, l[t][i], s);
-          const int g = t * 8 + c * 2 + i;
-          const int64_t rec = piece * a.chunk_rows + g;
-          if (g < n && r == 0)
-            a.own_ml[rec] = make_float2(m[t][i] * unit[t][i], broken ? kAtBadPage : l[t][i] * 0x1p-7f);
+        for (int s = 4; s < 32; s <<= 1) l[t][i] += __shfl_xor_sync(0xFFFFFFFFu, l[t][i], s);
+        const int g = t * 8 + c * 2 + i;
+        const int64_t rec = piece * a.chunk_rows + g;
+        // what the weights refer to, to the last bit: a query that saw no score refers to nothing
+        const float ref = m[t][i] == kA4Least ? kNone : far ? m[t][i] * unit[t][i] : 7.f - base[t][i];
+        if (g < n && r == 0) a.own_ml[rec] = make_float2(ref, broken ? kAtBadPage : l[t][i] * 0x1p-7f);
 #pragma unroll
-          for (int k = 0; k < NG; ++k) {
-            const float middle = __shfl_sync(0xFFFFFFFFu, z[t][i], (2 * k + 1) * 4 + c) * 0x1p-7f;
-            const int d = k * 32 + r * 4;
-            if (g < n && d < x.cache.head_dim)
-              *reinterpret_cast<float4 *>(a.own_o + rec * x.cache.head_dim + d) =
-                  make_float4(fmaf(o[t][2 * k][i], low, middle), fmaf(o[t][2 * k][2 + i], high, middle),
-                              fmaf(o[t][2 * k + 1][i], low, middle), fmaf(o[t][2 * k + 1][2 + i], high, middle));
-          }
+        for (int k = 0; k < NG; ++k) {
+          const float middle = __shfl_sync(0xFFFFFFFFu, z[t][i], (2 * k + 1) * 4 + c) * 0x1p-7f;
+          const int d = k * 32 + r * 4;
+          if (g < n && d < x.cache.head_dim)
+            *reinterpret_cast<float4 *>(a.own_o + rec * x.cache.head_dim + d) =
+                make_float4(fmaf(o[t][2 * k][i], low, middle), fmaf(o[t][2 * k][2 + i], high, middle),
+                            fmaf(o[t][2 * k + 1][i], low, middle), fmaf(o[t][2 * k + 1][2 + i], high, middle));
         }
       }
-      fresh = true;
     }
-    if (++stage == kStages) stage = 0;
-    a4_next(a, now);
+    fresh = true;
+    a4_item_next(a, now);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
