@@ -79,7 +79,7 @@ static cudaError_t a4_split(const A4Args &a, int dev, cudaStream_t s) {
 }
 template <int NG>
 static cudaError_t a4_split_as(const A4Args &a, int eights, int dev, cudaStream_t s) {
-  const bool whole = a.x.cache.page_size % kA4Tile == 0;
+  const bool whole = a.x.cache.page_size % kA4Half == 0;
   if (eights == 1) return whole ? a4_split<NG, 1, true>(a, dev, s) : a4_split<NG, 1, false>(a, dev, s);
   if (eights == 2) return whole ? a4_split<NG, 2, true>(a, dev, s) : a4_split<NG, 2, false>(a, dev, s);
   if constexpr (NG <= 2) {
@@ -142,7 +142,8 @@ int ms_kv4_attention(const ms_kv4_attention_args *args, ms_stream_t stream) {
   for (int i = 0; i < 31; ++i)
     if (x.cache.page_size == 1ll << i) a.page_shift = i;
   {  // records that an output may have: the warps spread over the items, but no more than the longest has room for
-    const int64_t items = x.rows * x.cache.kv_heads * p.chunks, tiles = (x.table_width * x.cache.page_size + ms::kA4Tile - 1) / ms::kA4Tile;
+    a.tile = ms::kA4Half * (p.eights == 1 ? ms::kA4Halves<1> : ms::kA4Halves<2>);
+    const int64_t items = x.rows * x.cache.kv_heads * p.chunks, tiles = (x.table_width * x.cache.page_size + a.tile - 1) / a.tile;
     a.merge_wide = std::min(p.split_warps / items + 1, (tiles + ms::kA4Item) / (ms::kA4Item + 1) + 1) > 24;
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

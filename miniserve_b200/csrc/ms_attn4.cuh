@@ -15,9 +15,9 @@
 namespace ms {
 
 constexpr int kA4Warps = 4;                // warps of a split CTA
-constexpr int kA4Tile = 16;                // keys of a tile: the M of the score products, the K of the output's
+constexpr int kA4Half = 16;                // keys of a product: the M of the scores', the K of the output's
 constexpr int kA4Item = 2;                 // cost of an item's queries and record, in tiles
-constexpr int kA4Stages = 4;               // tiles of a warp's ring
+constexpr int kA4Stages = 3;               // tiles of a warp's ring
 constexpr float kA4Least = -3e38f;         // refers to nothing yet: every score is far above it
 constexpr int64_t kA4MaxRows = 1 << 20;
 constexpr int kA4MaxTokens = 1024;         // of a row
@@ -25,16 +25,20 @@ constexpr int kA4MaxTokens = 1024;         // of a row
 // rows of 16 bytes lie in different banks.
 template <int NG>
 constexpr int kA4Pitch = NG <= 3 ? 48 : 80;
-template <int NG>
-constexpr int kA4Stage = 2 * kA4Tile * kA4Pitch<NG> + 2 * kA4Tile * 16;  // K and V codes, K and V parameters
+// Products of a tile: a tile of 32 keys pays for its copies, page and checks
+// once, where registers have room for its scores.
+template <int NQ>
+constexpr int kA4Halves = NQ <= 1 ? 2 : 1;
+template <int NG, int NQ>
+constexpr int kA4Stage = kA4Halves<NQ> * kA4Half * 2 * (kA4Pitch<NG> + 16);  // K and V codes, K and V parameters
 // Queries of more than four fragments a lane stay in shared memory: registers
 // are for the output's.
 template <int NG, int NQ>
 constexpr bool kA4QShared = NG * NQ > 4;
 template <int NG, int NQ>
-constexpr int kA4Queries = kA4QShared<NG, NQ> ? NG * NQ * 32 * 24 : 0;  // bytes of a warp's
+constexpr int kA4Queries = kA4QShared<NG, NQ> ? NG * NQ * 512 : 0;  // bytes of a warp's
 template <int NG, int NQ>
-constexpr int kA4Shared = kA4Warps * (kA4Stages * kA4Stage<NG> + kA4Queries<NG, NQ>);
+constexpr int kA4Shared = kA4Warps * (kA4Stages * kA4Stage<NG, NQ> + kA4Queries<NG, NQ>);
 // Split CTAs of an SM, by what their registers allow.
 template <int NG, int NQ>
 constexpr int kA4Ctas = NG <= 2 ? (NQ <= 1 ? 4 : NQ <= 3 ? 3 : 2) : (NQ <= 1 ? 3 : 2);
@@ -61,6 +65,7 @@ struct A4Args {
   int q_wide;      // q's heads start 16-byte aligned
   int page_shift;  // log2 of the page size, or -1
   int merge_wide;  // the merge gives each output a CTA
+  int tile;        // keys of the split kernel's tiles
 };
 
 // Keys of a row: its tokens' largest length; 0 where one of them does not fit
@@ -75,9 +80,7 @@ __device__ __forceinline__ int a4_keys(const ms_kv4_attention_args &x, int64_t b
   }
   return bad ? 0 : most;
 }
-__device__ __forceinline__ int64_t a4_units(int keys) {
-  return keys > 0 ? (keys + kA4Tile - 1) / kA4Tile + kA4Item : 0;
-}
+__device__ __forceinline__ int64_t a4_units(int keys, int tile) { return keys > 0 ? (keys + tile - 1) / tile + kA4Item : 0; }
 
 // Walks over a warp's tiles: the split kernel's sequence is rows' items (key
 // head and chunk) in order, each of kA4Item units and one unit a tile.  A warp's
@@ -86,8 +89,8 @@ struct A4Walk {
   int b, left;  // left: units of the share past this item
   int hc, tile, end, keys;
 };
-__device__ __forceinline__ int a4_tiles(int keys) { return (keys + kA4Tile - 1) / kA4Tile; }
 // The next item's tiles within the share; tile == end where none are left.
+template <int kTile>
 __device__ __forceinline__ void a4_item_next(const A4Args &a, A4Walk &w) {
   w.tile = w.end = 0;
   if (w.left <= kA4Item) return;
@@ -98,7 +101,7 @@ __device__ __forceinline__ void a4_item_next(const A4Args &a, A4Walk &w) {
       w.keys = a4_keys(a.x, ++w.b, bad);
     } while (w.keys == 0);
   }
-  const int take = min(w.left, a4_tiles(w.keys) + kA4Item);
+  const int take = min(w.left, (w.keys + kTile - 1) / kTile + kA4Item);
   w.left -= take;
   w.end = take - kA4Item;
 }
@@ -132,12 +135,11 @@ __device__ __forceinline__ void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
 }
 // The upper eight rows of the product, of an A whose lower ones are zero.
 __device__ __forceinline__ void a4_mma_top(float (&d)[2], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
-  float none0, none1;
+  [[maybe_unused]] float none0, none1;
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
       : "+f"(d[0]), "+f"(d[1]), "=f"(none0), "=f"(none1)
       : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
-  (void)none0, (void)none1;
 }
 __device__ __forceinline__ uint32_t a4_pack(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
@@ -147,7 +149,7 @@ __device__ __forceinline__ float a4_low(uint32_t u) { return __low2float(*reinte
 
 // Split kernel.  All rows' items form one sequence; every warp takes an equal,
 // contiguous share of it, whatever the rows' lengths, and works alone: a ring
-// of tiles of 16 keys filled with asynchronous copies of the codes and
+// of tiles of 32 or 16 keys filled with asynchronous copies of the codes and
 // parameters as they lie in the cache, a page lookup a tile ahead of its
 // copies, and products of m16n8k16 with the keys (S^T = K Q^T) and the values
 // (O^T += V^T P^T) as A.  Where its share meets an item's tiles, it leaves one
@@ -159,18 +161,17 @@ __device__ __forceinline__ float a4_low(uint32_t u) { return __low2float(*reinte
 // exact (subnormal), so that one AND makes two operands.  What a word's other
 // nibbles need is one shift.  With scale s_g and middle z_g of group g:
 //
-//   q . k = sum_g s_g (q_g . c_g - 8 sum q_g) + sum_g z_g sum q_g
+//   q . k = sum_g s_g (q_g . c_g) + sum_g (z_g - 8 s_g) sum q_g
 //   o     = sum_j (p_j s_jg) (c_j - 8) + sum_j p_j z_jg
 //
-// K: the -8 sum q_g is the product's C operand; s_g weighs a group's sums in
-// fp32; the middles' sum is one more product, of the parameters as they lie
-// with the queries' sums in two fp16 halves.  V: p s_g is rounded to fp16 once,
+// K: s_g weighs a group's sums in fp32; the rest is one more product, of the
+// parameters as they lie with the queries' sums in two fp16 halves.  V: p s_g is rounded to fp16 once,
 // -8 times the same rounded weights is one more product with constants, so
 // that a weight's rounding meets c - 8 and not c; the middles are one product
 // with p.
 //
 // Queries enter as fp16, scaled by a power of two that puts a row's largest in
-// [2^9, 2^10): entries down to 2^-23 of it are exact.  Weights are at most 2^8
+// [2^5, 2^6): entries are off by 2^-26 of it at most.  Weights are at most 2^8
 // of what they refer to (it moves only when a score passes it by 2^8), scaled up
 // by 2^7 (and up to 2^0.5: references are whole numbers), and by the power of two
 // below 1 over the largest value scale met, so that fp16 holds them with 2^-21
@@ -179,7 +180,8 @@ template <int NG, int NQ, bool kWhole>
 __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
     ms_attn4_split_kernel(const __grid_constant__ A4Args a) {
   constexpr int kThreads = kA4Warps * 32;
-  constexpr int kPitch = kA4Pitch<NG>, kStage = kA4Stage<NG>, kStages = kA4Stages;
+  constexpr int kPitch = kA4Pitch<NG>, kStage = kA4Stage<NG, NQ>, kStages = kA4Stages;
+  constexpr int kHalves = kA4Halves<NQ>, kTile = kHalves * kA4Half;
   constexpr int kRow = NG <= 2 ? 32 : NG * 16;  // bytes of a token's codes in the cache
   constexpr int kPieces = kRow / 16;            // 16-byte pieces of them
   constexpr int kPairs = NG <= 2 ? 2 : 4;       // pairs of parameters in the cache
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
   bool bad;
   {
     int64_t n = 0;
-    for (int64_t b = r0; b < r1; ++b) n += a4_units(a4_keys(x, b, bad));
+    for (int64_t b = r0; b < r1; ++b) n += a4_units(a4_keys(x, b, bad), kTile);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t v = __shfl_up_sync(0xFFFFFFFFu, n, o);
@@ -221,7 +223,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
       a.base[b] = n * hcs;
       const int keys = a4_keys(x, b, bad);
       x.status[b] = bad ? MS_ROW_BAD_LENGTH : MS_ROW_OK;
-      n += a4_units(keys);
+      n += a4_units(keys, kTile);
     }
     if (tid == 0) a.header->share = share;
   }
@@ -239,118 +241,121 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
     load.b = (int)min(rows, lo * run);
     int64_t first = sums[lo] * hcs;
     load.keys = a4_keys(x, load.b, bad);
-    while (first + a4_units(load.keys) * hcs <= u0) {
-      first += a4_units(load.keys) * hcs;
+    while (first + a4_units(load.keys, kTile) * hcs <= u0) {
+      first += a4_units(load.keys, kTile) * hcs;
       load.keys = a4_keys(x, ++load.b, bad);
     }
-    const int64_t units = a4_units(load.keys);
+    const int64_t units = a4_units(load.keys, kTile);
     load.hc = (int)((u0 - first) / units);
     const int64_t at = u0 - first - load.hc * units, take = min(u1 - u0, units - at);
     load.left = (int)(u1 - u0 - take);
     load.tile = (int)max((int64_t)0, at - kA4Item);
     load.end = (int)(at + take) - kA4Item;
-    if (load.end <= load.tile) a4_item_next(a, load);
+    if (load.end <= load.tile) a4_item_next<kTile>(a, load);
   }
   A4Walk now = load;
   unsigned char *mine = a4_ring + warp * kStages * kStage;
   const uint32_t ring = smem_addr(mine);
-  constexpr int kV = kA4Tile * kPitch, kKp = 2 * kV, kVp = kKp + kA4Tile * 16;  // of a stage
+  constexpr int kV = kTile * kPitch, kKp = 2 * kV, kVp = kKp + kTile * 16;  // of a stage
   if (kPairs == 2) {  // the parameters' rows are 16 bytes there too: what lies behind the two pairs stays zero
     for (int s = 0; s < kStages; ++s)
-      *reinterpret_cast<uint4 *>(mine + s * kStage + kKp + lane * 16) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < kHalves; ++i)
+        *reinterpret_cast<uint4 *>(mine + s * kStage + kKp + (i * 32 + lane) * 16) = make_uint4(0, 0, 0, 0);
     __syncwarp();
   }
   const int page_size = (int)x.cache.page_size;
 
-  // Copies.  Where tiles lie in one page each, a lane's places in the cache are
-  // stepped along the page; a new page's id is loaded a tile ahead of its use.
-  // Else lanes 0-15 (and 16-31 again) look up the tile's keys.
-  int page = -1;         // loaded, of the next tile (or the lane's key of it)
-  int fresh_page = 1;    // it is a new page, or every tile's keys are looked up
-  int offset = 0;        // in it
-  int room = 0;          // tokens of the page from the next tile on
-  int head = 0;          // of the next tile
-  int live_keys = 0;     // of the next tile; 0 where none is left
-  int64_t code_at = 0, param_at = 0;  // the lane's, of the tile copied last
-  bool good = false;     // its page is one
-  uint32_t met = 0;      // bit i: the tile issued i tiles ago met a bad page
-  auto look = [&](bool item) {  // at tile load.tile, the first of an item's or the one after the last
+  // Copies.  Where a half's keys lie in one page, it is looked up once for all lanes; else lanes 0-15 (and 16-31 again)
+  // look up the half's keys.  Page ids are loaded a tile ahead of their use.
+  int page[kHalves], offset[kHalves];
+  int head = 0;       // of the next tile
+  int live_keys = 0;  // of the next tile; 0 where none is left
+  uint32_t met = 0;   // bit i: the tile issued i tiles ago met a bad page
+  auto look = [&](bool item) {  // at tile load.tile, the first of an item's or not
     live_keys = 0;
     if (load.tile >= load.end) return;
     if (item) head = load.hc / a.chunks;
-    live_keys = load.keys - load.tile * kA4Tile;
-    if (kWhole) {
-      room -= kA4Tile;
-      fresh_page = item || room <= 0;
-      if (fresh_page) {
-        const int j = load.tile * kA4Tile, p = a.page_shift >= 0 ? j >> a.page_shift : j / page_size;
-        offset = j - p * page_size;
-        room = page_size - offset;
-        page = load_in(x.table + load.b * x.table_row + p);
-      }
-    } else {
-      const int j = load.tile * kA4Tile + (lane & 15);
-      page = 0, offset = 0;
+    live_keys = load.keys - load.tile * kTile;
+#pragma unroll
+    for (int i = 0; i < kHalves; ++i) {
+      const int j = load.tile * kTile + i * kA4Half + (kWhole ? 0 : lane & 15);
+      page[i] = offset[i] = 0;
       if (j < load.keys) {
         const int p = a.page_shift >= 0 ? j >> a.page_shift : j / page_size;
-        offset = j - p * page_size;
-        page = load_in(x.table + load.b * x.table_row + p);
+        offset[i] = j - p * page_size;
+        page[i] = load_in(x.table + load.b * x.table_row + p);
       }
     }
   };
   auto step = [&]() {
     if (load.tile >= load.end) return;  // none is left
-    bool item = ++load.tile >= load.end;
-    if (item) a4_item_next(a, load);
+    const bool item = ++load.tile >= load.end;
+    if (item) a4_item_next<kTile>(a, load);
     look(item);
   };
-  constexpr int kCopies = (kA4Tile * kPieces + 31) / 32;  // of a tile's codes of the keys
+  constexpr int kCopies = (kTile * kPieces + 31) / 32;  // of a tile's codes of the keys, and of the values
   auto issue = [&](int stage) {
     const uint32_t dst = ring + stage * kStage;
-    if (kWhole) {
-      if (fresh_page) {
-        good = page >= 0 && page < x.cache.pages;
-        const int64_t row = ((int64_t)page * x.cache.kv_heads + head) * page_size + offset;
-        code_at = good ? row * kRow + lane * 16 : 0;
-        param_at = good ? (row + (lane & 15)) * (kPairs * 4) : 0;
-      } else if (good) {
-        code_at += kA4Tile * kRow;
-        param_at += kA4Tile * kPairs * 4;
-      }
-      met = (met << 1) | (live_keys > 0 && !good);
-      const unsigned char *ks = x.cache.k_codes + code_at, *vs = x.cache.v_codes + code_at;
-      const char *ps = static_cast<const char *>(lane < 16 ? x.cache.k_params : x.cache.v_params) + param_at;
-      const int rows_here = good ? live_keys : 0;
+    int64_t row[kHalves];  // of the codes and parameters of a half's first key, or of the lane's; -1: none
+    bool wrong = false;
+#pragma unroll
+    for (int i = 0; i < kHalves; ++i) {
+      const bool live = i * kA4Half + (kWhole ? 0 : lane & 15) < live_keys, good = page[i] >= 0 && page[i] < x.cache.pages;
+      wrong = wrong || (live && !good);
+      row[i] = live && good ? ((int64_t)page[i] * x.cache.kv_heads + head) * page_size + offset[i] : -1;
+    }
+    met = (met << 1) | (kWhole ? wrong : __any_sync(0xFFFFFFFFu, wrong));
+    if (kWhole && live_keys >= kTile && !wrong) {  // all of the tile
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
-        const int at = i * 32 + lane, r = at / kPieces, piece = at - r * kPieces;
-        const bool live = rows_here >= kA4Tile || r < rows_here;
-        if (kA4Tile * kPieces % 32 == 0 || r < kA4Tile) {
-          copy16(dst + r * kPitch + piece * 16, live ? ks + i * 512 : x.cache.k_codes, live);
-          copy16(dst + kV + r * kPitch + piece * 16, live ? vs + i * 512 : x.cache.v_codes, live);
+        const int at = i * 32 + lane, r = at / kPieces, half = kPieces == 3 ? r >> 4 : i * 32 / kPieces / kA4Half;
+        const int64_t off = row[kHalves == 1 ? 0 : half] * kRow + (at - half * kA4Half * kPieces) * 16;
+        if (kTile * kPieces % 32 == 0 || r < kTile) {
+          copy16(dst + r * kPitch + (at - r * kPieces) * 16, x.cache.k_codes + off, true);
+          copy16(dst + kV + r * kPitch + (at - r * kPieces) * 16, x.cache.v_codes + off, true);
         }
       }
-      const bool live = (lane & 15) < rows_here;
-      if (kPairs == 4) copy16(dst + kKp + lane * 16, live ? ps : x.cache.k_params, live);
-      else copy8(dst + kKp + lane * 16, live ? ps : x.cache.k_params, live);
-    } else {
-      const bool mine_live = (lane & 15) < live_keys, fine = page >= 0 && page < x.cache.pages;
-      met = (met << 1) | __any_sync(0xFFFFFFFFu, mine_live && !fine);
-      const int64_t row = mine_live && fine ? ((int64_t)page * x.cache.kv_heads + head) * page_size + offset : -1;
+      const int64_t off = ((kHalves > 1 && lane >= 16 ? row[kHalves - 1] : row[0]) + (lane & 15)) * (kPairs * 4);
+      const char *ks = static_cast<const char *>(x.cache.k_params) + off, *vs = static_cast<const char *>(x.cache.v_params) + off;
+      if (kHalves == 1) {
+        if (kPairs == 4) copy16(dst + kKp + lane * 16, lane < 16 ? ks : vs, true);
+        else copy8(dst + kKp + lane * 16, lane < 16 ? ks : vs, true);
+      } else if (kPairs == 4) {
+        copy16(dst + kKp + lane * 16, ks, true);
+        copy16(dst + kVp + lane * 16, vs, true);
+      } else {
+        copy8(dst + kKp + lane * 16, ks, true);
+        copy8(dst + kVp + lane * 16, vs, true);
+      }
+      return;
+    }
+    // the row of key r of the tile, or -1
+    auto row_of = [&](int r) {
+      int64_t at = -1;
 #pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        const int at = i * 32 + lane, r = at / kPieces, piece = at - r * kPieces;
-        const int64_t from = __shfl_sync(0xFFFFFFFFu, row, r & 15);
-        const bool live = from >= 0 && r < kA4Tile;
-        const int64_t off = live ? from * kRow + piece * 16 : 0;
-        if (kA4Tile * kPieces % 32 == 0 || r < kA4Tile) {
-          copy16(dst + r * kPitch + piece * 16, x.cache.k_codes + off, live);
-          copy16(dst + kV + r * kPitch + piece * 16, x.cache.v_codes + off, live);
-        }
+      for (int i = 0; i < kHalves; ++i) {
+        const int64_t from = kWhole ? (row[i] >= 0 ? row[i] + (r & 15) : -1) : __shfl_sync(0xFFFFFFFFu, row[i], r & 15);
+        if (r >> 4 == i) at = from;
       }
-      const char *src = static_cast<const char *>(lane < 16 ? x.cache.k_params : x.cache.v_params) + (row >= 0 ? row * (kPairs * 4) : 0);
-      if (kPairs == 4) copy16(dst + kKp + lane * 16, src, row >= 0);
-      else copy8(dst + kKp + lane * 16, src, row >= 0);
+      return r < live_keys ? at : -1;
+    };
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int at = i * 32 + lane, r = at / kPieces, piece = at - r * kPieces;
+      const int64_t from = row_of(r), off = from >= 0 ? from * kRow + piece * 16 : 0;
+      if (kTile * kPieces % 32 == 0 || r < kTile) {
+        copy16(dst + r * kPitch + piece * 16, x.cache.k_codes + off, from >= 0);
+        copy16(dst + kV + r * kPitch + piece * 16, x.cache.v_codes + off, from >= 0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kHalves; ++i) {
+      const int64_t from = row_of(kHalves == 1 ? lane & 15 : lane), off = from >= 0 ? from * (kPairs * 4) : 0;
+      const bool key = kHalves == 1 ? lane < 16 : i == 0;
+      const char *src = static_cast<const char *>(key ? x.cache.k_params : x.cache.v_params) + off;
+      if (kPairs == 4) copy16(dst + kKp + (i * 32 + lane) * 16, src, from >= 0);
+      else copy8(dst + kKp + (i * 32 + lane) * 16, src, from >= 0);
     }
   };
 
@@ -361,13 +366,11 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
     step();
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  // Queries as B: pairs of entries (8c, 8c + 4), (8c + 1, 8c + 5) 2^-4, ... of a group, and -8 2^-24 times the groups'
-  // sums of queries 2c and 2c + 1.
+  // Queries as B: pairs of entries (8c, 8c + 4), (8c + 1, 8c + 5) 2^-4, ... of a group.
   constexpr bool kQShared = kA4QShared<NG, NQ>;
   uint32_t qf[kQShared ? 1 : NQ][NG][4];
-  float q8[kQShared ? 1 : NQ][NG][2];
   unsigned char *q_shared = a4_ring + kA4Warps * kStages * kStage + warp * kA4Queries<NG, NQ> + lane * 16;
-  uint32_t qs[NQ][2];          // (0, sum of group c) in two halves
+  uint32_t qs[NQ][2];          // (-8 times, once) the sum of group c, in two halves
   float o[NQ][2 * NG][4];      // entries 32 g + 4 r + 2 i (0, 1) and the next (2, 3), of queries 2c and 2c + 1
   float z[NQ][2];              // the middles' part: row r is parameter r of a key
   // of queries 2c and 2c + 1: what a score of 1 is in units of log2, the score that weights refer to, the one past which
@@ -383,6 +386,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
   bool fresh = true, broken = false;
   int stage = 0;
   const int r = lane >> 2, c = lane & 3;
+  const bool scale_lane = (r & 1) == 0 && r < 2 * NG;  // its rows of the parameters are scales
   while (now.tile < now.end) {
     issue(stage == 0 ? kStages - 1 : stage - 1);
     step();
@@ -421,8 +425,8 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
         }
         most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
-        // 2^(9 - floor(log2 most)), as long as it and 1 over it are normal numbers
-        const int power = most > 0.f ? min(126, 9 + 127 - (int)(__float_as_uint(most) >> 23)) : 0;
+        // 2^(5 - floor(log2 most)), as long as it and 1 over it are normal numbers
+        const int power = most > 0.f ? min(126, 5 + 127 - (int)(__float_as_uint(most) >> 23)) : 0;
         const float up = __uint_as_float((uint32_t)(power + 127) << 23), down = __uint_as_float((uint32_t)(127 - power) << 23);
         float sum[NG];
 #pragma unroll
@@ -441,15 +445,11 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
           }
           sum[k] += __shfl_xor_sync(0xFFFFFFFFu, sum[k], 1);
           sum[k] += __shfl_xor_sync(0xFFFFFFFFu, sum[k], 2);
-          const float s0 = -0x1p-21f * __shfl_sync(0xFFFFFFFFu, sum[k], 8 * c),
-                      s1 = -0x1p-21f * __shfl_sync(0xFFFFFFFFu, sum[k], 8 * c + 4);
           if constexpr (kQShared) {
             *reinterpret_cast<uint4 *>(q_shared + (t * NG + k) * 512) = make_uint4(f[0], f[1], f[2], f[3]);
-            *reinterpret_cast<float2 *>(q_shared - lane * 8 + NQ * NG * 512 + (t * NG + k) * 256) = make_float2(s0, s1);
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) qf[t][k][i] = f[i];
-            q8[t][k][0] = s0, q8[t][k][1] = s1;
           }
         }
         float own = 0.f;
@@ -457,12 +457,14 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
         for (int k = 0; k < NG; ++k)
           if (c == k) own = sum[k];
         const float high = __half2float(__float2half_rn(own));
-        qs[t][0] = a4_pack(0.f, high);
-        qs[t][1] = a4_pack(0.f, own - high);
+        qs[t][0] = a4_pack(-8.f * high, high);
+        qs[t][1] = a4_pack(-8.f * (own - high), own - high);
         // of the queries that this lane's columns of a product are
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          unit[t][i] = fmaxf(a.scale_log2 * __shfl_sync(0xFFFFFFFFu, down, 8 * c + 4 * i), 1e-38f);  // 0 times -inf is no number
+          // neither 0 nor infinite: 0 times -inf is no number
+          unit[t][i] = a.scale_log2 * (NQ == 1 ? 0x1p24f : 1.f) * __shfl_sync(0xFFFFFFFFu, down, 8 * c + 4 * i);
+          unit[t][i] = fminf(fmaxf(unit[t][i], 1e-38f), 1e38f);
           const int g2 = t * 8 + 2 * c + i;
           len[t][i] = g2 < n ? load_in(x.lengths + now.b * x.length_row + (first + g2) / a.group) : 0x7FFFFFFF;
           least = min(least, len[t][i]);
@@ -485,84 +487,86 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
     broken |= (met >> (kStages - 1)) & 1;
     const uint32_t kst = ring + stage * kStage;
     unsigned char *here = mine + stage * kStage;
-    // rows of the matrices that ldmatrix takes: keys 0-7 and 8-15 of a group, then of the next
+    // rows of the matrices that ldmatrix takes: keys 0-7 and 8-15 of a half and group, then of the next group
     const uint32_t mat = (uint32_t)((lane & 15) * kPitch + (lane >> 4) * 16);
-    float sc[NQ][4];
-    {
+    float sc[kHalves][NQ][4];
+#pragma unroll
+    for (int hf = 0; hf < kHalves; ++hf) {
+      const uint32_t kcodes = kst + hf * kA4Half * kPitch + mat;
+      const unsigned char *params = here + kKp + hf * kA4Half * 16;
       uint32_t p[2];
-      ldmatrix2(p, kst + kKp + (lane & 15) * 16);
+      ldmatrix2(p, kst + kKp + (hf * kA4Half + (lane & 15)) * 16);
       if (NG == 1 || NG == 3)
         if (c >= NG) p[0] = p[1] = 0;
       uint32_t pr[2][4];  // (scale, middle) of the groups of keys r and r + 8
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (kPairs == 4) *reinterpret_cast<uint4 *>(pr[i]) = *reinterpret_cast<const uint4 *>(here + kKp + (r + 8 * i) * 16);
-        else *reinterpret_cast<uint2 *>(pr[i]) = *reinterpret_cast<const uint2 *>(here + kKp + (r + 8 * i) * 16);
+        if (kPairs == 4) *reinterpret_cast<uint4 *>(pr[i]) = *reinterpret_cast<const uint4 *>(params + (r + 8 * i) * 16);
+        else *reinterpret_cast<uint2 *>(pr[i]) = *reinterpret_cast<const uint2 *>(params + (r + 8 * i) * 16);
       }
 #pragma unroll
-      for (int t = 0; t < NQ; ++t) a4_mma(sc[t], p[0], p[1], p[0], p[1], qs[t][0], qs[t][1], 0.f, 0.f);
+      for (int t = 0; t < NQ; ++t) {
+        a4_mma(sc[hf][t], p[0], p[1], p[0], p[1], qs[t][0], qs[t][1], 0.f, 0.f);
+        if (NQ == 1) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[hf][t][i] *= 0x1p-24f;  // or the scales by 2^24: fewer of these
+        }
+      }
       uint32_t f[4];
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        if ((g & 1) == 0) ldmatrix4(f, kst + mat + g * 16);
+        if ((g & 1) == 0) ldmatrix4(f, kcodes + g * 16);
         const uint32_t w0 = f[2 * (g & 1)], w1 = f[2 * (g & 1) + 1], w2 = w0 >> 8, w3 = w1 >> 8;
-        const float s0 = a4_low(pr[0][g]) * 0x1p24f, s1 = a4_low(pr[1][g]) * 0x1p24f;
+        const float s0 = a4_low(pr[0][g]) * (NQ == 1 ? 1.f : 0x1p24f), s1 = a4_low(pr[1][g]) * (NQ == 1 ? 1.f : 0x1p24f);
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
           uint4 b;
-          float2 from;
-          if constexpr (kQShared) {
-            b = *reinterpret_cast<const uint4 *>(q_shared + (t * NG + g) * 512);
-            from = *reinterpret_cast<const float2 *>(q_shared - lane * 8 + NQ * NG * 512 + (t * NG + g) * 256);
-          } else {
-            b = make_uint4(qf[t][g][0], qf[t][g][1], qf[t][g][2], qf[t][g][3]);
-            from = make_float2(q8[t][g][0], q8[t][g][1]);
-          }
+          if constexpr (kQShared) b = *reinterpret_cast<const uint4 *>(q_shared + (t * NG + g) * 512);
+          else b = make_uint4(qf[t][g][0], qf[t][g][1], qf[t][g][2], qf[t][g][3]);
           float d[4];
-          a4_mma(d, w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, b.x, b.y, from.x, from.y);
+          a4_mma(d, w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, b.x, b.y, 0.f, 0.f);
           a4_mma(d, w2 & 0x000F000Fu, w3 & 0x000F000Fu, w2 & 0x00F000F0u, w3 & 0x00F000F0u, b.z, b.w);
-          sc[t][0] = fmaf(s0, d[0], sc[t][0]);
-          sc[t][1] = fmaf(s0, d[1], sc[t][1]);
-          sc[t][2] = fmaf(s1, d[2], sc[t][2]);
-          sc[t][3] = fmaf(s1, d[3], sc[t][3]);
+          sc[hf][t][0] = fmaf(s0, d[0], sc[hf][t][0]);
+          sc[hf][t][1] = fmaf(s0, d[1], sc[hf][t][1]);
+          sc[hf][t][2] = fmaf(s1, d[2], sc[hf][t][2]);
+          sc[hf][t][3] = fmaf(s1, d[3], sc[hf][t][3]);
         }
       }
     }
-    const int j0 = now.tile * kA4Tile;
-    const bool partial = j0 + kA4Tile > least;  // some query does not see some key
+    const int j0 = now.tile * kTile;
+    const bool partial = j0 + kTile > least;  // some query does not see some key
     if (partial) {
 #pragma unroll
-      for (int t = 0; t < NQ; ++t)
+      for (int hf = 0; hf < kHalves; ++hf)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (j0 + r >= len[t][i]) sc[t][i] = kNone;
-          if (j0 + r + 8 >= len[t][i]) sc[t][2 + i] = kNone;
-        }
-    }
-    // the values' parameters
-    uint32_t vr[2][4];
+        for (int t = 0; t < NQ; ++t)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (kPairs == 4) *reinterpret_cast<uint4 *>(vr[i]) = *reinterpret_cast<const uint4 *>(here + kVp + (r + 8 * i) * 16);
-      else *reinterpret_cast<uint2 *>(vr[i]) = *reinterpret_cast<const uint2 *>(here + kVp + (r + 8 * i) * 16);
+          for (int i = 0; i < 2; ++i) {
+            if (j0 + hf * kA4Half + r >= len[t][i]) sc[hf][t][i] = kNone;
+            if (j0 + hf * kA4Half + r + 8 >= len[t][i]) sc[hf][t][2 + i] = kNone;
+          }
     }
     // A masked key's weight of 0 must not meet a middle that is no number: it is taken out of the products, and put
     // back for the queries that see the key.
     uint32_t lost[NQ] = {};  // bits g, 8 + g: queries 2c and 2c + 1 see a key whose group g is no number
     if (partial) {
-      uint32_t none[2] = {0, 0};
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int hf = 0; hf < kHalves; ++hf) {
+        uint32_t none[2] = {0, 0};
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
-          if ((vr[i][g] & 0x7C00u) == 0x7C00u || (vr[i][g] & 0x7C000000u) == 0x7C000000u) none[i] |= 1u << g;
-      if (__any_sync(0xFFFFFFFFu, none[0] | none[1])) {
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const uint32_t u = *reinterpret_cast<const uint32_t *>(here + kVp + (hf * kA4Half + r + 8 * i) * 16 + g * 4);
+            if ((u & 0x7C00u) == 0x7C00u || (u & 0x7C000000u) == 0x7C000000u) none[i] |= 1u << g;
+          }
+        if (!__any_sync(0xFFFFFFFFu, none[0] | none[1])) continue;
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
-          if (sc[t][0] != kNone) lost[t] |= none[0];
-          if (sc[t][1] != kNone) lost[t] |= none[0] << 8;
-          if (sc[t][2] != kNone) lost[t] |= none[1];
-          if (sc[t][3] != kNone) lost[t] |= none[1] << 8;
+          if (sc[hf][t][0] != kNone) lost[t] |= none[0];
+          if (sc[hf][t][1] != kNone) lost[t] |= none[0] << 8;
+          if (sc[hf][t][2] != kNone) lost[t] |= none[1];
+          if (sc[hf][t][3] != kNone) lost[t] |= none[1] << 8;
 #pragma unroll
           for (int s = 4; s < 32; s <<= 1) lost[t] |= __shfl_xor_sync(0xFFFFFFFFu, lost[t], s);
         }
@@ -570,36 +574,41 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int g = 0; g < NG; ++g)
-            if (none[i] & (1u << g)) {
-              vr[i][g] = 0;
-              *reinterpret_cast<uint32_t *>(here + kVp + (r + 8 * i) * 16 + g * 4) = 0;
-            }
+            if (none[i] & (1u << g)) *reinterpret_cast<uint32_t *>(here + kVp + (hf * kA4Half + r + 8 * i) * 16 + g * 4) = 0;
         __syncwarp();
       }
     }
-    float vs[2][NG], most = 0.f;
+    // the values' parameters as A: row r is parameter r (an even one is a scale), of keys 2c and 2c + 1, and 8 on
+    uint32_t vp[kHalves][2];
+    __half2 most = __float2half2_rn(0.f);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      vs[0][g] = a4_low(vr[0][g]), vs[1][g] = a4_low(vr[1][g]);
-      most = fmaxf(most, fmaxf(vs[0][g], vs[1][g]));
+    for (int hf = 0; hf < kHalves; ++hf) {
+      ldmatrix2t(vp[hf], kst + kVp + (hf * kA4Half + (lane & 15)) * 16);
+      most = __hmax2(most, __hmax2(*reinterpret_cast<__half2 *>(&vp[hf][0]), *reinterpret_cast<__half2 *>(&vp[hf][1])));
     }
-    bool moves = most > v_most;
+    bool moves = scale_lane && (__low2float(most) > v_most || __high2float(most) > v_most);
 #pragma unroll
     for (int t = 0; t < NQ; ++t)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) moves = moves || fmaxf(sc[t][i], sc[t][2 + i]) > lim[t][i];
-    if (__any_sync(0xFFFFFFFFu, moves)) {
-      if (most > 65504.f) {  // an infinite scale spoils its own group alone
-        most = 0.f;
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-          most = fmaxf(most, fmaxf(vs[0][g] <= 65504.f ? vs[0][g] : 0.f, vs[1][g] <= 65504.f ? vs[1][g] : 0.f));
+      for (int i = 0; i < 2; ++i) {
+        float high = fmaxf(sc[0][t][i], sc[0][t][2 + i]);
+        if (kHalves > 1) high = fmaxf(high, fmaxf(sc[kHalves - 1][t][i], sc[kHalves - 1][t][2 + i]));
+        moves = moves || high > lim[t][i];
       }
+    if (__any_sync(0xFFFFFFFFu, moves)) {
+      float largest = 0.f;  // value scale; an infinite one spoils its own group alone
 #pragma unroll
-      for (int s = 1; s < 32; s <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, s));
+      for (int hf = 0; hf < kHalves; ++hf)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 f = __half22float2(*reinterpret_cast<__half2 *>(&vp[hf][i]));
+          if (scale_lane) largest = fmaxf(largest, fmaxf(f.x <= 65504.f ? f.x : 0.f, f.y <= 65504.f ? f.y : 0.f));
+        }
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, s));
       float v_factor = 1.f;
-      if (most > v_most) {  // 2^-(floor(log2 most) + 1)
-        const int e = (int)(__float_as_uint(most) >> 23) - 126;
+      if (largest > v_most) {  // 2^-(floor(log2 largest) + 1)
+        const int e = (int)(__float_as_uint(largest) >> 23) - 126;
         const float next = __uint_as_float((uint32_t)(127 - e) << 23);
         v_factor = next / v_unit;
         v_unit = next;
@@ -611,7 +620,8 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
       for (int t = 0; t < NQ; ++t) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          top[t][i] = fmaxf(sc[t][i], sc[t][2 + i]);
+          top[t][i] = fmaxf(sc[0][t][i], sc[0][t][2 + i]);
+          if (kHalves > 1) top[t][i] = fmaxf(top[t][i], fmaxf(sc[kHalves - 1][t][i], sc[kHalves - 1][t][2 + i]));
 #pragma unroll
           for (int s = 4; s < 32; s <<= 1) top[t][i] = fmaxf(top[t][i], __shfl_xor_sync(0xFFFFFFFFu, top[t][i], s));
           top[t][i] = fmaxf(top[t][i], m[t][i]);
@@ -640,44 +650,52 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
       }
       far = next_far;
     }
-    uint32_t vp[2];
-    ldmatrix2t(vp, kst + kVp + (lane & 15) * 16);
-    uint32_t pw[NQ][NG][2];  // weights times the groups' scales as B: keys 2c and 2c + 1 of query r, then keys + 8
 #pragma unroll
-    for (int g = 0; g < NG; ++g) vs[0][g] *= v_unit, vs[1][g] *= v_unit;
-    if (far) {  // the difference from m, which is exact near it; the base's rounding would be whole units
+    for (int hf = 0; hf < kHalves; ++hf) {
+      if (far) {  // the difference from m, which is exact near it; the base's rounding would be whole units
 #pragma unroll
-      for (int t = 0; t < NQ; ++t)
+        for (int t = 0; t < NQ; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[t][i] = at_exp2(fmaf(sc[t][i] - m[t][i & 1], unit[t][i & 1], 7.f));
-    } else {
+          for (int i = 0; i < 4; ++i) sc[hf][t][i] = at_exp2(fmaf(sc[hf][t][i] - m[t][i & 1], unit[t][i & 1], 7.f));
+      } else {
 #pragma unroll
-      for (int t = 0; t < NQ; ++t)
+        for (int t = 0; t < NQ; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[t][i] = at_exp2(fmaf(sc[t][i], unit[t][i & 1], base[t][i & 1]));
-    }
-#pragma unroll
-    for (int t = 0; t < NQ; ++t) {
-      const float(&w)[4] = sc[t];
-      l[t][0] += w[0] + w[2];
-      l[t][1] += w[1] + w[3];
-      a4_mma_top(z[t], vp[0], vp[1], movmatrix(a4_pack(w[0], w[1])), movmatrix(a4_pack(w[2], w[3])));
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        pw[t][g][0] = movmatrix(a4_pack(w[0] * vs[0][g], w[1] * vs[0][g]));
-        pw[t][g][1] = movmatrix(a4_pack(w[2] * vs[1][g], w[3] * vs[1][g]));
-      }
-      if (partial && lost[t]) {
-        const float nan = __uint_as_float(0x7FFFFFFFu);
-        if ((r & 1) && (lost[t] >> (r >> 1)) & 1) z[t][0] = nan;
-        if ((r & 1) && (lost[t] >> (8 + (r >> 1))) & 1) z[t][1] = nan;
+          for (int i = 0; i < 4; ++i) sc[hf][t][i] = at_exp2(fmaf(sc[hf][t][i], unit[t][i & 1], base[t][i & 1]));
       }
     }
-    {
+#pragma unroll
+    for (int hf = 0; hf < kHalves; ++hf) {
+      const unsigned char *params = here + kVp + hf * kA4Half * 16;
+      uint32_t vr[2][4];  // (scale, middle) of the groups of keys r and r + 8
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (kPairs == 4) *reinterpret_cast<uint4 *>(vr[i]) = *reinterpret_cast<const uint4 *>(params + (r + 8 * i) * 16);
+        else *reinterpret_cast<uint2 *>(vr[i]) = *reinterpret_cast<const uint2 *>(params + (r + 8 * i) * 16);
+      }
+      float vs[2][NG];
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) vs[i][g] = a4_low(vr[i][g]) * (NQ == 1 ? 1.f : v_unit);
+      uint32_t pw[NQ][NG][2];  // weights times the groups' scales as B: keys 2c and 2c + 1 of query r, then keys + 8
+#pragma unroll
+      for (int t = 0; t < NQ; ++t) {
+        float w[4] = {sc[hf][t][0], sc[hf][t][1], sc[hf][t][2], sc[hf][t][3]};
+        l[t][0] += w[0] + w[2];
+        l[t][1] += w[1] + w[3];
+        a4_mma_top(z[t], vp[hf][0], vp[hf][1], movmatrix(a4_pack(w[0], w[1])), movmatrix(a4_pack(w[2], w[3])));
+        if (NQ == 1) w[0] *= v_unit, w[1] *= v_unit, w[2] *= v_unit, w[3] *= v_unit;  // or the scales: fewer of these
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          pw[t][g][0] = movmatrix(a4_pack(w[0] * vs[0][g], w[1] * vs[0][g]));
+          pw[t][g][1] = movmatrix(a4_pack(w[2] * vs[1][g], w[3] * vs[1][g]));
+        }
+      }
       uint32_t f[4];
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        if ((g & 1) == 0) ldmatrix4t(f, kst + kV + mat + g * 16);
+        if ((g & 1) == 0) ldmatrix4t(f, kst + kV + hf * kA4Half * kPitch + mat + g * 16);
         const uint32_t w0 = f[2 * (g & 1)], w1 = f[2 * (g & 1) + 1], w2 = w0 >> 8, w3 = w1 >> 8;
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
@@ -689,6 +707,15 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
           a4_mma(o[t][2 * g + 1], w2 & 0x000F000Fu, w2 & 0x00F000F0u, w3 & 0x000F000Fu, w3 & 0x00F000F0u, b0, b1);
         }
       }
+    }
+    if (partial) {
+#pragma unroll
+      for (int t = 0; t < NQ; ++t)
+        if (lost[t]) {
+          const float nan = __uint_as_float(0x7FFFFFFFu);
+          if ((r & 1) && (lost[t] >> (r >> 1)) & 1) z[t][0] = nan;
+          if ((r & 1) && (lost[t] >> (8 + (r >> 1))) & 1) z[t][1] = nan;
+        }
     }
     __syncwarp();  // the stage is read: the next round's copies may overwrite it
     if (++stage == kStages) stage = 0;
@@ -704,7 +731,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
         const int g = t * 8 + c * 2 + i;
         const int64_t rec = piece * a.chunk_rows + g;
         // what the weights refer to, to the last bit: a query that saw no score refers to nothing
-        const float ref = m[t][i] == kA4Least ? kNone : far ? m[t][i] * unit[t][i] : 7.f - base[t][i];
+        const float ref = m[t][i] == kA4Least ? kNone : far ? fminf(fmaxf(m[t][i] * unit[t][i], -3e38f), 3e38f) : 7.f - base[t][i];
         if (g < n && r == 0) a.own_ml[rec] = make_float2(ref, broken ? kAtBadPage : l[t][i] * 0x1p-7f);
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
@@ -718,7 +745,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
       }
     }
     fresh = true;
-    a4_item_next(a, now);
+    a4_item_next<kTile>(a, now);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -751,7 +778,7 @@ __global__ void __launch_bounds__((kWarps > 1 ? kWarps : kMgNarrow) * 32) ms_att
   int64_t own = 0;
   int pieces = 0;
   if (keys > 0) {  // the warps whose shares meet the item's tiles
-    const int64_t units = a4_units(keys), u = start + hc * units, w = (u + kA4Item) / share;
+    const int64_t units = a4_units(keys, a.tile), u = start + hc * units, w = (u + kA4Item) / share;
     own = (b * hcs + hc + w) * a.chunk_rows + q - chunk * a.chunk_rows;
     pieces = (int)((u + units - 1) / share - w) + 1;
   }
