@@ -131,6 +131,8 @@ int ms_kv4_attention(const ms_kv4_attention_args *args, ms_stream_t stream) {
   a.layout = ms::k4_layout(x.cache.head_dim);
   a.group = p.group, a.queries = p.queries, a.chunks = p.chunks, a.chunk_rows = p.chunk_rows;
   a.split_warps = p.split_warps;
+  a.code_head = x.cache.page_size * a.layout.row_bytes;
+  a.code_page = a.code_head * x.cache.kv_heads;
   char *w = static_cast<char *>(x.workspace);
   a.header = reinterpret_cast<ms::A4Header *>(w);
   a.base = reinterpret_cast<int64_t *>(w + p.base);

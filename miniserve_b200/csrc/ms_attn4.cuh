@@ -66,6 +66,7 @@ struct A4Args {
   int page_shift;  // log2 of the page size, or -1
   int merge_wide;  // the merge gives each output a CTA
   int tile;        // keys of the split kernel's tiles
+  int64_t code_page, code_head;  // bytes of a page's codes of the keys, and of one head of it
 };
 
 // Keys of a row: its tokens' largest length; 0 where one of them does not fit
@@ -121,14 +122,14 @@ __device__ __forceinline__ void ldmatrix2t(uint32_t (&r)[2], uint32_t addr) {
 // d = a b + c, and d += a b.
 __device__ __forceinline__ void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1, float c0, float c1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -136,10 +137,16 @@ __device__ __forceinline__ void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
 // The upper eight rows of the product, of an A whose lower ones are zero.
 __device__ __forceinline__ void a4_mma_top(float (&d)[2], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
   [[maybe_unused]] float none0, none1;
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
       : "+f"(d[0]), "+f"(d[1]), "=f"(none0), "=f"(none1)
       : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+}
+// movmatrix for values alone: the compiler may move it, as it may the products.
+__device__ __forceinline__ uint32_t a4_turn(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t a4_pack(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
@@ -267,15 +274,20 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
   const int page_size = (int)x.cache.page_size;
 
   // Copies.  Where a half's keys lie in one page, it is looked up once for all lanes; else lanes 0-15 (and 16-31 again)
-  // look up the half's keys.  Page ids are loaded a tile ahead of their use.
+  // look up the half's keys.  Page ids are loaded a tile ahead of their use, and a tile's addresses are a page's, a
+  // head's and a lane's parts: this is work for every 32 keys.
   int page[kHalves], offset[kHalves];
-  int head = 0;       // of the next tile
-  int live_keys = 0;  // of the next tile; 0 where none is left
-  uint32_t met = 0;   // bit i: the tile issued i tiles ago met a bad page
+  const int *table = nullptr;  // of the next tile's row
+  int64_t head_at = 0;         // its head's codes in a page
+  int live_keys = 0;           // of the next tile; 0 where none is left
+  uint32_t met = 0;            // bit i: the tile issued i tiles ago met a bad page
   auto look = [&](bool item) {  // at tile load.tile, the first of an item's or not
     live_keys = 0;
     if (load.tile >= load.end) return;
-    if (item) head = load.hc / a.chunks;
+    if (item) {
+      head_at = load.hc / a.chunks * a.code_head;
+      table = x.table + load.b * x.table_row;
+    }
     live_keys = load.keys - load.tile * kTile;
 #pragma unroll
     for (int i = 0; i < kHalves; ++i) {
@@ -283,8 +295,8 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
       page[i] = offset[i] = 0;
       if (j < load.keys) {
         const int p = a.page_shift >= 0 ? j >> a.page_shift : j / page_size;
-        offset[i] = j - p * page_size;
-        page[i] = load_in(x.table + load.b * x.table_row + p);
+        offset[i] = a.page_shift >= 0 ? j & (page_size - 1) : j - p * page_size;
+        page[i] = load_in(table + p);
       }
     }
   };
@@ -295,47 +307,62 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
     look(item);
   };
   constexpr int kCopies = (kTile * kPieces + 31) / 32;  // of a tile's codes of the keys, and of the values
+  const unsigned char *k_lane = x.cache.k_codes + lane * 16, *v_lane = x.cache.v_codes + lane * 16;
+  const uint32_t d_lane = ring + lane / kPieces * kPitch + lane % kPieces * 16;  // of copy 0
+  auto params_of = [](int64_t code) { return kPairs * 4 * 4 == kRow ? code >> 2 : code / kRow * (kPairs * 4); };
   auto issue = [&](int stage) {
-    const uint32_t dst = ring + stage * kStage;
-    int64_t row[kHalves];  // of the codes and parameters of a half's first key, or of the lane's; -1: none
+    int64_t code[kHalves];  // the codes' place of a half's first key, or of the lane's
     bool wrong = false;
 #pragma unroll
     for (int i = 0; i < kHalves; ++i) {
-      const bool live = i * kA4Half + (kWhole ? 0 : lane & 15) < live_keys, good = page[i] >= 0 && page[i] < x.cache.pages;
-      wrong = wrong || (live && !good);
-      row[i] = live && good ? ((int64_t)page[i] * x.cache.kv_heads + head) * page_size + offset[i] : -1;
+      const bool live = i * kA4Half + (kWhole ? 0 : lane & 15) < live_keys;
+      wrong = wrong || (live && (unsigned)page[i] >= (unsigned)x.cache.pages);
+      code[i] = page[i] * a.code_page + head_at + (uint32_t)offset[i] * (int64_t)kRow;
     }
     met = (met << 1) | (kWhole ? wrong : __any_sync(0xFFFFFFFFu, wrong));
     if (kWhole && live_keys >= kTile && !wrong) {  // all of the tile
+      const uint32_t dst = d_lane + stage * kStage;
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
-        const int at = i * 32 + lane, r = at / kPieces, half = kPieces == 3 ? r >> 4 : i * 32 / kPieces / kA4Half;
-        const int64_t off = row[kHalves == 1 ? 0 : half] * kRow + (at - half * kA4Half * kPieces) * 16;
-        if (kTile * kPieces % 32 == 0 || r < kTile) {
-          copy16(dst + r * kPitch + (at - r * kPieces) * 16, x.cache.k_codes + off, true);
-          copy16(dst + kV + r * kPitch + (at - r * kPieces) * 16, x.cache.v_codes + off, true);
+        if (kPieces == 3) {
+          const int at = i * 32 + lane, r = at / kPieces;
+          const int64_t off = (kHalves > 1 && r >= kA4Half ? code[kHalves - 1] - kA4Half * kRow : code[0]) + i * 512;
+          const uint32_t to = ring + stage * kStage + r * kPitch + (at - r * kPieces) * 16;
+          if (kTile * kPieces % 32 == 0 || r < kTile) {
+            copy16(to, k_lane + off, true);
+            copy16(to + kV, v_lane + off, true);
+          }
+        } else {
+          constexpr int kEach = kCopies / kHalves;  // of a half
+          const int64_t off = code[i / kEach] + i % kEach * 512;
+          copy16(dst + i * (32 / kPieces) * kPitch, k_lane + off, true);
+          copy16(dst + kV + i * (32 / kPieces) * kPitch, v_lane + off, true);
         }
       }
-      const int64_t off = ((kHalves > 1 && lane >= 16 ? row[kHalves - 1] : row[0]) + (lane & 15)) * (kPairs * 4);
+      const int64_t off = params_of(kHalves > 1 && lane >= 16 ? code[kHalves - 1] : code[0]) + (lane & 15) * (kPairs * 4);
       const char *ks = static_cast<const char *>(x.cache.k_params) + off, *vs = static_cast<const char *>(x.cache.v_params) + off;
+      const uint32_t to = ring + stage * kStage + kKp + lane * 16;
       if (kHalves == 1) {
-        if (kPairs == 4) copy16(dst + kKp + lane * 16, lane < 16 ? ks : vs, true);
-        else copy8(dst + kKp + lane * 16, lane < 16 ? ks : vs, true);
+        if (kPairs == 4) copy16(to, lane < 16 ? ks : vs, true);
+        else copy8(to, lane < 16 ? ks : vs, true);
       } else if (kPairs == 4) {
-        copy16(dst + kKp + lane * 16, ks, true);
-        copy16(dst + kVp + lane * 16, vs, true);
+        copy16(to, ks, true);
+        copy16(to + kTile * 16, vs, true);
       } else {
-        copy8(dst + kKp + lane * 16, ks, true);
-        copy8(dst + kVp + lane * 16, vs, true);
+        copy8(to, ks, true);
+        copy8(to + kTile * 16, vs, true);
       }
       return;
     }
-    // the row of key r of the tile, or -1
-    auto row_of = [&](int r) {
+    // the codes' place of key r of the tile, or -1
+    const uint32_t dst = ring + stage * kStage;
+    auto code_of = [&](int r) {
       int64_t at = -1;
 #pragma unroll
       for (int i = 0; i < kHalves; ++i) {
-        const int64_t from = kWhole ? (row[i] >= 0 ? row[i] + (r & 15) : -1) : __shfl_sync(0xFFFFFFFFu, row[i], r & 15);
+        const bool fine = i * kA4Half + (kWhole ? 0 : lane & 15) < live_keys && (unsigned)page[i] < (unsigned)x.cache.pages;
+        const int64_t own = fine ? code[i] : -1;
+        const int64_t from = kWhole ? (own >= 0 ? own + (r & 15) * kRow : -1) : __shfl_sync(0xFFFFFFFFu, own, r & 15);
         if (r >> 4 == i) at = from;
       }
       return r < live_keys ? at : -1;
@@ -343,7 +370,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
       const int at = i * 32 + lane, r = at / kPieces, piece = at - r * kPieces;
-      const int64_t from = row_of(r), off = from >= 0 ? from * kRow + piece * 16 : 0;
+      const int64_t from = code_of(r), off = from >= 0 ? from + piece * 16 : 0;
       if (kTile * kPieces % 32 == 0 || r < kTile) {
         copy16(dst + r * kPitch + piece * 16, x.cache.k_codes + off, from >= 0);
         copy16(dst + kV + r * kPitch + piece * 16, x.cache.v_codes + off, from >= 0);
@@ -351,7 +378,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
     }
 #pragma unroll
     for (int i = 0; i < kHalves; ++i) {
-      const int64_t from = row_of(kHalves == 1 ? lane & 15 : lane), off = from >= 0 ? from * (kPairs * 4) : 0;
+      const int64_t from = code_of(kHalves == 1 ? lane & 15 : lane), off = from >= 0 ? params_of(from) : 0;
       const bool key = kHalves == 1 ? lane < 16 : i == 0;
       const char *src = static_cast<const char *>(key ? x.cache.k_params : x.cache.v_params) + off;
       if (kPairs == 4) copy16(dst + kKp + (i * 32 + lane) * 16, src, from >= 0);
@@ -512,24 +539,45 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
           for (int i = 0; i < 4; ++i) sc[hf][t][i] *= 0x1p-24f;  // or the scales by 2^24: fewer of these
         }
       }
-      uint32_t f[4];
+      // the groups' first products, then their second ones, which wait for them
+      uint32_t f[(NG + 1) / 2][4];
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        if ((g & 1) == 0) ldmatrix4(f, kcodes + g * 16);
-        const uint32_t w0 = f[2 * (g & 1)], w1 = f[2 * (g & 1) + 1], w2 = w0 >> 8, w3 = w1 >> 8;
-        const float s0 = a4_low(pr[0][g]) * (NQ == 1 ? 1.f : 0x1p24f), s1 = a4_low(pr[1][g]) * (NQ == 1 ? 1.f : 0x1p24f);
+      for (int g = 0; g < NG; g += 2) ldmatrix4(f[g / 2], kcodes + g * 16);
+      constexpr int kAt = kQShared ? 1 : NG;  // groups at a time: registers
 #pragma unroll
-        for (int t = 0; t < NQ; ++t) {
-          uint4 b;
-          if constexpr (kQShared) b = *reinterpret_cast<const uint4 *>(q_shared + (t * NG + g) * 512);
-          else b = make_uint4(qf[t][g][0], qf[t][g][1], qf[t][g][2], qf[t][g][3]);
-          float d[4];
-          a4_mma(d, w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, b.x, b.y, 0.f, 0.f);
-          a4_mma(d, w2 & 0x000F000Fu, w3 & 0x000F000Fu, w2 & 0x00F000F0u, w3 & 0x00F000F0u, b.z, b.w);
-          sc[hf][t][0] = fmaf(s0, d[0], sc[hf][t][0]);
-          sc[hf][t][1] = fmaf(s0, d[1], sc[hf][t][1]);
-          sc[hf][t][2] = fmaf(s1, d[2], sc[hf][t][2]);
-          sc[hf][t][3] = fmaf(s1, d[3], sc[hf][t][3]);
+      for (int g0 = 0; g0 < NG; g0 += kAt) {
+        float d[kAt][NQ][4];
+        uint4 b[kAt][NQ];
+#pragma unroll
+        for (int k = 0; k < kAt; ++k) {
+          const int g = g0 + k;
+          const uint32_t w0 = f[g / 2][2 * (g & 1)], w1 = f[g / 2][2 * (g & 1) + 1];
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) {
+            if constexpr (kQShared) b[k][t] = *reinterpret_cast<const uint4 *>(q_shared + (t * NG + g) * 512);
+            else b[k][t] = make_uint4(qf[t][g][0], qf[t][g][1], qf[t][g][2], qf[t][g][3]);
+            a4_mma(d[k][t], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, b[k][t].x, b[k][t].y, 0.f, 0.f);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kAt; ++k) {
+          const int g = g0 + k;
+          const uint32_t w2 = f[g / 2][2 * (g & 1)] >> 8, w3 = f[g / 2][2 * (g & 1) + 1] >> 8;
+#pragma unroll
+          for (int t = 0; t < NQ; ++t)
+            a4_mma(d[k][t], w2 & 0x000F000Fu, w3 & 0x000F000Fu, w2 & 0x00F000F0u, w3 & 0x00F000F0u, b[k][t].z, b[k][t].w);
+        }
+#pragma unroll
+        for (int k = 0; k < kAt; ++k) {
+          const int g = g0 + k;
+          const float s0 = a4_low(pr[0][g]) * (NQ == 1 ? 1.f : 0x1p24f), s1 = a4_low(pr[1][g]) * (NQ == 1 ? 1.f : 0x1p24f);
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) {
+            sc[hf][t][0] = fmaf(s0, d[k][t][0], sc[hf][t][0]);
+            sc[hf][t][1] = fmaf(s0, d[k][t][1], sc[hf][t][1]);
+            sc[hf][t][2] = fmaf(s1, d[k][t][2], sc[hf][t][2]);
+            sc[hf][t][3] = fmaf(s1, d[k][t][3], sc[hf][t][3]);
+          }
         }
       }
     }
@@ -684,14 +732,22 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
         float w[4] = {sc[hf][t][0], sc[hf][t][1], sc[hf][t][2], sc[hf][t][3]};
         l[t][0] += w[0] + w[2];
         l[t][1] += w[1] + w[3];
-        a4_mma_top(z[t], vp[hf][0], vp[hf][1], movmatrix(a4_pack(w[0], w[1])), movmatrix(a4_pack(w[2], w[3])));
+        a4_mma_top(z[t], vp[hf][0], vp[hf][1], a4_turn(a4_pack(w[0], w[1])), a4_turn(a4_pack(w[2], w[3])));
         if (NQ == 1) w[0] *= v_unit, w[1] *= v_unit, w[2] *= v_unit, w[3] *= v_unit;  // or the scales: fewer of these
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          pw[t][g][0] = movmatrix(a4_pack(w[0] * vs[0][g], w[1] * vs[0][g]));
-          pw[t][g][1] = movmatrix(a4_pack(w[2] * vs[1][g], w[3] * vs[1][g]));
+          pw[t][g][0] = a4_turn(a4_pack(w[0] * vs[0][g], w[1] * vs[0][g]));
+          pw[t][g][1] = a4_turn(a4_pack(w[2] * vs[1][g], w[3] * vs[1][g]));
         }
       }
+      // -8 2^-24 and -8 2^-20, of the rows whose codes are in the lower and the upper nibble; then the codes
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int t = 0; t < NQ; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            a4_mma(o[t][2 * g + i], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pw[t][g][0], pw[t][g][1]);
       uint32_t f[4];
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -699,12 +755,8 @@ __global__ void __launch_bounds__(kA4Warps * 32, kA4Ctas<NG, NQ>)
         const uint32_t w0 = f[2 * (g & 1)], w1 = f[2 * (g & 1) + 1], w2 = w0 >> 8, w3 = w1 >> 8;
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
-          const uint32_t b0 = pw[t][g][0], b1 = pw[t][g][1];
-          // -8 2^-24 and -8 2^-20, of the rows whose codes are in the lower and the upper nibble
-          a4_mma(o[t][2 * g], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
-          a4_mma(o[t][2 * g + 1], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
-          a4_mma(o[t][2 * g], w0 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x000F000Fu, w1 & 0x00F000F0u, b0, b1);
-          a4_mma(o[t][2 * g + 1], w2 & 0x000F000Fu, w2 & 0x00F000F0u, w3 & 0x000F000Fu, w3 & 0x00F000F0u, b0, b1);
+          a4_mma(o[t][2 * g], w0 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x000F000Fu, w1 & 0x00F000F0u, pw[t][g][0], pw[t][g][1]);
+          a4_mma(o[t][2 * g + 1], w2 & 0x000F000Fu, w2 & 0x00F000F0u, w3 & 0x000F000Fu, w3 & 0x00F000F0u, pw[t][g][0], pw[t][g][1]);
         }
       }
     }
