@@ -30,6 +30,25 @@ namespace ms {
 
 constexpr int kK4Threads = 256;
 
+// Quotients of numbers below 2^16 (or, by divisors up to 16, below 2^28) from a
+// product: u / d is the high word of u ceil(2^32 / d).
+struct K4Divisor {
+  uint32_t d, inverse;
+};
+static K4Divisor k4_divisor(int64_t d) { return K4Divisor{(uint32_t)d, (uint32_t)((0x100000000ull + d - 1) / d)}; }
+__device__ __forceinline__ int k4_over(int u, const K4Divisor &d) { return d.d == 1 ? u : (int)__umulhi((uint32_t)u, d.inverse); }
+
+__device__ __forceinline__ float k4_min(float x, float y) {  // a NaN stays
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float k4_max(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+
 // kV entries as floats.
 template <typename T, int kV>
 __device__ __forceinline__ void k4_load(const T *p, float (&x)[kV]) {
@@ -102,10 +121,12 @@ struct K4AppendArgs {
   ms_kv4_append_args a;
   K4Layout layout;
   int page_shift;
-  int q_blocks;           // the first blocks: queries
+  int q_blocks;             // the first blocks: queries
   int q_tokens, kv_tokens;  // tokens of a block
-  int chunks;             // 8-entry chunks of a stored head
-  int piece, q_piece;     // entries loaded at once (8, 4 or 1) of the keys and values, and of the queries
+  int q_slots;              // threads' heads of a token: h, and h + q_slots
+  int piece, q_piece;       // entries loaded at once (8, 4 or 1) of the keys and values, and of the queries
+  K4Divisor units, q_token;     // of a head's pieces of the queries, and of a token's
+  K4Divisor chunks, kv_token;   // of a stored head's 8-entry chunks, and of a token's
 };
 
 constexpr int kK4Tokens = 64;  // tokens of a block, at most
@@ -120,73 +141,137 @@ __device__ __forceinline__ int64_t k4_position(const ms_kv4_append_args &a, int6
   return good ? at : 0;
 }
 
+// kV entries as they are, and one of them (two of them, where kV > 1).
 template <typename T, int kV>
-__device__ __forceinline__ void k4_store(T *p, const float (&x)[kV]) {
-  if constexpr (kV == 1) {
-    kv_from_float(x[0], *p);
-  } else {
-    uint32_t u[kV / 2];
+struct K4Raw {
+  uint32_t u[kV / 2];
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (kV == 8) *reinterpret_cast<uint4 *>(u) = load_in(reinterpret_cast<const uint4 *>(p));
+    else *reinterpret_cast<uint2 *>(u) = load_in(reinterpret_cast<const uint2 *>(p));
+  }
+  __device__ __forceinline__ void store(T *p) const {
+    if constexpr (kV == 8) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(u);
+    else *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(u);
+  }
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < kV / 2; ++i) u[i] = kv_narrow<T>(x[2 * i], x[2 * i + 1]);
-    if constexpr (kV == 8) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<uint4 *>(u);
-    else *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<uint2 *>(u);
+    for (int i = 0; i < kV / 2; ++i) u[i] = 0;
+  }
+};
+template <typename T>
+struct K4Raw<T, 1> {
+  T x;
+  __device__ __forceinline__ void load(const T *p) { x = load_in(p); }
+  __device__ __forceinline__ void store(T *p) const { *p = x; }
+  __device__ __forceinline__ void clear() { kv_from_float(0.f, x); }
+};
+// Pairs of x and y turned by cosines c and sines s.
+template <typename T, bool kInterleaved, int kV>
+__device__ __forceinline__ void k4_turn(K4Raw<T, kV> &x, K4Raw<T, kV> &y, const float (&c)[kV], const float (&s)[kV]) {
+  if constexpr (kV == 1) {
+    const float f = kv_to_float(x.x), g = kv_to_float(y.x);
+    kv_from_float(f * c[0] - g * s[0], x.x);
+    kv_from_float(g * c[0] + f * s[0], y.x);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kV / 2; ++k) {
+      const float2 f = kv_widen<T>(x.u[k]), g = kv_widen<T>(y.u[k]);
+      if (kInterleaved) {  // word k of x is pair k, word k of y is pair kV / 2 + k
+        const int i = kV / 2 + k;
+        x.u[k] = kv_narrow<T>(f.x * c[k] - f.y * s[k], f.y * c[k] + f.x * s[k]);
+        y.u[k] = kv_narrow<T>(g.x * c[i] - g.y * s[i], g.y * c[i] + g.x * s[i]);
+      } else {  // word k holds the first (x) and second (y) entries of pairs 2k and 2k + 1
+        x.u[k] = kv_narrow<T>(f.x * c[2 * k] - g.x * s[2 * k], f.y * c[2 * k + 1] - g.y * s[2 * k + 1]);
+        y.u[k] = kv_narrow<T>(g.x * c[2 * k] + f.x * s[2 * k], g.y * c[2 * k + 1] + f.y * s[2 * k + 1]);
+      }
+    }
   }
 }
 
-// Queries: a thread owns both sides of kV pairs (or 2 kV copied entries) of a
-// head, so that q_out may be q itself.
+// Queries: a thread owns both sides of kV pairs (or 2 kV copied entries) of up
+// to two heads, which share its cosines and sines; q_out may be q itself.  Its
+// loads are issued before anything that depends on the token's position.
 template <typename T, bool kInterleaved, int kV>
 __device__ __forceinline__ void k4_queries(const K4AppendArgs &p) {
   const ms_kv4_append_args &a = p.a;
-  const int units = a.cache.head_dim / (2 * kV), half = a.rotary >> 1;
+  const int half = a.rotary >> 1;
   const int64_t t0 = (int64_t)blockIdx.x * p.q_tokens;
-  const int per_token = a.heads * units;
-  const int items = (int)min((int64_t)p.q_tokens, a.tokens - t0) * per_token;
+  const int tokens = (int)min((int64_t)p.q_tokens, a.tokens - t0), items = tokens * (int)p.q_token.d;
   for (int u = threadIdx.x; u < items; u += kK4Threads) {
-    const int tl = u / per_token, w = u - tl * per_token;
-    const int h = w / units, j = w - h * units;
+    const int tl = tokens == 1 ? 0 : k4_over(u, p.q_token), w = u - tl * (int)p.q_token.d;
+    const int h = k4_over(w, p.units), j = w - h * (int)p.units.d;
     const int64_t t = t0 + tl;
-    const bool rotates = j * 2 * kV < a.rotary;
+    const bool rotates = j * 2 * kV < a.rotary, both = h + p.q_slots < a.heads;
     const int lo = rotates && !kInterleaved ? j * kV : j * 2 * kV, hi = rotates && !kInterleaved ? lo + half : lo + kV;
     const T *src = static_cast<const T *>(a.q) + t * a.q_token + h * a.q_head;
-    float x[kV], y[kV];
-    k4_load<T, kV>(src + lo, x);
-    k4_load<T, kV>(src + hi, y);
+    K4Raw<T, kV> x[2], y[2];
+    x[0].load(src + lo), y[0].load(src + hi);
+    if (both) {
+      const T *next = src + p.q_slots * a.q_head;
+      x[1].load(next + lo), y[1].load(next + hi);
+    }
     bool good;
     const int64_t at = k4_position(a, t, good);
-    if (!good) {
-#pragma unroll
-      for (int i = 0; i < kV; ++i) x[i] = y[i] = 0.f;
-    } else if (rotates) {
-      float c[kV], s[kV];
+    float c[kV], s[kV];
+    if (rotates) {
       k4_table<kV>(a.table + at * a.rotary + j * kV, c);
       k4_table<kV>(a.table + at * a.rotary + half + j * kV, s);
-      auto turn = [](float &f, float &g, float cosine, float sine) {
-        const float first = f * cosine - g * sine;
-        g = g * cosine + f * sine;
-        f = first;
-      };
-      if constexpr (kInterleaved && kV > 1) {
-#pragma unroll
-        for (int i = 0; i < kV / 2; ++i) {
-          turn(x[2 * i], x[2 * i + 1], c[i], s[i]);
-          turn(y[2 * i], y[2 * i + 1], c[kV / 2 + i], s[kV / 2 + i]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kV; ++i) turn(x[i], y[i], c[i], s[i]);
-      }
     }
     T *dst = static_cast<T *>(a.q_out) + t * a.q_out_token + h * a.q_out_head;
-    k4_store<T, kV>(dst + lo, x);
-    k4_store<T, kV>(dst + hi, y);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (i == 1 && !both) break;
+      if (!good) x[i].clear(), y[i].clear();
+      else if (rotates) k4_turn<T, kInterleaved, kV>(x[i], y[i], c, s);
+      x[i].store(dst + lo), y[i].store(dst + hi);
+      dst += p.q_slots * a.q_out_head;
+    }
   }
 }
 
-// Keys and values: a thread takes 8 entries of one head, and four neighbouring
-// threads a group, whose extremes two shuffles find.  A token's keys and
-// values are all one block's, so that its status is written once, whatever its
-// groups hold.
+// Eight entries (none where `inside` is not set) of a group that four
+// neighbouring threads share: its codes, its parameters, and whether fp16 does
+// not hold it.
+__device__ __forceinline__ uint32_t k4_encode(const float (&y)[8], bool inside, __half2 &param, bool &lost) {
+  float lo = __uint_as_float(0x7F800000u), hi = -lo;
+  if (inside) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lo = k4_min(lo, y[i]), hi = k4_max(hi, y[i]);
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    lo = k4_min(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
+    hi = k4_max(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
+  }
+  param = __halves2half2(__float2half_rn(0.f), __float2half_rn(0.f));
+  lost = false;
+  if (hi < lo) return 0;  // the padding behind a head
+  const __half scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)),
+               middle = __float2half_rn(__fadd_rn(lo, 8.f * __half2float(scale)));
+  const float s = __half2float(scale), m = __half2float(middle);
+  if (!(s <= 65504.f && fabsf(m) <= 65504.f)) {  // what fp16 does not hold, and what is not a number, reads back as NaN
+    param = __halves2half2(__float2half_rn(0.f), __ushort_as_half(0x7FFF));
+    lost = true;
+    return 0x88888888u;
+  }
+  param = __halves2half2(scale, middle);
+  const float inverse = s > 0.f ? __frcp_rn(s) : 0.f;
+  uint32_t word = 0;
+  if (inside) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // the nearest whole number from the low bits of its sum with 1.5 * 2^23 (+ 8)
+      const float step = fminf(fmaxf(__fmul_rn(__fsub_rn(y[i], m), inverse), -8.f), 7.f);
+      word |= (__float_as_uint(__fadd_rn(step, 12582920.f)) & 15u) << (4 * i);
+    }
+  }
+  return word;
+}
+
+// Keys and values: a thread takes 8 entries of a key head and the same 8 of its
+// value head, and four neighbouring threads a group of each.  A token's keys
+// and values are all one block's, so that its status is written once, whatever
+// its groups hold.
 template <typename T, bool kInterleaved, int kV>
 __device__ __forceinline__ void k4_quantise(const K4AppendArgs &p, int *flags) {
   const ms_kv4_append_args &a = p.a;
@@ -194,74 +279,45 @@ __device__ __forceinline__ void k4_quantise(const K4AppendArgs &p, int *flags) {
   const int tokens = (int)min((int64_t)p.kv_tokens, a.tokens - t0);
   for (int i = threadIdx.x; i < tokens; i += kK4Threads) flags[i] = 0;
   __syncthreads();
-  const int per_token = 2 * a.cache.kv_heads * p.chunks;
-  const int items = tokens * per_token;
+  const int items = tokens * (int)p.kv_token.d;
   for (int u0 = threadIdx.x & ~31; u0 < items; u0 += kK4Threads) {  // whole warps: the shuffles
     const int u = u0 + (threadIdx.x & 31);
     const bool live = u < items;
-    const int tl = live ? u / per_token : 0, w = live ? u - tl * per_token : 0;
-    const int side = w / p.chunks, chunk = w - side * p.chunks;
-    const bool key = side < a.cache.kv_heads;
-    const int h = key ? side : side - a.cache.kv_heads;
+    const int tl = live && tokens > 1 ? k4_over(u, p.kv_token) : 0, w = live ? u - tl * (int)p.kv_token.d : 0;
+    const int h = k4_over(w, p.chunks), chunk = w - h * (int)p.chunks.d;
     const int64_t t = t0 + tl;
     const int64_t slot = load_in(a.slots + t);
     bool good;
     const int64_t at = k4_position(a, t, good);
     int status = good ? 0 : MS_ROW_BAD_POSITION;
     if (slot >= a.cache.pages * a.cache.page_size) status |= MS_ROW_BAD_SLOT;
-    const bool write = live && slot >= 0 && status == 0;
-    const bool inside = write && chunk * 8 < a.cache.head_dim;
-    float y[8];
-    float lo = __uint_as_float(0x7F800000u), hi = -lo;
-    bool finite = true;
+    const bool write = live && slot >= 0 && status == 0, inside = write && chunk * 8 < a.cache.head_dim;
+    float y[2][8];
     if (inside) {
-      const T *src = key ? static_cast<const T *>(a.k) + t * a.k_token + h * a.k_head
-                         : static_cast<const T *>(a.v) + t * a.v_token + h * a.v_head;
-      k4_entries<T, kInterleaved, kV>(src, chunk * 8, key, a.rotary, a.table + at * a.rotary, y);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        lo = fminf(lo, y[i]);
-        hi = fmaxf(hi, y[i]);
-        finite = finite && fabsf(y[i]) <= 3.402823466e38f;
-      }
+      k4_entries<T, kInterleaved, kV>(static_cast<const T *>(a.v) + t * a.v_token + h * a.v_head, chunk * 8, false, a.rotary,
+                                      nullptr, y[1]);
+      k4_entries<T, kInterleaved, kV>(static_cast<const T *>(a.k) + t * a.k_token + h * a.k_head, chunk * 8, true, a.rotary,
+                                      a.table + at * a.rotary, y[0]);
     }
+    uint32_t word[2];
+    __half2 param[2];
+    bool lost[2];
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
-    }
-    const uint32_t all = __ballot_sync(0xFFFFFFFFu, finite);
-    finite = ((all >> (threadIdx.x & 28)) & 15u) == 15u;  // the group's four threads
-    uint32_t word = 0;
-    __half scale = __float2half_rn(0.f), middle = scale;
-    if (hi >= lo || !finite) {  // not the padding behind a head
-      scale = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f));
-      middle = __float2half_rn(__fadd_rn(lo, 8.f * __half2float(scale)));
-      const float s = __half2float(scale), m = __half2float(middle);
-      finite = finite && fabsf(s) <= 65504.f && fabsf(m) <= 65504.f;
-      if (!finite) {  // what fp16 does not hold, and what is not a number, reads back as NaN
-        scale = __float2half_rn(0.f);
-        middle = __ushort_as_half(0x7FFF);
-        word = 0x88888888u;
-        status |= MS_ROW_NONFINITE;
-      } else if (inside) {
-        const float inverse = s > 0.f ? __frcp_rn(s) : 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float code = rintf(__fmul_rn(__fsub_rn(y[i], m), inverse)) + 8.f;
-          word |= (uint32_t)__float2int_rn(fminf(fmaxf(code, 0.f), 15.f)) << (4 * i);
-        }
-      }
+    for (int side = 0; side < 2; ++side) {
+      word[side] = k4_encode(y[side], inside, param[side], lost[side]);
+      if (lost[side]) status |= MS_ROW_NONFINITE;
     }
     if (write) {
       int64_t page, offset;
       kv_place(slot, a.cache.page_size, p.page_shift, page, offset);
       const int64_t row = (page * a.cache.kv_heads + h) * a.cache.page_size + offset;
-      uint8_t *codes = key ? a.cache.k_codes : a.cache.v_codes;
-      void *params = key ? a.cache.k_params : a.cache.v_params;
-      *reinterpret_cast<uint32_t *>(codes + row * p.layout.row_bytes + chunk * 4) = word;
-      if ((chunk & 3) == 0)
-        static_cast<__half2 *>(params)[row * p.layout.groups + (chunk >> 2)] = __halves2half2(scale, middle);
+      const int64_t code_at = row * p.layout.row_bytes + chunk * 4, param_at = row * p.layout.groups + (chunk >> 2);
+      *reinterpret_cast<uint32_t *>(a.cache.k_codes + code_at) = word[0];
+      *reinterpret_cast<uint32_t *>(a.cache.v_codes + code_at) = word[1];
+      if ((chunk & 3) == 0) {
+        static_cast<__half2 *>(a.cache.k_params)[param_at] = param[0];
+        static_cast<__half2 *>(a.cache.v_params)[param_at] = param[1];
+      }
     }
     if (live && (chunk & 3) == 0 && status) atomicOr(&flags[tl], status);
   }
@@ -271,7 +327,7 @@ __device__ __forceinline__ void k4_quantise(const K4AppendArgs &p, int *flags) {
 }
 
 template <typename T, bool kInterleaved>
-__global__ void __launch_bounds__(kK4Threads) ms_kv4_append_kernel(const __grid_constant__ K4AppendArgs p) {
+__global__ void __launch_bounds__(kK4Threads, 4) ms_kv4_append_kernel(const __grid_constant__ K4AppendArgs p) {
   __shared__ int flags[kK4Tokens];
   grid_wait();
   if ((int)blockIdx.x < p.q_blocks) {
@@ -289,18 +345,46 @@ struct K4ReadArgs {
   ms_kv4_read_args a;
   K4Layout layout;
   int page_shift;
-  int chunks;  // 8-entry chunks of a head
   int tokens;  // tokens of a block
   int wide;    // outputs are stored in 16 bytes
+  K4Divisor chunks, token;  // of a head's 8-entry chunks, and of a token's
 };
 
+// Eight entries of codes and (scale, middle), as pairs of T.  A code in a half's
+// low bits over the bits of 1024 is 1024 + code: less 1032, exact, it is code - 8.
 template <typename T>
-__device__ __forceinline__ uint32_t k4_narrow(float x, float y) {
-  if constexpr (sizeof(T) == 2 && __is_same(T, __half)) {  // finite entries stay finite
-    x = fabsf(x) <= 3.402823466e38f ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
-    y = fabsf(y) <= 3.402823466e38f ? fminf(fmaxf(y, -65504.f), 65504.f) : y;
+__device__ __forceinline__ void k4_decode(uint32_t word, __half2 param, uint32_t (&out)[4]) {
+  const __half2 less = __floats2half2_rn(-1032.f, -1032.f);
+  __half2 step[4];  // entries i and i + 4
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = ((word >> (4 * i)) & 0x000F000Fu) | 0x64006400u;
+    step[i] = __hadd2(*reinterpret_cast<const __half2 *>(&u), less);
   }
-  return kv_narrow<T>(x, y);
+  const float s = __low2float(param), m = __high2float(param);
+  if constexpr (__is_same(T, __half)) {
+    const __half2 s2 = __low2half2(param), m2 = __high2half2(param);
+    __half2 y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = __hfma2(step[i], s2, m2);  // rounded once
+    if (!(fmaf(8.f, fabsf(s), fabsf(m)) <= 65000.f)) {  // finite entries stay finite, NaN stays
+      const __half2 most = __floats2half2_rn(65504.f, 65504.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = __hmax2_nan(__hmin2_nan(y[i], most), __hneg2(most));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half2 low = __lows2half2(y[2 * i], y[2 * i + 1]), high = __highs2half2(y[2 * i], y[2 * i + 1]);
+      out[i] = *reinterpret_cast<const uint32_t *>(&low), out[2 + i] = *reinterpret_cast<const uint32_t *>(&high);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 f = __half22float2(step[2 * i]), g = __half22float2(step[2 * i + 1]);
+      out[i] = kv_narrow<T>(fmaf(s, f.x, m), fmaf(s, g.x, m));
+      out[2 + i] = kv_narrow<T>(fmaf(s, f.y, m), fmaf(s, g.y, m));
+    }
+  }
 }
 
 // A thread takes 8 entries of a key head and the same 8 of its value head.
@@ -309,11 +393,10 @@ __global__ void __launch_bounds__(kK4Threads) ms_kv4_read_kernel(const __grid_co
   grid_wait();
   const ms_kv4_read_args &a = p.a;
   const int64_t t0 = (int64_t)blockIdx.x * p.tokens;
-  const int per_token = a.cache.kv_heads * p.chunks;
-  const int items = (int)min((int64_t)p.tokens, a.tokens - t0) * per_token;
+  const int tokens = (int)min((int64_t)p.tokens, a.tokens - t0), items = tokens * (int)p.token.d;
   for (int u = threadIdx.x; u < items; u += kK4Threads) {
-    const int tl = u / per_token, w = u - tl * per_token;
-    const int h = w / p.chunks, chunk = w - h * p.chunks;
+    const int tl = tokens == 1 ? 0 : k4_over(u, p.token), w = u - tl * (int)p.token.d;
+    const int h = k4_over(w, p.chunks), chunk = w - h * (int)p.chunks.d;
     const int64_t t = t0 + tl, slot = load_in(a.slots + t);
     const bool bad = slot >= a.cache.pages * a.cache.page_size, live = slot >= 0 && !bad;
     if (w == 0 && a.status) a.status[t] = bad ? MS_ROW_BAD_SLOT : MS_ROW_OK;
@@ -335,13 +418,8 @@ __global__ void __launch_bounds__(kK4Threads) ms_kv4_read_kernel(const __grid_co
       T *dst = side ? static_cast<T *>(a.v_out) + t * a.v_token + h * a.v_head
                     : static_cast<T *>(a.k_out) + t * a.k_token + h * a.k_head;
       dst += chunk * 8;
-      const float s = __low2float(param[side]), m = __high2float(param[side]);
       uint32_t out[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = (float)((int)((word[side] >> (8 * i)) & 15) - 8), y = (float)((int)((word[side] >> (8 * i + 4)) & 15) - 8);
-        out[i] = k4_narrow<T>(fmaf(s, x, m), fmaf(s, y, m));
-      }
+      k4_decode<T>(word[side], param[side], out);
       if (p.wide) {
         *reinterpret_cast<uint4 *>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
       } else {
@@ -391,7 +469,7 @@ int ms_kv4_append(const ms_kv4_append_args *args, ms_stream_t stream) {
     return MS_E_INVALID;
   p.layout = ms::k4_layout(a.cache.head_dim);
   p.page_shift = ms::kv_page_shift(a.cache.page_size);
-  p.chunks = p.layout.row_bytes / 4;
+  p.chunks = ms::k4_divisor(p.layout.row_bytes / 4);
   // the largest pieces that strides and bases allow: of the keys and values those that lie on one side of a rotation,
   // of the queries those that come in pairs
   const bool table = a.rotary == 0 || (reinterpret_cast<uintptr_t>(a.table) & 15) == 0;
@@ -406,10 +484,13 @@ int ms_kv4_append(const ms_kv4_append_args *args, ms_stream_t stream) {
   p.q_piece = largest([&](int v) {
     return a.rotary % (2 * v) == 0 && (q_strides & (v - 1)) == 0 && (q_bases & (2 * v - 1)) == 0;
   });
-  const int64_t kv_items = 2ll * a.cache.kv_heads * p.chunks;
-  const int64_t q_items = (int64_t)a.heads * (a.cache.head_dim / (2 * p.q_piece));
+  p.units = ms::k4_divisor(a.cache.head_dim / (2 * p.q_piece));
+  p.q_slots = (a.heads + 1) / 2;
+  const int64_t kv_items = (int64_t)a.cache.kv_heads * p.chunks.d, q_items = (int64_t)p.q_slots * p.units.d;
+  p.kv_token = ms::k4_divisor(kv_items);
+  p.q_token = ms::k4_divisor(q_items ? q_items : 1);
   p.kv_tokens = ms::k4_tokens(a.tokens, kv_items, 4);
-  p.q_tokens = q_items ? ms::k4_tokens(a.tokens, q_items, 4) : 1;
+  p.q_tokens = q_items ? ms::k4_tokens(a.tokens, q_items, 2) : 1;
   p.q_blocks = q_items ? (int)((a.tokens + p.q_tokens - 1) / p.q_tokens) : 0;
   const int64_t blocks = p.q_blocks + (a.tokens + p.kv_tokens - 1) / p.kv_tokens;
   if (blocks > 0x7FFFFFFFll) return MS_E_INVALID;
@@ -432,8 +513,9 @@ int ms_kv4_read(const ms_kv4_read_args *args, ms_stream_t stream) {
   if (!a.slots || !a.k_out || !a.v_out) return MS_E_INVALID;
   p.layout = ms::k4_layout(a.cache.head_dim);
   p.page_shift = ms::kv_page_shift(a.cache.page_size);
-  p.chunks = a.cache.head_dim / 8;
-  p.tokens = ms::k4_tokens(a.tokens, (int64_t)a.cache.kv_heads * p.chunks, 4);
+  p.chunks = ms::k4_divisor(a.cache.head_dim / 8);
+  p.token = ms::k4_divisor((int64_t)a.cache.kv_heads * p.chunks.d);
+  p.tokens = ms::k4_tokens(a.tokens, p.token.d, 4);
   p.wide = ((a.k_token | a.k_head | a.v_token | a.v_head) & 7) == 0 &&
            ((reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out)) & 15) == 0;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
