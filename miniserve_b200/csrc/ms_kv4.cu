@@ -43,6 +43,16 @@ __device__ __forceinline__ float k4_min(float x, float y) {  // a NaN stays
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
   return r;
 }
+__device__ __forceinline__ float k4_min3(float x, float y, float z) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+__device__ __forceinline__ float k4_max3(float x, float y, float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 __device__ __forceinline__ float k4_max(float x, float y) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
@@ -236,7 +246,7 @@ __device__ __forceinline__ uint32_t k4_encode(const float (&y)[8], bool inside, 
   float lo = __uint_as_float(0x7F800000u), hi = -lo;
   if (inside) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) lo = k4_min(lo, y[i]), hi = k4_max(hi, y[i]);
+    for (int i = 0; i < 8; i += 2) lo = k4_min3(lo, y[i], y[i + 1]), hi = k4_max3(hi, y[i], y[i + 1]);
   }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
@@ -301,11 +311,11 @@ __device__ __forceinline__ void k4_quantise(const K4AppendArgs &p, int *flags) {
     }
     uint32_t word[2];
     __half2 param[2];
-    bool lost[2];
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-      word[side] = k4_encode(y[side], inside, param[side], lost[side]);
-      if (lost[side]) status |= MS_ROW_NONFINITE;
+      bool lost;
+      word[side] = k4_encode(y[side], inside, param[side], lost);
+      if (lost) status |= MS_ROW_NONFINITE;
     }
     if (write) {
       int64_t page, offset;
@@ -347,6 +357,7 @@ struct K4ReadArgs {
   int page_shift;
   int tokens;  // tokens of a block
   int wide;    // outputs are stored in 16 bytes
+  int slots, heads;         // threads' heads of a token: h, and h + slots where heads is 2
   K4Divisor chunks, token;  // of a head's 8-entry chunks, and of a token's
 };
 
@@ -387,7 +398,8 @@ __device__ __forceinline__ void k4_decode(uint32_t word, __half2 param, uint32_t
   }
 }
 
-// A thread takes 8 entries of a key head and the same 8 of its value head.
+// A thread takes 8 entries of a key head and the same 8 of its value head, of one
+// or two heads.
 template <typename T>
 __global__ void __launch_bounds__(kK4Threads) ms_kv4_read_kernel(const __grid_constant__ K4ReadArgs p) {
   grid_wait();
@@ -400,35 +412,45 @@ __global__ void __launch_bounds__(kK4Threads) ms_kv4_read_kernel(const __grid_co
     const int64_t t = t0 + tl, slot = load_in(a.slots + t);
     const bool bad = slot >= a.cache.pages * a.cache.page_size, live = slot >= 0 && !bad;
     if (w == 0 && a.status) a.status[t] = bad ? MS_ROW_BAD_SLOT : MS_ROW_OK;
-    uint32_t word[2] = {0, 0};
-    __half2 param[2];
-    param[0] = param[1] = __halves2half2(__float2half_rn(0.f), __float2half_rn(0.f));
-    if (live) {
-      int64_t page, offset;
-      kv_place(slot, a.cache.page_size, p.page_shift, page, offset);
-      const int64_t row = (page * a.cache.kv_heads + h) * a.cache.page_size + offset;
-      const int64_t code_at = row * p.layout.row_bytes + chunk * 4, param_at = row * p.layout.groups + (chunk >> 2);
-      word[0] = load_in(reinterpret_cast<const uint32_t *>(a.cache.k_codes + code_at));
-      word[1] = load_in(reinterpret_cast<const uint32_t *>(a.cache.v_codes + code_at));
-      param[0] = load_in(static_cast<const __half2 *>(a.cache.k_params) + param_at);
-      param[1] = load_in(static_cast<const __half2 *>(a.cache.v_params) + param_at);
+    int64_t page = 0, offset = 0;
+    if (live) kv_place(slot, a.cache.page_size, p.page_shift, page, offset);
+    const int64_t row = (page * a.cache.kv_heads + h) * a.cache.page_size + offset;
+    const int64_t code_at = row * p.layout.row_bytes + chunk * 4, param_at = row * p.layout.groups + (chunk >> 2);
+    uint32_t word[2][2];
+    __half2 param[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // all loads first
+      word[i][0] = word[i][1] = 0;
+      param[i][0] = param[i][1] = __halves2half2(__float2half_rn(0.f), __float2half_rn(0.f));
+      if (live && (i == 0 || (p.heads > 1 && h + p.slots < a.cache.kv_heads))) {
+        const int64_t rows = i * p.slots * a.cache.page_size;
+        word[i][0] = load_in(reinterpret_cast<const uint32_t *>(a.cache.k_codes + code_at + rows * p.layout.row_bytes));
+        word[i][1] = load_in(reinterpret_cast<const uint32_t *>(a.cache.v_codes + code_at + rows * p.layout.row_bytes));
+        param[i][0] = load_in(static_cast<const __half2 *>(a.cache.k_params) + param_at + rows * p.layout.groups);
+        param[i][1] = load_in(static_cast<const __half2 *>(a.cache.v_params) + param_at + rows * p.layout.groups);
+      }
     }
+    T *k = static_cast<T *>(a.k_out) + t * a.k_token + h * a.k_head + chunk * 8;
+    T *v = static_cast<T *>(a.v_out) + t * a.v_token + h * a.v_head + chunk * 8;
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      T *dst = side ? static_cast<T *>(a.v_out) + t * a.v_token + h * a.v_head
-                    : static_cast<T *>(a.k_out) + t * a.k_token + h * a.k_head;
-      dst += chunk * 8;
-      uint32_t out[4];
-      k4_decode<T>(word[side], param[side], out);
-      if (p.wide) {
-        *reinterpret_cast<uint4 *>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
-      } else {
+    for (int i = 0; i < 2; ++i) {
+      if (i == 1 && !(p.heads > 1 && h + p.slots < a.cache.kv_heads)) break;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const T *pair = reinterpret_cast<const T *>(&out[i]);
-          dst[2 * i] = pair[0], dst[2 * i + 1] = pair[1];
+      for (int side = 0; side < 2; ++side) {
+        T *dst = side ? v : k;
+        uint32_t out[4];
+        k4_decode<T>(word[i][side], param[i][side], out);
+        if (p.wide) {
+          *reinterpret_cast<uint4 *>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const T *pair = reinterpret_cast<const T *>(&out[j]);
+            dst[2 * j] = pair[0], dst[2 * j + 1] = pair[1];
+          }
         }
       }
+      k += p.slots * a.k_head, v += p.slots * a.v_head;
     }
   }
 }
@@ -514,7 +536,9 @@ int ms_kv4_read(const ms_kv4_read_args *args, ms_stream_t stream) {
   p.layout = ms::k4_layout(a.cache.head_dim);
   p.page_shift = ms::kv_page_shift(a.cache.page_size);
   p.chunks = ms::k4_divisor(a.cache.head_dim / 8);
-  p.token = ms::k4_divisor((int64_t)a.cache.kv_heads * p.chunks.d);
+  p.heads = a.tokens * a.cache.kv_heads * p.chunks.d > 4ll * 148 * 2048 ? 2 : 1;
+  p.slots = (a.cache.kv_heads + p.heads - 1) / p.heads;
+  p.token = ms::k4_divisor((int64_t)p.slots * p.chunks.d);
   p.tokens = ms::k4_tokens(a.tokens, p.token.d, 4);
   p.wide = ((a.k_token | a.k_head | a.v_token | a.v_head) & 7) == 0 &&
            ((reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out)) & 15) == 0;
