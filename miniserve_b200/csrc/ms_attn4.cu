@@ -20,19 +20,10 @@ namespace ms {
 static int64_t a4_round(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct A4Plan {
-  int group, queries, chunks, chunk_rows, eights;
+  int group, queries, chunks, chunk_rows, sixteens;  // sixteens of the wide kernel, or 0
   int64_t split_warps;
   int64_t base, own_o, own_ml, bytes;  // workspace: a header, the rows' first units, the records
 };
-
-// CTAs of an SM that the kernel of these sizes is built for.
-static int a4_ctas(int groups, int eights) {
-  if (groups <= 2) {
-    constexpr int ctas[5] = {kA4Ctas<2, 1>, kA4Ctas<2, 2>, kA4Ctas<2, 3>, kA4Ctas<2, 4>, kA4Ctas<2, 5>};
-    return ctas[eights - 1];
-  }
-  return eights == 1 ? kA4Ctas<4, 1> : kA4Ctas<4, 2>;
-}
 
 static A4Plan a4_plan(int64_t rows, int tokens, int heads, int kv_heads, int head_dim, int sms) {
   A4Plan p{};
@@ -42,8 +33,8 @@ static A4Plan a4_plan(int64_t rows, int tokens, int heads, int kv_heads, int hea
   // as few items as hold all query rows, and those of equal sizes
   p.chunks = (p.queries + a4_most(groups) - 1) / a4_most(groups);
   p.chunk_rows = (p.queries + p.chunks - 1) / p.chunks;
-  p.eights = (p.chunk_rows + 7) / 8;
-  p.split_warps = (int64_t)sms * a4_ctas(groups, p.eights) * kA4Warps;
+  p.sixteens = p.chunk_rows <= kA4Narrow ? 0 : (p.chunk_rows + 15) / 16;
+  p.split_warps = (int64_t)sms * (p.sixteens ? a4_wide_ctas(groups, p.sixteens) : a4_narrow_ctas(groups)) * kA4Warps;
   const int64_t pieces = rows * kv_heads * p.chunks + p.split_warps;
   int64_t at = 256;  // A4Header
   p.base = at, at = a4_round(at + rows * 8);
@@ -65,29 +56,39 @@ static bool a4_sizes(int64_t rows, int32_t tokens, int32_t heads, int32_t kv_hea
          rows * tokens * heads <= 0x7FFFFFFFll;
 }
 
-template <int NG, int NQ, bool kWhole>
-static cudaError_t a4_split(const A4Args &a, int dev, cudaStream_t s) {
-  static std::atomic<int> ready[kMaxDevices];
+template <typename K>
+static cudaError_t a4_launch(K *kernel, int shared, std::atomic<int> (&ready)[kMaxDevices], const A4Args &a, int dev, cudaStream_t s) {
   if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
-  auto *kernel = ms_attn4_split_kernel<NG, NQ, kWhole>;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kA4Shared<NG, NQ>);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
     if (e != cudaSuccess) return e;
     ready[dev].store(1, std::memory_order_release);
   }
-  return launch_dependent(kernel, (unsigned)(a.split_warps / kA4Warps), kA4Warps * 32, kA4Shared<NG, NQ>, s, a);
+  return launch_dependent(kernel, (unsigned)(a.split_warps / kA4Warps), kA4Warps * 32, shared, s, a);
 }
-template <int NG>
-static cudaError_t a4_split_as(const A4Args &a, int eights, int dev, cudaStream_t s) {
-  const bool whole = a.x.cache.page_size % kA4Half == 0;
-  if (eights == 1) return whole ? a4_split<NG, 1, true>(a, dev, s) : a4_split<NG, 1, false>(a, dev, s);
-  if (eights == 2) return whole ? a4_split<NG, 2, true>(a, dev, s) : a4_split<NG, 2, false>(a, dev, s);
+template <int NG, bool kWhole>
+static cudaError_t a4_narrow(const A4Args &a, int dev, cudaStream_t s) {
+  static std::atomic<int> ready[kMaxDevices];
+  return a4_launch(ms_attn4_narrow_kernel<NG, kWhole>, kA4NarrowShared<NG>, ready, a, dev, s);
+}
+template <int NG, int NP, bool kWhole>
+static cudaError_t a4_wide(const A4Args &a, int dev, cudaStream_t s) {
+  static std::atomic<int> ready[kMaxDevices];
+  return a4_launch(ms_attn4_wide_kernel<NG, NP, kWhole>, kA4WideShared<NG, NP>, ready, a, dev, s);
+}
+template <int NG, bool kWhole>
+static cudaError_t a4_split(const A4Args &a, int sixteens, int dev, cudaStream_t s) {
+  if (sixteens == 0) return a4_narrow<NG, kWhole>(a, dev, s);
+  if (sixteens == 1) return a4_wide<NG, 1, kWhole>(a, dev, s);
   if constexpr (NG <= 2) {
-    if (eights == 3) return whole ? a4_split<NG, 3, true>(a, dev, s) : a4_split<NG, 3, false>(a, dev, s);
-    if (eights == 5) return whole ? a4_split<NG, 5, true>(a, dev, s) : a4_split<NG, 5, false>(a, dev, s);
-    if (eights == 4) return whole ? a4_split<NG, 4, true>(a, dev, s) : a4_split<NG, 4, false>(a, dev, s);
+    if (sixteens == 2) return a4_wide<NG, 2, kWhole>(a, dev, s);
+    if (sixteens == 3) return a4_wide<NG, 3, kWhole>(a, dev, s);
   }
   return cudaErrorInvalidValue;
+}
+template <int NG>
+static cudaError_t a4_split_as(const A4Args &a, int sixteens, int dev, cudaStream_t s) {
+  return a.x.cache.page_size % kA4Half == 0 ? a4_split<NG, true>(a, sixteens, dev, s) : a4_split<NG, false>(a, sixteens, dev, s);
 }
 template <typename T, int DP>
 static cudaError_t a4_merge(const A4Args &a, cudaStream_t s) {
@@ -144,16 +145,15 @@ int ms_kv4_attention(const ms_kv4_attention_args *args, ms_stream_t stream) {
   for (int i = 0; i < 31; ++i)
     if (x.cache.page_size == 1ll << i) a.page_shift = i;
   {  // records that an output may have: the warps spread over the items, but no more than the longest has room for
-    a.tile = ms::kA4Half * (p.eights == 1 ? ms::kA4Halves<1> : ms::kA4Halves<2>);
-    const int64_t items = x.rows * x.cache.kv_heads * p.chunks, tiles = (x.table_width * x.cache.page_size + a.tile - 1) / a.tile;
+      const int64_t items = x.rows * x.cache.kv_heads * p.chunks, tiles = (x.table_width * x.cache.page_size + ms::kA4Tile - 1) / ms::kA4Tile;
     a.merge_wide = std::min(p.split_warps / items + 1, (tiles + ms::kA4Item) / (ms::kA4Item + 1) + 1) > 24;
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   switch (a.layout.used) {
-    case 1: e = ms::a4_split_as<1>(a, p.eights, dev, s); break;
-    case 2: e = ms::a4_split_as<2>(a, p.eights, dev, s); break;
-    case 3: e = ms::a4_split_as<3>(a, p.eights, dev, s); break;
-    default: e = ms::a4_split_as<4>(a, p.eights, dev, s); break;
+    case 1: e = ms::a4_split_as<1>(a, p.sixteens, dev, s); break;
+    case 2: e = ms::a4_split_as<2>(a, p.sixteens, dev, s); break;
+    case 3: e = ms::a4_split_as<3>(a, p.sixteens, dev, s); break;
+    default: e = ms::a4_split_as<4>(a, p.sixteens, dev, s); break;
   }
   if (e == cudaSuccess) {
     const bool narrow = x.cache.head_dim <= 64;
