@@ -25,15 +25,16 @@ struct A4Plan {
   int64_t base, own_o, own_ml, bytes;  // workspace: a header, the rows' first units, the records
 };
 
-static A4Plan a4_plan(int64_t rows, int tokens, int heads, int kv_heads, int head_dim, int sms) {
+static A4Plan a4_plan(int64_t rows, int tokens, int heads, int kv_heads, int head_dim, bool fine, int sms) {
   A4Plan p{};
   const int groups = k4_layout(head_dim).used;
   p.group = heads / kv_heads;
   p.queries = tokens * p.group;
   // as few items as hold all query rows, and those of equal sizes
-  p.chunks = (p.queries + a4_most(groups) - 1) / a4_most(groups);
+  p.chunks = (p.queries + a4_most(groups, fine) - 1) / a4_most(groups, fine);
   p.chunk_rows = (p.queries + p.chunks - 1) / p.chunks;
-  p.sixteens = p.chunk_rows <= kA4Narrow ? 0 : (p.chunk_rows + 15) / 16;
+  const int sixteen = fine ? 8 : 16;
+  p.sixteens = p.chunk_rows <= a4_narrow(fine) ? 0 : (p.chunk_rows + sixteen - 1) / sixteen;
   p.split_warps = (int64_t)sms * (p.sixteens ? a4_wide_ctas(groups, p.sixteens) : a4_narrow_ctas(groups)) * kA4Warps;
   const int64_t pieces = rows * kv_heads * p.chunks + p.split_warps;
   int64_t at = 256;  // A4Header
@@ -66,29 +67,32 @@ static cudaError_t a4_launch(K *kernel, int shared, std::atomic<int> (&ready)[kM
   }
   return launch_dependent(kernel, (unsigned)(a.split_warps / kA4Warps), kA4Warps * 32, shared, s, a);
 }
-template <int NG, bool kWhole>
-static cudaError_t a4_narrow(const A4Args &a, int dev, cudaStream_t s) {
+template <int NG, bool kFine, bool kWhole>
+static cudaError_t a4_split_narrow(const A4Args &a, int dev, cudaStream_t s) {
   static std::atomic<int> ready[kMaxDevices];
-  return a4_launch(ms_attn4_narrow_kernel<NG, kWhole>, kA4NarrowShared<NG>, ready, a, dev, s);
+  return a4_launch(ms_attn4_narrow_kernel<NG, kFine, kWhole>, kA4NarrowShared<NG>, ready, a, dev, s);
 }
-template <int NG, int NP, bool kWhole>
-static cudaError_t a4_wide(const A4Args &a, int dev, cudaStream_t s) {
+template <int NG, int NP, bool kFine, bool kWhole>
+static cudaError_t a4_split_wide(const A4Args &a, int dev, cudaStream_t s) {
   static std::atomic<int> ready[kMaxDevices];
-  return a4_launch(ms_attn4_wide_kernel<NG, NP, kWhole>, kA4WideShared<NG, NP>, ready, a, dev, s);
+  return a4_launch(ms_attn4_wide_kernel<NG, NP, kFine, kWhole>, kA4WideShared<NG, NP>, ready, a, dev, s);
 }
-template <int NG, bool kWhole>
+template <int NG, bool kFine, bool kWhole>
 static cudaError_t a4_split(const A4Args &a, int sixteens, int dev, cudaStream_t s) {
-  if (sixteens == 0) return a4_narrow<NG, kWhole>(a, dev, s);
-  if (sixteens == 1) return a4_wide<NG, 1, kWhole>(a, dev, s);
+  if (sixteens == 0) return a4_split_narrow<NG, kFine, kWhole>(a, dev, s);
+  if (sixteens == 1) return a4_split_wide<NG, 1, kFine, kWhole>(a, dev, s);
   if constexpr (NG <= 2) {
-    if (sixteens == 2) return a4_wide<NG, 2, kWhole>(a, dev, s);
-    if (sixteens == 3) return a4_wide<NG, 3, kWhole>(a, dev, s);
+    if (sixteens == 2) return a4_split_wide<NG, 2, kFine, kWhole>(a, dev, s);
+    if (sixteens == 3) return a4_split_wide<NG, 3, kFine, kWhole>(a, dev, s);
   }
   return cudaErrorInvalidValue;
 }
 template <int NG>
 static cudaError_t a4_split_as(const A4Args &a, int sixteens, int dev, cudaStream_t s) {
-  return a.x.cache.page_size % kA4Half == 0 ? a4_split<NG, true>(a, sixteens, dev, s) : a4_split<NG, false>(a, sixteens, dev, s);
+  const bool whole = a.x.cache.page_size % kA4Half == 0;
+  if (a.x.dtype == MS_DTYPE_F16)
+    return whole ? a4_split<NG, true, true>(a, sixteens, dev, s) : a4_split<NG, true, false>(a, sixteens, dev, s);
+  return whole ? a4_split<NG, false, true>(a, sixteens, dev, s) : a4_split<NG, false, false>(a, sixteens, dev, s);
 }
 template <typename T, int DP>
 static cudaError_t a4_merge(const A4Args &a, cudaStream_t s) {
@@ -106,7 +110,9 @@ int64_t ms_kv4_attention_workspace(int64_t rows, int32_t tokens, int32_t heads, 
   if (!ms::a4_sizes(rows, tokens, heads, kv_heads, head_dim)) return 0;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  return ms::a4_plan(rows, tokens, heads, kv_heads, head_dim, ms::a4_sms(dev)).bytes;
+  const int sms = ms::a4_sms(dev);  // of either type
+  return std::max(ms::a4_plan(rows, tokens, heads, kv_heads, head_dim, false, sms).bytes,
+                  ms::a4_plan(rows, tokens, heads, kv_heads, head_dim, true, sms).bytes);
 }
 
 int ms_kv4_attention(const ms_kv4_attention_args *args, ms_stream_t stream) {
@@ -125,7 +131,7 @@ int ms_kv4_attention(const ms_kv4_attention_args *args, ms_stream_t stream) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return ms::cuda_fail(e);
-  const ms::A4Plan p = ms::a4_plan(x.rows, x.tokens, x.heads, x.cache.kv_heads, x.cache.head_dim, ms::a4_sms(dev));
+  const ms::A4Plan p = ms::a4_plan(x.rows, x.tokens, x.heads, x.cache.kv_heads, x.cache.head_dim, x.dtype == MS_DTYPE_F16, ms::a4_sms(dev));
   if (x.workspace_bytes < p.bytes) return MS_E_INVALID;
   ms::A4Args a{};
   a.x = x;
@@ -145,7 +151,8 @@ int ms_kv4_attention(const ms_kv4_attention_args *args, ms_stream_t stream) {
   for (int i = 0; i < 31; ++i)
     if (x.cache.page_size == 1ll << i) a.page_shift = i;
   {  // records that an output may have: the warps spread over the items, but no more than the longest has room for
-      const int64_t items = x.rows * x.cache.kv_heads * p.chunks, tiles = (x.table_width * x.cache.page_size + ms::kA4Tile - 1) / ms::kA4Tile;
+      const int64_t items = x.rows * x.cache.kv_heads * p.chunks;
+      const int64_t tiles = (x.table_width * x.cache.page_size + ms::kA4Tile - 1) / ms::kA4Tile;
     a.merge_wide = std::min(p.split_warps / items + 1, (tiles + ms::kA4Item) / (ms::kA4Item + 1) + 1) > 24;
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

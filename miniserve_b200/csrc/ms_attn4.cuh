@@ -23,12 +23,12 @@ constexpr float kA4Least = -3e38f;         // refers to nothing yet: every score
 constexpr int64_t kA4MaxRows = 1 << 20;
 constexpr int kA4MaxTokens = 1024;         // of a row
 // Query rows of an item: up to eight in the narrow kernel, in the wide one as many
-// sixteens as registers have room for.  64 rows of ragged keys, eight queries a
-// key head: 62 us narrow, 86 us wide (half of each product is empty).  128 rows
-// of five tokens and seven heads a key head: 65 us as one item of three
-// sixteens, 80 us as two of two, 69 us as three of one.
-constexpr int kA4Narrow = 8;
-__host__ __device__ constexpr int a4_most(int groups) { return groups <= 2 ? 48 : 16; }
+// sixteens as registers have room for; half of them where a query takes two rows
+// (`fine`, below).  Two rows of 131072 keys, four queries a key head: 86 us narrow,
+// 127 us wide.  128 rows of five tokens and seven heads a key head: 66 us as one
+// item of three sixteens, 80 us as two of two, 69 us as three of one.
+__host__ __device__ constexpr int a4_narrow(bool fine) { return fine ? 4 : 8; }
+__host__ __device__ constexpr int a4_most(int groups, bool fine) { return (groups <= 2 ? 48 : 16) >> (fine ? 1 : 0); }
 // Split CTAs of an SM, by what their registers allow.
 __host__ __device__ constexpr int a4_narrow_ctas(int groups) { return groups <= 2 ? 4 : 3; }
 __host__ __device__ constexpr int a4_wide_ctas(int groups, int sixteens) { return groups <= 2 && sixteens <= 1 ? 3 : 2; }
@@ -156,6 +156,22 @@ __device__ __forceinline__ uint32_t a4_turn(uint32_t x) {
 __device__ __forceinline__ uint32_t a4_pack(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
   return *reinterpret_cast<const uint32_t *>(&h);
+}
+// Of halves, subnormal ones too.
+__device__ __forceinline__ uint32_t a4_add(uint32_t x, uint32_t y) {
+  uint32_t z;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
+  return z;
+}
+// Two weights as fp16, less what `rest` has of them as such: where it is all ones,
+// what their rounding left.
+template <bool kFine>
+__device__ __forceinline__ uint32_t a4_weights(float x, float y, uint32_t rest) {
+  const uint32_t whole = a4_pack(x, y);
+  if (!kFine) return whole;
+  const uint32_t less = whole & rest;
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&less));
+  return a4_pack(x - f.x, y - f.y);
 }
 __device__ __forceinline__ float a4_low(uint32_t u) { return __low2float(*reinterpret_cast<const __half2 *>(&u)); }
 
@@ -521,20 +537,27 @@ __device__ __forceinline__ bool a4_none(uint32_t u) {
 //
 // K: s_g weighs a group's sums in fp32; the rest is one more product, of the
 // parameters as they lie with the queries' sums in two fp16 halves.  V: p s_g is
-// rounded to fp16 once, -8 times the same rounded weights is one more product
-// with constants, so that a weight's rounding meets c - 8 and not c; the middles
-// are one product with p.
+// rounded to fp16 once, and its rounding meets c - 8 and not c: the narrow kernel
+// adds -8 times the same rounded weights, one more product with constants, the
+// wide one subtracts 8 from the codes, which are many products' operands there.
+// Either keeps the sums small: what a product's sum loses at its end would else
+// grow with the keys.  The middles are one product with p.
 //
 // Queries' entries are off by 2^-26 of a row's largest at most.  Weights are at
 // most 2^8 of what they refer to (it moves only when a score passes it by 2^8),
 // scaled up by 2^7 (and up to 2^0.5: references are whole numbers), and by the
 // power of two below 1 over the largest value scale met, so that fp16 holds them
-// with 2^-21 and less of the largest at full precision.
+// with 2^-21 and less of the largest at full precision.  p s_g and p are off by
+// 2^-12 of themselves, which beside a bf16 answer's own 2^-9 is nothing and beside
+// an fp16 answer's 2^-12 is as much again: for fp16 (kFine) a query takes two rows
+// of a product, one of its weights and one of what rounding left of them (2^-23),
+// and their sums are added at the end (64 ragged rows, four queries a key head: 62
+// -> 67 us; the answers' error from 1.5 of what rounding them costs to 1.0).
 //
 // Narrow: up to eight query rows, S^T = K Q^T and O^T += V^T P^T, keys and values
 // as A, so that no half of a product is empty; P^T changes fragments with
-// movmatrix.
-template <int NG, bool kWhole>
+// movmatrix.  kFine: four, columns 4 to 7 being what rounding left of 0 to 3.
+template <int NG, bool kFine, bool kWhole>
 __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
     ms_attn4_narrow_kernel(const __grid_constant__ A4Args a) {
   using R = A4Ring<NG>;
@@ -552,6 +575,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
   const int hcs = x.cache.kv_heads * a.chunks;
   const bool scale_lane = (r & 1) == 0 && r < 2 * NG;  // its rows of the values' parameters are scales
   uint32_t qf[NG][4], qs[2];  // query r's operands
+  const uint32_t rest = kFine && c >= 2 ? 0xFFFFFFFFu : 0u;
   float o[2 * NG][4];         // entries 32 g + 4 r + 2 i (0, 1) and the next (2, 3), of queries 2c and 2c + 1
   float z[2];                 // the middles' part: row r is parameter r of a key
   // of queries 2c and 2c + 1: what a score of 2^-24 is in units of log2, the score that weights refer to, the one past
@@ -569,16 +593,16 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
     if (fresh) {
       const int h = now.hc / a.chunks, first = (now.hc - h * a.chunks) * a.chunk_rows;
       n = min(a.chunk_rows, a.queries - first);
-      const int q = first + (r < n ? r : 0), token = q / a.group;
+      const int own = r & (a4_narrow(kFine) - 1), q = first + (own < n ? own : 0), token = q / a.group;
       float sum[NG], down;
       uint32_t u[NG][4];
-      a4_query_load<NG>(a, r < n, now.b * x.q_row + token * x.q_token + (h * a.group + q - token * a.group) * x.q_head, u);
+      a4_query_load<NG>(a, own < n, now.b * x.q_row + token * x.q_token + (h * a.group + q - token * a.group) * x.q_head, u);
       a4_query<NG>(a, u, qf, sum, down);
       a4_sums<NG>(sum, qs[0], qs[1]);
       least = 0x7FFFFFFF;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {  // of the queries that this lane's columns of a product are
-        const int g = 2 * c + i;
+        const int g = (2 * c + i) & (a4_narrow(kFine) - 1);
         unit[i] = a4_unit(a.scale_log2 * 0x1p24f * __shfl_sync(0xFFFFFFFFu, down, g * 4));
         len[i] = g < n ? load_in(x.lengths + now.b * x.length_row + (first + g) / a.group) : 0x7FFFFFFF;
         least = min(least, len[i]);
@@ -742,15 +766,16 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
       float w[4] = {sc[hf][0], sc[hf][1], sc[hf][2], sc[hf][3]};
       l[0] += w[0] + w[2];
       l[1] += w[1] + w[3];
-      a4_mma_top(z, vp[hf][0], vp[hf][1], a4_turn(a4_pack(w[0], w[1])), a4_turn(a4_pack(w[2], w[3])));
+      a4_mma_top(z, vp[hf][0], vp[hf][1], a4_turn(a4_weights<kFine>(w[0], w[1], rest)),
+                 a4_turn(a4_weights<kFine>(w[2], w[3], rest)));
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] *= v_scale.unit;
       uint32_t pw[NG][2];  // weights times the groups' scales as B: keys 2c and 2c + 1 of query r, then keys + 8
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const float s0 = a4_low(vr[0][g]), s1 = a4_low(vr[1][g]);
-        pw[g][0] = a4_turn(a4_pack(w[0] * s0, w[1] * s0));
-        pw[g][1] = a4_turn(a4_pack(w[2] * s1, w[3] * s1));
+        pw[g][0] = a4_turn(a4_weights<kFine>(w[0] * s0, w[1] * s0, rest));
+        pw[g][1] = a4_turn(a4_weights<kFine>(w[2] * s1, w[3] * s1, rest));
       }
       // -8 2^-24 and -8 2^-20, of the rows whose codes are in the lower and the upper nibble; then the codes
 #pragma unroll
@@ -773,6 +798,17 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
     if (++stage == kA4Stages) stage = 0;
     if (++now.tile < now.end) continue;
     const int64_t piece = (int64_t)now.b * hcs + now.hc + (int64_t)blockIdx.x * kA4Warps + warp;
+    if (kFine) {  // lanes c and c + 2 have the same queries
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        z[i] += __shfl_xor_sync(0xFFFFFFFFu, z[i], 2);
+#pragma unroll
+        for (int k = 0; k < 2 * NG; ++k) {
+          o[k][i] += __shfl_xor_sync(0xFFFFFFFFu, o[k][i], 2);
+          o[k][2 + i] += __shfl_xor_sync(0xFFFFFFFFu, o[k][2 + i], 2);
+        }
+      }
+    }
     const float low = 0x1p17f / v_scale.unit, up = 0x1p13f / v_scale.unit;  // 2^24 and 2^20 without the weights' 2^7
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -805,11 +841,13 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
 // lane's.  A code is made an operand once for all sixteens: with operands of
 // eight queries each (movmatrix for every weight) 128 rows of five tokens took 82
 // us.  All queries of an item are loaded before the first is used (one after
-// another: 73 us, now 65).
-template <int NG, int NP, bool kWhole>
+// another: 73 us, now 66).  kFine: eight queries a sixteen, row r + 8 being what
+// rounding left of row r.
+template <int NG, int NP, bool kFine, bool kWhole>
 __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
     ms_attn4_wide_kernel(const __grid_constant__ A4Args a) {
   using R = A4Ring<NG>;
+  constexpr int kOwn = kFine ? 1 : 2;  // a lane's queries of a sixteen
   constexpr int kPitch = R::kPitch, kStage = R::kStage;
   const float kNone = __uint_as_float(0xFF800000u);
   extern __shared__ __align__(128) unsigned char a4_ring[];
@@ -827,12 +865,8 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
   const int hcs = x.cache.kv_heads * a.chunks;
   const bool scale_lane = (r & 1) == 0 && r < 2 * NG;
   float o[NP][NG][4][4];      // entries 32 g + 8 c + i (0) and + 4 + i (1) of row r, then of row r + 8
-  float eights[NP][4];        // -8 2^-24 times the sums of weights times scales of group c, of row r (0) and row r + 8 (2)
   float z[NP][4];             // the scales' and the middles' parts of group c, of row r, then of row r + 8
-  float unit[NP][2], lim[NP][2], base[NP][2], l[NP][2];  // as m
-  uint32_t eight[NG];         // -8 2^-24 in column 2 g alone
-#pragma unroll
-  for (int g = 0; g < NG; ++g) eight[g] = r == 2 * g ? 0x80088008u : 0u;
+  float unit[NP][kOwn], lim[NP][kOwn], base[NP][kOwn], l[NP][kOwn];  // as m
   int least = 0, n = 0;
   A4Scale v_scale;
   bool far = false, fresh = true, broken = false;
@@ -843,27 +877,29 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
       const int h = now.hc / a.chunks, first = (now.hc - h * a.chunks) * a.chunk_rows;
       n = min(a.chunk_rows, a.queries - first);
       least = 0x7FFFFFFF;
-      uint32_t u[NP][2][NG][4];  // all loads before the first is waited for
+      uint32_t u[NP][kOwn][NG][4];  // all loads before the first is waited for
 #pragma unroll
       for (int t = 0; t < NP; ++t)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int g = t * 16 + r + 8 * i, q = first + (g < n ? g : 0), token = q / a.group;
+        for (int i = 0; i < kOwn; ++i) {
+          const int g = (t * kOwn + i) * 8 + r, q = first + (g < n ? g : 0), token = q / a.group;
           a4_query_load<NG>(a, g < n, now.b * x.q_row + token * x.q_token + (h * a.group + q - token * a.group) * x.q_head, u[t][i]);
           if (g < n) least = min(least, load_in(x.lengths + now.b * x.length_row + token));
         }
 #pragma unroll
       for (int t = 0; t < NP; ++t) {
-        uint32_t f[2][NG][4], parts[4];
+        uint32_t f[2][NG][4] = {}, parts[4] = {};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kOwn; ++i) {
           float sum[NG], down;
           a4_query<NG>(a, u[t][i], f[i], sum, down);
           a4_sums<NG>(sum, parts[i], parts[2 + i]);
           unit[t][i] = a4_unit(a.scale_log2 * down);
           lim[t][i] = kA4Least;
-          base[t][i] = l[t][i] = z[t][i] = z[t][2 + i] = eights[t][i] = eights[t][2 + i] = 0.f;
+          base[t][i] = l[t][i] = 0.f;
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[t][i] = 0.f;
         qs[t * 32] = make_uint4(parts[0], parts[1], parts[2], parts[3]);
         m[t * 32] = make_float2(kA4Least, kA4Least);
 #pragma unroll
@@ -891,7 +927,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
       const int j0 = now.tile * kA4Tile + hf * kA4Half;
       if (j0 >= now.keys) break;
       unsigned char *kps = here + R::kKp + hf * kA4Half * 16, *vps = here + R::kVp + hf * kA4Half * 16;
-      float sc[NP][2][4];  // keys 8 j + 2c and the next, of row r, then of row r + 8
+      float sc[NP][2][2 * kOwn];  // keys 8 j + 2c and the next, of row r, then of row r + 8
       {
         uint32_t p[2];
         ldmatrix2(p, smem_addr(kps) + (lane & 15) * 16);
@@ -901,7 +937,12 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
         for (int t = 0; t < NP; ++t) {
           const uint4 q = qs[t * 32];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) a4_mma(sc[t][j], q.x, q.y, q.z, q.w, p[j], p[j], 0.f, 0.f);
+          for (int j = 0; j < 2; ++j) {
+            float d[4];
+            a4_mma(d, q.x, q.y, q.z, q.w, p[j], p[j], 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 2 * kOwn; ++i) sc[t][j][i] = d[i];
+          }
         }
         float2 s[2][NG];  // scales of keys 8 j + 2c and the next
 #pragma unroll
@@ -924,7 +965,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-              for (int i = 0; i < 4; i += 2) {
+              for (int i = 0; i < 2 * kOwn; i += 2) {
                 const float2 y = at_fma2(s[j][g], make_float2(d[j][i], d[j][i + 1]), make_float2(sc[t][j][i], sc[t][j][i + 1]));
                 sc[t][j][i] = y.x, sc[t][j][i + 1] = y.y;
               }
@@ -946,8 +987,8 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
 #pragma unroll
         for (int t = 0; t < NP; ++t) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int g = t * 16 + r + 8 * i;
+          for (int i = 0; i < kOwn; ++i) {
+            const int g = (t * kOwn + i) * 8 + r;
             const int len = min(now.keys, g < n ? load_in(x.lengths + now.b * x.length_row + (first + g) / a.group) : 0x7FFFFFFF);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -977,7 +1018,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
 #pragma unroll
       for (int t = 0; t < NP; ++t)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < kOwn; ++i)
           moves = moves || fmaxf(fmaxf(sc[t][0][2 * i], sc[t][0][2 * i + 1]), fmaxf(sc[t][1][2 * i], sc[t][1][2 * i + 1])) > lim[t][i];
       if (__any_sync(0xFFFFFFFFu, moves)) {
         const float factor = v_scale.fit(a4_largest(vp, scale_lane));
@@ -986,7 +1027,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
 #pragma unroll
         for (int t = 0; t < NP; ++t)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < kOwn; ++i) {
             float y = fmaxf(fmaxf(sc[t][0][2 * i], sc[t][0][2 * i + 1]), fmaxf(sc[t][1][2 * i], sc[t][1][2 * i + 1]));
             y = fmaxf(y, __shfl_xor_sync(0xFFFFFFFFu, y, 1));
             y = fmaxf(y, __shfl_xor_sync(0xFFFFFFFFu, y, 2));
@@ -998,72 +1039,86 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
 #pragma unroll
         for (int t = 0; t < NP; ++t)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < kOwn; ++i) {
             const float whole = rintf(top[t][i] * unit[t][i]);
             const float f = a4_moved(old[t][i], 7.f - base[t][i], far, top[t][i], whole, next_far, unit[t][i]);
             lim[t][i] = top[t][i] == kA4Least ? kA4Least : top[t][i] + 8.f / unit[t][i];
             base[t][i] = next_far ? 7.f : 7.f - whole;
             l[t][i] *= f;
-            z[t][2 * i] *= f, z[t][2 * i + 1] *= f;
             const float fo = f * factor;
-            eights[t][2 * i] *= fo;
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
+            for (int e = 2 * i; e < (kFine ? 4 : 2 * i + 2); ++e) {
+              z[t][e] *= f;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) o[t][g][k][2 * i] *= fo, o[t][g][k][2 * i + 1] *= fo;
+              for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[t][g][k][e] *= fo;
+            }
           }
         far = next_far;
 #pragma unroll
-        for (int t = 0; t < NP; ++t) m[t * 32] = make_float2(top[t][0], top[t][1]);
+        for (int t = 0; t < NP; ++t) m[t * 32] = make_float2(top[t][0], top[t][kOwn - 1]);
       }
       if (far) {  // the difference from m, which is exact near it; the base's rounding would be whole units
 #pragma unroll
         for (int t = 0; t < NP; ++t) {
           const float2 by = m[t * 32];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) sc[t][k >> 2][k & 3] -= (k & 2) ? by.y : by.x;
+          for (int k = 0; k < 4 * kOwn; ++k) sc[t][k / (2 * kOwn)][k % (2 * kOwn)] -= (k & 2) && !kFine ? by.y : by.x;
         }
       }
       float2 s[2][NG];  // scales of values 8 j + 2c and the next
 #pragma unroll
       for (int j = 0; j < 2; ++j) a4_pair_scales<NG>(vps + (8 * j + 2 * c) * 16, v_scale.unit, s[j]);
-      uint32_t f[(NG + 1) / 2][4];
+      uint32_t v[NG][4][2], f[4];  // codes less 8
 #pragma unroll
-      for (int g = 0; g < NG; g += 2) ldmatrix4t(f[g / 2], kst + R::kV + hf * kA4Half * kPitch + mat + g * 16);
+      for (int g = 0; g < NG; ++g) {
+        if ((g & 1) == 0) ldmatrix4t(f, kst + R::kV + hf * kA4Half * kPitch + mat + g * 16);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t even = f[2 * (g & 1) + j], odd = even >> 8;
+          v[g][0][j] = a4_add(even & 0x000F000Fu, 0x80088008u);
+          v[g][1][j] = a4_add(even & 0x00F000F0u, 0x80808080u);
+          v[g][2][j] = a4_add(odd & 0x000F000Fu, 0x80088008u);
+          v[g][3][j] = a4_add(odd & 0x00F000F0u, 0x80808080u);
+        }
+      }
 #pragma unroll
       for (int t = 0; t < NP; ++t) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < kOwn; ++i)
 #pragma unroll
             for (int k = 2 * i; k < 2 * i + 2; ++k) sc[t][j][k] = at_exp2(fmaf(sc[t][j][k], unit[t][i], base[t][i]));
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < kOwn; ++i)
           l[t][i] += (sc[t][0][2 * i] + sc[t][0][2 * i + 1]) + (sc[t][1][2 * i] + sc[t][1][2 * i + 1]);
         // weights as A: keys 2c and 2c + 1 of rows r and r + 8, then keys + 8
-        a4_mma(z[t], a4_pack(sc[t][0][0], sc[t][0][1]), a4_pack(sc[t][0][2], sc[t][0][3]), a4_pack(sc[t][1][0], sc[t][1][1]),
-               a4_pack(sc[t][1][2], sc[t][1][3]), vp[0][0], vp[0][1]);
+        uint32_t p[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          p[2 * j] = a4_pack(sc[t][j][0], sc[t][j][1]);
+          p[2 * j + 1] = kFine ? a4_weights<true>(sc[t][j][0], sc[t][j][1], 0xFFFFFFFFu)
+                               : a4_pack(sc[t][j][2 * kOwn - 2], sc[t][j][2 * kOwn - 1]);
+        }
+        a4_mma(z[t], p[0], p[1], p[2], p[3], vp[0][0], vp[0][1]);
         if (lost[t]) {
           if ((lost[t] >> c) & 1) z[t][1] = __uint_as_float(0x7FFFFFFFu);
           if ((lost[t] >> (8 + c)) & 1) z[t][3] = __uint_as_float(0x7FFFFFFFu);
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          uint32_t p[4];
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < kOwn; ++i) {
               const float2 y = a4_mul2(make_float2(sc[t][j][2 * i], sc[t][j][2 * i + 1]), s[j][g]);
               p[2 * j + i] = a4_pack(y.x, y.y);
+              if (kFine) p[2 * j + 1] = a4_weights<true>(y.x, y.y, 0xFFFFFFFFu);
             }
-          a4_mma(eights[t], p[0], p[1], p[2], p[3], eight[g], eight[g]);
-          const uint32_t w0 = f[g / 2][2 * (g & 1)], w1 = f[g / 2][2 * (g & 1) + 1], w2 = w0 >> 8, w3 = w1 >> 8;
-          a4_mma(o[t][g][0], p[0], p[1], p[2], p[3], w0 & 0x000F000Fu, w1 & 0x000F000Fu);
-          a4_mma(o[t][g][1], p[0], p[1], p[2], p[3], w0 & 0x00F000F0u, w1 & 0x00F000F0u);
-          a4_mma(o[t][g][2], p[0], p[1], p[2], p[3], w2 & 0x000F000Fu, w3 & 0x000F000Fu);
-          a4_mma(o[t][g][3], p[0], p[1], p[2], p[3], w2 & 0x00F000F0u, w3 & 0x00F000F0u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a4_mma(o[t][g][i], p[0], p[1], p[2], p[3], v[g][i][0], v[g][i][1]);
         }
       }
     }
@@ -1071,21 +1126,31 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
     if (++stage == kA4Stages) stage = 0;
     if (++now.tile < now.end) continue;
     const int64_t piece = (int64_t)now.b * hcs + now.hc + (int64_t)blockIdx.x * kA4Warps + warp;
-    const float low = 0x1p17f / v_scale.unit;  // 2^24 without the weights' 2^7
+    const float low = 0x1p17f / v_scale.unit, up = 0x1p13f / v_scale.unit;  // 2^24 and 2^20 without the weights' 2^7
 #pragma unroll
     for (int t = 0; t < NP; ++t) {
+      if (kFine) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+        for (int e = 0; e < 2; ++e) {
+          z[t][e] += z[t][2 + e];
+#pragma unroll
+          for (int k = 0; k < NG; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[t][k][j][e] += o[t][k][j][2 + e];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
         l[t][i] += __shfl_xor_sync(0xFFFFFFFFu, l[t][i], 1);
         l[t][i] += __shfl_xor_sync(0xFFFFFFFFu, l[t][i], 2);
-        const int g = t * 16 + r + 8 * i;
+        const int g = (t * kOwn + i) * 8 + r;
         const int64_t rec = piece * a.chunk_rows + g;
         if (g < n && c == 0)
-          a.own_ml[rec] = make_float2(a4_record_reference(i ? m[t * 32].y : m[t * 32].x, base[t][i], far, unit[t][i]), broken ? kAtBadPage : l[t][i] * 0x1p-7f);
+          a.own_ml[rec] = make_float2(a4_record_reference(i ? m[t * 32].y : m[t * 32].x, base[t][i], far, unit[t][i]),
+                                      broken ? kAtBadPage : l[t][i] * 0x1p-7f);
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
           const float middle = __shfl_sync(0xFFFFFFFFu, z[t][2 * i + 1], (lane & 28) + k) * 0x1p-7f;
-          const float eighth = __shfl_sync(0xFFFFFFFFu, eights[t][2 * i], (lane & 28) + k);
           const int d = k * 32 + c * 8;
           if (g < n && d < x.cache.head_dim) {
             float4 *to = reinterpret_cast<float4 *>(a.own_o + rec * x.cache.head_dim + d);
@@ -1094,7 +1159,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
             for (int e = 0; e < 2; ++e)
 #pragma unroll
               for (int j = 0; j < 4; ++j)
-                y[e][j] = fmaf(fmaf(o[t][k][j][2 * i + e], j & 1 ? 0.0625f : 1.f, eighth), low, middle);
+                y[e][j] = fmaf(o[t][k][j][2 * i + e], j & 1 ? up : low, middle);
             to[0] = make_float4(y[0][0], y[0][1], y[0][2], y[0][3]);
             to[1] = make_float4(y[1][0], y[1][1], y[1][2], y[1][3]);
           }
