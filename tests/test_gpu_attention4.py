@@ -317,6 +317,77 @@ def test_repeats_are_equal_and_graphs_replay():
 
 
 @gpu
+@pytest.mark.parametrize("T,H,Hkv,D", [(1, 1, 1, 16), (1, 8, 2, 64), (1, 8, 1, 128), (5, 14, 2, 64), (3, 12, 1, 48), (4, 64, 1, 96)])
+def test_fp16_is_rounded_once(T, H, Hkv, D):
+    """Of one key the weight is 1, whatever its score: only the answer's rounding
+    (2^-11) and what two halves of a weight leave (2^-22 each of two parts,
+    and fp16's steps below its normal range) are left of the error."""
+    p = Problem(2, T, H, Hkv, D, [[1] * T, [1] * T], 16, dtype=FP16, seed=T + H + D)
+    out, lse, status = p.run()
+    assert not status.any()
+    for b in range(2):
+        c, s, z = p.keys(b, 1, p.cache.v_codes, p.cache.v_params)
+        want = (z + s * (c - 8)).expand(Hkv, H // Hkv, D)
+        room = (s * (c - 8).abs() + z.abs()).expand(Hkv, H // Hkv, D)
+        for t in range(T):
+            err = (out[b, t].double().view(Hkv, H // Hkv, D) - want).abs()
+            assert bool((err <= 2.0 ** -11 * want.abs() + 2.0 ** -20 * room + 2.0 ** -25).all()), (b, t)
+
+
+@gpu
+@pytest.mark.parametrize("T,H,D", [(1, 4, 64), (1, 8, 64), (2, 8, 64), (3, 8, 128)])
+def test_long_items_keep_their_precision(T, H, D):
+    """Items of thousands of keys a warp, whose answers are sums of terms of both
+    signs far smaller than the sum of their magnitudes: over an answer the
+    error's mean square is at most that of its own rounding, a third of the
+    square of 2^-11 of the entries, and a tenth of the root for what else there
+    is (weights to 2^-20 or so, in terms whose signs differ)."""
+    B, n = (320, 32768) if D == 64 else (200, 16384)
+    p = Problem(1, T, H, 1, D, [[n - t for t in range(T)]], 16, dtype=FP16, seed=T + H)
+    p.q = p.q.expand(B, T, H, D).contiguous()
+    p.q *= torch.rand((B, 1, 1, 1), generator=torch.Generator(device="cuda").manual_seed(8), device="cuda").half()
+    p.pages, p.lengths = p.pages.expand(B, -1).contiguous(), p.lengths.expand(B, -1).contiguous()
+    out, lse, status = p.run()
+    assert not status.any()
+    for b in (0, B // 3, B - 1):
+        for t in range(T):
+            c, s, z = p.keys(b, n - t, p.cache.k_codes, p.cache.k_params)
+            w = torch.softmax(p.q[b, t].double() @ (z + s * (c - 8))[0].T * D ** -0.5, -1)
+            c, s, z = p.keys(b, n - t, p.cache.v_codes, p.cache.v_params)
+            want = w @ (z + s * (c - 8))[0]
+            err = (out[b, t].double() - want).norm() / want.norm()
+            assert float(err) <= 1.1 * 2.0 ** -11 / 3 ** 0.5, (b, t, float(err))
+
+
+@gpu
+@pytest.mark.parametrize("H,Hkv,T", [(6, 2, 4), (2, 1, 2), (28, 2, 3)])
+def test_nan_and_infinite_parameters_fp16(H, Hkv, T):
+    """As for bf16: a value's group that is no number reaches the tokens that see it, and its group alone."""
+    p = Problem(1, T, H, Hkv, 64, [[20] * (T - 1) + [40]], 16, dtype=FP16)
+    clean = p.run()
+    pg, off = int(p.pages[0, 1]), 14  # key 30
+    p.cache.v_params[pg, 0, off, 0, 1] = math.nan
+    p.cache.v_params[pg, 0, off, 1, 0] = math.inf
+    out, lse, status = p.run()
+    assert not status.any() and torch.equal(lse, clean[1])
+    seen = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+    seen[0, T - 1, :H // Hkv] = True
+    assert torch.equal(out.isnan(), seen)
+    assert torch.equal(out[~seen], clean[0][~seen])
+    p.cache.v_params[pg, 0, off, 1, 0] = 0.25
+    out = p.run()[0]
+    assert torch.equal(out.isnan(), seen & (torch.arange(64, device="cuda") < 32))
+
+
+@gpu
+@pytest.mark.parametrize("H,Hkv,T", [(8, 2, 1), (8, 1, 1), (14, 2, 5)])
+@pytest.mark.parametrize("spread,scale", [(0.0, None), (1e-5, None), (60.0, None), (1.5, 4.0)])
+def test_scores_of_any_size_fp16(H, Hkv, T, spread, scale):
+    p = Problem(2, T, H, Hkv, 64, [100, 513], 16, spread=spread, dtype=FP16)
+    p.check(*p.run(scale=scale), scale=scale)
+
+
+@gpu
 def test_over_appended_tokens():
     """What append_kv4 wrote, against attention over what read_kv4 gives back."""
     gen = torch.Generator(device="cuda").manual_seed(4)
