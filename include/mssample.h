@@ -70,14 +70,15 @@ enum {
   MS_ROW_BAD_SLOT = 32,       /* ms_kv_append, ms_kv4_append: slot past the
                                  cache; nothing is written to the cache for the
                                  token (ms_kv4_read: it reads as zeros) */
-  MS_ROW_BAD_POSITION = 64,   /* ms_kv_append: position outside the table;
-                                 nothing is written to the cache, the
-                                 token's q_out is zero */
-  MS_ROW_BAD_LENGTH = 128,    /* ms_prefix_attention: length below 0 or past
-                                 the row's pages; the row's output is 0 and
-                                 its lse -inf */
-  MS_ROW_BAD_PAGE = 256,      /* ms_prefix_attention: a page that the row or
-                                 the prefix uses is outside the cache; as above */
+  MS_ROW_BAD_POSITION = 64,   /* ms_kv_append, ms_kv4_append: position outside
+                                 the table; nothing is written to the cache,
+                                 the token's q_out is zero */
+  MS_ROW_BAD_LENGTH = 128,    /* ms_prefix_attention, ms_kv4_attention: length
+                                 below 0 or past the row's pages; the row's
+                                 output is 0 and its lse -inf */
+  MS_ROW_BAD_PAGE = 256,      /* ms_prefix_attention, ms_kv4_attention: a page
+                                 that the row or the prefix uses is outside the
+                                 cache; as above */
   MS_ROW_WAIT_TIMEOUT = 512,  /* ms_prefix_attention: a wait inside the kernel
                                  of the shared prefix was given up after 1 s;
                                  the heads concerned have output 0 and lse
@@ -619,7 +620,8 @@ int ms_kv4_read(const ms_kv4_read_args *args, ms_stream_t stream);
  *
  * k_j and v_j being what the cache stands for, not rounded; scores and sums in
  * fp32, the weights (times the values' scales) rounded to fp16 for their
- * product with the codes, out rounded once.  A token that sees no key has out
+ * product with the codes (for an fp16 out to two halves, 2^-22), out rounded
+ * once.  A token that sees no key has out
  * 0 and lse -inf.  What the cache holds past the keys that a token sees is not
  * used for it, NaN and infinities included.  A row with a length below 0 or
  * past its pages has out 0 and lse -inf for all its tokens and is flagged

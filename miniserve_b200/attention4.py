@@ -31,7 +31,8 @@ def attention_kv4(q, cache: KvCache4, pages, lengths, *, scale: Optional[float] 
     bits.  A token that sees no key has out 0 and lse -inf; so have all tokens
     of a row flagged MS_ROW_BAD_LENGTH, and the heads of a row flagged
     MS_ROW_BAD_PAGE that met the page.  What the cache holds past a token's
-    keys does not touch its result.
+    keys does not touch its result.  Scores and sums are fp32; weights are
+    rounded to fp16 (for fp16 queries to two halves), the result once.
     """
     entry = _lib.binding()
     try:

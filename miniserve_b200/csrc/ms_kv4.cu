@@ -15,7 +15,11 @@
 // rotated entries are not rounded to the model's type in between.
 //
 // Both are bound by bytes: an append reads each entry in 2 bytes and writes
-// 5 bits of it, a read back the reverse.
+// 5 bits of it, a read back the reverse.  Measured: 20011 tokens of 32 query and
+// 8 + 8 key and value heads of 128 in 98 us, 436 MB at 4.4 TB/s (two thirds of a
+// plain copy's rate: every entry costs some ten operations, issue slots are 60 %
+// busy and 44 % of the warps resident); 8 tokens in 3.7 us, a launch.  65536
+// tokens of 8 heads of 128 read back in 62 us, 352 MB at 5.7 TB/s.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -281,7 +285,8 @@ __device__ __forceinline__ uint32_t k4_encode(const float (&y)[8], bool inside, 
 // Keys and values: a thread takes 8 entries of a key head and the same 8 of its
 // value head, and four neighbouring threads a group of each.  A token's keys
 // and values are all one block's, so that its status is written once, whatever
-// its groups hold.
+// its groups hold.  (A thread for keys or values alone finds slot, position and
+// addresses twice: 20011 tokens appended and read back 169 us, so 121.)
 template <typename T, bool kInterleaved, int kV>
 __device__ __forceinline__ void k4_quantise(const K4AppendArgs &p, int *flags) {
   const ms_kv4_append_args &a = p.a;
@@ -399,7 +404,8 @@ __device__ __forceinline__ void k4_decode(uint32_t word, __half2 param, uint32_t
 }
 
 // A thread takes 8 entries of a key head and the same 8 of its value head, of one
-// or two heads.
+// or, where that leaves threads enough for the GPU four times over, two heads
+// (65536 tokens: 71 us with one, 62 with two).
 template <typename T>
 __global__ void __launch_bounds__(kK4Threads) ms_kv4_read_kernel(const __grid_constant__ K4ReadArgs p) {
   grid_wait();
@@ -455,8 +461,10 @@ __global__ void __launch_bounds__(kK4Threads) ms_kv4_read_kernel(const __grid_co
   }
 }
 
-// Tokens of a block: each thread a few items, so that a block's start and end
-// are paid for, but no fewer blocks than fill the GPU.
+// Tokens of a block: each thread up to `items` items, so that a block's start and
+// end are paid for, but no fewer blocks than fill the GPU.  20011 tokens appended
+// and read back, four items of keys and values and two of queries: 119 us; one
+// and two 126, eight and two 122, four and one 123.
 static int k4_tokens(int64_t tokens, int64_t per_token, int items) {
   const int64_t fill = tokens * per_token / (148 * 8 * kK4Threads);
   const int64_t each = fill < 1 ? 1 : fill < items ? fill : items;

@@ -14,6 +14,10 @@
 // position.  A draw compares with the running mass at every one of the
 // vocabulary's borders, so that its weights and sums are in 64 bits: with 32
 // about one draw in a thousand would land beside its token.
+//
+// Measured, four drafts a row over 151936 fp32 logits: 64 rows 63 us, of which
+// the sums, 175 MB at 5.2 TB/s, are 33 and the draws 30 (latency: fp64 operations
+// one after the other, and the sums' way through the cluster); one row 16 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -733,7 +737,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
 
 // Entries of a slice: about three slices for each warp that an SM has room for,
 // but 4096 entries (what a slice costs besides its entries is that of 1000), or
-// what fills the GPU once, of 1024 entries at least.
+// what fills the GPU once, of 1024 entries at least.  64 rows: 69 us with one
+// slice a warp, 63 with three and with six.
 static void vf_slices(int64_t positions, int64_t vocab, int *slices, int *slice) {
   const int64_t warps = 148ll * kVfSums * (kVfThreads / 32);
   auto each = [&](int64_t all) {
@@ -767,6 +772,8 @@ static cudaError_t vf_draw(const VfArgs &a, cudaStream_t s) {
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+// Draws by CTAs of 1024 threads where every row's cluster has SMs of its own: one
+// row takes 16.4 us so and 19.2 with 256 threads; 64 rows 85 us and 63.
 template <int DT>
 static cudaError_t vf_run(const VfArgs &a, cudaStream_t s) {
   const int64_t items = a.x.rows * (a.x.drafts + 1) * a.slices;
@@ -802,7 +809,8 @@ int ms_verify_drafts(const ms_verify_args *args, ms_stream_t stream) {
   a.records = static_cast<ms::VfRecord *>(x.workspace);
   ms::vf_slices(x.rows * (x.drafts + 1), x.vocab, &a.slices, &a.slice);
   if (x.rows * (x.drafts + 1) > 0x7FFFFFFFll / a.slices) return MS_E_INVALID;
-  // CTAs of a row: as many as one wave has room for (four of 256 threads an SM), so that every row's draw runs at once
+  // CTAs of a row: as many as one wave has room for (four of 256 threads an SM), so that every row's draw runs at once.
+  // 200 rows of 32003 logits in clusters of two 37.7 us, of four 37.9, of one 42.4; 64 of 151936 of eight 63, of four 75.
   a.ranks = ms::kVfCluster;
   while (a.ranks > 1 && x.rows * a.ranks > 148 * 4) a.ranks >>= 1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
