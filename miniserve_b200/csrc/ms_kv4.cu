@@ -34,8 +34,9 @@ namespace ms {
 
 constexpr int kK4Threads = 256;
 
-// Quotients of numbers below 2^16 (or, by divisors up to 16, below 2^28) from a
-// product: u / d is the high word of u ceil(2^32 / d).
+// Quotients of numbers below 2^16 (or, by divisors up to 64, below 2^26) from a
+// product: u / d is the high word of u ceil(2^32 / d), as long as u times what
+// the ceiling adds (less than d) is below 2^32.
 struct K4Divisor {
   uint32_t d, inverse;
 };

@@ -23,6 +23,7 @@ So |out - exact| <= u sum p (s |c - 8| + |z|) + (4 e + 2^-19 + (n + 64) 2^-22) R
 + 2^-30 n (16 S + Z) + U |exact| + 2^-25, and lse is within 2 e + 2^-20 + (n +
 64) 2^-23 + 2^-22 |lse|.
 """
+import copy
 import math
 
 import pytest
@@ -385,6 +386,91 @@ def test_nan_and_infinite_parameters_fp16(H, Hkv, T):
 def test_scores_of_any_size_fp16(H, Hkv, T, spread, scale):
     p = Problem(2, T, H, Hkv, 64, [100, 513], 16, spread=spread, dtype=FP16)
     p.check(*p.run(scale=scale), scale=scale)
+
+
+def rows_of(p, rows):
+    """The problem of some rows alone, for check."""
+    part = copy.copy(p)
+    part.q, part.pages, part.lens = p.q[rows], p.pages[rows], [p.lens[b] for b in rows]
+    return part
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("T,H,Hkv", [(1, 4, 1), (1, 8, 1), (3, 14, 2)])
+def test_queries_that_are_no_numbers(T, H, Hkv, dtype):
+    """A query that holds a NaN or an infinity gives NaN, and nothing else does."""
+    p = Problem(3, T, H, Hkv, 64, [50, 300, 7], 16, dtype=dtype)
+    p.q[1, T - 1, 1, 40] = math.nan
+    p.q[2, 0, H - 1, 3] = math.inf
+    out, lse, status = p.run()
+    bad = torch.zeros(lse.shape, dtype=torch.bool, device="cuda")
+    bad[1, T - 1, 1] = bad[2, 0, H - 1] = True
+    assert not status.any() and torch.equal(lse.isnan(), bad) and torch.equal(out.isnan(), bad[..., None].expand_as(out))
+    clean = copy.copy(p)
+    clean.q = torch.where(bad[..., None], 0.0, p.q)
+    want = clean.run()
+    clean.check(torch.where(bad[..., None], want[0], out), torch.where(bad, want[1], lse), status)
+
+
+@gpu
+@pytest.mark.parametrize("T,H", [(1, 4), (1, 8), (2, 14)])
+def test_scores_past_whole_numbers(T, H):
+    """Scores so large that one key has all the weight: the answer is its value."""
+    p = Problem(2, T, H, 1 if H < 14 else 2, 64, [100, 513], 16, spread=1e30)
+    out, lse, status = p.run()
+    assert not status.any()
+    for b in range(2):
+        for t in range(T):
+            c, s, z = p.keys(b, p.lens[b][t], p.cache.k_codes, p.cache.k_params)
+            score = p.q[b, t].double().view(s.shape[0], -1, 64) @ (z + s * (c - 8)).transpose(1, 2) / 8
+            top, place = score.max(-1)
+            assert bool(((lse[b, t].double().view_as(top) - top).abs() <= 2.0 ** -18 * score.abs().amax(-1)).all())
+            c, s, z = p.keys(b, p.lens[b][t], p.cache.v_codes, p.cache.v_params)
+            want = torch.gather(z + s * (c - 8), 1, place[..., None].expand(-1, -1, 64))
+            err = (out[b, t].double().view_as(want) - want).abs()
+            assert bool((err <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * (s.max() * 8 + z.abs().max())).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_many_tokens_heads_and_rows(dtype):
+    p = Problem(1, 1024, 4, 1, 64, [1500], 16, dtype=dtype)
+    out, lse, status = p.run()
+    p.check(out, lse, status, tokens=[0, 1, 511, 700, 1023])
+    p = Problem(2, 1, 250, 2, 128, [333, 40], 64, dtype=dtype)
+    p.check(*p.run())
+    p = Problem(20011, 2, 3, 1, 48, [(b * 7) % 6 for b in range(20011)], 4, dtype=dtype)
+    out, lse, status = p.run()
+    assert not status.any()
+    rows = [0, 1, 2, 5, 9999, 20009, 20010]
+    rows_of(p, rows).check(out[rows], lse[rows], status[rows])
+
+
+@gpu
+def test_out_may_be_q():
+    p = Problem(5, 3, 14, 2, 64, [5, 100, 0, 37, 600], 16)
+    want = p.run()
+    out, lse, status = p.run(out=p.q)
+    assert out is p.q and torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+@gpu
+def test_calls_on_two_streams():
+    """Two calls under way at once have workspaces of their own."""
+    p = Problem(64, 1, 14, 2, 64, [(91 * i) % 700 for i in range(64)], 16)
+    r = Problem(16, 4, 14, 2, 64, [(301 * i) % 3000 for i in range(16)], 16, seed=5)
+    want = p.run(), r.run()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (problem, stream) in enumerate(zip((p, r), streams)):
+            with torch.cuda.stream(stream):
+                got[i].append(problem.run())
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, y) for one in got[i] for x, y in zip(one, want[i]))
 
 
 @gpu
