@@ -543,7 +543,10 @@ __device__ __forceinline__ bool a4_none(uint32_t u) {
 //   q . k = sum_g s_g (q_g . c_g) + sum_g (z_g - 8 s_g) sum q_g
 //   o     = sum_j (p_j s_jg) (c_j - 8) + sum_j p_j z_jg
 //
-// K: s_g weighs a group's sums in fp32; the rest is one more product, of the
+// K: words are shifted so that codes are c 2^-22 and c 2^-18: a product's terms are
+// aligned as if a subnormal factor had the smallest normal exponent, and cut off,
+// so that two bits more leave a fifth of the scores' error (lse of one key 1.1e-6
+// off as c 2^-24, 2e-7 so).  s_g weighs a group's sums in fp32; the rest is one more product, of the
 // parameters as they lie with the queries' sums in two fp16 halves.  V: p s_g is
 // rounded to fp16 once, and its rounding meets c - 8 and not c: the narrow kernel
 // adds -8 times the same rounded weights, one more product with constants, the
@@ -586,7 +589,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
   const uint32_t rest = kFine && c >= 2 ? 0xFFFFFFFFu : 0u;
   float o[2 * NG][4];         // entries 32 g + 4 r + 2 i (0, 1) and the next (2, 3), of queries 2c and 2c + 1
   float z[2];                 // the middles' part: row r is parameter r of a key
-  // of queries 2c and 2c + 1: what a score of 2^-24 is in units of log2, the score that weights refer to, the one past
+  // of queries 2c and 2c + 1: what a score of 2^-22 is in units of log2, the score that weights refer to, the one past
   // which they do no longer, 7 less the whole number nearest to it in units of log2, the sum of weights, keys seen
   float unit[2], m[2], lim[2], base[2], l[2];
   int len[2];
@@ -611,7 +614,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
 #pragma unroll
       for (int i = 0; i < 2; ++i) {  // of the queries that this lane's columns of a product are
         const int g = (2 * c + i) & (a4_narrow(kFine) - 1);
-        unit[i] = a4_unit(a.scale_log2 * 0x1p24f * __shfl_sync(0xFFFFFFFFu, down, g * 4));
+        unit[i] = a4_unit(a.scale_log2 * 0x1p22f * __shfl_sync(0xFFFFFFFFu, down, g * 4));
         len[i] = g < n ? load_in(x.lengths + now.b * x.length_row + (first + g) / a.group) : 0x7FFFFFFF;
         least = min(least, len[i]);
         len[i] = min(len[i], now.keys);
@@ -632,7 +635,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
     const uint32_t kst = smem_addr(here);
     // rows of the matrices that ldmatrix takes: keys 0-7 and 8-15 of a half and group, then of the next group
     const uint32_t mat = (uint32_t)((lane & 15) * kPitch + (lane >> 4) * 16);
-    float sc[kA4Halves][4];  // in units of 2^24: the scales stay as they are
+    float sc[kA4Halves][4];  // in units of 2^22: the scales stay as they are
 #pragma unroll
     for (int hf = 0; hf < kA4Halves; ++hf) {
       const unsigned char *params = here + R::kKp + hf * kA4Half * 16;
@@ -648,7 +651,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
       }
       a4_mma(sc[hf], p[0], p[1], p[0], p[1], qs[0], qs[1], 0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sc[hf][i] *= 0x1p-24f;
+      for (int i = 0; i < 4; ++i) sc[hf][i] *= 0x1p-22f;
       // the groups' first products, then their second ones, which wait for them
       uint32_t f[(NG + 1) / 2][4];
       float d[NG][4];
@@ -656,13 +659,13 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
       for (int g = 0; g < NG; g += 2) ldmatrix4(f[g / 2], kst + hf * kA4Half * kPitch + mat + g * 16);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint32_t w0 = f[g / 2][2 * (g & 1)], w1 = f[g / 2][2 * (g & 1) + 1];
-        a4_mma(d[g], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[g][0], qf[g][1], 0.f, 0.f);
+        const uint32_t w0 = f[g / 2][2 * (g & 1)] << 2, w1 = f[g / 2][2 * (g & 1) + 1] << 2;
+        a4_mma(d[g], w0 & 0x003C003Cu, w1 & 0x003C003Cu, w0 & 0x03C003C0u, w1 & 0x03C003C0u, qf[g][0], qf[g][1], 0.f, 0.f);
       }
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint32_t w0 = f[g / 2][2 * (g & 1)] >> 8, w1 = f[g / 2][2 * (g & 1) + 1] >> 8;
-        a4_mma(d[g], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qf[g][2], qf[g][3]);
+        const uint32_t w0 = f[g / 2][2 * (g & 1)] >> 6, w1 = f[g / 2][2 * (g & 1) + 1] >> 6;
+        a4_mma(d[g], w0 & 0x003C003Cu, w1 & 0x003C003Cu, w0 & 0x03C003C0u, w1 & 0x03C003C0u, qf[g][2], qf[g][3]);
       }
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -954,7 +957,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
         }
         float2 s[2][NG];  // scales of keys 8 j + 2c and the next
 #pragma unroll
-        for (int j = 0; j < 2; ++j) a4_pair_scales<NG>(kps + (8 * j + 2 * c) * 16, 0x1p24f, s[j]);
+        for (int j = 0; j < 2; ++j) a4_pair_scales<NG>(kps + (8 * j + 2 * c) * 16, 0x1p22f, s[j]);
         uint32_t f[4];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -966,10 +969,10 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
             float d[2][4];
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-              a4_mma(d[j], q0.x, q0.y, q0.z, q0.w, w[j] & 0x000F000Fu, w[j] & 0x00F000F0u, 0.f, 0.f);
+              a4_mma(d[j], q0.x, q0.y, q0.z, q0.w, (w[j] << 2) & 0x003C003Cu, (w[j] << 2) & 0x03C003C0u, 0.f, 0.f);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-              a4_mma(d[j], q1.x, q1.y, q1.z, q1.w, (w[j] >> 8) & 0x000F000Fu, (w[j] >> 8) & 0x00F000F0u);
+              a4_mma(d[j], q1.x, q1.y, q1.z, q1.w, (w[j] >> 6) & 0x003C003Cu, (w[j] >> 6) & 0x03C003C0u);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
