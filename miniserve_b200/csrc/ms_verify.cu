@@ -327,7 +327,8 @@ __device__ __forceinline__ VfScale vf_scale(double c, double heat, float top) {
   s.c = c;
   s.plain = fabs((double)top) * c < 35184372088832.0 && c < 1e290;  // 2^45
   s.base = kVfMagic - (s.plain ? kVfSteps * ceil((double)top * c * (1.0 / kVfSteps)) : 0.0);
-  s.least = s.plain ? (float)fmax((double)top - kVfLeast * 0.69314718055994530942 * heat, -3.4e38) : top;
+  // rounded up, which passes no value of `top`: a value below 2^-1000 would wrap the power's exponent
+  s.least = s.plain ? __double2float_ru(fmax((double)top - kVfLeast * 0.69314718055994530942 * heat, -3.4e38)) : top;
   return s;
 }
 // Relative to 2^(R / 128) or, of scales that are not plain, to the largest

@@ -362,3 +362,27 @@ def test_entry_point_refusals():
         assert call(**bad) == -1, bad
     assert L.ms_verify_drafts(None, None) == -1
     assert L.ms_verify_workspace(0, 1, 10) == 0 and L.ms_verify_workspace(1, 256, 10) == 0
+
+
+@gpu
+@pytest.mark.parametrize("top", [20.0, 50.0, 100.0])
+@pytest.mark.parametrize("heat", [1e-10, 1e-9, 2e-9, 1e-8, 5e-8, 1e-6])
+def test_near_ties_at_small_temperatures(heat, top):
+    """The second largest logit a few units in the last place below the largest,
+    hundreds or thousands of octaves apart in weight: neighbours, and at the
+    row's two ends."""
+    V, cases = 3001, [(ulps, at) for ulps in (1, 2, 5, 20) for at in ((1500, 1501), (7, 2990), (2990, 7))]
+    logits, _, uniforms, q = problem(len(cases), 2, V, seed=14, sharp=0.5, fewer=False)
+    step = float(torch.tensor(top) - torch.nextafter(torch.tensor(top), torch.tensor(0.0)))
+    first, second = (torch.tensor([at[i] for _, at in cases], device="cuda") for i in range(2))
+    rows = torch.arange(len(cases), device="cuda")
+    logits[rows, :, first] = top
+    logits[rows, :, second] = top - step * torch.tensor([float(u) for u, _ in cases], device="cuda")[:, None]
+    none = torch.full_like(first, -1)
+    for drafts in ((none, none), (first, second), (second, first), (first, first)):
+        drafts = torch.stack(drafts, 1)
+        check(logits, drafts, uniforms, None, heat)
+        given = q * 0.3
+        for at, much in ((first, 0.3), (second, 0.4)):
+            given[rows, :, at] = much
+        check(logits, drafts, uniforms, given, heat)
