@@ -312,6 +312,7 @@ __device__ const VfPowers vf_powers{};
 
 constexpr double kVfMagic = 6755399441055744.0;  // 1.5 * 2^52: the low word of a sum with it is a whole number
 constexpr double kVfLeast = 1000.0;              // weights below 2^-1000 count as 0
+constexpr double kVfMost = 3.4028234663852886e38;  // the largest fp32 value
 
 struct VfScale {
   double c;     // steps of a unit of logit
@@ -328,7 +329,7 @@ __device__ __forceinline__ VfScale vf_scale(double c, double heat, float top) {
   s.plain = fabs((double)top) * c < 35184372088832.0 && c < 1e290;  // 2^45
   s.base = kVfMagic - (s.plain ? kVfSteps * ceil((double)top * c * (1.0 / kVfSteps)) : 0.0);
   // rounded up, which passes no value of `top`: a value below 2^-1000 would wrap the power's exponent
-  s.least = s.plain ? __double2float_ru(fmax((double)top - kVfLeast * 0.69314718055994530942 * heat, -3.4e38)) : top;
+  s.least = s.plain ? __double2float_ru(fmax((double)top - kVfLeast * 0.69314718055994530942 * heat, -kVfMost)) : top;
   return s;
 }
 // Relative to 2^(R / 128) or, of scales that are not plain, to the largest

@@ -386,3 +386,17 @@ def test_near_ties_at_small_temperatures(heat, top):
         for at, much in ((first, 0.3), (second, 0.4)):
             given[rows, :, at] = much
         check(logits, drafts, uniforms, given, heat)
+
+
+@gpu
+@pytest.mark.parametrize("heat", [1.0, 1e26, 1e30, 1e300])
+def test_lowest_logits_alone(heat):
+    """Rows whose only values are the type's lowest, which a mask may write: they share the probability."""
+    V, low = 2500, torch.finfo(torch.float32).min
+    logits = torch.full((3, 2, V), low, device="cuda")
+    logits[1, :, ::3] = -math.inf
+    logits[2, :, 40:] = -math.inf
+    drafts = torch.tensor([[-1], [4], [39]], device="cuda")
+    uniforms = torch.tensor([[0.5, 0.30013], [0.9, 0.7], [0.9, 0.999]], dtype=torch.float64, device="cuda")
+    check(logits, drafts, uniforms, None, heat)
+    check(logits, drafts, uniforms, torch.full((3, 1, V), 1e-3, device="cuda"), heat)
