@@ -131,14 +131,28 @@ __device__ __forceinline__ float2 vf_mul2(float2 a, float2 b) {
       : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
   return *reinterpret_cast<float2 *>(&d);
 }
-// A unit of logit in units of log2: finite and not 0, so that it makes neither
-// a number of 0 times infinity.
-__device__ __forceinline__ float vf_unit(double heat) {
-  return heat == 0.0 ? 1.f : (float)fmin(fmax(1.4426950408889634 / heat, 1e-37), 3e38);
+__device__ __forceinline__ float2 vf_fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)), "l"(*reinterpret_cast<uint64_t *>(&c)));
+  return *reinterpret_cast<float2 *>(&d);
+}
+// A difference of logits in units of log2 is its `part` times `by`: finite and
+// not 0, so that neither makes a number of 0 times infinity.  The part is one
+// half where logits past fp32's largest difference still weigh something.
+struct VfUnit {
+  float part, by;
+};
+__device__ __forceinline__ VfUnit vf_unit(double heat) {
+  if (heat == 0.0) return VfUnit{1.f, 1.f};
+  const double unit = 1.4426950408889634 / heat;
+  // (float)1.4e-45, the least fp32 value, times the largest difference is 1e-6
+  return unit < 1e-30 ? VfUnit{0.5f, (float)fmax(2.0 * unit, 1.4e-45)} : VfUnit{1.f, (float)fmin(unit, 3e38)};
 }
 // A sum of weights relative to `from`, as one relative to `to`, which is not below it.
-__device__ __forceinline__ double vf_moved(double sum, float from, float to, float unit) {
-  return from == to || sum == 0.0 ? sum : sum * (double)vf_exp2((from - to) * unit);
+__device__ __forceinline__ double vf_moved(double sum, float from, float to, VfUnit unit) {
+  return from == to || sum == 0.0 ? sum : sum * (double)vf_exp2(fmaf(from, unit.part, -to * unit.part) * unit.by);
 }
 
 // A thread's values so far.
@@ -150,7 +164,7 @@ struct VfSum {
 
 // One more batch of values, piece s's at s * 32 pieces from place `first` on.
 template <int kPieces, int kVec>
-__device__ __forceinline__ void vf_add(VfSum &a, float (&v)[kPieces][kVec], int first, bool greedy, float unit) {
+__device__ __forceinline__ void vf_add(VfSum &a, float (&v)[kPieces][kVec], int first, bool greedy, VfUnit unit) {
   const float kNone = __uint_as_float(0xFF800000u), kInf = __uint_as_float(0x7F800000u);
   float most = kNone;
 #pragma unroll
@@ -183,12 +197,13 @@ __device__ __forceinline__ void vf_add(VfSum &a, float (&v)[kPieces][kVec], int 
   if (greedy || a.top == kNone) return;
   float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   if (a.top < kInf) {
-    const float2 from = make_float2(-a.top, -a.top), by = make_float2(unit, unit);
+    const float2 from = make_float2(-a.top * unit.part, -a.top * unit.part), part_of = make_float2(unit.part, unit.part),
+                 by = make_float2(unit.by, unit.by);
 #pragma unroll
     for (int s = 0; s < kPieces; ++s)
 #pragma unroll
       for (int k = 0; k < kVec; k += 2) {
-        const float2 t = vf_mul2(vf_add2(make_float2(v[s][k], v[s][k + 1]), from), by);
+        const float2 t = vf_mul2(vf_fma2(make_float2(v[s][k], v[s][k + 1]), part_of, from), by);
         part[(k >> 1) & 1] = vf_add2(part[(k >> 1) & 1], make_float2(vf_exp2(t.x), vf_exp2(t.y)));
       }
   } else {  // infinite values share the weight
@@ -223,7 +238,7 @@ __global__ void __launch_bounds__(kVfThreads, kVfSums) ms_verify_sums_kernel(con
   const double heat = load_in(x.temperature + b);
   if (vf_drafts(x, b, i) < i || !vf_heat(heat)) return;
   const bool greedy = heat == 0.0;
-  const float unit = vf_unit(heat);
+  const VfUnit unit = vf_unit(heat);
   const typename V::T *row = static_cast<const typename V::T *>(x.logits) + b * x.logits_row + i * x.logits_pos;
   // 16-byte pieces: the first one starts before the row where the row does not start on one.  Pieces `inner` .. `outer`
   // - 1 lie in the row as a whole.
@@ -399,7 +414,7 @@ struct VfShared {
   int index[kVfMaxDrafts + 1], flags[kVfMaxDrafts + 1];
   bool none[kVfMaxDrafts + 1];               // all values are -inf
   double c, heat;
-  float unit;
+  VfUnit unit;
   int stop, drafts, status;
 };
 
@@ -474,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
     meet();
     return;
   }
-  const float unit = sh.unit;
+  const VfUnit unit = sh.unit;
   const bool greedy = sh.heat == 0.0;
   auto logits = [&](int i) { return static_cast<const typename V::T *>(x.logits) + b * x.logits_row + i * x.logits_pos; };
   for (int i = warp; i <= n; i += kWarps) {  // the positions' records

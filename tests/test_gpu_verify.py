@@ -400,3 +400,17 @@ def test_lowest_logits_alone(heat):
     uniforms = torch.tensor([[0.5, 0.30013], [0.9, 0.7], [0.9, 0.999]], dtype=torch.float64, device="cuda")
     check(logits, drafts, uniforms, None, heat)
     check(logits, drafts, uniforms, torch.full((3, 1, V), 1e-3, device="cuda"), heat)
+
+
+@gpu
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("heat", [1e32, 1e36, 1e37, 1e38, 3e38, 1e39, 1e42])
+def test_logits_as_large_as_the_temperature(heat, probs):
+    """Logits over all of fp32's range, at temperatures where they weigh alike."""
+    logits, drafts, uniforms, q = problem(20, 3, 1200, seed=15, probs=probs)
+    big = torch.finfo(torch.float32).max
+    logits.clamp_(-3, 3)
+    logits *= min(big / 3, heat / 2)
+    logits[::2, :, ::5] = -big
+    logits[1::4, :, 3::7] = big
+    check(logits, drafts, uniforms, q, heat)
