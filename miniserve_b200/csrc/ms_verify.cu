@@ -523,6 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
     const int flags = __reduce_or_sync(0xFFFFFFFFu, all.flags);
     const double z = vf_warp_sum(vf_moved(all.sum, all.top, top, unit));
     if (lane == 0) {
+      if (top == kNone) index = 0;  // all are as large
       sh.index[i] = index, sh.flags[i] = flags, sh.none[i] = top == kNone;
       double p = 0.0;
       if (greedy) {
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
   };
   if (greedy || none) {
     if (rank == 0 && !greedy) give_up(MS_ROW_ALL_MASKED | flags);
-    if (rank == 0 && greedy && warp == 0) finish(none ? 0 : sh.index[f], 1.0);
+    if (rank == 0 && greedy && warp == 0) finish(sh.index[f], 1.0);
     __syncwarp();
     meet();
     return;

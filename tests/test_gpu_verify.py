@@ -414,3 +414,17 @@ def test_logits_as_large_as_the_temperature(heat, probs):
     logits[::2, :, ::5] = -big
     logits[1::4, :, 3::7] = big
     check(logits, drafts, uniforms, q, heat)
+
+
+@gpu
+def test_greedy_over_positions_without_a_value():
+    """The first largest of a position that holds nothing but -inf is token 0: a draft of it is accepted."""
+    logits, drafts, uniforms, q = problem(4, 3, 700, seed=16, fewer=False)
+    best = logits.argmax(-1)
+    drafts.copy_(best[:, :3])
+    logits[:3, 1] = -math.inf
+    logits[2, 1] = math.nan
+    drafts[0, 1], drafts[1, 1], drafts[2, 1] = 0, 5, 0
+    tokens, counts, status = check(logits, drafts, uniforms, q, 0.0)
+    assert counts.tolist() == [4, 2, 4, 4] and tokens[0].tolist() == [int(best[0, 0]), 0, int(best[0, 2]), int(best[0, 3])]
+    assert status.tolist() == [0, 0, _lib.MS_ROW_NONFINITE, 0]
