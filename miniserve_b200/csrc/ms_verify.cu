@@ -401,8 +401,11 @@ __device__ __forceinline__ bool vf_find(double mass, double r, bool end, double 
 // than the draft gave them, and what it gave those; what is left by the exact z.
 enum { kVfAll, kVfMore, kVfTaken, kVfRest, kVfKinds };
 
+constexpr int kVfRun = 8;  // batches whose draft probabilities are summed in fp32
+
 template <int kThreads>
 struct VfShared {
+  double given[kThreads];                    // the runs' sums of a thread
   double power[kVfSteps * kVfCopies];
   double sum[kVfKinds][kThreads / 32];       // of the CTA's warps
   double mass[kVfKinds][kVfCluster];         // of the cluster's CTAs, in index order
@@ -426,10 +429,11 @@ struct VfShared {
 //
 // What the draft's probabilities leave, max(w / z - q, 0), needs the whole z of
 // the weights w first.  One pass is enough all the same: the first kernel's z is
-// known to 1e-7, and the entries that it puts on the wrong side of w / z = q are
+// known to 1e-6, and the entries that it puts on the wrong side of w / z = q are
 // those where next to nothing is left, so that the sum over its side, S = sum (w
-// / z - q) and Q = sum q, is S + (S + Q) (z / z' - 1) for the exact z' to 1e-13,
-// with Q to 1e-6.  Where all that is left is itself small (a draft model that is
+// / z - q) and Q = sum q, is S + (S + Q) (z / z' - 1) for the exact z' to 2e-12,
+// with Q to 2e-6 of itself (fp32 over a row of 2^24 tokens, a CTA's: borders were
+// off by 1e-10).  Where all that is left is itself small (a draft model that is
 // the target, nearly), a second pass takes the exact z.
 //
 // fp64 operations take some 40 cycles one after the other, and divisions several
@@ -467,6 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
       sh.unit = vf_unit(heat);
     }
   }
+  sh.given[tid] = 0.0;
   if (tid < 2 * kVfSteps) {
     const int step = tid >> 1;
     const double g = __hiloint2double(__double2hiint(entry) - (step << 13), __double2loint(entry));
@@ -629,11 +634,18 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
         for (int k = 0; k < kBatch; ++k)
           if (j0 + 32 * k < end) add(t[k & 1], given[k & 1], v[k], d[k], j + 32 * k != without, kind);
       }
+      if constexpr (kind.value == kVfMore) {
+        constexpr int kRun = 32 * kBatch * kVfRun;
+        if (((j0 - (int)lo) & (kRun - 1)) == kRun - 32 * kBatch) {
+          sh.given[tid] += (double)(given[0] + given[1]);
+          given[0] = given[1] = 0.f;
+        }
+      }
     }
     s[0] = vf_warp_sum(t[0][0] + t[1][0]);
     if constexpr (kind.value == kVfMore) {
       s[1] = vf_warp_sum(t[0][1] + t[1][1]);
-      s[2] = vf_warp_sum((double)(given[0] + given[1]));
+      s[2] = vf_warp_sum(sh.given[tid] + (double)(given[0] + given[1]));
     }
   };
   // Every CTA's sums of its part to all of them, at places `slot` on.
@@ -664,7 +676,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
     cluster_sync();
   };
   // A lane's part of the row, of CTAs or of warps, as the draw sees it: nothing where what is left of a part is within
-  // the rounding of its sums.
+  // the rounding of its sums: of Q 33 roundings to fp32, 2e-6, in the part of it that the exact z moves, and per / 64
+  // roundings of 2^-53.  What the sums find left is at most what is left by the exact z, but for that: a part that is
+  // chosen holds an entry to draw.
   int slot = kVfAll;
   double moved = 0.0;  // by the exact z, over the first kernel's: its share less 1
   auto mass = [&](const double *of, int pitch, int count) {
@@ -672,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
     if (slot != kVfMore) return of[slot * pitch + lane];
     const double left = of[kVfMore * pitch + lane], all = left + of[kVfTaken * pitch + lane];
     const double rest = fma(all, moved, left);
-    return rest > 1e-13 * all ? rest : 0.0;
+    return rest > fma(fabs(moved), 2e-6, fma((double)per, 0x1p-57, 1e-13)) * all ? rest : 0.0;
   };
   auto whole = [&]() { return vf_warp_sum(mass(&sh.mass[0][0], kVfCluster, ranks)); };
   double all;

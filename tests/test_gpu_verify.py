@@ -428,3 +428,33 @@ def test_greedy_over_positions_without_a_value():
     tokens, counts, status = check(logits, drafts, uniforms, q, 0.0)
     assert counts.tolist() == [4, 2, 4, 4] and tokens[0].tolist() == [int(best[0, 0]), 0, int(best[0, 2]), int(best[0, 3])]
     assert status.tolist() == [0, 0, _lib.MS_ROW_NONFINITE, 0]
+
+
+@gpu
+def test_draws_beside_borders_of_long_rows():
+    """2^24 tokens, a CTA a row: u lies 2^-37 (twice what a weight may be off by)
+    beside a border of what the draft leaves.  One token holds a fifteenth of p,
+    the others are 20 octaves below it, so that an error of the weights' unit
+    moves their sum; the draft's share of them lies in the second half alone, so
+    that an error of it moves the first half's borders."""
+    V, B = 1 << 24, 600
+    # a temperature whose factor log2(e) / T is rounded by almost half a unit in the last place of fp32
+    heat = max((1.0 + i * 1e-4 for i in range(400)),
+               key=lambda t: abs(float(torch.tensor(1.4426950408889634 / t)) * t / 1.4426950408889634 - 1.0))
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    base = torch.rand((2, V), generator=gen, device="cuda") * 0.01
+    base[:, V // 2 + 3] = 14.0 * heat
+    p = torch.softmax(base[0].double() / heat, 0)
+    q = torch.zeros(V, device="cuda")
+    q[V // 2:] = 0.47 * float(p[0])
+    q[V - 1] = 1e-3
+    mass = (p - q.double()).clamp(min=0).cumsum(0)
+    at = torch.randint(V // 8, V // 2, (B,), generator=gen, device="cuda")
+    above = torch.arange(B, device="cuda") % 2
+    uniforms = torch.full((B, 2), 0.9, dtype=torch.float64, device="cuda")
+    uniforms[:, 1] = mass[at] / mass[-1] + (above * 2 - 1) * 2.0 ** -37
+    tokens, probs, counts, status = verify_drafts(base.expand(B, 2, V), torch.full((B, 1), V - 1, device="cuda"), uniforms,
+                                                  draft_probs=q.expand(B, 1, V), temperature=heat)
+    assert not status.any() and bool((counts == 1).all())
+    assert torch.equal(tokens[:, 0], at + above)
+    assert bool(((probs[:, 0].double() - p[tokens[:, 0]]).abs() <= p[tokens[:, 0]] * 2.0 ** -23).all())
