@@ -32,7 +32,7 @@
 namespace ms {
 
 constexpr int kVfThreads = 128;   // of a CTA that sums slices
-constexpr int kVfSums = 7;        // such CTAs of an SM
+constexpr int kVfSums = 6;        // such CTAs of an SM: what their rings leave room for
 constexpr int kVfPieces = 4;      // 16-byte pieces of a lane's batch of values
 constexpr int kVfStages = 4;      // batches of a warp's ring
 constexpr int kVfCluster = 8;     // CTAs of a row's draw, at most
@@ -769,8 +769,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
 
 // Entries of a slice: about three slices for each warp that an SM has room for,
 // but 4096 entries (what a slice costs besides its entries is that of 1000), or
-// what fills the GPU once, of 1024 entries at least.  64 rows: 69 us with one
-// slice a warp, 63 with three and with six.
+// what fills the GPU once, of 1024 entries at least.  64 rows: 66 us with one
+// slice a warp, 65 with two to six.
 static void vf_slices(int64_t positions, int64_t vocab, int *slices, int *slice) {
   const int64_t warps = 148ll * kVfSums * (kVfThreads / 32);
   auto each = [&](int64_t all) {
