@@ -539,8 +539,9 @@ int ms_int8_linear(const void *x, int dtype, int64_t ldx, int64_t M, const int8_
  *   params  [pages, kv_heads, page_size, groups, 2] fp16
  *   entry i stands for  middle[i / 32] + scale[i / 32] (code[i] - 8)
  *
- * for the keys and the values each, contiguous, the bases 16-byte aligned
- * (MS_E_UNSUPPORTED otherwise).  What lies behind a head's entries and its
+ * for the keys and the values each, contiguous, the codes' bases 16-byte
+ * aligned, the parameters' to groups * 4 bytes (MS_E_UNSUPPORTED otherwise; a
+ * range of a cache's pages is a cache).  What lies behind a head's entries and its
  * ceil(head_dim / 32) parameters is not used.
  */
 typedef struct {

@@ -373,12 +373,12 @@ Cache4 cache4(PyObject *const *o) {
   check("v_codes", vc, at::kByte, r.device, kc.sizes());
   check("v_params", vp, at::kHalf, r.device, kp.sizes());
   if (kc.numel() == 0) refuse(PyExc_ValueError, "the cache is empty");
-  uintptr_t bases = 0;
   for (const at::Tensor *t : {&kc, &kp, &vc, &vp}) {
     if (!t->is_contiguous()) refuse(PyExc_ValueError, "the cache's tensors must be contiguous");
-    bases |= reinterpret_cast<uintptr_t>(t->const_data_ptr());
+    const int64_t align = t == &kp || t == &vp ? groups * 4 : 16;
+    if (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & (align - 1))
+      refuse(PyExc_ValueError, "the cache's codes must start 16-byte aligned, its parameters ", groups * 4, "-byte aligned");
   }
-  if (bases & 15) refuse(PyExc_ValueError, "the cache's tensors must start 16-byte aligned");
   r.c.pages = kc.size(0), r.c.kv_heads = (int32_t)kc.size(1), r.c.page_size = kc.size(2), r.c.head_dim = (int32_t)dim;
   r.c.k_codes = static_cast<uint8_t *>(kc.data_ptr()), r.c.k_params = kp.data_ptr();
   r.c.v_codes = static_cast<uint8_t *>(vc.data_ptr()), r.c.v_params = vp.data_ptr();

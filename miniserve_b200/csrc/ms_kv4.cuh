@@ -27,9 +27,10 @@ inline int k4_check(const ms_kv4_cache &c) {
     return MS_E_INVALID;
   // the last byte's address is a 64-bit offset
   if (c.pages > 0x7FFFFFFFFFFFll / c.page_size / c.kv_heads) return MS_E_INVALID;
+  // a slot's parameters are copied at once, its codes by 16 bytes: a range of a cache's pages lies so too
   if (c.head_dim % 16 || c.head_dim > 128 ||
-      ((reinterpret_cast<uintptr_t>(c.k_codes) | reinterpret_cast<uintptr_t>(c.k_params) |
-        reinterpret_cast<uintptr_t>(c.v_codes) | reinterpret_cast<uintptr_t>(c.v_params)) & 15))
+      ((reinterpret_cast<uintptr_t>(c.k_codes) | reinterpret_cast<uintptr_t>(c.v_codes)) & 15) ||
+      ((reinterpret_cast<uintptr_t>(c.k_params) | reinterpret_cast<uintptr_t>(c.v_params)) & (k4_layout(c.head_dim).groups * 4 - 1)))
     return MS_E_UNSUPPORTED;
   return MS_OK;
 }

@@ -34,8 +34,10 @@ class KvCache4:
     holds entries 2j, in its low four bits, and 2j + 1) and ``k_params``,
     ``v_params`` fp16 [pages, kv_heads, page_size, groups, 2], the scale and the
     middle of every 32 entries (``groups``: 2 or 4, as many as padded needs).
-    Entry i stands for ``middle + scale * (code - 8)``.  All are contiguous;
-    a range of pages (``cache[first:last]``) is a cache too.
+    Entry i stands for ``middle + scale * (code - 8)``.  All are contiguous
+    and start aligned: codes to 16 bytes, parameters to a slot's (8 for two
+    groups, 16 for four).  A range of pages (``cache[first:last]``) is a cache
+    too.
 
     ``dtype`` (bfloat16 or float16) is the model's type: what ``append_kv4``
     takes and ``read_kv4`` gives.  ``head_dim`` is a multiple of 16 up to 128.
@@ -61,6 +63,9 @@ class KvCache4:
                 raise ValueError(f"{name} is on {t.device}, k_codes on {k_codes.device}")
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
+            align = groups * 4 if kind == torch.float16 else 16
+            if t.data_ptr() % align:
+                raise ValueError(f"{name} must start {align}-byte aligned")
         if not k_codes.numel():
             raise ValueError("the cache is empty")
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params

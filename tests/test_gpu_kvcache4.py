@@ -408,3 +408,71 @@ def test_call_refusals():
             read_kv4(cache, *args, **kw)
     with pytest.raises(TypeError):
         read_kv4(cache, slots, k_out=k.half())
+
+
+@gpu
+@pytest.mark.parametrize("dim,kv,page", [(64, 1, 5), (48, 3, 1), (16, 1, 7), (80, 1, 3), (128, 1, 1)])
+def test_any_range_of_pages(dim, kv, page):
+    """Ranges that start at an odd page of odd size, where a page's parameters
+    are 8 bytes off the 16-byte grid: the bytes, what is read back and the
+    attention are those of a cache of its own."""
+    from miniserve_b200 import attention_kv4
+    gen = generator(11)
+    T = 6 * page
+    k, v = (torch.randn((T, kv, dim), generator=gen, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn((2, 3, 2 * kv, dim), generator=gen, device="cuda").bfloat16()
+    rope, positions = rope_table(T, 16), torch.arange(T, device="cuda")
+    slots = torch.randperm(T, generator=gen, device="cuda")
+    pages = torch.tensor([[0, 3, 5], [4, 1, 2]], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([[3 * page - 2, 3 * page - 1, 3 * page], [1, 0, 2 * page]], dtype=torch.int32, device="cuda").clamp(min=0)
+    want = KvCache4.empty(6, page, kv, dim)
+    append_kv4(want, k, v, slots, positions=positions, rope=rope)
+    read = read_kv4(want, slots)
+    many = q.repeat(1, 6, 1, 1), lengths.repeat(1, 6)  # eighteen tokens a row: the other kernel
+    seen = attention_kv4(q, want, pages, lengths), attention_kv4(many[0], want, pages, many[1])
+    for first in (1, 2, 3):
+        whole = KvCache4.empty(11, page, kv, dim)
+        part = whole[first:first + 6]
+        append_kv4(part, k, v, slots, positions=positions, rope=rope)
+        for a, b in zip(want._args[:4], part._args[:4]):
+            assert torch.equal(a, b)
+        assert not bool(whole[:first].k_params.any()) and not bool(whole[first + 6:].v_params.any())
+        for a, b in zip(read, read_kv4(part, slots)):
+            assert torch.equal(a, b)
+        for a, b in zip(seen[0], attention_kv4(q, part, pages, lengths)):
+            assert torch.equal(a, b)
+        for a, b in zip(seen[1], attention_kv4(many[0], part, pages, many[1])):
+            assert torch.equal(a, b)
+
+
+def test_bases_off_their_grid():
+    """Codes lie on 16 bytes and parameters on a slot's 8 or 16: what does not is refused as the cache is made, and by
+    the entry points."""
+    import ctypes
+    for dim, row, groups in ((64, 32, 2), (96, 48, 4)):
+        codes, params = torch.zeros((3, 1, 5, row), dtype=torch.uint8), torch.zeros((3, 1, 5, groups, 2), dtype=torch.float16)
+        cache = KvCache4(codes, params, codes.clone(), params.clone(), head_dim=dim, dtype=BF16)
+        assert cache[1:].pages == 2 and cache[1:2].pages == 1
+        for name in ("k_codes", "k_params", "v_codes", "v_params"):
+            like = getattr(cache, name)
+            step = 8 if like.dtype == torch.uint8 else 2
+            moved = torch.zeros(like.numel() + step, dtype=like.dtype)[step:].view(like.shape)
+            with pytest.raises(ValueError, match=name):
+                KvCache4(**{**{n: getattr(cache, n) for n in ("k_codes", "k_params", "v_codes", "v_params")}, name: moved},
+                         head_dim=dim, dtype=BF16)
+    L = _lib.lib()
+    some = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(some) + 255) // 256 * 256
+
+    def call(dim, **other):
+        c = _lib.Kv4Cache(**{**dict(kv_heads=1, head_dim=dim, pages=3, page_size=5, k_codes=p, k_params=p, v_codes=p, v_params=p),
+                             **other})
+        return {L.ms_kv4_append(_lib.Kv4AppendArgs(dtype=1, tokens=0, cache=c), None),
+                L.ms_kv4_read(_lib.Kv4ReadArgs(dtype=1, tokens=0, cache=c), None),
+                L.ms_kv4_attention(_lib.Kv4AttentionArgs(dtype=1, tokens=1, heads=1, rows=0, scale=1.0, cache=c), None)}
+
+    for name in ("k_params", "v_params"):
+        assert call(64, **{name: p + 8}) == {0} and call(96, **{name: p + 8}) == {-4}
+        assert call(64, **{name: p + 4}) == {-4}
+    for name in ("k_codes", "v_codes"):
+        assert call(64, **{name: p + 8}) == {-4}
