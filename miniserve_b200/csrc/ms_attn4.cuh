@@ -486,8 +486,9 @@ __device__ __forceinline__ float a4_moved(float m, float old, bool far, float to
 __device__ __forceinline__ float a4_record_reference(float m, float base, bool far, float unit) {
   return m == kA4Least ? __uint_as_float(0xFF800000u) : far ? fminf(fmaxf(m * unit, -3e38f), 3e38f) : 7.f - base;
 }
-// The largest value scale of a tile, from its values' parameters as products take
-// them (rows of even parameters); an infinite one spoils its own group alone.
+// The largest value scale of a tile, of either sign, from its values' parameters as
+// products take them (rows of even parameters); an infinite one spoils its own group
+// alone.
 template <int kHalves>  // of the tile
 __device__ __forceinline__ float a4_largest(const uint32_t (&vp)[kHalves][2], bool scale_lane) {
   float largest = 0.f;
@@ -495,7 +496,7 @@ __device__ __forceinline__ float a4_largest(const uint32_t (&vp)[kHalves][2], bo
   for (int hf = 0; hf < kHalves; ++hf)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&vp[hf][i]));
+      const float2 f = __half22float2(__habs2(*reinterpret_cast<const __half2 *>(&vp[hf][i])));
       if (scale_lane) largest = fmaxf(largest, fmaxf(f.x <= 65504.f ? f.x : 0.f, f.y <= 65504.f ? f.y : 0.f));
     }
 #pragma unroll
@@ -717,7 +718,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
 #pragma unroll
     for (int hf = 0; hf < kA4Halves; ++hf) {
       ldmatrix2t(vp[hf], kst + R::kVp + (hf * kA4Half + (lane & 15)) * 16);
-      most = __hmax2(most, __hmax2(*reinterpret_cast<__half2 *>(&vp[hf][0]), *reinterpret_cast<__half2 *>(&vp[hf][1])));
+      most = __hmax2(most, __hmax2(__habs2(*reinterpret_cast<__half2 *>(&vp[hf][0])), __habs2(*reinterpret_cast<__half2 *>(&vp[hf][1]))));
     }
     bool moves = scale_lane && (__low2float(most) > v_scale.most || __high2float(most) > v_scale.most);
     float high[2];
@@ -1024,7 +1025,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
       // the values' parameters as B: column r is parameter r, of keys 2c and 2c + 1, and 8 on
       uint32_t vp[1][2];
       ldmatrix2t(vp[0], smem_addr(vps) + (lane & 15) * 16);
-      const __half2 most = __hmax2(*reinterpret_cast<__half2 *>(&vp[0][0]), *reinterpret_cast<__half2 *>(&vp[0][1]));
+      const __half2 most = __hmax2(__habs2(*reinterpret_cast<__half2 *>(&vp[0][0])), __habs2(*reinterpret_cast<__half2 *>(&vp[0][1])));
       bool moves = scale_lane && (__low2float(most) > v_scale.most || __high2float(most) > v_scale.most);
 #pragma unroll
       for (int t = 0; t < NP; ++t)

@@ -593,3 +593,29 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(TypeError, match="CUDA"):
         attention_kv4(torch.zeros((1, 4, 64), dtype=BF16), cache, torch.zeros((1, 1), dtype=torch.int32),
                       torch.zeros(1, dtype=torch.int32))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("share", [0.5, 1.0])
+@pytest.mark.parametrize("T,H,Hkv,D", [(1, 8, 2, 64), (1, 4, 1, 128), (5, 14, 2, 64), (3, 8, 1, 96)])
+def test_scales_of_either_sign(T, H, Hkv, D, dtype, share):
+    """m + s (c - 8) is m + (-s) ((16 - c) - 8): a cache of some scales' other
+    sign stands for the same entries, whatever their size."""
+    def scales(p):
+        for codes in (p.cache.k_codes, p.cache.v_codes):  # no code of 0: 16 is none
+            codes.copy_(codes | (((codes & 15) == 0) + 16 * ((codes >> 4) == 0)).to(torch.uint8))
+        p.cache.v_params[..., :p.used_groups, 0] *= 2.0 ** 13
+    p = Problem(3, T, H, Hkv, D, [300, 17, 90], 16, dtype=dtype, scales=scales)
+    p.check(*p.run())
+    gen = torch.Generator(device="cuda").manual_seed(18)
+    mirrored = copy.copy(p)
+    tensors = [t.clone() for t in p.cache._args[:4]]
+    for codes, params in (tensors[:2], tensors[2:]):
+        for g in range(params.shape[-2]):
+            turn = torch.rand(params.shape[:3], generator=gen, device="cuda") < share
+            part = codes[..., 16 * g:16 * g + 16]
+            part.copy_(torch.where(turn[..., None], (16 - (part & 15)) | ((16 - (part >> 4)) << 4), part))
+            params[..., g, 0] = torch.where(turn, -params[..., g, 0], params[..., g, 0])
+    mirrored.cache = KvCache4(*tensors, head_dim=D, dtype=dtype)
+    p.check(*mirrored.run())
