@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) ms_verify_draw_kern
   finish(token, vf_weight(scale, V::one(row + token), sh.power) * share);
 }
 
-// Entries of a slice: about three slices for each warp that an SM has room for,
+// Entries of a slice: about four slices for each warp that an SM has room for,
 // but 4096 entries (what a slice costs besides its entries is that of 1000), or
 // what fills the GPU once, of 1024 entries at least.  64 rows: 66 us with one
 // slice a warp, 65 with two to six.
@@ -777,7 +777,7 @@ static void vf_slices(int64_t positions, int64_t vocab, int *slices, int *slice)
     const int64_t want = std::max<int64_t>(1, (all + positions - 1) / positions);
     return ((vocab + want - 1) / want + 1023) / 1024 * 1024;
   };
-  *slice = (int)std::max(each(3 * warps), std::min<int64_t>(4096, each(warps)));
+  *slice = (int)std::max(each(4 * warps), std::min<int64_t>(4096, each(warps)));
   *slices = (int)((vocab + 8 + *slice - 1) / *slice);  // 8: a row may start inside a piece
 }
 
