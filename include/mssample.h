@@ -622,8 +622,10 @@ int ms_kv4_read(const ms_kv4_read_args *args, ms_stream_t stream);
  * k_j and v_j being what the cache stands for, not rounded; scores and sums in
  * fp32, the weights (times the values' scales) rounded to fp16 for their
  * product with the codes (for an fp16 out to two halves, 2^-22), out rounded
- * once.  A token that sees no key has out
- * 0 and lse -inf.  What the cache holds past the keys that a token sees is not
+ * once.  These products are held down to 2^-31 of the largest weight times the
+ * largest value scale of the head's keys: entries of groups whose scale is less
+ * than 2^-20 of that one's lose bits.  A token that sees no key has out 0 and
+ * lse -inf.  What the cache holds past the keys that a token sees is not
  * used for it, NaN and infinities included.  A row with a length below 0 or
  * past its pages has out 0 and lse -inf for all its tokens and is flagged
  * MS_ROW_BAD_LENGTH; one that uses a page outside the cache has so for the
@@ -688,7 +690,7 @@ int64_t ms_kv4_attention_workspace(int64_t rows, int32_t tokens, int32_t heads, 
  * subtracted an infinity, a negative entry or a NaN (read as 0).
  *
  * Acceptance is decided with sums of fp32 weights (within 1e-6 of p), draws
- * with fp64 weights and sums.  drafts is at most 255.  The struct is read on the host
+ * with fp64 weights and sums (2^-38 of each weight).  drafts is at most 255.  The struct is read on the host
  * during the call; strides count entries.  workspace: ms_verify_workspace(...)
  * bytes, 16-byte aligned, this call's until it has finished.
  */

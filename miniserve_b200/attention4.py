@@ -32,7 +32,9 @@ def attention_kv4(q, cache: KvCache4, pages, lengths, *, scale: Optional[float] 
     of a row flagged MS_ROW_BAD_LENGTH, and the heads of a row flagged
     MS_ROW_BAD_PAGE that met the page.  What the cache holds past a token's
     keys does not touch its result.  Scores and sums are fp32; weights are
-    rounded to fp16 (for fp16 queries to two halves), the result once.
+    rounded to fp16 (for fp16 queries to two halves), the result once; entries
+    whose 32 share a scale below 2^-20 of the largest value scale of the head's
+    keys lose bits.
     """
     entry = _lib.binding()
     try:

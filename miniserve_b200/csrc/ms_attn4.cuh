@@ -525,9 +525,10 @@ __device__ __forceinline__ bool a4_none(uint32_t u) {
 // 64 ragged rows (up to 8192 keys of 4 heads of 128, four queries each, fp16) take
 // 67 us, 202 MB at 3.0 TB/s; 2 rows of 131072 keys of 8 such heads (bf16) 86 us,
 // 325 MB at 3.8 TB/s; 128 rows of five tokens (4096 keys of 2 heads of 64, seven
-// queries each) 66 us; 8 rows of up to 700 keys 11.4 us, latency.  Some 400
-// operations for 16 keys of four groups, 26 of them products; issue slots are half
-// busy, three warps a scheduler (registers), the tensor pipe a quarter.
+// queries each) 66 us; 8 rows of up to 700 keys 11.3 us, latency.  16 keys cost a
+// warp some 400 operations (four groups in bf16, 26 of them products), 440 in fp16,
+// 500 in the wide kernel; in the narrow one issue slots are half busy, three warps a
+// scheduler (registers), the tensor pipe a quarter.
 //
 // All rows' items form one sequence; every warp takes an equal,
 // contiguous share of it, whatever the rows' lengths, and works alone: a ring of
@@ -559,9 +560,12 @@ __device__ __forceinline__ bool a4_none(uint32_t u) {
 // most 2^8 of what they refer to (it moves only when a score passes it by 2^8),
 // scaled up by 2^7 (and up to 2^0.5: references are whole numbers), and by the
 // power of two below 1 over the largest value scale met, so that fp16 holds them
-// with 2^-21 and less of the largest at full precision.  p s_g and p are off by
-// 2^-12 of themselves, which beside a bf16 answer's own 2^-9 is nothing and beside
-// an fp16 answer's 2^-12 is as much again: for fp16 (kFine) a query takes two rows
+// with 2^-21 and less of the largest at full precision; a smaller one is off by up to
+// 2^-31 of the largest, so that a group whose scale is 2^-20 of the largest met loses
+// bits of its codes' part.  p s_g and p are off by 2^-12 of themselves.  Beside a bf16
+// answer's own 2^-9 that adds 1 to 2 % to its error (0.00172 for 0.00169); taking what
+// rounding leaves there too would cost 93 us for 87 (2 rows of 131072 keys) and 91 for
+// 66 (five tokens).  Beside an fp16 answer's 2^-12 it is as much again: for fp16 (kFine) a query takes two rows
 // of a product, one of its weights and one of what rounding left of them (2^-23),
 // and their sums are added at the end (64 ragged rows, four queries a key head: 62
 // -> 67 us; the answers' error from 1.5 of what rounding them costs to 1.0).

@@ -16,10 +16,11 @@
 //
 // Both are bound by bytes: an append reads each entry in 2 bytes and writes
 // 5 bits of it, a read back the reverse.  Measured: 20011 tokens of 32 query and
-// 8 + 8 key and value heads of 128 in 98 us, 436 MB at 4.4 TB/s (two thirds of a
-// plain copy's rate: every entry costs some ten operations, issue slots are 60 %
-// busy and 44 % of the warps resident); 8 tokens in 3.7 us, a launch.  65536
-// tokens of 8 heads of 128 read back in 62 us, 352 MB at 5.7 TB/s.
+// 8 + 8 key and value heads of 128 in 94 us, 436 MB at 4.6 TB/s (70 % of a plain
+// copy's rate: every entry costs some ten operations, issue slots are 60 % busy and
+// 44 % of the warps resident; a thread loads both sides of a key's pairs and turns
+// one, and every key head loads the table again); 8 tokens in 2.2 us, a launch.
+// 65536 tokens of 8 heads of 128 read back in 62 us, 352 MB at 5.7 TB/s.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

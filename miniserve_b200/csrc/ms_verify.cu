@@ -9,15 +9,15 @@
 //
 // Two kernels.  The first reads every position's logits once, for their largest
 // values and the sums of their weights in fp32 (bound by bytes): what the
-// decisions compare with is off by 1e-7, which decides one case in ten million
-// otherwise.  The second, a cluster of CTAs a row, decides and draws from one
+// decisions compare with is off by up to 1e-6, which decides at most one case in a
+// million otherwise.  The second, a cluster of CTAs a row, decides and draws from one
 // position.  A draw compares with the running mass at every one of the
 // vocabulary's borders, so that its weights and sums are in 64 bits: with 32
 // about one draw in a thousand would land beside its token.
 //
-// Measured, four drafts a row over 151936 fp32 logits: 64 rows 63 us, of which
-// the sums, 175 MB at 5.2 TB/s, are 33 and the draws 30 (latency: fp64 operations
-// one after the other, and the sums' way through the cluster); one row 16 us.
+// Measured, four drafts a row over 151936 fp32 logits: 64 rows 64 us, of which
+// the sums, 175 MB at 5.2 TB/s, are 34 and the draws 30 (latency: fp64 operations
+// one after the other, and the sums' way through the cluster); one row 17 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
