@@ -475,7 +475,8 @@ __device__ __forceinline__ void a4_sums(const float (&sum)[NG], uint32_t &high, 
   high = a4_pack(-8.f * h, h);
   low = a4_pack(-8.f * (own - h), own - h);
 }
-// A score's unit in units of log2: neither 0 nor infinite, for 0 times -inf is no number.
+// A score's unit in units of log2: neither 0 nor infinite, for 0 times -inf is no number.  (Scores whose unit is held to
+// 1e38 differ by 2^50 and more where they differ: their weights stay 0 and 1.)
 __device__ __forceinline__ float a4_unit(float unit) { return fminf(fmaxf(unit, 1e-38f), 1e38f); }
 // What weights that refer to score m are to be multiplied by when they come to
 // refer to score `top`: where scores are far (past 2^20 units of log2) weights
@@ -483,8 +484,9 @@ __device__ __forceinline__ float a4_unit(float unit) { return fminf(fmaxf(unit, 
 __device__ __forceinline__ float a4_moved(float m, float old, bool far, float top, float whole, bool next_far, float unit) {
   return at_exp2(far ? (next_far ? (m - top) * unit : fmaf(m, unit, -whole)) : (next_far ? fmaf(-top, unit, old) : old - whole));
 }
-__device__ __forceinline__ float a4_record_reference(float m, float base, bool far, float unit) {
-  return m == kA4Least ? __uint_as_float(0xFF800000u) : far ? fminf(fmaxf(m * unit, -3e38f), 3e38f) : 7.f - base;
+// A record's reference in units of log2, of a score m in units of 1 / `by`.
+__device__ __forceinline__ float a4_record_reference(float m, float base, bool far, float by, float unit) {
+  return m == kA4Least ? __uint_as_float(0xFF800000u) : far ? fminf(fmaxf(m * by * unit, -3e38f), 3e38f) : 7.f - base;
 }
 // The largest value scale of a tile, of either sign, from its values' parameters as
 // products take them (rows of even parameters); an infinite one spoils its own group
@@ -580,6 +582,9 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
   constexpr int kPitch = R::kPitch, kStage = R::kStage, kPairs = R::kPairs;
   const float kNone = __uint_as_float(0xFF800000u);
   extern __shared__ __align__(128) unsigned char a4_ring[];
+  // Of the warps' queries, what a score of 1 is in units of log2: a score's own unit here is 2^22 times that, past fp32
+  // where scale times q passes 1e31, and a record's reference is not.
+  __shared__ float plain_units[kA4Warps][8];
   grid_wait();  // the call's first kernel
   grid_release();
   A4Walk now;
@@ -615,6 +620,8 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
       a4_query_load<NG>(a, own < n, now.b * x.q_row + token * x.q_token + (h * a.group + q - token * a.group) * x.q_head, u);
       a4_query<NG>(a, u, qf, sum, down);
       a4_sums<NG>(sum, qs[0], qs[1]);
+      __syncwarp();  // the last item's have been read
+      if (c == 0) plain_units[warp][r] = a4_unit(a.scale_log2 * down);
       least = 0x7FFFFFFF;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {  // of the queries that this lane's columns of a product are
@@ -833,7 +840,8 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_narrow_ctas(NG))
       const int g = c * 2 + i;
       const int64_t rec = piece * a.chunk_rows + g;
       if (g < n && r == 0)
-        a.own_ml[rec] = make_float2(a4_record_reference(m[i], base[i], far, unit[i]), broken ? kAtBadPage : l[i] * 0x1p-7f);
+        a.own_ml[rec] = make_float2(a4_record_reference(m[i], base[i], far, 0x1p22f, plain_units[warp][g]),
+                                    broken ? kAtBadPage : l[i] * 0x1p-7f);
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         const float middle = __shfl_sync(0xFFFFFFFFu, z[i], (2 * k + 1) * 4 + c) * 0x1p-7f;
@@ -1162,7 +1170,7 @@ __global__ void __launch_bounds__(kA4Warps * 32, a4_wide_ctas(NG, NP))
         const int g = (t * kOwn + i) * 8 + r;
         const int64_t rec = piece * a.chunk_rows + g;
         if (g < n && c == 0)
-          a.own_ml[rec] = make_float2(a4_record_reference(i ? m[t * 32].y : m[t * 32].x, base[t][i], far, unit[t][i]),
+          a.own_ml[rec] = make_float2(a4_record_reference(i ? m[t * 32].y : m[t * 32].x, base[t][i], far, 1.f, unit[t][i]),
                                       broken ? kAtBadPage : l[t][i] * 0x1p-7f);
 #pragma unroll
         for (int k = 0; k < NG; ++k) {

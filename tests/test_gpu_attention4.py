@@ -619,3 +619,25 @@ def test_scales_of_either_sign(T, H, Hkv, D, dtype, share):
             params[..., g, 0] = torch.where(turn, -params[..., g, 0], params[..., g, 0])
     mirrored.cache = KvCache4(*tensors, head_dim=D, dtype=dtype)
     p.check(*mirrored.run())
+
+
+@gpu
+@pytest.mark.parametrize("spread,scale", [(1e35, None), (1.5, 1e35), (1e4, 1e31)])
+@pytest.mark.parametrize("T,H,dtype", [(1, 4, BF16), (1, 8, BF16), (2, 14, BF16), (1, 4, FP16), (3, 8, FP16)])
+def test_scores_near_the_end_of_fp32(T, H, dtype, spread, scale):
+    """Scores of 1e35 and more: lse is the largest one, within what scores may be
+    off by, and nothing is infinite or NaN."""
+    if dtype == FP16:
+        spread = min(spread, 1e4)
+    p = Problem(2, T, H, 1 if H < 14 else 2, 64, [100, 3000], 16, dtype=dtype, spread=spread)
+    by = 0.125 if scale is None else scale
+    out, lse, status = p.run(scale=scale)
+    assert not status.any() and bool(out.isfinite().all())
+    for b in range(2):
+        for t in range(T):
+            c, s, z = p.keys(b, p.lens[b][t], p.cache.k_codes, p.cache.k_params)
+            q = p.q[b, t].double().view(s.shape[0], -1, 64)
+            want = (q @ (z + s * (c - 8)).transpose(1, 2)).amax(-1) * by
+            mag = (q.abs() @ (s * (c + 8) + z.abs()).transpose(1, 2)).amax(-1) * by
+            assert bool((mag < 2e38).all())
+            assert bool(((lse[b, t].double().view_as(want) - want).abs() <= 2.0 ** -18 * mag).all())
